@@ -202,6 +202,95 @@ int tb_attention_bwd(const void* d_Q, const void* d_K, const void* d_V, const vo
                      const float* d_lse, float* d_delta, float* d_dQ, float* d_dK, float* d_dV, int B, int H, int T,
                      int hd, float scale, void* stream);
 
+/* ---- a paged cache of keys and values --------------------------------------------- */
+
+/* No counterpart in the reference, which has no KV cache (training/generate.c:186-212); TbDecoder's own cache holds
+ * sequences of one length in lockstep.  These operators serve sequences of different lengths over one pool of pages:
+ * append a chunk of new tokens (position rotation included), let the chunk attend to all that is cached, read rows back.
+ *
+ * The pool belongs to the caller.  Key (or value) row t of sequence s and key head h is row
+ *     [page = table[s * table_ld + t / page_size]][h][t % page_size]   of  K (V)  [pages][heads][page_size][head_dim].
+ * TB_KV_BF16: rows of bf16, head_dim a multiple of 8 up to 128.  TB_KV_E4M3: rows of 8-bit floats (4 exponent bits, 3 of
+ * significand, largest 448) with one float32 scale per row in k_scale (v_scale) [pages][heads][page_size], head_dim a multiple of
+ * 16 up to 128; a row stands for code * scale.  page_size is 16, 32, 64, 128 or 256.  Table entries behind a sequence's last row
+ * are not looked at, and rows of a page behind it may hold anything, NaN included.  Pointers 16-byte aligned.
+ *
+ * A batch is given by device arrays, so that a captured call can be replayed with other lengths: the new rows of sequence s
+ * are rows q_start[s] .. q_start[s + 1] - 1 of the row arrays (ascending, q_start [seqs + 1]), the sequence has kv_len[s] keys
+ * with them, so that its new rows sit at positions kv_len[s] - n .. kv_len[s] - 1.  A sequence may have no new row.  Rows
+ * behind q_start[seqs] are left as they are.
+ * A page outside the pool, a position or a length outside what the call allows is left out and reported by the next
+ * tb_check (code 71 or 75: page, 72 or 76: length or position); nothing outside the arrays is read or written. */
+#define TB_KV_BF16 0
+#define TB_KV_E4M3 1
+typedef struct TbKvCache {
+    void *K, *V;
+    float *k_scale, *v_scale;        /* TB_KV_E4M3 only, else NULL */
+    const int32_t* table;            /* [seqs][table_ld] */
+    int32_t type, pages, page_size, heads, head_dim, seqs, table_ld;
+} TbKvCache;
+
+/* how a rotated vector's pairs lie: (2k, 2k + 1) as tb_gemm_qkv_rope_bf16 has them, or (k, k + rot_dim / 2) */
+#define TB_ROPE_PAIRS 0
+#define TB_ROPE_HALVES 1
+
+/* Rows [q | k | v] of `rows` new tokens (float32, or bf16 with qkv_bf16 != 0; q_heads, heads and heads vectors of head_dim;
+ * leading dimension ld_qkv, a multiple of 16 bytes): the first rot_dim elements of every q and k vector are rotated by the
+ * angles of the row's position (tables cos, sin [positions, rot_dim / 2] float32, so that any frequencies and any scaling for long
+ * contexts are the caller's; rot_dim 0: no rotation), q leaves as bf16 [rows, q_heads * head_dim] (leading dimension ld_q, a
+ * multiple of 8), k and v go to their places in the cache.  Float32 arithmetic.  TB_KV_E4M3: scale = max(largest
+ * magnitude of the row / 448, 2^-126), codes are the nearest to value / scale, halves to the even code; a row with an
+ * infinity or NaN in it reads back as NaN.  q_heads a multiple of heads. */
+int tb_kv_append(const TbKvCache* cache, const int32_t* d_q_start, const int32_t* d_kv_len, const void* d_qkv, int qkv_bf16,
+                 int64_t ld_qkv, int rows, int q_heads, const float* d_cos, const float* d_sin, int positions, int rot_dim,
+                 int rope_form, void* d_Q, int64_t ld_q, void* stream);
+
+/* Rows of the cache as bf16 (code * scale, rounded once): rows start[s] .. start[s + 1] - 1 of d_K and d_V receive keys and values
+ * first[s], first[s] + 1, .. of sequence s (first NULL: from 0).  Head h of row r goes to r * ld_row + h * ld_head
+ * (multiples of 8): ld_head = head_dim gives [rows, heads * head_dim], ld_head = rows * head_dim one matrix per head as
+ * tb_attention_fwd reads them.  d_K or d_V may be NULL. */
+int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_first, int rows, void* d_K, void* d_V,
+               int64_t ld_row, int64_t ld_head, void* stream);
+
+/* Causal attention of the new rows over the cache (their own keys included: append first):
+ *   att[r, h] = sum_t p_t V_t,  p = softmax over t <= position of r of  scale * <Q[r, h], K_t>,  key head h * heads / q_heads.
+ * d_Q, d_att: bf16 [rows, q_heads * head_dim] (leading dimensions multiples of 8).  d_lse (optional): float [rows, q_heads], natural
+ * log of the row's sum of exponentials.  Keys behind a row's position have no influence on it, whatever they hold.  A row without
+ * any key (kv_len below the number of new rows) gets zeros and lse -infinity.
+ * max_q and max_kv bound the new rows and the keys of any one sequence (host numbers: they size the launch, and a captured
+ * call may be replayed with any lengths within them).  d_workspace: tb_attention_paged_workspace(..) bytes, 16-byte aligned,
+ * contents of no concern (NULL where that is 0); calls that can overlap on the GPU need one each. */
+int64_t tb_attention_paged_workspace(const TbKvCache* cache, int rows, int q_heads, int max_q, int max_kv);
+int tb_attention_paged(const TbKvCache* cache, const int32_t* d_q_start, const int32_t* d_kv_len, const void* d_Q, int64_t ld_q,
+                       int rows, int q_heads, int max_q, int max_kv, float scale, void* d_att, int64_t ld_att, float* d_lse,
+                       void* d_workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- rules on logits ---------------------------------------------------------------- */
+
+/* No counterpart in the reference (training/generate.c:57-73 samples from the plain logits).  Between the LM head
+ * and the choice of a token, for row s of [rows, vocab] float32 logits, in this order:
+ *   z = z > 0 ? z / repetition[s] : z * repetition[s]     for tokens among the row's prompt or output ids
+ *   z -= frequency[s] * c,  c = how often the token is among the row's output ids
+ *   z -= presence[s]                                      where c > 0
+ *   z += the sum of the row's bias entries for the token (in the order of the list)
+ *   z = -infinity                                         where the row's mask does not allow the token
+ * Any pointer may be NULL: that rule is left out.  Ids outside the vocabulary are passed over (padding).  A mask that
+ * allows nothing leaves a row of -infinity. */
+typedef struct TbLogitRules {
+    const uint32_t* prompt; const int32_t* prompt_len;     /* [rows][prompt_ld]: the first prompt_len[s] ids of row s */
+    const uint32_t* output; const int32_t* output_len;     /* [rows][output_ld] */
+    const float *repetition, *frequency, *presence;        /* [rows]; repetition > 0, 1 for none */
+    const int32_t* bias_start; const uint32_t* bias_id; const float* bias_value;   /* entries bias_start[s] .. bias_start[s + 1] - 1 */
+    const uint32_t* mask; const int32_t* mask_row;         /* [masks][mask_ld] words, bit v % 32 of word v / 32 set: allowed; mask_row
+                                                              [rows]: the row's mask, -1 for none (NULL: mask s for row s) */
+    int32_t prompt_ld, output_ld, masks, mask_ld, bias_entries;
+} TbLogitRules;
+
+/* d_out may be d_logits (in place) or another matrix that does not overlap it.  Ids of a row number less than 2^30; a length or an
+ * index outside its array is cut to it or left out, and reported by the next tb_check (code 81). */
+int tb_logits_adjust(const TbLogitRules* rules, const float* d_logits, int64_t ld_logits, float* d_out, int64_t ld_out, int rows,
+                     int vocab, void* stream);
+
 /* ---- GPU-resident trainer ---------------------------------------------------- */
 
 /* GpuTrainer (model/gpu_train.h:51-80).  Parameters, gradients and Adam state are flat

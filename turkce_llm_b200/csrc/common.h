@@ -198,6 +198,11 @@ int make_operand_map_f32(CUtensorMap* map, const float* ptr, long long inner, lo
 int make_operand_map4(CUtensorMap* map, const bf16* ptr, long long inner, long long rows, long long ld,
                       long long n0, long long stride0, long long n1, long long stride1, int box_rows);
 
+// a pool of cache pages seen as [blocks][rows][inner], blocks of one head of a page.  es = 2: bf16, box of 64 elements (128-byte
+// swizzle), es = 1: bytes, box of box_inner (as they lie)
+int make_cache_map(CUtensorMap* map, const void* ptr, int es, long long inner, long long rows, long long blocks, int box_inner,
+                   int box_rows);
+
 // ---- fused causal attention (attention.cu); Q, K, V bf16 [B*H, T, hd] (hd <= 64, multiple of 8)
 // forward: att bf16 [B*T, H*hd] (heads merged), lse float [B*H, T] (natural-log sum of exponentials)
 // (lse may be NULL; kv_rows_per_head > T when K and V live in a KV cache with that many rows per head)
@@ -257,6 +262,11 @@ int lmhead_argmax_ctas(const DeviceCtx* ctx, int S, int V, int K);
 int launch_lmhead_argmax(DeviceCtx* ctx, const bf16* X, const bf16* E, int S, int V, int K, bool table_is_stable,
                          unsigned long long* best, unsigned int* ticket, uint32_t* tok, uint32_t* out, int* state,
                          int out_ld, int advance_pos, float* logits, long long ld_logits, cudaStream_t st);
+
+// Penalties, biases and masks on [rows, V] logits (logit_rules.cu; in may be out)
+struct LogitRuleArgs;
+int launch_logit_rules(DeviceCtx* ctx, const LogitRuleArgs& r, const float* in, long long ld_in, float* out, long long ld_out, int rows, int V,
+                       cudaStream_t st);
 
 // Linear layer of a decode step for S <= 64 rows (decode_linear.cu): y32 [S, N] = X W + bias (+ residual), or with
 // h16 given (N = 2F) h16 [S, F] = silu(gate) * up.  X is bf16 [S, K], or x32 float32 [S, K] with the RMSNorm

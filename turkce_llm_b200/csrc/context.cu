@@ -131,6 +131,15 @@ int device_error_result(DeviceCtx* ctx) {
         // the ticket words and packed maxima behind the error word go back to zero as well: a kernel that
         // gave up may have left them half-way
         cudaMemset(ctx->d_err, 0, 1024);
+        // (codes of arguments that only the device sees: the kernel has left them out and gone on)
+        const char* what = h == 71 || h == 75   ? "a page table names a page outside the pool"
+                           : h == 72 || h == 76 ? "a length or position of a batch is outside what its call allows"
+                           : h == 81            ? "a length or index of the rules on logits is outside its array"
+                                                : nullptr;
+        if (what) {
+            set_error("%s (code %d); what it concerns was left out", what, h);
+            return -3;
+        }
         const char* who = h == 1 ? "TMA producer" : h == 2 ? "MMA issuer" : h == 3 ? "epilogue" : "kernel";
         set_error("a kernel gave up on a bounded wait (%s, code %d); its output is invalid", who, h);
         return -3;

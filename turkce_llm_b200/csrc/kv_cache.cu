@@ -1,0 +1,330 @@
+// Writing new tokens' keys and values into a paged cache, position rotation included, and reading rows of it back.
+//
+// Both kernels move bytes and do little else: eight elements of one head per thread, so that a head of 64 is one 256-byte
+// (float32), 128-byte (bf16) or 64-byte (8-bit) piece of consecutive threads on either side.  A warp belongs to one row
+// (token), and finds the row's sequence, position and page once for all its heads.
+#include "paged.cuh"
+
+#include <algorithm>
+
+namespace tb {
+
+int check_cache(const TbKvCache* c, const char* who) {
+    TB_CHECK(c != nullptr, "%s: NULL cache", who);
+    TB_CHECK(c->K && c->V && c->table, "%s: the cache has a NULL pool or table", who);
+    TB_CHECK(c->type == TB_KV_BF16 || c->type == TB_KV_E4M3, "%s: unknown cache type %d", who, c->type);
+    const int step = c->type == TB_KV_E4M3 ? 16 : 8;
+    TB_CHECK(c->head_dim >= step && c->head_dim <= 128 && c->head_dim % step == 0, "%s: head_dim must be a multiple of %d up to 128 (got %d)",
+             who, step, c->head_dim);
+    TB_CHECK(c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128 || c->page_size == 256,
+             "%s: page_size must be 16, 32, 64, 128 or 256 (got %d)", who, c->page_size);
+    TB_CHECK(c->pages > 0 && c->heads > 0 && c->seqs > 0 && c->table_ld > 0, "%s: cache dims must be positive", who);
+    TB_CHECK((long long)c->pages * c->heads < (1LL << 31), "%s: pages * heads must be below 2^31", who);
+    TB_CHECK((long long)c->table_ld * c->page_size < (1LL << 31), "%s: table_ld * page_size must be below 2^31", who);
+    TB_CHECK(c->seqs <= 65535, "%s: at most 65535 sequences (got %d)", who, c->seqs);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(c->K) | reinterpret_cast<uintptr_t>(c->V);
+    TB_CHECK((at & 15u) == 0, "%s: the pools must be 16-byte aligned", who);
+    if (c->type == TB_KV_E4M3) {
+        TB_CHECK(c->k_scale && c->v_scale, "%s: an 8-bit cache needs both scale arrays", who);
+        TB_CHECK(((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 15u) == 0,
+                 "%s: the scale arrays must be 16-byte aligned", who);
+    } else {
+        TB_CHECK(!c->k_scale && !c->v_scale, "%s: a bf16 cache has no scales", who);
+    }
+    return 0;
+}
+
+namespace {
+
+constexpr int KV_THREADS = 256;
+constexpr int KV_WARPS = KV_THREADS / 32;
+
+struct AppendParams {
+    PagedView v;
+    const int *q_start, *kv_len;
+    const void* x; long long ld_x;
+    int rows, H, warps_per_row, threads_log2;        // threads per head: 1 << threads_log2
+    const float *cos_t, *sin_t;
+    int positions, half;                              // rot_dim / 2
+    bf16* Q; long long ld_q;
+    void *K, *V;
+    float *ks, *vs;
+    int* err;
+};
+
+template <bool BF16_IN>
+__device__ __forceinline__ void load8(const void* x, long long at, float (&f)[8]) {
+    if (BF16_IN) {
+        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(x) + at);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 p = bf16_floats(u[i]);
+            f[2 * i] = p.x; f[2 * i + 1] = p.y;
+        }
+    } else {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
+        const float4 a = p[0], b = p[1];
+        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    }
+}
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+    return make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
+}
+
+// Rotated elements are a cos - b sin and a sin + b cos with every product rounded, the same sums whichever thread forms them.
+template <bool BF16_IN, bool HALVES, bool E4M3>
+__global__ void __launch_bounds__(KV_THREADS)
+kv_append_kernel(const AppendParams p) {
+    __shared__ float swap[HALVES ? KV_WARPS : 1][HALVES ? 32 * 9 : 1];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned w = blockIdx.x * KV_WARPS + warp;
+    const int row = (int)(w / (unsigned)p.warps_per_row), part = (int)(w - (unsigned)row * (unsigned)p.warps_per_row);
+    if (row >= p.rows) return;                                   // (whole warps)
+    const int hd = p.v.hd, G = p.v.heads;
+    const int head = (part << (5 - p.threads_log2)) + (lane >> p.threads_log2);
+    const int e0 = (lane & ((1 << p.threads_log2) - 1)) * 8;     // first of this thread's elements
+    const bool mine = head < p.H + 2 * G && e0 < hd;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (mine) load8<BF16_IN>(p.x, (long long)row * p.ld_x + (long long)head * hd + e0, x);      // (needs nothing of the batch)
+    const int s = sequence_of(p.q_start, p.v.seqs, row);
+    if (s < 0) return;
+    const int end = p.q_start[s + 1], len = p.kv_len[s];
+    if (row >= end) return;                                      // behind the last sequence
+    const long long pos = (long long)len - end + row;
+    if (pos < 0 || pos >= (long long)p.v.table_ld << p.v.page_shift || (p.half > 0 && pos >= p.positions)) {
+        if (lane == 0) atomicExch(p.err, 72);
+        return;
+    }
+    const int page = p.v.table[(long long)s * p.v.table_ld + (pos >> p.v.page_shift)];
+    if (p.half > 0 && part * (32 >> p.threads_log2) < p.H + G) {     // (a warp of values alone has nothing to rotate)
+        const bool turns = head < p.H + G;
+        const float* ct = p.cos_t + pos * p.half;
+        const float* st = p.sin_t + pos * p.half;
+        if (!HALVES) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = (e0 >> 1) + i;
+                if (mine && turns && k < p.half) {
+                    const float c = ct[k], d = st[k], a = x[2 * i], b = x[2 * i + 1];
+                    x[2 * i] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, d));
+                    x[2 * i + 1] = __fadd_rn(__fmul_rn(a, d), __fmul_rn(b, c));
+                }
+            }
+        } else {
+            // the partner's elements through shared memory: element e of this head at (e / 8) * 9 + e % 8 from the head's first
+            float* sw = swap[warp];
+            const int base = (lane >> p.threads_log2 << p.threads_log2) * 9;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sw[lane * 9 + i] = x[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = e0 + i;
+                if (mine && turns && e < 2 * p.half) {
+                    const bool low = e < p.half;
+                    const int k = low ? e : e - p.half, o = low ? e + p.half : e - p.half;
+                    const float other = sw[base + (o >> 3) * 9 + (o & 7)], c = ct[k], d = st[k];
+                    x[i] = low ? __fsub_rn(__fmul_rn(x[i], c), __fmul_rn(other, d)) : __fadd_rn(__fmul_rn(other, d), __fmul_rn(x[i], c));
+                }
+            }
+        }
+    }
+    if (mine && head < p.H) {
+        *reinterpret_cast<uint4*>(p.Q + (long long)row * p.ld_q + (long long)head * hd + e0) = pack8(x);
+    }
+    // largest magnitude of the row: as integers, so that NaN is larger than infinity and infinity than the rest
+    uint32_t big = 0u;
+    if (E4M3) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
+        for (int o = (1 << p.threads_log2) >> 1; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+    }
+    if (!mine || head < p.H) return;
+    if ((unsigned)page >= (unsigned)p.v.pages) {
+        atomicExch(p.err, 71);
+        return;
+    }
+    const bool key = head < p.H + G;
+    const long long at = (((long long)page * G + (head - p.H - (key ? 0 : G))) << p.v.page_shift) + (pos & ((1 << p.v.page_shift) - 1));
+    if (!E4M3) {
+        *reinterpret_cast<uint4*>(static_cast<bf16*>(key ? p.K : p.V) + at * hd + e0) = pack8(x);
+    } else {
+        float scale = __fdiv_rn(__uint_as_float(big), 448.0f);
+        if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;          // (stays NaN where it is)
+        uint32_t c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = e4m3_pair(quotient_to_odd(x[2 * i], scale), quotient_to_odd(x[2 * i + 1], scale));
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(key ? p.K : p.V) + at * hd + e0) =
+            make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+        if (e0 == 0) (key ? p.ks : p.vs)[at] = scale;
+    }
+}
+
+struct ReadParams {
+    PagedView v;
+    const int *start, *first;
+    int rows, warps_per_row, threads_log2, kinds;     // kinds: 1 or 2 of K and V
+    const void *A, *B;                                // the pools read (B: the second one)
+    const float *as, *bs;
+    bf16 *oA, *oB;
+    long long ld_row, ld_head;
+    int* err;
+};
+
+template <bool E4M3>
+__global__ void __launch_bounds__(KV_THREADS)
+kv_read_kernel(const ReadParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned w = blockIdx.x * KV_WARPS + warp;
+    const int row = (int)(w / (unsigned)p.warps_per_row), part = (int)(w - (unsigned)row * (unsigned)p.warps_per_row);
+    if (row >= p.rows) return;
+    const int hd = p.v.hd, G = p.v.heads;
+    const int head = (part << (5 - p.threads_log2)) + (lane >> p.threads_log2);
+    const int e0 = (lane & ((1 << p.threads_log2) - 1)) * 8;
+    const int s = sequence_of(p.start, p.v.seqs, row);
+    if (s < 0 || row >= p.start[s + 1]) return;
+    const long long t = (long long)row - p.start[s] + (p.first ? p.first[s] : 0);
+    if (t < 0 || t >= (long long)p.v.table_ld << p.v.page_shift) {
+        if (lane == 0) atomicExch(p.err, 72);
+        return;
+    }
+    const int page = p.v.table[(long long)s * p.v.table_ld + (t >> p.v.page_shift)];
+    if ((unsigned)page >= (unsigned)p.v.pages) {
+        if (lane == 0) atomicExch(p.err, 71);
+        return;
+    }
+    if (head >= p.kinds * G || e0 >= hd) return;
+    const bool first = head < G;
+    const int h = first ? head : head - G;
+    const long long at = (((long long)page * G + h) << p.v.page_shift) + (t & ((1 << p.v.page_shift) - 1));
+    uint4 out;
+    if (!E4M3) {
+        out = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(first ? p.A : p.B) + at * hd + e0);
+    } else {
+        const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(first ? p.A : p.B) + at * hd + e0);
+        const float scale = (first ? p.as : p.bs)[at];
+        const uint32_t u[4] = {c.x & 0xffffu, c.x >> 16, c.y & 0xffffu, c.y >> 16};
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = e4m3_floats(u[i]);
+            o[i] = bf16_pair(f.x * scale, f.y * scale);
+        }
+        out = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    *reinterpret_cast<uint4*>((first ? p.oA : p.oB) + (long long)row * p.ld_row + h * p.ld_head + e0) = out;
+}
+
+// threads per head (a power of two that divides a warp), warps per row, and the blocks for all rows
+int shape_of(int hd, int heads, int rows, int* threads_log2, int* warps_per_row, long long* blocks) {
+    int t = 0;
+    while ((8 << t) < hd) ++t;
+    *threads_log2 = t;
+    const int per_warp = 32 >> t;
+    *warps_per_row = (heads + per_warp - 1) / per_warp;
+    *blocks = ((long long)rows * *warps_per_row + KV_WARPS - 1) / KV_WARPS;
+    return 0;
+}
+
+}  // namespace
+
+int launch_kv_append(DeviceCtx* ctx, const TbKvCache* c, const int* q_start, const int* kv_len, const void* x, bool x_bf16, long long ld_x,
+                     int rows, int H, const float* cos_t, const float* sin_t, int positions, int rot_dim, int form, bf16* Q,
+                     long long ld_q, cudaStream_t st) {
+    AppendParams p;
+    p.v = paged_view(c);
+    p.q_start = q_start; p.kv_len = kv_len; p.x = x; p.ld_x = ld_x; p.rows = rows; p.H = H;
+    p.cos_t = cos_t; p.sin_t = sin_t; p.positions = positions; p.half = rot_dim / 2;
+    p.Q = Q; p.ld_q = ld_q; p.K = c->K; p.V = c->V; p.ks = c->k_scale; p.vs = c->v_scale; p.err = ctx->d_err;
+    long long blocks;
+    shape_of(c->head_dim, H + 2 * c->heads, rows, &p.threads_log2, &p.warps_per_row, &blocks);
+    TB_CHECK(blocks < (1LL << 31) / KV_WARPS, "tb_kv_append: too many rows");
+    typedef void (*Kernel)(AppendParams);
+    const bool halves = form == TB_ROPE_HALVES && rot_dim > 0, e4m3 = c->type == TB_KV_E4M3;
+    static const Kernel kernels[8] = {
+        kv_append_kernel<false, false, false>, kv_append_kernel<false, false, true>, kv_append_kernel<false, true, false>,
+        kv_append_kernel<false, true, true>, kv_append_kernel<true, false, false>, kv_append_kernel<true, false, true>,
+        kv_append_kernel<true, true, false>, kv_append_kernel<true, true, true>};
+    const double n = (double)rows * c->head_dim;
+    prof_mark(ctx, "kv_append", 0.0, n * ((H + 2.0 * c->heads) * (x_bf16 ? 2 : 4) + 2.0 * H + 2.0 * c->heads * (e4m3 ? 1 : 2)), st);
+    TB_CUDA(launch_kernel(kernels[(x_bf16 ? 4 : 0) + (halves ? 2 : 0) + (e4m3 ? 1 : 0)], dim3((unsigned)blocks), dim3(KV_THREADS), 0, st, p));
+    ctx->launches++;
+    prof_close(ctx, st);
+    return 0;
+}
+
+int launch_kv_read(DeviceCtx* ctx, const TbKvCache* c, const int* start, const int* first, int rows, bf16* K, bf16* V, long long ld_row,
+                   long long ld_head, cudaStream_t st) {
+    ReadParams p;
+    p.v = paged_view(c);
+    p.start = start; p.first = first; p.rows = rows; p.kinds = K && V ? 2 : 1;
+    p.A = K ? c->K : c->V; p.as = K ? c->k_scale : c->v_scale; p.oA = K ? K : V;
+    p.B = c->V; p.bs = c->v_scale; p.oB = V;
+    p.ld_row = ld_row; p.ld_head = ld_head; p.err = ctx->d_err;
+    long long blocks;
+    shape_of(c->head_dim, p.kinds * c->heads, rows, &p.threads_log2, &p.warps_per_row, &blocks);
+    TB_CHECK(blocks < (1LL << 31) / KV_WARPS, "tb_kv_read: too many rows");
+    const bool e4m3 = c->type == TB_KV_E4M3;
+    prof_mark(ctx, "kv_read", 0.0, (double)rows * p.kinds * c->heads * c->head_dim * (e4m3 ? 3 : 4), st);
+    TB_CUDA(launch_kernel(e4m3 ? kv_read_kernel<true> : kv_read_kernel<false>, dim3((unsigned)blocks), dim3(KV_THREADS), 0, st, p));
+    ctx->launches++;
+    prof_close(ctx, st);
+    return 0;
+}
+
+}  // namespace tb
+
+using namespace tb;
+
+extern "C" {
+
+int tb_kv_append(const TbKvCache* cache, const int32_t* d_q_start, const int32_t* d_kv_len, const void* d_qkv, int qkv_bf16,
+                 int64_t ld_qkv, int rows, int q_heads, const float* d_cos, const float* d_sin, int positions, int rot_dim,
+                 int rope_form, void* d_Q, int64_t ld_q, void* stream) {
+    TB_TRY(check_cache(cache, "tb_kv_append"));
+    TB_CHECK(rows >= 0, "tb_kv_append: rows must not be negative");
+    TB_CHECK(d_q_start && d_kv_len, "tb_kv_append: NULL batch array");
+    TB_CHECK(rows == 0 || (d_qkv && d_Q), "tb_kv_append: NULL operand");
+    TB_CHECK(q_heads > 0 && q_heads % cache->heads == 0, "tb_kv_append: %d query heads cannot share %d key heads", q_heads, cache->heads);
+    const int per16 = qkv_bf16 ? 8 : 4;
+    const long long width = ((long long)q_heads + 2LL * cache->heads) * cache->head_dim;
+    TB_CHECK(ld_qkv >= width && ld_qkv % per16 == 0, "tb_kv_append: ld_qkv must be a multiple of %d and at least %lld (got %lld)", per16, width,
+             (long long)ld_qkv);
+    TB_CHECK(ld_q >= (long long)q_heads * cache->head_dim && ld_q % 8 == 0, "tb_kv_append: ld_q must be a multiple of 8 and at least %lld (got %lld)",
+             (long long)q_heads * cache->head_dim, (long long)ld_q);
+    TB_CHECK(((reinterpret_cast<uintptr_t>(d_qkv) | reinterpret_cast<uintptr_t>(d_Q)) & 15u) == 0, "tb_kv_append: rows must be 16-byte aligned");
+    TB_CHECK(rot_dim >= 0 && rot_dim <= cache->head_dim && rot_dim % 2 == 0, "tb_kv_append: rot_dim must be even and at most head_dim (got %d)", rot_dim);
+    TB_CHECK(rope_form == TB_ROPE_PAIRS || rope_form == TB_ROPE_HALVES, "tb_kv_append: unknown rotation form %d", rope_form);
+    TB_CHECK(rot_dim == 0 || (d_cos && d_sin && positions > 0), "tb_kv_append: a rotation needs both tables");
+    if (rows == 0) return 0;
+    DeviceCtx* ctx;
+    TB_TRY(get_ctx(&ctx));
+    return launch_kv_append(ctx, cache, d_q_start, d_kv_len, d_qkv, qkv_bf16 != 0, ld_qkv, rows, q_heads, d_cos, d_sin, positions, rot_dim,
+                            rope_form, static_cast<bf16*>(d_Q), ld_q, static_cast<cudaStream_t>(stream));
+}
+
+int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_first, int rows, void* d_K, void* d_V, int64_t ld_row,
+               int64_t ld_head, void* stream) {
+    TB_TRY(check_cache(cache, "tb_kv_read"));
+    TB_CHECK(rows >= 0, "tb_kv_read: rows must not be negative");
+    TB_CHECK(d_start, "tb_kv_read: NULL row starts");
+    TB_CHECK(d_K || d_V, "tb_kv_read: both outputs are NULL");
+    TB_CHECK(ld_row >= cache->head_dim && ld_row % 8 == 0 && ld_head >= cache->head_dim && ld_head % 8 == 0,
+             "tb_kv_read: ld_row and ld_head must be multiples of 8 and at least head_dim (got %lld, %lld)", (long long)ld_row,
+             (long long)ld_head);
+    TB_CHECK(ld_row >= (cache->heads - 1) * ld_head + cache->head_dim || ld_head >= (rows - 1LL) * ld_row + cache->head_dim,
+             "tb_kv_read: rows of ld_row %lld and heads of ld_head %lld lie over one another", (long long)ld_row, (long long)ld_head);
+    TB_CHECK(((reinterpret_cast<uintptr_t>(d_K) | reinterpret_cast<uintptr_t>(d_V)) & 15u) == 0, "tb_kv_read: outputs must be 16-byte aligned");
+    if (rows == 0) return 0;
+    DeviceCtx* ctx;
+    TB_TRY(get_ctx(&ctx));
+    return launch_kv_read(ctx, cache, d_start, d_first, rows, static_cast<bf16*>(d_K), static_cast<bf16*>(d_V), ld_row, ld_head,
+                          static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,26 @@
+// The rules on logits as the library's own callers give them (the entry point's arrays, and a step between a row's lengths, 0
+// where all rows share one), and how rows are cut into slices.  The slices are host arithmetic without CUDA types.
+#pragma once
+#include <cstdint>
+
+namespace tb {
+
+// Columns of the vocabulary per CTA: a multiple of 32 (a mask word belongs to one CTA) up to 4096.  As many as give every SM
+// four CTAs, so that few rows spread over the chip and many rows do not read their ids more often than needed.
+inline int logit_rules_slice(int rows, int V, int sms) {
+    const long long want = 4LL * sms;
+    long long slices = (want + rows - 1) / rows;
+    long long s = (V + slices - 1) / slices;
+    s = (s + 31) / 32 * 32;
+    return (int)(s < 512 ? 512 : s > 4096 ? 4096 : s);
+}
+
+struct LogitRuleArgs {
+    const uint32_t* prompt = nullptr; const int* prompt_len = nullptr; int prompt_ld = 0, prompt_len_stride = 1;
+    const uint32_t* output = nullptr; const int* output_len = nullptr; int output_ld = 0, output_len_stride = 1;
+    const float *repetition = nullptr, *frequency = nullptr, *presence = nullptr;
+    const int* bias_start = nullptr; const uint32_t* bias_id = nullptr; const float* bias_value = nullptr; int bias_entries = 0;
+    const uint32_t* mask = nullptr; const int* mask_row = nullptr; int masks = 0, mask_ld = 0;
+};
+
+}  // namespace tb

@@ -1,0 +1,83 @@
+// What the kernels over a paged cache share: the view of the pool, which sequence a row belongs to, and 8-bit codes.
+#pragma once
+#include "../../include/turkce_b200.h"
+#include "common.h"
+
+namespace tb {
+
+struct PagedView {
+    const int* table;
+    int pages, page_shift, heads, hd, seqs, table_ld;
+};
+
+// host: the checks that every entry point makes of a cache
+int check_cache(const TbKvCache* c, const char* who);
+inline int page_shift_of(int page_size) {
+    int s = 0;
+    while ((1 << s) < page_size) ++s;
+    return s;
+}
+inline PagedView paged_view(const TbKvCache* c) {
+    PagedView v;
+    v.table = c->table;
+    v.pages = c->pages; v.page_shift = page_shift_of(c->page_size); v.heads = c->heads; v.hd = c->head_dim;
+    v.seqs = c->seqs; v.table_ld = c->table_ld;
+    return v;
+}
+
+#ifdef __CUDACC__
+
+// The sequence whose rows hold `row`: the last one that starts at or before it; -1 where none does.  A warp looks at 32
+// starts per step, so that up to 32 sequences take one read and up to 1024 take two.  All lanes of the warp call it with the
+// same row.
+__device__ __forceinline__ int sequence_of(const int* __restrict__ start, int seqs, int row) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = seqs;
+    while (true) {
+        const int step = (hi - lo + 31) >> 5;
+        const int i = lo + lane * step;
+        const unsigned below = __ballot_sync(0xffffffffu, i < hi && start[i] <= row);
+        const int n = __popc(below);
+        if (n == 0) return -1;
+        lo += (n - 1) * step;
+        hi = min(lo + step, hi);
+        if (hi - lo <= 1) return lo;
+    }
+}
+
+// x / scale as the nearest 8-bit float (4 exponent bits, 3 of significand), halves to the even one.  The quotient of float32
+// numbers is rounded already; where it was, its last bit is set instead (a number strictly between two floats keeps to its side
+// of every middle of two codes), so that the code is the one nearest to the true quotient.
+__device__ __forceinline__ float quotient_to_odd(float x, float scale) {
+    const float q = __fdiv_rn(x, scale);
+    const float rest = __fmaf_rn(-q, scale, x);
+    uint32_t b = __float_as_uint(q);
+    if (rest != 0.0f && fabsf(q) < INFINITY) {
+        if ((rest < 0.0f) != (x < 0.0f) && (b & 0x7fffffffu) != 0u) b -= 1u;      // |q| was rounded up
+        b |= 1u;
+    }
+    return __uint_as_float(b);
+}
+__device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// two codes -> two float32 / a pair of bf16 (exact)
+__device__ __forceinline__ float2 e4m3_floats(uint32_t two) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+    float2 f;
+    asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(f.x), "=f"(f.y) : "r"(h));
+    return f;
+}
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 bf16_floats(uint32_t two) {
+    return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
+}
+
+#endif
+}  // namespace tb

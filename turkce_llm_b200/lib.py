@@ -12,7 +12,24 @@ NN, NT, TN = 0, 1, 2
 PREC_BF16, PREC_TF32, PREC_FP32 = 0, 1, 2
 CAUSAL_NONE, CAUSAL_SKIP_UPPER, CAUSAL_K_PREFIX, CAUSAL_K_SUFFIX = 0, 1, 2, 3
 
+KV_BF16, KV_E4M3 = 0, 1
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+
 _vp, _i, _i64, _f = C.c_void_p, C.c_int, C.c_int64, C.c_float
+
+
+class KvCacheStruct(C.Structure):
+    """TbKvCache of include/turkce_b200.h."""
+    _fields_ = [(n, C.c_void_p) for n in ("K", "V", "k_scale", "v_scale", "table")] + \
+               [(n, C.c_int32) for n in ("type", "pages", "page_size", "heads", "head_dim", "seqs", "table_ld")]
+
+
+class LogitRulesStruct(C.Structure):
+    """TbLogitRules of include/turkce_b200.h."""
+    _fields_ = [(n, C.c_void_p) for n in ("prompt", "prompt_len", "output", "output_len", "repetition", "frequency", "presence",
+                                          "bias_start", "bias_id", "bias_value", "mask", "mask_row")] + \
+               [(n, C.c_int32) for n in ("prompt_ld", "output_ld", "masks", "mask_ld", "bias_entries")]
+
 
 # name -> (restype, argtypes); every symbol include/turkce_b200.h declares is listed here
 SIGNATURES = {
@@ -45,6 +62,11 @@ SIGNATURES = {
     "tb_gemm_qkv_rope_bf16": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
     "tb_decode_linear": (_i, [_vp, _vp, _vp, _f, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "tb_lmhead_argmax_bf16": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _i64, _i, _vp]),
+    "tb_kv_append": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i, _i, _vp, _vp, _i, _i, _i, _vp, _i64, _vp]),
+    "tb_kv_read": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i64, _i64, _vp]),
+    "tb_attention_paged_workspace": (_i64, [_vp, _i, _i, _i, _i]),
+    "tb_attention_paged": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _f, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "tb_logits_adjust": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _i, _vp]),
     "tb_decoder_create": (_i, [C.POINTER(_vp), _i, _i, _i, _i, _i, _i, _i, _f, _vp]),
     "tb_decoder_destroy": (_i, [_vp]),
     "tb_decoder_total_scalars": (_i64, [_vp]),
