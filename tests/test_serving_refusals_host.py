@@ -27,8 +27,8 @@ def append(c, starts=A, lens=A, qkv=A, bf16=0, ld=512, rows=4, heads=4, cos=A, s
     return ("tb_kv_append", C.byref(c), starts, lens, qkv, bf16, ld, rows, heads, cos, sin, positions, rot, form, q, ld_q, None)
 
 
-def attend(c, starts=A, lens=A, q=A, ld_q=256, rows=4, heads=4, max_q=2, max_kv=40, att=2 * A, ld_att=256, lse=None, ws=None, n=0):
-    return ("tb_attention_paged", C.byref(c), starts, lens, q, ld_q, rows, heads, max_q, max_kv, 0.125, att, ld_att, lse, ws, n, None)
+def attend(c, starts=A, lens=A, q=A, ld_q=256, rows=4, heads=4, max_q=2, max_kv=40, att=2 * A, ld_att=256, lse=None, ws=None, n=0, scale=0.125):
+    return ("tb_attention_paged", C.byref(c), starts, lens, q, ld_q, rows, heads, max_q, max_kv, scale, att, ld_att, lse, ws, n, None)
 
 
 def read(c, starts=A, first=None, rows=4, k=A, v=A, ld_row=128, ld_head=64):
@@ -62,7 +62,8 @@ def test_append_refuses(over, match):
     (dict(starts=None), "NULL operand"), (dict(lens=None), "NULL operand"), (dict(q=None), "NULL operand"), (dict(att=None), "NULL operand"),
     (dict(rows=-1), "negative"), (dict(max_q=-1), "negative"), (dict(max_kv=-1), "negative"), (dict(heads=5), "cannot share"),
     (dict(ld_q=248), "leading dimensions"), (dict(ld_att=260), "leading dimensions"), (dict(q=A + 8), "aligned"), (dict(ws=A + 4, n=99), "aligned"),
-    (dict(att=A), "over the queries"), (dict(rows=1 << 30), "2\\^31")])
+    (dict(att=A), "over the queries"), (dict(heads=260, ld_q=260 * 64, ld_att=260 * 64), "at most 128"), (dict(scale=0.0), "positive and finite"),
+    (dict(scale=-1.0), "positive and finite"), (dict(scale=float("inf")), "positive and finite"), (dict(scale=float("nan")), "positive and finite"), (dict(rows=1 << 30), "2\\^31")])
 def test_attention_refuses(over, match):
     refused(match, *attend(struct(), **over))
 

@@ -6,13 +6,14 @@
 // are taken by different CTAs where there are few sequences; each leaves (o, m, l) and paged_combine_kernel adds them in the order
 // of the pieces.
 //
-// An 8-bit key's scale multiplies its score, an 8-bit value's scale its probability before that is rounded to bf16, so the codes
-// enter the tensor cores as they are (exact in bf16) and nothing is rounded more often than with a bf16 cache.
+// 8-bit codes enter the tensor cores as f16, which holds each of them, against queries in f16 (every bf16 row, scaled by a power of
+// two) and probabilities in f16.  A key's scale multiplies its score.
 #include "paged.cuh"
 #include "paged_plan.h"
 #include "ptx.cuh"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace tb {
@@ -26,8 +27,9 @@ struct PagedAttParams {
     const float *ks, *vs;
     bf16* att; long long ld_att;
     float* lse;                      // [rows, H] or NULL
-    float* part_o; float2* part_ml;  // [splits][rows * H][hd], [splits][rows * H]
-    int rows, H, group, max_q, max_kv, split_keys;
+    float* part_o; float2* part_ml;  // [2 grid][16][hd], [2 grid][16]: results of items that a CTA shares with its neighbours
+    long long* before;               // [seqs + 1]: blocks of one head in front of a sequence
+    int rows, H, group, max_q, max_kv, grid, whole;
     float scale_log2;
     int* err;
 };
@@ -43,9 +45,16 @@ __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0
 }
 
 // ------------------------------------------------------------------------------- few rows: mma fragments
-// CTA = 16 query rows of one key head and one piece of the cache; four warps with 16 keys of every stage of 64 each, a fifth one
-// that fills the ring.  What counts here is bytes: the rows are padded to 16 and the tensor work is still small beside the keys
-// and values that come in.  A warp keeps maximum, sum and accumulator of its own keys; they are put together at the end.
+// Sequences whose new rows, times the heads that share a key head, are at most 16: single tokens, and a few of them.  What counts
+// here is bytes: an item is one (sequence, key head), its rows are padded to the 16 of a fragment, and the tensor work is still
+// small beside the keys and values that come in.  A CTA of four warps, 16 keys of every block of 64 each, and a fifth one that
+// fills a ring of blocks.  A warp keeps maximum, sum and accumulator of its own keys; they are put together at the item's end.
+//
+// The grid is as many CTAs as the chip holds, and the blocks of all items, laid end to end, are dealt to them in equal runs: the
+// ring goes on from item to item without a pause, and sequences of any lengths keep every SM equally long.  An item that
+// lies in several runs is added up by paged_combine_kernel in the order of the runs.  (One CTA per item and piece of 1024 keys: 47 us
+// for 64 sequences of 400 .. 4096 keys and 6 heads of 64, 35 % of it a tail; pieces of 256 keys: 65 us, a start for each.)
+// Where no sequence has more than PA_WHOLE keys, an item is one CTA's and there is nothing to add.
 //
 // Fragments without a shuffle: the contraction over the head dimension may take the elements in any order, so lane (r, c) of a
 // key's fragment (r = lane / 4, c = lane % 4) holds elements 16 c .. 16 c + 15 of key r, two 16-byte reads, and the queries lie
@@ -53,149 +62,317 @@ __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0
 // with byte permutes; accumulator tile i then holds elements 8 (2c) + i and 8 (2c + 1) + i of rows r and r + 8.
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = (PA_WARPS + 1) * 32;
-constexpr int PA_STAGES = 4;
+enum { PA_FIRST = 1, PA_LAST = 2, PA_FINAL = 4, PA_SLOT = 8, PA_END = 16 };
 
 template <int NH, bool E4M3>
 struct RowsShape {
     static constexpr int ROW_BYTES = E4M3 ? 64 * NH : 128;                   // of one 64-element (8 bits: all) column block
     static constexpr int BLOCK = PA_KEYS * ROW_BYTES;                        // one column block of 64 keys
     static constexpr int TILE = E4M3 ? BLOCK : NH * BLOCK;
-    static constexpr int STAGE = 2 * TILE + (E4M3 ? 2 * PA_KEYS * 4 : 0);
-    static constexpr int SMEM = 1024 + PA_STAGES * STAGE + 256;
+    static constexpr int Q_BYTES = PA_ROWS * 128 * NH;
+    static constexpr int O_SCALE = 2 * TILE, O_Q = O_SCALE + (E4M3 ? 2 * PA_KEYS * 4 : 0), O_WHAT = O_Q + Q_BYTES;
+    static constexpr int STAGE = (O_WHAT + 32 + 1023) / 1024 * 1024;
+    static constexpr int STAGES = E4M3 ? (NH == 1 ? 5 : 3) : (NH == 1 ? 4 : 3);
+    static constexpr int LD = 64 * NH + 4;                                   // floats per row of a warp's result
+    static constexpr int O_OUT = STAGES * STAGE;
+    static constexpr int O_BARS = O_OUT + PA_WARPS * PA_ROWS * (LD + 2) * 4;
+    static constexpr int SMEM = 1024 + O_BARS + 2 * STAGES * 8 + 16;
+    static constexpr int PER_SM = SMEM <= 75 * 1024 ? 3 : SMEM <= 113 * 1024 ? 2 : 1;
 };
 
-__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, std::false_type) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// two 8-bit codes -> a pair of bf16
-__device__ __forceinline__ uint32_t e4m3_bf16(uint32_t two) {
-    const float2 f = e4m3_floats(two);
-    return bf16_pair(f.x, f.y);
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, std::true_type) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two 8-bit codes (low half of the word) -> a pair of f16, exact
+__device__ __forceinline__ uint32_t e4m3_f16(uint32_t two) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+    return h;
+}
+__device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(hi), "f"(lo));
+    return h;
+}
+// a value's scale as 2^exponent * part, |part| < 2, and 2^-exponent.  (Infinity and NaN are their own part.)
+struct ScaleParts { float exponent, part, down; };
+__device__ __forceinline__ ScaleParts scale_parts(float s) {
+    const uint32_t b = __float_as_uint(s), e = (b >> 23) & 255u;
+    ScaleParts r;
+    r.exponent = __uint_as_float(0x4b000000u | e) - 8388735.0f;                        // e - 127
+    r.part = __uint_as_float((b & 0x807fffffu) | 0x3f800000u);
+    r.down = __uint_as_float((254u - min(e, 253u)) << 23);
+    if (e == 0u) { r.exponent = -126.f; r.part = s * 8.507059173e37f; r.down = 8.507059173e37f; }      // 2^126
+    if (e == 255u) { r.exponent = 0.f; r.part = s; r.down = 1.f; }
+    return r;
+}
+
+// A named barrier for the warps that wait for one another: whether all of them say so.  (A warp whose wait ran out comes here too and says
+// no, so that nobody waits for it.)
+__device__ __forceinline__ bool all_of(bool mine, int barrier, int threads) {
+    int whole;
+    asm volatile("{\n\t.reg .pred P, Q;\n\tsetp.ne.s32 P, %1, 0;\n\tbar.red.and.pred Q, %2, %3, P;\n\tselp.s32 %0, 1, 0, Q;\n\t}"
+                 : "=r"(whole) : "r"(mine ? 1 : 0), "r"(barrier), "r"(threads) : "memory");
+    return whole != 0;
+}
+
+// blocks of one head of a sequence that the kernel for few rows takes
+__device__ __forceinline__ int row_blocks(const PagedAttParams& p, bool ok, int n, int kv) {
+    return ok && n > 0 && n * p.group <= PA_ROWS ? max(1, (kv + PA_KEYS - 1) / PA_KEYS) : 0;
+}
+__device__ __forceinline__ long long run_length(const PagedAttParams& p, long long total) {
+    const long long per = (total + p.grid - 1) / p.grid;
+    return per < PA_LEAST ? PA_LEAST : per;
 }
 
 template <int NH, bool E4M3>
-__global__ void __launch_bounds__(PA_THREADS)
+__global__ void __launch_bounds__(PA_THREADS, (RowsShape<NH, E4M3>::PER_SM))
 paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedAttParams p) {
     typedef RowsShape<NH, E4M3> Sh;
+    typedef std::integral_constant<bool, E4M3> Kind;
+    constexpr int STAGES = Sh::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + PA_STAGES * Sh::STAGE);
-    uint64_t* empty = full + PA_STAGES;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + PA_STAGES);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sh::O_BARS);
+    uint64_t* empty = full + STAGES;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + STAGES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < PA_STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], PA_WARPS); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], PA_WARPS); }
         *abort_flag = 0;
         fence_mbar_init();
     }
     __syncthreads();
     pdl_wait();
-    const int split = blockIdx.x, s = blockIdx.z;
-    const int head = blockIdx.y % p.v.heads, tile = blockIdx.y / p.v.heads;
-    int q0, n, kv;
-    if (!batch_of(p, s, q0, n, kv)) {
-        if (threadIdx.x == 0) atomicExch(p.err, 76);
-        return;
-    }
-    const int row0 = tile * PA_ROWS, nrows = min(PA_ROWS, n * p.group - row0);
-    if (nrows <= 0) return;
-    const int first_pos = kv - n + row0 / p.group, last_pos = kv - n + (row0 + nrows - 1) / p.group;
-    const int kv_end = last_pos + 1;                              // (no more than kv; negative for rows without a key)
-    const bool whole = kv <= p.split_keys;                        // one piece: the result is final
-    const int k_begin = split * p.split_keys, k_end = min(k_begin + p.split_keys, kv_end);
-    if (k_begin > 0 && k_begin >= kv_end) return;                 // (piece 0 of a row without keys writes its zeros)
-    const int stages = k_end > k_begin ? (k_end - k_begin + PA_KEYS - 1) / PA_KEYS : 0;
 
     if (warp == PA_WARPS) {
-        // ---- producer: a lane per piece of a page; the table is read 32 entries at a time, one round ahead
-        const int piece_shift = min(p.v.page_shift, 6), pieces = PA_KEYS >> piece_shift;      // keys per copy, copies per stage
+        // ---- producer: finds this CTA's items, and fills the ring with their blocks.  A lane per piece of a page.
+        const int heads = p.v.heads, seqs = p.v.seqs;
+        const int piece_shift = min(p.v.page_shift, 6), pieces = PA_KEYS >> piece_shift;      // keys per copy, copies per block
         const int piece_keys = 1 << piece_shift, per_page_shift = p.v.page_shift - piece_shift;
-        const int* table = p.v.table + (long long)s * p.v.table_ld;
-        const int first_piece = k_begin >> piece_shift, last_piece = (k_end + piece_keys - 1) >> piece_shift;
-        auto page_at = [&](int piece) -> int {
-            if (piece >= last_piece) return 0;
-            const int pg = table[piece >> per_page_shift];
-            if ((unsigned)pg < (unsigned)p.v.pages) return pg;
-            atomicExch(p.err, 75);
-            return 0;
-        };
-        int held = first_piece, pages_now = page_at(first_piece + lane), pages_next = page_at(first_piece + 32 + lane);
-        bool ok = true;
-        for (int i = 0; i < stages && ok; ++i) {
-            const int st = i % PA_STAGES;
-            const int at = first_piece + i * pieces;
-            if (at >= held + 32) { held += 32; pages_now = pages_next; pages_next = page_at(held + 32 + lane); }
-            const int piece = at + lane;
-            const int pg = __shfl_sync(0xffffffffu, pages_now, (at - held + lane) & 31);
-            const int count = min(pieces, last_piece - at);       // copies of this stage
-            if (i >= PA_STAGES) ok = mbar_wait(&empty[st], (uint32_t)((i / PA_STAGES) & 1) ^ 1u, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            uint8_t* sK = smem + st * Sh::STAGE;
-            uint8_t* sV = sK + Sh::TILE;
-            if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)(count * piece_keys * (2 * Sh::TILE / PA_KEYS + (E4M3 ? 8 : 0))));
-            __syncwarp();
-            if (lane < count) {
-                const int block = pg * p.v.heads + head, r0 = (piece & ((1 << per_page_shift) - 1)) << piece_shift;
-                const int o = lane << piece_shift;
-#pragma unroll
-                for (int b = 0; b < (E4M3 ? 1 : NH); ++b) {
-                    tma_load_3d(sK + b * Sh::BLOCK + o * Sh::ROW_BYTES, &tmK, &full[st], b * 64, r0, block);
-                    tma_load_3d(sV + b * Sh::BLOCK + o * Sh::ROW_BYTES, &tmV, &full[st], b * 64, r0, block);
+        int s = 0, h = 0, b = 0;              // the next block: of sequence s, head h
+        long long left = 0;                   // blocks of this CTA's run that are still to come
+        if (p.whole) {
+            s = (int)(blockIdx.x / (unsigned)heads);
+            h = (int)(blockIdx.x % (unsigned)heads);
+        } else {
+            // all sequences' blocks, a sequence per lane
+            long long total = 0;
+            for (int s0 = 0; s0 < seqs; s0 += 32) {
+                int q0, n, kv, nb = 0;
+                if (s0 + lane < seqs) {
+                    const bool ok = batch_of(p, s0 + lane, q0, n, kv);
+                    if (!ok) atomicExch(p.err, 76);
+                    nb = row_blocks(p, ok, n, kv);
                 }
-                if (E4M3) {
-                    float* sc = reinterpret_cast<float*>(sK + 2 * Sh::TILE);
-                    const long long row = ((long long)block << p.v.page_shift) + r0;
-                    bulk_load(sc + o, p.ks + row, (uint32_t)piece_keys * 4u, &full[st]);
-                    bulk_load(sc + PA_KEYS + o, p.vs + row, (uint32_t)piece_keys * 4u, &full[st]);
+                long long incl = nb;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += x;
+                }
+                if (blockIdx.x == 0 && s0 + lane < seqs) p.before[s0 + lane] = total + incl - nb;
+                total += __shfl_sync(0xffffffffu, incl, 31);
+            }
+            if (blockIdx.x == 0 && lane == 0) p.before[seqs] = total;
+            total *= heads;
+            const long long per = run_length(p, total), first = per * blockIdx.x;
+            left = min(per, total - first);
+            if (left > 0) {
+                long long at = 0;
+                for (int s0 = 0; s0 < seqs; s0 += 32) {
+                    int q0, n, kv, nb = 0;
+                    if (s0 + lane < seqs) {
+                        const bool ok = batch_of(p, s0 + lane, q0, n, kv);
+                        nb = row_blocks(p, ok, n, kv);
+                    }
+                    long long incl = nb;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+                        if (lane >= o) incl += x;
+                    }
+                    const unsigned ends_behind = __ballot_sync(0xffffffffu, (at + incl) * heads > first);
+                    if (ends_behind) {
+                        const int who = __ffs(ends_behind) - 1;
+                        const long long rest = first - (at + __shfl_sync(0xffffffffu, incl - nb, who)) * heads;
+                        const int blocks = __shfl_sync(0xffffffffu, nb, who);
+                        s = s0 + who; h = (int)(rest / blocks); b = (int)(rest - (long long)h * blocks);
+                        break;
+                    }
+                    at += __shfl_sync(0xffffffffu, incl, 31);
                 }
             }
-            __syncwarp();
+        }
+        int i = 0;                            // blocks put into the ring
+        bool ok = true;
+        auto slot_free = [&]() {
+            if (i >= STAGES) ok = mbar_wait(&empty[i % STAGES], (uint32_t)((i / STAGES) & 1) ^ 1u, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            return ok;
+        };
+        while (ok && (p.whole ? s < seqs : left > 0)) {
+            int q0, n, kv;
+            const bool fine = batch_of(p, s, q0, n, kv);
+            if (!fine && p.whole && lane == 0) atomicExch(p.err, 76);
+            const int nb = row_blocks(p, fine, n, kv);
+            const int b_end = p.whole ? nb : (int)min((long long)nb, b + left);
+            const int* table = p.v.table + (long long)s * p.v.table_ld;
+            const int last_piece = (kv + piece_keys - 1) >> piece_shift;
+            auto page_at = [&](int piece) -> int {
+                if (piece >= last_piece) return 0;
+                const int pg = table[piece >> per_page_shift];
+                if ((unsigned)pg < (unsigned)p.v.pages) return pg;
+                atomicExch(p.err, 75);
+                return 0;
+            };
+            // the table is read 32 pieces at a time, one round ahead
+            int held = b * pieces, now = 0, next = 0;
+            if (b < b_end) { now = page_at(held + lane); next = page_at(held + 32 + lane); }
+            const int flags = p.whole || (b == 0 && b_end == nb) ? PA_FINAL : b == 0 ? PA_SLOT : 0;
+            const int b_begin = b;
+            for (; b < b_end; ++b) {
+                const int at = b * pieces;
+                if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
+                const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
+                const int count = max(0, min(pieces, last_piece - at));      // copies of this block
+                if (!slot_free()) break;
+                uint8_t* st = smem + (i % STAGES) * Sh::STAGE;
+                uint64_t* bar = &full[i % STAGES];
+                const bool first = b == b_begin;
+                if (lane == 0) {
+                    int* what = reinterpret_cast<int*>(st + Sh::O_WHAT);
+                    what[0] = flags | (first ? PA_FIRST : 0) | (b == b_end - 1 ? PA_LAST : 0);
+                    what[1] = b * PA_KEYS; what[2] = q0; what[3] = n; what[4] = kv; what[5] = h;
+                    mbar_expect_tx(bar, (uint32_t)(count * piece_keys * (2 * Sh::TILE / PA_KEYS + (E4M3 ? 8 : 0)) +
+                                                   (first ? n * p.group * p.v.hd * 2 : 0)));
+                }
+                __syncwarp();
+                if (first && lane < n)
+                    bulk_load(st + Sh::O_Q + lane * p.group * p.v.hd * 2, p.Q + (long long)(q0 + lane) * p.ld_q + (long long)h * p.group * p.v.hd,
+                              (uint32_t)(p.group * p.v.hd * 2), bar);
+                if (lane < count) {
+                    const int block = pg * heads + h, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift;
+                    const int o = lane << piece_shift;
+#pragma unroll
+                    for (int c = 0; c < (E4M3 ? 1 : NH); ++c) {
+                        tma_load_3d(st + c * Sh::BLOCK + o * Sh::ROW_BYTES, &tmK, bar, c * 64, r0, block);
+                        tma_load_3d(st + Sh::TILE + c * Sh::BLOCK + o * Sh::ROW_BYTES, &tmV, bar, c * 64, r0, block);
+                    }
+                    if (E4M3) {
+                        float* sc = reinterpret_cast<float*>(st + Sh::O_SCALE);
+                        const long long row = ((long long)block << p.v.page_shift) + r0;
+                        bulk_load(sc + o, p.ks + row, (uint32_t)piece_keys * 4u, bar);
+                        bulk_load(sc + PA_KEYS + o, p.vs + row, (uint32_t)piece_keys * 4u, bar);
+                    }
+                }
+                __syncwarp();
+                ++i;
+            }
+            if (p.whole) {
+                b = 0;
+                h += (int)(gridDim.x % (unsigned)heads);
+                s += (int)(gridDim.x / (unsigned)heads);
+                if (h >= heads) { h -= heads; ++s; }
+            } else {
+                left -= b - b_begin;
+                if (b >= nb) {
+                    b = 0;
+                    if (nb == 0 || ++h == heads) { h = 0; ++s; }
+                }
+            }
+        }
+        if (ok && slot_free() && lane == 0) {
+            *reinterpret_cast<int*>(smem + (i % STAGES) * Sh::STAGE + Sh::O_WHAT) = PA_END;
+            mbar_arrive(&full[i % STAGES]);
         }
         pdl_launch_dependents_now();
         if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 73); }
-        // (the CTA stays until what was asked for has arrived: the consumers wait for every stage)
+        // (the consumers wait for everything that has been asked for)
         return;
     }
 
     const int r = lane >> 2, c = lane & 3;
+    float* so = reinterpret_cast<float*>(smem + Sh::O_OUT);
+    float2* sml = reinterpret_cast<float2*>(so + PA_WARPS * PA_ROWS * Sh::LD);
     // query fragments: elements 16 c .. of rows r and r + 8, head-dimension block by block
     uint32_t qf[NH][4][4];
-    int pos[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int rr = r + 8 * i;
-        const int tok = (row0 + min(rr, nrows - 1)) / p.group, g = (row0 + min(rr, nrows - 1)) % p.group;
-        pos[i] = kv - n + tok;
-        const bf16* q = p.Q + (long long)(q0 + tok) * p.ld_q + (long long)(head * p.group + g) * p.v.hd;
-#pragma unroll
-        for (int b = 0; b < NH; ++b)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int e = 64 * b + 16 * c + 8 * h;
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (e < p.v.hd && rr < nrows) w = *reinterpret_cast<const uint4*>(q + e);
-                qf[b][2 * h][i] = w.x; qf[b][2 * h][2 + i] = w.y; qf[b][2 * h + 1][i] = w.z; qf[b][2 * h + 1][2 + i] = w.w;
-            }
-    }
-    float o[8 * NH][4];
-#pragma unroll
-    for (int i = 0; i < 8 * NH; ++i) { o[i][0] = 0.f; o[i][1] = 0.f; o[i][2] = 0.f; o[i][3] = 0.f; }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float row_factor[2] = {p.scale_log2, p.scale_log2};
+    int pos[2] = {0, 0}, first_pos = 0, last_pos = 0, nrows = 0;
+    float o[8 * NH][4], m[2], l[2];
     bool ok = true;
-    for (int i = 0; i < stages; ++i) {
-        const int st = i % PA_STAGES;
-        if (!mbar_wait(&full[st], (uint32_t)((i / PA_STAGES) & 1), abort_flag)) { ok = false; break; }
+    for (int i = 0;; ++i) {
+        const int st = i % STAGES;
+        if (!mbar_wait(&full[st], (uint32_t)((i / STAGES) & 1), abort_flag)) {
+            if (lane == 0) *abort_flag = 1;
+            all_of(false, 1, 128);
+            ok = false;
+            break;
+        }
         const uint8_t* sK = smem + st * Sh::STAGE;
         const uint8_t* sV = sK + Sh::TILE;
-        const float* sc = reinterpret_cast<const float*>(sK + 2 * Sh::TILE);
-        const int kk = 16 * warp, k0 = k_begin + i * PA_KEYS + kk;         // this warp's 16 keys
-        if (k0 < k_end) {
+        const float* sc = reinterpret_cast<const float*>(sK + Sh::O_SCALE);
+        const int4 what = *reinterpret_cast<const int4*>(sK + Sh::O_WHAT);             // flags, first key, first row, new rows
+        const int2 more = *reinterpret_cast<const int2*>(sK + Sh::O_WHAT + 16);        // keys, head
+        if (what.x & PA_END) { all_of(true, 1, 128); break; }
+        const int kv = more.x, n = what.w;
+        if (what.x & PA_FIRST) {
+            nrows = n * p.group;
+            first_pos = kv - n; last_pos = kv - 1;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int rr = r + 8 * x;
+                pos[x] = kv - n + min(rr, nrows - 1) / p.group;
+                const uint8_t* q = sK + Sh::O_Q + rr * p.v.hd * 2;
+                uint32_t big = 0u;
+#pragma unroll
+                for (int b = 0; b < NH; ++b)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const int e = 64 * b + 16 * c + 8 * g;
+                        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                        if (e < p.v.hd && rr < nrows) w = *reinterpret_cast<const uint4*>(q + e * 2);
+                        qf[b][2 * g][x] = w.x; qf[b][2 * g][2 + x] = w.y; qf[b][2 * g + 1][x] = w.z; qf[b][2 * g + 1][2 + x] = w.w;
+                        if (E4M3) {
+                            const uint32_t a = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+                            big = max(big & 0xffffu, max(a & 0xffffu, a >> 16));
+                        }
+                    }
+                if (E4M3) {
+                    // as f16, the row scaled by a power of two so that its largest magnitude lies in [1, 2): exact but for what is
+                    // less than 2^-24 of it
+                    big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                    big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                    const int e = max((int)(big >> 7), 1);                             // (biased; 255: infinity or NaN)
+                    const float down = __uint_as_float((uint32_t)min(254 - e, 253) << 23), up = __uint_as_float((uint32_t)e << 23);
+                    const bool odd = e >= 254;                                         // (2^(127 - e) would be no normal number)
+                    row_factor[x] = odd ? p.scale_log2 : p.scale_log2 * up;
+#pragma unroll
+                    for (int b = 0; b < NH; ++b)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const float2 f = bf16_floats(qf[b][g][x + 2 * j]);
+                                qf[b][g][x + 2 * j] = odd ? f16_pair(f.x, f.y) : f16_pair(f.x * down, f.y * down);
+                            }
+                }
+                m[x] = -INFINITY; l[x] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8 * NH; ++e) { o[e][0] = 0.f; o[e][1] = 0.f; o[e][2] = 0.f; o[e][3] = 0.f; }
+        }
+        const int kk = 16 * warp, k0 = what.y + kk;                        // this warp's 16 keys
+        if (k0 <= last_pos) {
             // ---- scores of two tiles of 8 keys
             float z[2][4];
+            ScaleParts vs[2][2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 z[t][0] = z[t][1] = z[t][2] = z[t][3] = 0.f;
@@ -207,7 +384,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                         const uint4 x = *reinterpret_cast<const uint4*>(sK + key * Sh::ROW_BYTES + 64 * b + 16 * c);
                         const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) { w[2 * e] = e4m3_bf16(u[e] & 0xffffu); w[2 * e + 1] = e4m3_bf16(u[e] >> 16); }
+                        for (int e = 0; e < 4; ++e) { w[2 * e] = e4m3_f16(u[e]); w[2 * e + 1] = e4m3_f16(u[e] >> 16); }
                     } else {
                         // (128-byte swizzle: the 16-byte pieces of a row lie at piece ^ (row & 7))
                         const uint8_t* row = sK + b * Sh::BLOCK + key * 128;
@@ -216,14 +393,21 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                         w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) mma_bf16_16816(z[t], qf[b][e], w[2 * e], w[2 * e + 1]);
+                    for (int e = 0; e < 4; ++e) mma_16816(z[t], qf[b][e], w[2 * e], w[2 * e + 1], Kind());
                 }
-                float f0 = p.scale_log2, f1 = p.scale_log2;
                 if (E4M3) {
+                    // the key's scale on the score; the value's scale, but for a factor below 2, in the exponent of the probability
                     const float2 f = *reinterpret_cast<const float2*>(sc + kk + 8 * t + 2 * c);
-                    f0 *= f.x; f1 *= f.y;
+                    const float2 g = *reinterpret_cast<const float2*>(sc + PA_KEYS + kk + 8 * t + 2 * c);
+                    vs[t][0] = scale_parts(g.x); vs[t][1] = scale_parts(g.y);
+                    z[t][0] = fmaf(z[t][0], f.x * row_factor[0], vs[t][0].exponent);
+                    z[t][1] = fmaf(z[t][1], f.y * row_factor[0], vs[t][1].exponent);
+                    z[t][2] = fmaf(z[t][2], f.x * row_factor[1], vs[t][0].exponent);
+                    z[t][3] = fmaf(z[t][3], f.y * row_factor[1], vs[t][1].exponent);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[t][e] *= p.scale_log2;
                 }
-                z[t][0] *= f0; z[t][1] *= f1; z[t][2] *= f0; z[t][3] *= f1;
             }
             const bool edge = k0 + 15 > first_pos;                         // some row does not see all of these keys
             if (edge) {
@@ -255,23 +439,20 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             uint32_t pa[4];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                float f0 = 1.f, f1 = 1.f;
-                if (E4M3) {
-                    const float2 f = *reinterpret_cast<const float2*>(sc + PA_KEYS + kk + 8 * t + 2 * c);
-                    f0 = f.x; f1 = f.y;
-                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     // (a row that has seen no key yet: its maximum is -infinity, and so are its scores)
                     const float base = m[h] == -INFINITY ? 0.f : m[h];
-                    float p0 = ex2_approx(z[t][2 * h] - base), p1 = ex2_approx(z[t][2 * h + 1] - base);
-                    l[h] += p0 + p1;
+                    const float p0 = ex2_approx(z[t][2 * h] - base), p1 = ex2_approx(z[t][2 * h + 1] - base);
                     if (E4M3) {
-                        // (a masked key's scale may be anything)
-                        p0 = z[t][2 * h] == -INFINITY ? 0.f : p0 * f0;
-                        p1 = z[t][2 * h + 1] == -INFINITY ? 0.f : p1 * f1;
+                        // (a key that the row does not see may have any scale)
+                        const bool no0 = edge && z[t][2 * h] == -INFINITY, no1 = edge && z[t][2 * h + 1] == -INFINITY;
+                        l[h] += (no0 ? 0.f : p0 * vs[t][0].down) + (no1 ? 0.f : p1 * vs[t][1].down);
+                        pa[2 * t + h] = f16_pair(no0 ? 0.f : p0 * vs[t][0].part, no1 ? 0.f : p1 * vs[t][1].part);
+                    } else {
+                        l[h] += p0 + p1;
+                        pa[2 * t + h] = bf16_pair(p0, p1);
                     }
-                    pa[2 * t + h] = bf16_pair(p0, p1);
                 }
             }
             // ---- values
@@ -283,7 +464,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int key = kk + 2 * c + (j & 1) + 8 * (j >> 1);
-                        const bool seen = k0 - kk + key <= last;
+                        const bool seen = !at_edge.value || k0 - kk + key <= last;
                         if (E4M3) {
                             uint2 x = *reinterpret_cast<const uint2*>(sV + key * Sh::ROW_BYTES + 64 * b + 8 * r);
                             if (!seen) x = make_uint2(0u, 0u);
@@ -300,102 +481,96 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                         if (E4M3) {
                             // byte e of two keys side by side
                             const uint32_t sel = 0x0040u + 0x0011u * (e & 3);
-                            b0 = e4m3_bf16(__byte_perm(w[0][e >> 2], w[1][e >> 2], sel) & 0xffffu);
-                            b1 = e4m3_bf16(__byte_perm(w[2][e >> 2], w[3][e >> 2], sel) & 0xffffu);
+                            b0 = e4m3_f16(__byte_perm(w[0][e >> 2], w[1][e >> 2], sel));
+                            b1 = e4m3_f16(__byte_perm(w[2][e >> 2], w[3][e >> 2], sel));
                         } else {
                             const uint32_t sel = e & 1 ? 0x7632u : 0x5410u;
                             b0 = __byte_perm(w[0][e >> 1], w[1][e >> 1], sel);
                             b1 = __byte_perm(w[2][e >> 1], w[3][e >> 1], sel);
                         }
                         if (!at_edge.value) {
-                            mma_bf16_16816(o[8 * b + e], a, b0, b1);
+                            mma_16816(o[8 * b + e], a, b0, b1, Kind());
                         } else {
                             float d[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_bf16_16816(d, a, b0, b1);
+                            mma_16816(d, a, b0, b1, Kind());
                             if (pos[0] == last) { o[8 * b + e][0] += d[0]; o[8 * b + e][1] += d[1]; }
                             if (pos[1] == last) { o[8 * b + e][2] += d[2]; o[8 * b + e][3] += d[3]; }
                         }
                     }
                 }
             };
-            if (!edge) values(pa, 0x7fffffff, std::false_type());
+            if (!edge) values(pa, 0, std::false_type());
             else       // token by token: what a token does not see must not reach it, not even as 0 * infinity
                 for (int last = first_pos; last <= last_pos; ++last) values(pa, last, std::true_type());
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
+        if (!(what.x & PA_LAST)) continue;
+
+        // ---- the item's end: the four warps' results, [warp][16 rows][LD] floats, maxima and sums behind
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            float* dst = so + (warp * PA_ROWS + r + 8 * h) * Sh::LD + 16 * c;
+#pragma unroll
+            for (int b = 0; b < NH; ++b)
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    *reinterpret_cast<float4*>(dst + 64 * b + e) =
+                        make_float4(o[8 * b + e][2 * h], o[8 * b + e + 1][2 * h], o[8 * b + e + 2][2 * h], o[8 * b + e + 3][2 * h]);
+                    *reinterpret_cast<float4*>(dst + 64 * b + 8 + e) =
+                        make_float4(o[8 * b + e][2 * h + 1], o[8 * b + e + 1][2 * h + 1], o[8 * b + e + 2][2 * h + 1], o[8 * b + e + 3][2 * h + 1]);
+                }
+            if (c == 0) sml[warp * PA_ROWS + r + 8 * h] = make_float2(m[h], l[h]);
+        }
+        if (!all_of(true, 1, 128)) { ok = false; break; }
+        const int chunks = p.v.hd >> 3;                                    // eight elements per thread
+        for (int x = threadIdx.x; x < nrows * chunks; x += PA_WARPS * 32) {
+            const int rr = x / chunks, e = (x - rr * chunks) * 8;
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, sml[w * PA_ROWS + rr].x);
+            float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; ++w) {
+                const float2 ml = sml[w * PA_ROWS + rr];
+                if (ml.y == 0.f) continue;                                 // (no key of this warp's was visible)
+                const float f = ex2_approx(ml.x - M);
+                L += ml.y * f;
+                const float4* src = reinterpret_cast<const float4*>(so + (w * PA_ROWS + rr) * Sh::LD + e);
+                const float4 a = src[0], d = src[1];
+                acc[0] += a.x * f; acc[1] += a.y * f; acc[2] += a.z * f; acc[3] += a.w * f;
+                acc[4] += d.x * f; acc[5] += d.y * f; acc[6] += d.z * f; acc[7] += d.w * f;
+            }
+            const int tok = rr / p.group, hq = more.y * p.group + (rr - tok * p.group), row = what.z + tok;
+            if (what.x & PA_FINAL) {
+                const bool none = kv - n + tok < 0;                        // a row without a key
+                const float inv = none ? 0.f : 1.0f / L;
+                *reinterpret_cast<uint4*>(p.att + (long long)row * p.ld_att + (long long)hq * p.v.hd + e) =
+                    make_uint4(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv),
+                               bf16_pair(acc[4] * inv, acc[5] * inv), bf16_pair(acc[6] * inv, acc[7] * inv));
+                if (p.lse && e == 0) p.lse[(long long)row * p.H + hq] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+            } else {
+                const int slot = (2 * blockIdx.x + (what.x & PA_SLOT ? 1 : 0)) * PA_ROWS + rr;
+                float4* dst = reinterpret_cast<float4*>(p.part_o + (long long)slot * p.v.hd + e);
+                dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                if (e == 0) p.part_ml[slot] = make_float2(M, L);
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");                     // the buffer is read
     }
     if (!ok) {
         // (what was asked for may still arrive: the block keeps its memory a little longer)
         if (lane == 0) { *abort_flag = 1; atomicExch(p.err, 74); }
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
     }
-
-    // ---- the four warps' results: [warp][16 rows][64 NH + 4] floats over the ring, maxima and sums behind
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    }
-    asm volatile("bar.sync 1, 128;" ::: "memory");                         // every stage has been read
-    constexpr int LD = 64 * NH + 4;
-    float* so = reinterpret_cast<float*>(smem);
-    float2* sml = reinterpret_cast<float2*>(so + PA_WARPS * PA_ROWS * LD);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float* dst = so + (warp * PA_ROWS + r + 8 * h) * LD + 16 * c;
-#pragma unroll
-        for (int b = 0; b < NH; ++b)
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                *reinterpret_cast<float4*>(dst + 64 * b + e) =
-                    make_float4(o[8 * b + e][2 * h], o[8 * b + e + 1][2 * h], o[8 * b + e + 2][2 * h], o[8 * b + e + 3][2 * h]);
-                *reinterpret_cast<float4*>(dst + 64 * b + 8 + e) =
-                    make_float4(o[8 * b + e][2 * h + 1], o[8 * b + e + 1][2 * h + 1], o[8 * b + e + 2][2 * h + 1], o[8 * b + e + 3][2 * h + 1]);
-            }
-        if (c == 0) sml[warp * PA_ROWS + r + 8 * h] = make_float2(m[h], l[h]);
-    }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    const int chunks = p.v.hd >> 3;                                        // eight elements per thread
-    for (int x = threadIdx.x; x < nrows * chunks; x += PA_WARPS * 32) {
-        const int rr = x / chunks, e = (x - rr * chunks) * 8;
-        float M = -INFINITY, L = 0.f, f[PA_WARPS];
-#pragma unroll
-        for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, sml[w * PA_ROWS + rr].x);
-        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < PA_WARPS; ++w) {
-            const float2 ml = sml[w * PA_ROWS + rr];
-            f[w] = ml.y == 0.f ? 0.f : ex2_approx(ml.x - M);              // (a sum of 0: no key of this warp's was visible)
-            L += ml.y * f[w];
-            if (f[w] != 0.f) {
-                const float4* src = reinterpret_cast<const float4*>(so + (w * PA_ROWS + rr) * LD + e);
-                const float4 a = src[0], b = src[1];
-                acc[0] += a.x * f[w]; acc[1] += a.y * f[w]; acc[2] += a.z * f[w]; acc[3] += a.w * f[w];
-                acc[4] += b.x * f[w]; acc[5] += b.y * f[w]; acc[6] += b.z * f[w]; acc[7] += b.w * f[w];
-            }
-        }
-        const int tok = (row0 + rr) / p.group, hq = head * p.group + (row0 + rr) % p.group;
-        const long long at = (long long)(q0 + tok) * p.H + hq;
-        if (whole) {
-            const bool none = kv - n + tok < 0;                            // a row without a key
-            const float inv = none ? 0.f : 1.0f / L;
-            *reinterpret_cast<uint4*>(p.att + (long long)(q0 + tok) * p.ld_att + (long long)hq * p.v.hd + e) =
-                make_uint4(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv),
-                           bf16_pair(acc[4] * inv, acc[5] * inv), bf16_pair(acc[6] * inv, acc[7] * inv));
-            if (p.lse && e == 0) p.lse[at] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-        } else {
-            const long long slot = (long long)split * p.rows * p.H + at;
-            float4* dst = reinterpret_cast<float4*>(p.part_o + slot * p.v.hd + e);
-            dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-            dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-            if (e == 0) p.part_ml[slot] = make_float2(M, L);
-        }
-    }
 }
 
-// ------------------------------------------------------------------------------- pieces of a row, in their order
-// A warp per (row, head); rows of sequences that took one piece are final already.
+// ------------------------------------------------------------------------------- items of several runs, in the order of the runs
+// A warp per (row, head); items that lie in one run are final already.  The run that an item starts in has it as its last one
+// (slot 1 of that CTA), the others as their first (slot 0).
 constexpr int PC_WARPS = 8;
 __global__ void __launch_bounds__(PC_WARPS * 32)
 paged_combine_kernel(const PagedAttParams p) {
@@ -404,38 +579,44 @@ paged_combine_kernel(const PagedAttParams p) {
     const int lane = threadIdx.x & 31;
     const long long at = (long long)blockIdx.x * PC_WARPS + (threadIdx.x >> 5);
     if (at >= (long long)p.rows * p.H) return;
-    const int row = (int)(at / p.H), hq = (int)(at - (long long)row * p.H);
+    const int row = (int)(at / p.H), hq = (int)(at - (long long)row * p.H), h = hq / p.group;
     const int s = sequence_of(p.q_start, p.v.seqs, row);
     if (s < 0) return;
     int q0, n, kv;
-    if (!batch_of(p, s, q0, n, kv) || row >= q0 + n || kv <= p.split_keys) return;
-    const int pos = kv - n + row - q0;
-    const int pieces = pos < 0 ? 0 : pos / p.split_keys + 1;
-    const long long step = (long long)p.rows * p.H;
+    const bool fine = batch_of(p, s, q0, n, kv);
+    const int nb = row_blocks(p, fine, n, kv);
+    if (nb == 0 || row >= q0 + n) return;
+    const long long per = run_length(p, p.before[p.v.seqs] * p.v.heads), first = p.before[s] * p.v.heads + (long long)h * nb;
+    const int c0 = (int)(first / per), c1 = (int)((first + nb - 1) / per);
+    if (c0 == c1) return;
+    const int rr = (row - q0) * p.group + hq - h * p.group;
+    auto slot = [&](int c) { return (2 * c + (c == c0 ? 1 : 0)) * PA_ROWS + rr; };
     float M = -INFINITY, L = 0.f;
-    for (int i = 0; i < pieces; ++i) M = fmaxf(M, p.part_ml[i * step + at].x);
+    for (int c = c0; c <= c1; ++c) M = fmaxf(M, p.part_ml[slot(c)].x);
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     const int e = lane * 4;
-    for (int i = 0; i < pieces; ++i) {
-        const float2 ml = p.part_ml[i * step + at];
+    for (int c = c0; c <= c1; ++c) {
+        const float2 ml = p.part_ml[slot(c)];
         if (ml.y == 0.f) continue;
         const float f = ex2_approx(ml.x - M);
         L += ml.y * f;
         if (e < p.v.hd) {
-            const float4 a = *reinterpret_cast<const float4*>(p.part_o + (i * step + at) * p.v.hd + e);
+            const float4 a = *reinterpret_cast<const float4*>(p.part_o + (long long)slot(c) * p.v.hd + e);
             acc[0] += a.x * f; acc[1] += a.y * f; acc[2] += a.z * f; acc[3] += a.w * f;
         }
     }
-    const float inv = pos < 0 ? 0.f : 1.0f / L;
+    const bool none = kv - n + row - q0 < 0;
+    const float inv = none ? 0.f : 1.0f / L;
     if (e < p.v.hd)
         *reinterpret_cast<uint2*>(p.att + (long long)row * p.ld_att + (long long)hq * p.v.hd + e) =
             make_uint2(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv));
-    if (p.lse && lane == 0) p.lse[at] = pos < 0 ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    if (p.lse && lane == 0) p.lse[at] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 template <int NH, bool E4M3>
-int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, const PagedPlan& pl, cudaStream_t st) {
+int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cudaStream_t st) {
     typedef RowsShape<NH, E4M3> Sh;
+    static_assert(Sh::PER_SM == paged_per_sm(NH, E4M3), "the plan counts on as many CTAs per SM");
     CUtensorMap tmK, tmV;
     const int box_rows = std::min(c->page_size, PA_KEYS);
     TB_TRY(make_cache_map(&tmK, c->K, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
@@ -446,7 +627,594 @@ int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, con
         attr_set[ctx->device & 63] = true;
     }
     prof_mark(ctx, "paged_rows", 4.0 * p.rows * p.H * (double)p.max_kv * c->head_dim, 0.0, st);
-    TB_CUDA(launch_kernel(paged_rows_kernel<NH, E4M3>, dim3(pl.splits, c->heads * pl.tiles, c->seqs), dim3(PA_THREADS), Sh::SMEM, st, tmK, tmV, p));
+    TB_CUDA(launch_kernel(paged_rows_kernel<NH, E4M3>, dim3(p.grid), dim3(PA_THREADS), Sh::SMEM, st, tmK, tmV, p));
+    ctx->launches++;
+    prof_close(ctx, st);
+    return 0;
+}
+
+// ------------------------------------------------------------------------------- chunks: tcgen05
+// CTA = one tile of 128 query rows of a sequence: 128 / group tokens with the heads that share a key head side by side, so that
+// every key and value that comes in is used by all of them.  The roles are those of attention_fwd_kernel: a producer warp, one that
+// issues the products, and two groups of four softmax warps (thread = query row) that take the half blocks of 64 keys in turn,
+// with a score buffer, a probability buffer, a maximum, a sum and an accumulator in tensor memory each.  What is different:
+//  * keys and values come by one copy per piece of a page;
+//  * where a block holds keys that some row does not see (the chunk's own tokens, the rest of the last page), what is not finite
+//    among its values is set to zero before the product, because 0 * infinity would reach the rows that do not see it; a row that does
+//    see it gets it added at the end (add_what_is_not_finite);
+//  * 8-bit rows: four more warps turn codes into f16 tiles, a key per thread.  A value's scale goes into its tile against the largest
+//    scale so far (a power of two, which the accumulators follow as they follow the maximum): 11 bits of every value whose scale is
+//    within 2^-21 of the largest, and an absolute error below 2^-31 of the largest value behind that.
+constexpr int PT_ROWS = 128, PT_KEYS = 128;
+constexpr int PT_TILE = 128 * 128;                      // bytes of a [128][64] 16-bit tile
+
+template <int NH, bool E4M3>
+struct ChunkShape {
+    static constexpr int THREADS = E4M3 ? 448 : 320;
+    static constexpr int VST = NH == 2 && E4M3 ? 1 : 2;                  // stages of values
+    static constexpr int RAW = PT_KEYS * 64 * NH;                        // bytes of a block's codes
+    static constexpr int O_K = NH * PT_TILE, O_V = O_K + 2 * NH * PT_TILE, O_P = O_V + VST * NH * PT_TILE, O_RAW = O_P + 2 * PT_TILE;
+    static constexpr int O_SCALE = O_RAW + (E4M3 ? 2 * RAW : 0);         // scales as they come in: keys' and values', [2][128]
+    static constexpr int O_KS = O_SCALE + (E4M3 ? 2 * PT_KEYS * 4 : 0);  // [4][128] key scales * scale_log2
+    static constexpr int O_RF = O_KS + (E4M3 ? 4 * PT_KEYS * 4 : 0);     // [128] row factors
+    static constexpr int O_BARS = O_RF + (E4M3 ? PT_ROWS * 4 : 0);
+    // (bf16 heads of 64: exactly what lets two CTAs share an SM; 256 bytes of barriers behind the tiles or in the alignment's pad)
+    static constexpr int SMEM = 1024 + O_BARS + (NH == 1 && !E4M3 ? 0 : 256);
+    static constexpr int PER_SM = SMEM <= 113 * 1024 ? 2 : 1;
+    static constexpr int TMEM = NH == 1 ? 256 : 512;
+};
+
+struct PagedChunkParams {
+    PagedAttParams a;
+    int tokens, tiles;                // tokens per tile; tiles of max_q
+};
+
+__device__ __forceinline__ bool not_finite_16(uint32_t two) {            // either bf16 of a pair
+    return (two & 0x7f80u) == 0x7f80u || (two & 0x7f800000u) == 0x7f800000u;
+}
+
+// What the product left out: values that are not finite, of the keys from k0 on that the row sees, added to the row's columns 32 b ..
+// of every 64 in the staged result (bf16, 128-byte swizzle).  Rare; straight from the pool.
+template <int NH, bool E4M3>
+__device__ __forceinline__ void add_what_is_not_finite(const PagedAttParams& p, const uint8_t* V, int s, int head, int k0, int pos, int b, int r, uint8_t* row) {
+#pragma unroll 1
+    for (int k = k0; k <= pos; ++k) {
+        const int page = p.v.table[(long long)s * p.v.table_ld + (k >> p.v.page_shift)];
+        if ((unsigned)page >= (unsigned)p.v.pages) continue;
+        const long long at = (((long long)page * p.v.heads + head) << p.v.page_shift) + (k & ((1 << p.v.page_shift) - 1));
+        const float scale = E4M3 ? p.vs[at] : 1.f;
+#pragma unroll 1
+        for (int d = 0; d < p.v.hd; ++d) {
+            if (((d >> 5) & 1) != b) continue;
+            const float x = E4M3 ? e4m3_floats(V[at * p.v.hd + d]).x * scale : __bfloat162float(reinterpret_cast<const bf16*>(V)[at * p.v.hd + d]);
+            if (fabsf(x) < INFINITY) continue;
+            bf16* o = reinterpret_cast<bf16*>(row + (d >> 6) * PT_TILE + ((((d & 63) >> 3) ^ (r & 7)) << 4)) + (d & 7);
+            *o = __float2bfloat16_rn(__bfloat162float(*o) + x);
+        }
+    }
+}
+
+template <int NH, bool E4M3>
+__global__ void __launch_bounds__((ChunkShape<NH, E4M3>::THREADS), (ChunkShape<NH, E4M3>::PER_SM))
+paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const uint8_t* __restrict__ pool_v, const PagedChunkParams pp) {
+    typedef ChunkShape<NH, E4M3> Sh;
+    const PagedAttParams& p = pp.a;
+    constexpr int VST = Sh::VST;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+    uint8_t* smem = smem_raw + pad;
+    uint8_t *sQ = smem, *sK = smem + Sh::O_K, *sV = smem + Sh::O_V, *sP = smem + Sh::O_P;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(pad <= 768u ? smem + Sh::O_BARS : smem_raw);
+    uint64_t* q_full = bars;          // 1: the query tile has come
+    uint64_t* q_ready = bars + 1;     // (8 bits) and is f16
+    uint64_t* k_full = bars + 2;      // 2
+    uint64_t* k_empty = bars + 4;     // 2: the scores of both halves have been formed
+    uint64_t* v_full = bars + 6;      // 2
+    uint64_t* v_empty = bars + 8;     // 2
+    uint64_t* v_land = bars + 10;     // 1: values of a block that is looked through first
+    uint64_t* s_full = bars + 11;     // 2
+    uint64_t* s_free = bars + 13;     // 2
+    uint64_t* p_full = bars + 15;     // 2
+    uint64_t* o_full = bars + 17;     // 2
+    uint64_t* raw_full = bars + 19;   // (8 bits) 2: codes of keys with all scales, codes of values
+    uint64_t* raw_empty = bars + 21;  // 2
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* bad_value = abort_flag + 1;                              // a value that is not finite has been set to zero
+    volatile int* v_exponent = abort_flag + 2;                             // (8 bits) the last block's reference
+    float* v_moved = reinterpret_cast<float*>(tmem_slot + 4);              // (8 bits) [4]: 2^(reference before - reference) of a block
+    uint32_t* warp_most = tmem_slot + 8;                                   // (8 bits) [2][4]
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = blockIdx.x, s = blockIdx.z, tile = pp.tiles - 1 - (int)blockIdx.y;
+    pdl_wait();
+    int q0, n, kv;
+    if (!batch_of(p, s, q0, n, kv)) return;                                // (paged_rows_kernel reports it)
+    const int tok0 = tile * pp.tokens;
+    if (n * p.group <= PA_ROWS || tok0 >= n) return;
+    const int tokens = min(pp.tokens, n - tok0);
+    const int first_pos = kv - n + tok0, last_pos = first_pos + tokens - 1;
+    const int nkv = last_pos >= 0 ? last_pos / PT_KEYS + 1 : 0;            // blocks of keys
+    const int edge0 = max(0, first_pos + 1) / PT_KEYS;                     // the first block with a key that some row does not see
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1); mbar_init(q_ready, 4); mbar_init(v_land, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], E4M3 ? 4 : 1); mbar_init(&v_full[i], E4M3 ? 4 : 1);
+            mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1);
+            mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4);
+        }
+        *abort_flag = 0; *bad_value = 0; *v_exponent = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) { tmem_alloc(tmem_slot, Sh::TMEM); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tS = tmem_base, tO = tmem_base + 128;                   // two score buffers of 64, two accumulators of 64 NH columns
+
+    if (warp == 0) {
+        // ---- producer: a lane per piece of a page
+        const int piece_shift = min(p.v.page_shift, 7), pieces = PT_KEYS >> piece_shift, piece_keys = 1 << piece_shift;
+        const int per_page_shift = p.v.page_shift - piece_shift;
+        const int* table = p.v.table + (long long)s * p.v.table_ld;
+        const int last_piece = (last_pos + piece_keys) >> piece_shift;
+        auto page_at = [&](int piece) -> int {
+            if (piece >= last_piece) return 0;
+            const int pg = table[piece >> per_page_shift];
+            if ((unsigned)pg < (unsigned)p.v.pages) return pg;
+            atomicExch(p.err, 75);
+            return 0;
+        };
+        bool ok = true;
+        if (lane == 0 && nkv > 0) {
+            mbar_expect_tx(q_full, (uint32_t)(NH * pp.tokens * p.group * 128));
+            for (int c = 0; c < NH; ++c) tma_load_3d(sQ + c * PT_TILE, &tmQ, q_full, c * 64, head * p.group, q0 + tok0);
+        }
+        int held = 0, now = nkv > 0 ? page_at(lane) : 0, next = nkv > 0 ? page_at(32 + lane) : 0, landed = 0;
+        for (int j = 0; j < nkv && ok; ++j) {
+            const int at = j * pieces;
+            if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
+            const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
+            const int count = min(pieces, last_piece - at);
+            const int block = pg * p.v.heads + head, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift, o = lane << piece_shift;
+            const int st = j & 1;
+            if (!E4M3) {
+                const int vst = j % VST;
+                ok = mbar_wait(&k_empty[st], (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_expect_tx(&k_full[st], (uint32_t)(count * piece_keys * 128 * NH));
+                __syncwarp();
+                if (lane < count)
+                    for (int c = 0; c < NH; ++c) tma_load_3d(sK + (st * NH + c) * PT_TILE + o * 128, &tmK, &k_full[st], c * 64, r0, block);
+                ok = mbar_wait(&v_empty[vst], (uint32_t)((j / VST) & 1) ^ 1u, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const bool edge = j >= edge0;
+                uint64_t* bar = edge ? v_land : &v_full[vst];
+                uint8_t* tile_v = sV + vst * NH * PT_TILE;
+                if (lane == 0) mbar_expect_tx(bar, (uint32_t)(count * piece_keys * 128 * NH));
+                __syncwarp();
+                if (lane < count)
+                    for (int c = 0; c < NH; ++c) tma_load_3d(tile_v + c * PT_TILE + o * 128, &tmV, bar, c * 64, r0, block);
+                if (edge) {
+                    ok = mbar_wait(v_land, (uint32_t)(landed & 1), abort_flag);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    ++landed;
+                    const int seen = last_pos + 1 - j * PT_KEYS;           // rows of the tile that some query sees
+                    bool bad = false;
+                    for (int c = 0; c < NH; ++c)
+#pragma unroll 2
+                        for (int x = lane; x < PT_KEYS * 8; x += 32) {
+                            uint4* at16 = reinterpret_cast<uint4*>(tile_v + c * PT_TILE + x * 16);
+                            const uint4 w = *at16;
+                            if ((x >> 3) >= seen) {
+                                *at16 = make_uint4(0u, 0u, 0u, 0u);
+                            } else if (not_finite_16(w.x) || not_finite_16(w.y) || not_finite_16(w.z) || not_finite_16(w.w)) {
+                                bad = true;
+                                uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                                for (int e = 0; e < 4; ++e) {
+                                    if ((u[e] & 0x7f80u) == 0x7f80u) u[e] &= 0xffff0000u;
+                                    if ((u[e] & 0x7f800000u) == 0x7f800000u) u[e] &= 0xffffu;
+                                }
+                                *at16 = make_uint4(u[0], u[1], u[2], u[3]);
+                            }
+                        }
+                    if (bad) *bad_value = 1;
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&v_full[vst]);
+                }
+            } else {
+                for (int x = 0; x < 2 && ok; ++x) {
+                    ok = mbar_wait(&raw_empty[x], (uint32_t)(j & 1) ^ 1u, abort_flag);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(&raw_full[x], (uint32_t)(count * piece_keys * (64 * NH + (x == 0 ? 8 : 0))));
+                    __syncwarp();
+                    if (lane < count) {
+                        tma_load_3d(smem + Sh::O_RAW + x * Sh::RAW + o * 64 * NH, x == 0 ? &tmK : &tmV, &raw_full[x], 0, r0, block);
+                        if (x == 0) {
+                            float* sc = reinterpret_cast<float*>(smem + Sh::O_SCALE) + o;
+                            const long long row = ((long long)block << p.v.page_shift) + r0;
+                            bulk_load(sc, p.ks + row, (uint32_t)piece_keys * 4u, &raw_full[0]);
+                            bulk_load(sc + PT_KEYS, p.vs + row, (uint32_t)piece_keys * 4u, &raw_full[0]);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            __syncwarp();
+        }
+        pdl_launch_dependents_now();
+        if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 77); }
+    } else if (warp == 1) {
+        if (elect_one() && nkv > 0) {
+            const uint32_t fmt = E4M3 ? 0u : 1u;
+            const uint32_t idesc_s = umma_idesc(fmt, 0u, 0u, PT_ROWS, 64), idesc_o = umma_idesc(fmt, 0u, 1u, PT_ROWS, 64 * NH);
+            const uint64_t dQ = umma_desc_sw128(smem_u32(sQ), 16, 1024), dK0 = umma_desc_sw128(smem_u32(sK), 16, 1024);
+            const uint64_t dP0 = umma_desc_sw128(smem_u32(sP), 16, 1024), dV0 = umma_desc_sw128(smem_u32(sV), PT_TILE, 1024);
+            constexpr uint64_t TILE = PT_TILE >> 4, KSTEP = 32 >> 4, MNSTEP = 2048 >> 4;
+            const int nsub = 2 * nkv;
+            bool ok = mbar_wait(E4M3 ? q_ready : q_full, 0, abort_flag);
+            auto issue_scores = [&](int i) -> bool {
+                const int j = i >> 1, st = j & 1, b = i & 1;
+                if (b == 0 && !mbar_wait(&k_full[st], (uint32_t)((j >> 1) & 1), abort_flag)) return false;
+                if (!mbar_wait(&s_free[b], (uint32_t)((i >> 1) & 1) ^ 1u, abort_flag)) return false;
+                tc_fence_after();
+                const uint64_t dK = dK0 + (uint64_t)(st * NH) * TILE + (uint64_t)b * (TILE / 2);
+#pragma unroll
+                for (int k = 0; k < 4 * NH; ++k)
+                    umma_bf16(tS + (uint32_t)(b * 64), dQ + (k >> 2) * TILE + (k & 3) * KSTEP, dK + (k >> 2) * TILE + (k & 3) * KSTEP, idesc_s,
+                              k > 0 ? 1u : 0u);
+                umma_commit(&s_full[b]);
+                if (b == 1) umma_commit(&k_empty[st]);
+                return true;
+            };
+            if (ok) ok = issue_scores(0) && issue_scores(1);
+            for (int i = 0; i < nsub && ok; ++i) {
+                const int j = i >> 1, b = i & 1, vst = j % VST;
+                if (i + 2 < nsub && !issue_scores(i + 2)) { ok = false; break; }
+                if (!mbar_wait(&p_full[b], (uint32_t)(j & 1), abort_flag)) { ok = false; break; }
+                if (b == 0 && !mbar_wait(&v_full[vst], (uint32_t)((j / VST) & 1), abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint64_t dP = dP0 + (uint64_t)b * TILE, dV = dV0 + (uint64_t)(vst * NH) * TILE + (uint64_t)b * (4 * MNSTEP);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_bf16(tO + (uint32_t)(b * 64 * NH), dP + k * KSTEP, dV + k * MNSTEP, idesc_o, (i > 1 || k > 0) ? 1u : 0u);
+                umma_commit(&o_full[b]);
+                if (b == 1) umma_commit(&v_empty[vst]);
+            }
+            if (!ok) { *abort_flag = 1; atomicExch(p.err, 78); }
+        }
+    } else if (warp < 10) {
+        // ---- softmax
+        const int q = warp & 3, b = (warp - 2) >> 2, r = q * 32 + lane;
+        const int tok = min(r / p.group, tokens - 1);
+        const int pos = first_pos + tok;
+        const bool mine = r < tokens * p.group;
+        const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+        const uint32_t ts = tS + lane_base + (uint32_t)(b * 64), to = tO + lane_base + (uint32_t)(b * 64 * NH);
+        float m = -INFINITY, l = 0.f, c1 = p.scale_log2;
+        bool ok = true;
+        uint32_t v[2][32];
+        if (E4M3 && nkv > 0) {
+            ok = mbar_wait(q_ready, 0, abort_flag);
+            c1 = reinterpret_cast<const float*>(smem + Sh::O_RF)[r];
+        }
+        for (int j = 0; j < nkv && ok; ++j) {
+            if (E4M3 && !mbar_wait(&k_full[j & 1], (uint32_t)((j >> 1) & 1), abort_flag)) { ok = false; break; }
+            if (!mbar_wait(&s_full[b], (uint32_t)(j & 1), abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            tmem_ld32(ts, v[0]);
+            tmem_ld32(ts + 32, v[1]);
+            tmem_ld_wait();
+            float moved = 1.f;
+            if (E4M3) {
+                const float4* ks = reinterpret_cast<const float4*>(smem + Sh::O_KS) + (j & 3) * (PT_KEYS / 4) + b * 16;
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 f = ks[c * 8 + e / 4];
+                        const float2 x = __fmul2_rn(make_float2(__uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1])), make_float2(f.x, f.y));
+                        const float2 y = __fmul2_rn(make_float2(__uint_as_float(v[c][e + 2]), __uint_as_float(v[c][e + 3])), make_float2(f.z, f.w));
+                        v[c][e] = __float_as_uint(x.x); v[c][e + 1] = __float_as_uint(x.y);
+                        v[c][e + 2] = __float_as_uint(y.x); v[c][e + 3] = __float_as_uint(y.y);
+                    }
+                moved = v_moved[j & 3];
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[b]);
+            const bool edge = j >= edge0;
+            const int lim = edge ? pos - j * PT_KEYS - b * 64 : 64;         // columns e <= lim are allowed
+            float mx = -INFINITY;
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    mx = fmaxf(mx, e <= lim ? __uint_as_float(v[0][e]) : -INFINITY);
+                    mx = fmaxf(mx, e + 32 <= lim ? __uint_as_float(v[1][e]) : -INFINITY);
+                }
+            } else {
+                float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    m0 = fmaxf(m0, fmaxf(__uint_as_float(v[0][e]), __uint_as_float(v[1][e])));
+                    m1 = fmaxf(m1, fmaxf(__uint_as_float(v[0][e + 1]), __uint_as_float(v[1][e + 1])));
+                    m2 = fmaxf(m2, fmaxf(__uint_as_float(v[0][e + 2]), __uint_as_float(v[1][e + 2])));
+                    m3 = fmaxf(m3, fmaxf(__uint_as_float(v[0][e + 3]), __uint_as_float(v[1][e + 3])));
+                }
+                mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+            }
+            const float m_new = fmaxf(m, mx * c1);
+            float alpha = 1.0f;
+            if (m_new > m) {
+                alpha = ex2_approx(m - m_new);
+                l *= alpha;
+                m = m_new;
+            }
+            if (E4M3) alpha *= moved;
+            const bool move = __any_sync(0xffffffffu, alpha != 1.0f);
+            if (j > 0 && !mbar_wait(&o_full[b], (uint32_t)((j - 1) & 1), abort_flag)) { ok = false; break; }
+            const float2 c2 = make_float2(c1, c1), nm2 = make_float2(-m, -m);
+            float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            uint8_t* prow = sP + b * PT_TILE + r * 128;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const int e = 8 * g + 2 * h;
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1])), c2, nm2);
+                        float2 pr = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                        if (edge) {
+                            pr.x = e + 32 * c <= lim ? pr.x : 0.0f;
+                            pr.y = e + 1 + 32 * c <= lim ? pr.y : 0.0f;
+                        }
+                        ls[h & 1] = __fadd2_rn(ls[h & 1], pr);
+                        w[h] = E4M3 ? f16_pair(pr.x, pr.y) : bf16_pair(pr.x, pr.y);
+                    }
+                    *reinterpret_cast<uint4*>(prow + (((4 * c + g) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+            if (move && j > 0) {
+                tc_fence_after();
+#pragma unroll 1
+                for (int h2 = 0; h2 < 2 * NH; ++h2) {                       // (unrolled, it costs registers that the loop around it needs)
+                    tmem_ld32(to + (uint32_t)(h2 * 32), v[0]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[0][e] = __float_as_uint(__uint_as_float(v[0][e]) * alpha);
+                    tmem_st32(to + (uint32_t)(h2 * 32), v[0]);
+                }
+                tmem_st_wait();
+            }
+            tc_fence_before();
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[b]);
+        }
+        // ---- the two groups' results together
+        if (ok && nkv > 0)
+            ok = mbar_wait(&o_full[0], (uint32_t)((nkv - 1) & 1), abort_flag) && mbar_wait(&o_full[1], (uint32_t)((nkv - 1) & 1), abort_flag) &&
+                 mbar_wait(&v_full[(nkv - 1) % VST], (uint32_t)(((nkv - 1) / VST) & 1), abort_flag);        // (for bad_value)
+        float2* stat = reinterpret_cast<float2*>(sP);
+        if (ok) stat[b * PT_ROWS + r] = make_float2(m, l);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (ok) {
+            const bool none = pos < 0;                                      // a row without a key
+            const float2 s0 = stat[r], s1 = stat[PT_ROWS + r];
+            const float M = fmaxf(s0.x, s1.x);
+            const float e0 = s0.y == 0.f ? 0.f : ex2_approx(s0.x - M), e1 = s1.y == 0.f ? 0.f : ex2_approx(s1.x - M);
+            const float lt = s0.y * e0 + s1.y * e1;
+            float inv = none ? 0.f : 1.0f / lt;
+            const float unit = E4M3 ? exp2f((float)(*v_exponent - 127 - 6)) : 1.f;
+            const float w0 = e0 * inv * unit, w1 = e1 * inv * unit;
+            // as bf16 through the query tile, so that whole rows leave side by side
+            uint8_t* row = sQ + r * 128;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < NH; ++c) {
+                if (nkv > 0) {
+                    tmem_ld32(tO + lane_base + (uint32_t)(64 * c + 32 * b), v[0]);
+                    tmem_ld32(tO + lane_base + (uint32_t)(64 * NH + 64 * c + 32 * b), v[1]);
+                    tmem_ld_wait();
+                }
+                auto out = [&](int e) {
+                    return none ? 0.f : (e0 == 0.f ? 0.f : __uint_as_float(v[0][e]) * w0) + (e1 == 0.f ? 0.f : __uint_as_float(v[1][e]) * w1);
+                };
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    *reinterpret_cast<uint4*>(row + c * PT_TILE + (((4 * b + d) ^ (r & 7)) << 4)) =
+                        make_uint4(bf16_pair(out(8 * d), out(8 * d + 1)), bf16_pair(out(8 * d + 2), out(8 * d + 3)),
+                                   bf16_pair(out(8 * d + 4), out(8 * d + 5)), bf16_pair(out(8 * d + 6), out(8 * d + 7)));
+            }
+            if (*bad_value && mine && !none) add_what_is_not_finite<NH, E4M3>(p, pool_v, s, head, edge0 * PT_KEYS, pos, b, r, row);
+            if (p.lse && b == 0 && mine)
+                p.lse[(long long)(q0 + tok0 + r / p.group) * p.H + head * p.group + r % p.group] =
+                    none ? -INFINITY : (M + log2f(lt)) * 0.6931471805599453f;
+        }
+        if (all_of(ok, 1, 256)) {
+            const int per_row = p.v.hd >> 3;                                // 16-byte pieces of a row
+            for (int x = threadIdx.x - 64; x < tokens * p.group * per_row; x += 256) {
+                const int rr = x / per_row, e = x - rr * per_row, t = rr / p.group, g = rr - t * p.group;
+                const uint4 w = *reinterpret_cast<const uint4*>(sQ + (e >> 3) * PT_TILE + rr * 128 + (((e & 7) ^ (rr & 7)) << 4));
+                *reinterpret_cast<uint4*>(p.att + (long long)(q0 + tok0 + t) * p.ld_att + (long long)(head * p.group + g) * p.v.hd + e * 8) = w;
+            }
+        }
+        if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 79); }
+    } else if (E4M3) {
+        // ---- codes to f16: thread = query row once, then a key of every block
+        const int t = threadIdx.x - 320, q = warp - 10;
+        bool ok = true;
+        if (nkv > 0) ok = mbar_wait(q_full, 0, abort_flag);
+        if (nkv > 0 && ok) {
+            uint32_t most = 0u;
+            uint8_t* row = sQ + t * 128;
+#pragma unroll
+            for (int c = 0; c < NH; ++c)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(row + c * PT_TILE + (d << 4));
+                    const uint32_t a = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+                    most = max(most, max(a & 0xffffu, a >> 16));
+                }
+            // scaled by a power of two so that the row's largest magnitude lies in [1, 2): exact but for what is less than 2^-24 of it
+            const int e = max((int)(most >> 7), 1);
+            const bool odd = e >= 254;
+            const float down = odd ? 1.f : __uint_as_float((uint32_t)(254 - e) << 23), up = odd ? 1.f : __uint_as_float((uint32_t)e << 23);
+            reinterpret_cast<float*>(smem + Sh::O_RF)[t] = up;
+#pragma unroll
+            for (int c = 0; c < NH; ++c)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    uint4* at = reinterpret_cast<uint4*>(row + c * PT_TILE + (d << 4));
+                    uint4 w = *at;
+                    uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = bf16_floats(u[i]);
+                        u[i] = f16_pair(f.x * down, f.y * down);
+                    }
+                    *at = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready);
+        }
+        // Keys go one block ahead of the values, so that the next scores do not wait for this block's product.
+        const uint8_t* rk = smem + Sh::O_RAW + t * 64 * NH;
+        const uint8_t* rv = rk + Sh::RAW;
+        const float* sc = reinterpret_cast<const float*>(smem + Sh::O_SCALE);
+        int reference = 0;
+        float f_next = 0.f, f = 0.f;                                        // the factor of this key's value, of the next block and of this one
+        bool fin_next = true, fin = true;
+        auto keys = [&](int j) -> bool {
+            const int st = j & 1;
+            ok = ok && mbar_wait(&raw_full[0], (uint32_t)(j & 1), abort_flag);
+            const float vs = j * PT_KEYS + t <= last_pos ? sc[PT_KEYS + t] : 0.f;
+            const uint32_t ve = (__float_as_uint(vs) >> 23) & 255u;
+            fin_next = ve != 255u;
+            // the block's reference: the largest exponent of a value's scale so far
+            const uint32_t most = __reduce_max_sync(0xffffffffu, fin_next ? ve : 0u);
+            ok = ok && mbar_wait(&k_empty[st], (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag);
+            uint32_t* w4 = warp_most + (j & 1) * 4;
+            if (lane == 0) w4[q] = most;
+            if (!all_of(ok, 2, 128)) return false;
+            const int now = max(reference, (int)max(max(w4[0], w4[1]), max(w4[2], w4[3])));
+            reinterpret_cast<float*>(smem + Sh::O_KS)[(j & 3) * PT_KEYS + t] = sc[t] * p.scale_log2;
+            if (t == 0) {
+                const int d = now - reference;                              // (an accumulator that is still empty may be scaled by anything)
+                v_moved[j & 3] = d == 0 ? 1.f : d > 126 ? 0.f : __uint_as_float((uint32_t)(127 - d) << 23);
+                *v_exponent = now;
+            }
+            reference = now;
+            // code * scale * 2^(6 - reference), in two steps: 2^(127 - reference) alone may be no normal number
+            const int half_way = (127 - now) / 2;
+            f_next = fin_next ? vs * __uint_as_float((uint32_t)(127 + half_way) << 23) * __uint_as_float((uint32_t)(133 + 127 - now - half_way) << 23) : vs;
+            uint8_t* row = sK + st * NH * PT_TILE + t * 128;
+#pragma unroll
+            for (int c = 0; c < NH; ++c)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(rk + 64 * c + 16 * d);
+                    *reinterpret_cast<uint4*>(row + c * PT_TILE + (((2 * d) ^ (t & 7)) << 4)) =
+                        make_uint4(e4m3_f16(w.x), e4m3_f16(w.x >> 16), e4m3_f16(w.y), e4m3_f16(w.y >> 16));
+                    *reinterpret_cast<uint4*>(row + c * PT_TILE + (((2 * d + 1) ^ (t & 7)) << 4)) =
+                        make_uint4(e4m3_f16(w.z), e4m3_f16(w.z >> 16), e4m3_f16(w.w), e4m3_f16(w.w >> 16));
+                }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(&k_full[st]); mbar_arrive(&raw_empty[0]); }
+            return true;
+        };
+        auto nan_codes = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
+        if (nkv > 0) ok = keys(0);
+        for (int j = 0; j < nkv && ok; ++j) {
+            const int vst = j % VST;
+            f = f_next; fin = fin_next;
+            if (j + 1 < nkv && !keys(j + 1)) { ok = false; break; }
+            ok = mbar_wait(&raw_full[1], (uint32_t)(j & 1), abort_flag) && mbar_wait(&v_empty[vst], (uint32_t)((j / VST) & 1) ^ 1u, abort_flag);
+            if (!ok) {
+                if (lane == 0) *abort_flag = 1;
+                if (j + 2 < nkv) all_of(false, 2, 128);                     // (where the others meet in keys(j + 2))
+                break;
+            }
+            const bool seen = j * PT_KEYS + t <= last_pos, looked = j >= edge0 && seen;
+            bool bad = looked && !fin;
+            if (looked && fin) {
+                uint32_t has = 0u;
+#pragma unroll
+                for (int d = 0; d < 4 * NH; ++d) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(rv + 16 * d);
+                    has |= nan_codes(w.x) | nan_codes(w.y) | nan_codes(w.z) | nan_codes(w.w);
+                }
+                bad = has != 0u;
+            }
+            if (bad) *bad_value = 1;
+            const bool zero = !seen || (bad && !fin);
+            const uint32_t f2 = zero ? 0u : f16_pair(f, f);
+            uint8_t* row = sV + vst * NH * PT_TILE + t * 128;
+#pragma unroll
+            for (int c = 0; c < NH; ++c)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    uint4 w = *reinterpret_cast<const uint4*>(rv + 64 * c + 16 * d);
+                    if (zero) w = make_uint4(0u, 0u, 0u, 0u);
+                    if (bad) {                                              // NaN codes to zero
+                        w.x &= ~((nan_codes(w.x) >> 7) * 255u); w.y &= ~((nan_codes(w.y) >> 7) * 255u);
+                        w.z &= ~((nan_codes(w.z) >> 7) * 255u); w.w &= ~((nan_codes(w.w) >> 7) * 255u);
+                    }
+                    uint32_t u[8] = {w.x, w.x >> 16, w.y, w.y >> 16, w.z, w.z >> 16, w.w, w.w >> 16};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(u[i]) : "r"(e4m3_f16(u[i])), "r"(f2));
+                    *reinterpret_cast<uint4*>(row + c * PT_TILE + (((2 * d) ^ (t & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+                    *reinterpret_cast<uint4*>(row + c * PT_TILE + (((2 * d + 1) ^ (t & 7)) << 4)) = make_uint4(u[4], u[5], u[6], u[7]);
+                }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(&v_full[vst]); mbar_arrive(&raw_empty[1]); }
+        }
+        if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 80); }
+    }
+
+    __syncwarp();
+    if (*abort_flag) for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, Sh::TMEM); }
+}
+
+template <int NH, bool E4M3>
+int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cudaStream_t st) {
+    typedef ChunkShape<NH, E4M3> Sh;
+    PagedChunkParams pp;
+    pp.a = p;
+    pp.tokens = PT_ROWS / p.group;
+    pp.tiles = (p.max_q + pp.tokens - 1) / pp.tokens;
+    TB_CHECK(pp.tiles <= 65535, "tb_attention_paged: max_q %d is too much for one launch", p.max_q);
+    CUtensorMap tmQ, tmK, tmV;
+    TB_TRY(make_query_map(&tmQ, p.Q, c->head_dim, p.H, p.rows, p.ld_q, p.group, pp.tokens));
+    const int box_rows = std::min(c->page_size, PT_KEYS);
+    TB_TRY(make_cache_map(&tmK, c->K, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
+    TB_TRY(make_cache_map(&tmV, c->V, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
+    static bool attr_set[64] = {false};
+    if (!attr_set[ctx->device & 63]) {
+        TB_CUDA(cudaFuncSetAttribute(paged_chunk_kernel<NH, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+        attr_set[ctx->device & 63] = true;
+    }
+    prof_mark(ctx, "paged_chunk", 4.0 * p.rows * p.H * (double)p.max_kv * c->head_dim, 0.0, st);
+    TB_CUDA(launch_kernel(paged_chunk_kernel<NH, E4M3>, dim3(c->heads, pp.tiles, c->seqs), dim3(Sh::THREADS), Sh::SMEM, st, tmQ, tmK, tmV,
+                          static_cast<const uint8_t*>(c->V), pp));
     ctx->launches++;
     prof_close(ctx, st);
     return 0;
@@ -458,25 +1226,28 @@ int launch_attention_paged(DeviceCtx* ctx, const TbKvCache* c, const int* q_star
                            int H, int max_q, int max_kv, float scale, bf16* att, long long ld_att, float* lse, void* ws, int64_t ws_bytes,
                            cudaStream_t st) {
     const int group = H / c->heads;
-    const PagedPlan pl = paged_plan(c->seqs, c->heads, group, c->head_dim, rows, max_q, max_kv, ctx->sm_count);
+    const PagedPlan pl = paged_plan(c->seqs, c->heads, c->head_dim, c->type == TB_KV_E4M3, max_kv, ctx->sm_count);
     TB_CHECK(pl.workspace == 0 || (ws != nullptr && ws_bytes >= pl.workspace), "tb_attention_paged: the workspace has %lld bytes, %lld are needed",
              (long long)(ws ? ws_bytes : 0), (long long)pl.workspace);
-    TB_CHECK((long long)c->heads * pl.tiles <= 65535, "tb_attention_paged: max_q %d with %d heads is too much for one launch", max_q, H);
     PagedAttParams p;
     p.v = paged_view(c);
     p.q_start = q_start; p.kv_len = kv_len; p.Q = Q; p.ld_q = ld_q; p.ks = c->k_scale; p.vs = c->v_scale;
     p.att = att; p.ld_att = ld_att; p.lse = lse;
     p.part_o = static_cast<float*>(ws);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + (long long)pl.splits * rows * H * c->head_dim);
-    p.rows = rows; p.H = H; p.group = group; p.max_q = max_q; p.max_kv = max_kv; p.split_keys = pl.split_keys;
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + 2LL * pl.grid * PA_ROWS * c->head_dim);
+    p.before = reinterpret_cast<long long*>(p.part_ml + 2LL * pl.grid * PA_ROWS);
+    p.rows = rows; p.H = H; p.group = group; p.max_q = max_q; p.max_kv = max_kv; p.grid = pl.grid; p.whole = pl.whole ? 1 : 0;
     p.scale_log2 = scale * 1.4426950408889634f; p.err = ctx->d_err;
     const bool wide = c->head_dim > 64;
-    if (c->type == TB_KV_E4M3) TB_TRY(wide ? (launch_rows<2, true>(ctx, c, p, pl, st)) : (launch_rows<1, true>(ctx, c, p, pl, st)));
-    else TB_TRY(wide ? (launch_rows<2, false>(ctx, c, p, pl, st)) : (launch_rows<1, false>(ctx, c, p, pl, st)));
-    if (pl.splits > 1) {
+    if (max_q * (long long)group > PA_ROWS) {
+        if (c->type == TB_KV_E4M3) TB_TRY(wide ? (launch_chunks<2, true>(ctx, c, p, st)) : (launch_chunks<1, true>(ctx, c, p, st)));
+        else TB_TRY(wide ? (launch_chunks<2, false>(ctx, c, p, st)) : (launch_chunks<1, false>(ctx, c, p, st)));
+    }
+    if (c->type == TB_KV_E4M3) TB_TRY(wide ? (launch_rows<2, true>(ctx, c, p, st)) : (launch_rows<1, true>(ctx, c, p, st)));
+    else TB_TRY(wide ? (launch_rows<2, false>(ctx, c, p, st)) : (launch_rows<1, false>(ctx, c, p, st)));
+    if (!pl.whole) {
         const long long blocks = ((long long)rows * H + PC_WARPS - 1) / PC_WARPS;
-        TB_CHECK(blocks < (1LL << 31), "tb_attention_paged: too many rows");
-        prof_mark(ctx, "paged_combine", 0.0, (double)pl.workspace, st);
+        prof_mark(ctx, "paged_combine", 0.0, 0.0, st);
         TB_CUDA(launch_kernel(paged_combine_kernel, dim3((unsigned)blocks), dim3(PC_WARPS * 32), 0, st, p));
         ctx->launches++;
         prof_close(ctx, st);
@@ -492,6 +1263,7 @@ static int check_attention(const TbKvCache* cache, int rows, int q_heads, int ma
     TB_TRY(check_cache(cache, "tb_attention_paged"));
     TB_CHECK(rows >= 0 && max_q >= 0 && max_kv >= 0, "tb_attention_paged: rows, max_q and max_kv must not be negative");
     TB_CHECK(q_heads > 0 && q_heads % cache->heads == 0, "tb_attention_paged: %d query heads cannot share %d key heads", q_heads, cache->heads);
+    TB_CHECK(q_heads / cache->heads <= PT_ROWS, "tb_attention_paged: at most %d query heads share a key head (got %d)", PT_ROWS, q_heads / cache->heads);
     TB_CHECK((long long)rows * q_heads < (1LL << 31), "tb_attention_paged: rows * q_heads must be below 2^31");
     return 0;
 }
@@ -501,7 +1273,7 @@ extern "C" {
 int64_t tb_attention_paged_workspace(const TbKvCache* cache, int rows, int q_heads, int max_q, int max_kv) {
     DeviceCtx* ctx;
     if (check_attention(cache, rows, q_heads, max_q, max_kv) != 0 || get_ctx(&ctx) != 0) return -1;
-    return paged_plan(cache->seqs, cache->heads, q_heads / cache->heads, cache->head_dim, rows, std::min(max_q, rows), max_kv, ctx->sm_count).workspace;
+    return paged_plan(cache->seqs, cache->heads, cache->head_dim, cache->type == TB_KV_E4M3, max_kv, ctx->sm_count).workspace;
 }
 
 int tb_attention_paged(const TbKvCache* cache, const int32_t* d_q_start, const int32_t* d_kv_len, const void* d_Q, int64_t ld_q, int rows,
@@ -516,6 +1288,7 @@ int tb_attention_paged(const TbKvCache* cache, const int32_t* d_q_start, const i
              (long long)ld_att);
     TB_CHECK(((reinterpret_cast<uintptr_t>(d_Q) | reinterpret_cast<uintptr_t>(d_att) | reinterpret_cast<uintptr_t>(d_workspace)) & 15u) == 0,
              "tb_attention_paged: rows and workspace must be 16-byte aligned");
+    TB_CHECK(scale > 0.f && scale < INFINITY, "tb_attention_paged: scale must be positive and finite");
     TB_CHECK(d_Q != d_att, "tb_attention_paged: the result must not lie over the queries");
     DeviceCtx* ctx;
     TB_TRY(get_ctx(&ctx));

@@ -203,6 +203,9 @@ int make_operand_map4(CUtensorMap* map, const bf16* ptr, long long inner, long l
 int make_cache_map(CUtensorMap* map, const void* ptr, int es, long long inner, long long rows, long long blocks, int box_inner,
                    int box_rows);
 
+// rows of heads, [rows][heads][hd] with leading dimension ld: a box of 64 elements of box_heads heads of box_rows rows
+int make_query_map(CUtensorMap* map, const bf16* ptr, int hd, int heads, int rows, long long ld, int box_heads, int box_rows);
+
 // ---- fused causal attention (attention.cu); Q, K, V bf16 [B*H, T, hd] (hd <= 64, multiple of 8)
 // forward: att bf16 [B*T, H*hd] (heads merged), lse float [B*H, T] (natural-log sum of exponentials)
 // (lse may be NULL; kv_rows_per_head > T when K and V live in a KV cache with that many rows per head)

@@ -1522,6 +1522,19 @@ int make_cache_map(CUtensorMap* map, const void* ptr, int es, long long inner, l
     return 0;
 }
 
+int make_query_map(CUtensorMap* map, const bf16* ptr, int hd, int heads, int rows, long long ld, int box_heads, int box_rows) {
+    EncodeTiledFn enc = get_encode_fn();
+    TB_CHECK(enc != nullptr, "cuTensorMapEncodeTiled entry point not available");
+    cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
+    cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)ld * 2};
+    cuuint32_t box[3] = {64u, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+    cuuint32_t estr[3] = {1u, 1u, 1u};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    TB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code %d (head_dim=%d heads=%d rows=%d ld=%lld)", (int)r, hd, heads, rows, ld);
+    return 0;
+}
+
 int make_operand_map4(CUtensorMap* map, const bf16* ptr, long long inner, long long rows, long long ld,
                       long long n0, long long stride0, long long n1, long long stride1, int box_rows) {
     EncodeTiledFn enc = get_encode_fn();

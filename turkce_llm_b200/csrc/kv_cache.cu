@@ -43,7 +43,7 @@ struct AppendParams {
     PagedView v;
     const int *q_start, *kv_len;
     const void* x; long long ld_x;
-    int rows, H, warps_per_row, threads_log2;        // threads per head: 1 << threads_log2
+    int rows, H, parts, threads_log2;                 // warps per row; threads per head: 1 << threads_log2
     const float *cos_t, *sin_t;
     int positions, half;                              // rot_dim / 2
     bf16* Q; long long ld_q;
@@ -73,6 +73,7 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 }
 
 // Rotated elements are a cos - b sin and a sin + b cos with every product rounded, the same sums whichever thread forms them.
+// A warp takes every `parts`-th group of heads of its row, the next group's elements on their way while it works on one.
 template <bool BF16_IN, bool HALVES, bool E4M3>
 __global__ void __launch_bounds__(KV_THREADS)
 kv_append_kernel(const AppendParams p) {
@@ -81,14 +82,24 @@ kv_append_kernel(const AppendParams p) {
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned w = blockIdx.x * KV_WARPS + warp;
-    const int row = (int)(w / (unsigned)p.warps_per_row), part = (int)(w - (unsigned)row * (unsigned)p.warps_per_row);
+    const int row = (int)(w / (unsigned)p.parts), part = (int)(w - (unsigned)row * (unsigned)p.parts);
     if (row >= p.rows) return;                                   // (whole warps)
-    const int hd = p.v.hd, G = p.v.heads;
-    const int head = (part << (5 - p.threads_log2)) + (lane >> p.threads_log2);
+    const int hd = p.v.hd, G = p.v.heads, all = p.H + 2 * G;
+    const int per_warp = 32 >> p.threads_log2, step = per_warp * p.parts;
     const int e0 = (lane & ((1 << p.threads_log2) - 1)) * 8;     // first of this thread's elements
-    const bool mine = head < p.H + 2 * G && e0 < hd;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (mine) load8<BF16_IN>(p.x, (long long)row * p.ld_x + (long long)head * hd + e0, x);      // (needs nothing of the batch)
+    const long long x_row = (long long)row * p.ld_x + e0;
+    int group = part * per_warp, head = group + (lane >> p.threads_log2);
+    const bool lane_in = e0 < hd;
+    float x[8], nx[8];
+    auto fetch = [&](float (&f)[8], int h) {
+        if (lane_in && h < all) {
+            load8<BF16_IN>(p.x, x_row + (long long)h * hd, f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = 0.f;
+        }
+    };
+    fetch(x, head);                                              // (needs nothing of the batch)
     const int s = sequence_of(p.q_start, p.v.seqs, row);
     if (s < 0) return;
     const int end = p.q_start[s + 1], len = p.kv_len[s];
@@ -99,74 +110,89 @@ kv_append_kernel(const AppendParams p) {
         return;
     }
     const int page = p.v.table[(long long)s * p.v.table_ld + (pos >> p.v.page_shift)];
-    if (p.half > 0 && part * (32 >> p.threads_log2) < p.H + G) {     // (a warp of values alone has nothing to rotate)
-        const bool turns = head < p.H + G;
-        const float* ct = p.cos_t + pos * p.half;
-        const float* st = p.sin_t + pos * p.half;
-        if (!HALVES) {
+    const bool page_ok = (unsigned)page < (unsigned)p.v.pages;
+    if (!page_ok && lane == 0) atomicExch(p.err, 71);
+    const long long slot = ((long long)page * G << p.v.page_shift) + (pos & ((1 << p.v.page_shift) - 1));
+    // this thread's angles are the same in every head
+    float c[HALVES ? 8 : 4], d[HALVES ? 8 : 4];
+    if (p.half > 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = (e0 >> 1) + i;
-                if (mine && turns && k < p.half) {
-                    const float c = ct[k], d = st[k], a = x[2 * i], b = x[2 * i + 1];
-                    x[2 * i] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, d));
-                    x[2 * i + 1] = __fadd_rn(__fmul_rn(a, d), __fmul_rn(b, c));
-                }
-            }
-        } else {
-            // the partner's elements through shared memory: element e of this head at (e / 8) * 9 + e % 8 from the head's first
-            float* sw = swap[warp];
-            const int base = (lane >> p.threads_log2 << p.threads_log2) * 9;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sw[lane * 9 + i] = x[i];
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int e = e0 + i;
-                if (mine && turns && e < 2 * p.half) {
-                    const bool low = e < p.half;
-                    const int k = low ? e : e - p.half, o = low ? e + p.half : e - p.half;
-                    const float other = sw[base + (o >> 3) * 9 + (o & 7)], c = ct[k], d = st[k];
-                    x[i] = low ? __fsub_rn(__fmul_rn(x[i], c), __fmul_rn(other, d)) : __fadd_rn(__fmul_rn(other, d), __fmul_rn(x[i], c));
-                }
-            }
+        for (int i = 0; i < (HALVES ? 8 : 4); ++i) {
+            const int e = HALVES ? e0 + i : (e0 >> 1) + i, k = HALVES && e >= p.half ? e - p.half : e;
+            const bool turns = HALVES ? e < 2 * p.half : e < p.half;
+            c[i] = turns ? p.cos_t[pos * p.half + k] : 1.f;
+            d[i] = turns ? p.sin_t[pos * p.half + k] : 0.f;
         }
     }
-    if (mine && head < p.H) {
-        *reinterpret_cast<uint4*>(p.Q + (long long)row * p.ld_q + (long long)head * hd + e0) = pack8(x);
-    }
-    // largest magnitude of the row: as integers, so that NaN is larger than infinity and infinity than the rest
-    uint32_t big = 0u;
-    if (E4M3) {
+    for (; group < all; group += step, head += step) {
+        const bool mine = lane_in && head < all;
+        if (group + step < all) fetch(nx, head + step);
+        if (p.half > 0 && group < p.H + G) {                     // (a group of values alone has nothing to rotate)
+            const bool turns = head < p.H + G;
+            if (!HALVES) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
-        for (int o = (1 << p.threads_log2) >> 1; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-    }
-    if (!mine || head < p.H) return;
-    if ((unsigned)page >= (unsigned)p.v.pages) {
-        atomicExch(p.err, 71);
-        return;
-    }
-    const bool key = head < p.H + G;
-    const long long at = (((long long)page * G + (head - p.H - (key ? 0 : G))) << p.v.page_shift) + (pos & ((1 << p.v.page_shift) - 1));
-    if (!E4M3) {
-        *reinterpret_cast<uint4*>(static_cast<bf16*>(key ? p.K : p.V) + at * hd + e0) = pack8(x);
-    } else {
-        float scale = __fdiv_rn(__uint_as_float(big), 448.0f);
-        if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;          // (stays NaN where it is)
-        uint32_t c[4];
+                for (int i = 0; i < 4; ++i) {
+                    if (turns && (e0 >> 1) + i < p.half) {
+                        const float a = x[2 * i], b = x[2 * i + 1];
+                        x[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, d[i]));
+                        x[2 * i + 1] = __fadd_rn(__fmul_rn(a, d[i]), __fmul_rn(b, c[i]));
+                    }
+                }
+            } else {
+                // the partner's elements through shared memory: element e of this head at (e / 8) * 9 + e % 8 from the head's first
+                float* sw = swap[warp];
+                const int base = (lane >> p.threads_log2 << p.threads_log2) * 9;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = e4m3_pair(quotient_to_odd(x[2 * i], scale), quotient_to_odd(x[2 * i + 1], scale));
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(key ? p.K : p.V) + at * hd + e0) =
-            make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
-        if (e0 == 0) (key ? p.ks : p.vs)[at] = scale;
+                for (int i = 0; i < 8; ++i) sw[lane * 9 + i] = x[i];
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int e = e0 + i;
+                    if (mine && turns && e < 2 * p.half) {
+                        const bool low = e < p.half;
+                        const int o = low ? e + p.half : e - p.half;
+                        const float other = sw[base + (o >> 3) * 9 + (o & 7)];
+                        x[i] = low ? __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(other, d[i]))
+                                   : __fadd_rn(__fmul_rn(other, d[i]), __fmul_rn(x[i], c[i]));
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        // largest magnitude of the row: as integers, so that NaN is larger than infinity and infinity than the rest
+        uint32_t big = 0u;
+        if (E4M3 && group + per_warp > p.H) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
+            for (int o = (1 << p.threads_log2) >> 1; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+        }
+        if (mine && head < p.H) {
+            *reinterpret_cast<uint4*>(p.Q + (long long)row * p.ld_q + (long long)head * hd + e0) = pack8(x);
+        } else if (mine && page_ok) {
+            const bool key = head < p.H + G;
+            const long long at = slot + ((long long)(head - p.H - (key ? 0 : G)) << p.v.page_shift);
+            if (!E4M3) {
+                *reinterpret_cast<uint4*>(static_cast<bf16*>(key ? p.K : p.V) + at * hd + e0) = pack8(x);
+            } else {
+                float scale = __fdiv_rn(__uint_as_float(big), 448.0f);
+                if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;          // (stays NaN where it is)
+                uint32_t q[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[i] = e4m3_pair(quotient_to_odd(x[2 * i], scale), quotient_to_odd(x[2 * i + 1], scale));
+                *reinterpret_cast<uint2*>(static_cast<uint8_t*>(key ? p.K : p.V) + at * hd + e0) =
+                    make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+                if (e0 == 0) (key ? p.ks : p.vs)[at] = scale;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = nx[i];
     }
 }
 
 struct ReadParams {
     PagedView v;
     const int *start, *first;
-    int rows, warps_per_row, threads_log2, kinds;     // kinds: 1 or 2 of K and V
+    int rows, parts, threads_log2, kinds;             // warps per row, threads per head, 1 or 2 of K and V
     const void *A, *B;                                // the pools read (B: the second one)
     const float *as, *bs;
     bf16 *oA, *oB;
@@ -181,10 +207,10 @@ kv_read_kernel(const ReadParams p) {
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned w = blockIdx.x * KV_WARPS + warp;
-    const int row = (int)(w / (unsigned)p.warps_per_row), part = (int)(w - (unsigned)row * (unsigned)p.warps_per_row);
+    const int row = (int)(w / (unsigned)p.parts), part = (int)(w - (unsigned)row * (unsigned)p.parts);
     if (row >= p.rows) return;
-    const int hd = p.v.hd, G = p.v.heads;
-    const int head = (part << (5 - p.threads_log2)) + (lane >> p.threads_log2);
+    const int hd = p.v.hd, G = p.v.heads, all = p.kinds * G;
+    const int step = (32 >> p.threads_log2) * p.parts;
     const int e0 = (lane & ((1 << p.threads_log2) - 1)) * 8;
     const int s = sequence_of(p.start, p.v.seqs, row);
     if (s < 0 || row >= p.start[s + 1]) return;
@@ -198,37 +224,42 @@ kv_read_kernel(const ReadParams p) {
         if (lane == 0) atomicExch(p.err, 71);
         return;
     }
-    if (head >= p.kinds * G || e0 >= hd) return;
-    const bool first = head < G;
-    const int h = first ? head : head - G;
-    const long long at = (((long long)page * G + h) << p.v.page_shift) + (t & ((1 << p.v.page_shift) - 1));
-    uint4 out;
-    if (!E4M3) {
-        out = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(first ? p.A : p.B) + at * hd + e0);
-    } else {
-        const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(first ? p.A : p.B) + at * hd + e0);
-        const float scale = (first ? p.as : p.bs)[at];
-        const uint32_t u[4] = {c.x & 0xffffu, c.x >> 16, c.y & 0xffffu, c.y >> 16};
-        uint32_t o[4];
+    if (e0 >= hd) return;
+    const long long slot = ((long long)page * G << p.v.page_shift) + (t & ((1 << p.v.page_shift) - 1));
+#pragma unroll 4
+    for (int head = part * (32 >> p.threads_log2) + (lane >> p.threads_log2); head < all; head += step) {
+        const bool first = head < G;
+        const int h = first ? head : head - G;
+        const long long at = slot + ((long long)h << p.v.page_shift);
+        uint4 out;
+        if (!E4M3) {
+            out = __ldg(reinterpret_cast<const uint4*>(static_cast<const bf16*>(first ? p.A : p.B) + at * hd + e0));
+        } else {
+            const uint2 c = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(first ? p.A : p.B) + at * hd + e0));
+            const float scale = __ldg((first ? p.as : p.bs) + at);
+            const uint32_t u[4] = {c.x & 0xffffu, c.x >> 16, c.y & 0xffffu, c.y >> 16};
+            uint32_t o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = e4m3_floats(u[i]);
-            o[i] = bf16_pair(f.x * scale, f.y * scale);
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = e4m3_floats(u[i]);
+                o[i] = bf16_pair(f.x * scale, f.y * scale);
+            }
+            out = make_uint4(o[0], o[1], o[2], o[3]);
         }
-        out = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>((first ? p.oA : p.oB) + (long long)row * p.ld_row + h * p.ld_head + e0) = out;
     }
-    *reinterpret_cast<uint4*>((first ? p.oA : p.oB) + (long long)row * p.ld_row + h * p.ld_head + e0) = out;
 }
 
-// threads per head (a power of two that divides a warp), warps per row, and the blocks for all rows
-int shape_of(int hd, int heads, int rows, int* threads_log2, int* warps_per_row, long long* blocks) {
+// threads per head (a power of two that divides a warp), warps per row, and the blocks for all rows.  A warp takes its row's heads
+// one group after the other, and what it knows of the row once; where there are fewer rows than that keeps the chip busy with
+// (eight warps per SM), a row's groups go to different warps.
+void shape_of(const DeviceCtx* ctx, int hd, int heads, int rows, int* threads_log2, int* parts, long long* blocks) {
     int t = 0;
     while ((8 << t) < hd) ++t;
     *threads_log2 = t;
-    const int per_warp = 32 >> t;
-    *warps_per_row = (heads + per_warp - 1) / per_warp;
-    *blocks = ((long long)rows * *warps_per_row + KV_WARPS - 1) / KV_WARPS;
-    return 0;
+    const int per_warp = 32 >> t, groups = (heads + per_warp - 1) / per_warp;
+    *parts = (int)std::max<long long>(1, std::min<long long>(groups, 8LL * ctx->sm_count / rows));
+    *blocks = ((long long)rows * *parts + KV_WARPS - 1) / KV_WARPS;
 }
 
 }  // namespace
@@ -242,7 +273,7 @@ int launch_kv_append(DeviceCtx* ctx, const TbKvCache* c, const int* q_start, con
     p.cos_t = cos_t; p.sin_t = sin_t; p.positions = positions; p.half = rot_dim / 2;
     p.Q = Q; p.ld_q = ld_q; p.K = c->K; p.V = c->V; p.ks = c->k_scale; p.vs = c->v_scale; p.err = ctx->d_err;
     long long blocks;
-    shape_of(c->head_dim, H + 2 * c->heads, rows, &p.threads_log2, &p.warps_per_row, &blocks);
+    shape_of(ctx, c->head_dim, H + 2 * c->heads, rows, &p.threads_log2, &p.parts, &blocks);
     TB_CHECK(blocks < (1LL << 31) / KV_WARPS, "tb_kv_append: too many rows");
     typedef void (*Kernel)(AppendParams);
     const bool halves = form == TB_ROPE_HALVES && rot_dim > 0, e4m3 = c->type == TB_KV_E4M3;
@@ -267,7 +298,7 @@ int launch_kv_read(DeviceCtx* ctx, const TbKvCache* c, const int* start, const i
     p.B = c->V; p.bs = c->v_scale; p.oB = V;
     p.ld_row = ld_row; p.ld_head = ld_head; p.err = ctx->d_err;
     long long blocks;
-    shape_of(c->head_dim, p.kinds * c->heads, rows, &p.threads_log2, &p.warps_per_row, &blocks);
+    shape_of(ctx, c->head_dim, p.kinds * c->heads, rows, &p.threads_log2, &p.parts, &blocks);
     TB_CHECK(blocks < (1LL << 31) / KV_WARPS, "tb_kv_read: too many rows");
     const bool e4m3 = c->type == TB_KV_E4M3;
     prof_mark(ctx, "kv_read", 0.0, (double)rows * p.kinds * c->heads * c->head_dim * (e4m3 ? 3 : 4), st);

@@ -5,6 +5,8 @@
 
 namespace tb {
 
+constexpr int kLogitSlice = 4096;         // most columns per CTA: four per thread in four rounds
+
 // Columns of the vocabulary per CTA: a multiple of 32 (a mask word belongs to one CTA) up to 4096.  As many as give every SM
 // four CTAs, so that few rows spread over the chip and many rows do not read their ids more often than needed.
 inline int logit_rules_slice(int rows, int V, int sms) {
@@ -12,7 +14,7 @@ inline int logit_rules_slice(int rows, int V, int sms) {
     long long slices = (want + rows - 1) / rows;
     long long s = (V + slices - 1) / slices;
     s = (s + 31) / 32 * 32;
-    return (int)(s < 512 ? 512 : s > 4096 ? 4096 : s);
+    return (int)(s < 512 ? 512 : s > kLogitSlice ? kLogitSlice : s);
 }
 
 struct LogitRuleArgs {
