@@ -81,8 +81,6 @@ def attend(b, H, seed, max_q=None, max_kv=None, stride=0, check=True, scale=None
     lse = torch.full((b.rows + 3, H), 5.0, device="cuda")
     max_q, max_kv = max_q or max(1, max(b.new)), max(b.kv) if max_kv is None else max_kv
     ws = b.cache.workspace(H, b.rows + 3, max_q, max_kv)
-    if ws is not None:
-        ws.fill_(0xff)                                          # NaN
     b.cache.attend(qd, att[:, :width], b.q_start, b.kv_len, max_q, max_kv, scale=scale, lse=lse, workspace=ws)
     if check:
         from turkce_llm_b200 import lib

@@ -28,53 +28,63 @@ struct PagedAttParams {
     bf16* att; long long ld_att;
     float* lse;                      // [rows, H] or NULL
     float* part_o; float2* part_ml;  // [2 grid][16][hd], [2 grid][16]: results of items that a CTA shares with its neighbours
-    long long* before;               // [seqs + 1]: blocks of one head in front of a sequence
+    unsigned int* arrived;           // [grid], zero between launches: pieces written of the item that begins in a CTA's run and goes on
     int rows, H, group, max_q, max_kv, grid, whole;
     float scale_log2;
     int* err;
 };
 
 // the sequence's first row, number of new rows and number of keys; false where they are outside what the call allows
+__device__ __forceinline__ bool batch_ok(const PagedAttParams& p, int q0, int q1, int kv) {
+    const int n = q1 - q0;
+    return q0 >= 0 && q1 >= q0 && q1 <= p.rows && n <= p.max_q && kv >= 0 && kv <= p.max_kv &&
+           kv <= (long long)p.v.table_ld << p.v.page_shift;
+}
 __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0, int& n, int& kv) {
     q0 = p.q_start[s];
     const int q1 = p.q_start[s + 1];
     kv = p.kv_len[s];
     n = q1 - q0;
-    return q0 >= 0 && q1 >= q0 && q1 <= p.rows && n <= p.max_q && kv >= 0 && kv <= p.max_kv &&
-           kv <= (long long)p.v.table_ld << p.v.page_shift;
+    return batch_ok(p, q0, q1, kv);
 }
 
 // ------------------------------------------------------------------------------- few rows: mma fragments
 // Sequences whose new rows, times the heads that share a key head, are at most 16: single tokens, and a few of them.  What counts
 // here is bytes: an item is one (sequence, key head), its rows are padded to the 16 of a fragment, and the tensor work is still
-// small beside the keys and values that come in.  A CTA of four warps, 16 keys of every block of 64 each, and a fifth one that
-// fills a ring of blocks.  A warp keeps maximum, sum and accumulator of its own keys; they are put together at the item's end.
+// small beside the keys and values that come in.  A CTA of four warps, each with a quarter of the keys of every block, and a fifth one
+// that fills a ring of blocks.  A warp keeps maximum, sum and accumulator of its own keys; they are put together at the item's end.
 //
 // The grid is as many CTAs as the chip holds, and the blocks of all items, laid end to end, are dealt to them in equal runs: the
 // ring goes on from item to item without a pause, and sequences of any lengths keep every SM equally long.  An item that
-// lies in several runs is added up by paged_combine_kernel in the order of the runs.  (One CTA per item and piece of 1024 keys: 47 us
-// for 64 sequences of 400 .. 4096 keys and 6 heads of 64, 35 % of it a tail; pieces of 256 keys: 65 us, a start for each.)
-// Where no sequence has more than PA_WHOLE keys, an item is one CTA's and there is nothing to add.
+// lies in several runs is added up by the CTA that is last with its piece, in the order of the runs.  (One CTA per item and piece of
+// 1024 keys: 47 us for 64 sequences of 400 .. 4096 keys and 6 heads of 64, 35 % of it a tail; pieces of 256 keys: 65 us, a start for
+// each.)  Where no sequence has more than PA_WHOLE keys, an item is one CTA's and there is nothing to add.
 //
 // Fragments without a shuffle: the contraction over the head dimension may take the elements in any order, so lane (r, c) of a
 // key's fragment (r = lane / 4, c = lane % 4) holds elements 16 c .. 16 c + 15 of key r, two 16-byte reads, and the queries lie
 // the same way.  Of a value's rows 2c, 2c + 1, 2c + 8, 2c + 9 it takes elements 8 r .. 8 r + 7, and pairs of two keys are made
 // with byte permutes; accumulator tile i then holds elements 8 (2c) + i and 8 (2c + 1) + i of rows r and r + 8.
+//
+// 8-bit rows of up to 64: as many bytes are twice the keys, and a step of a warp is 32 of them.
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = (PA_WARPS + 1) * 32;
-enum { PA_FIRST = 1, PA_LAST = 2, PA_FINAL = 4, PA_SLOT = 8, PA_END = 16 };
+constexpr int PA_SCAN = 4;               // sequences per lane of one look at the batch
+enum { PA_FIRST = 1, PA_LAST = 2, PA_FINAL = 4, PA_END = 8 };
 
 template <int NH, bool E4M3>
 struct RowsShape {
+    static constexpr int KEYS = paged_keys(NH, E4M3), KW = KEYS / PA_WARPS;      // keys per block and per warp
     static constexpr int ROW_BYTES = E4M3 ? 64 * NH : 128;                   // of one 64-element (8 bits: all) column block
-    static constexpr int BLOCK = PA_KEYS * ROW_BYTES;                        // one column block of 64 keys
+    static constexpr int BLOCK = KEYS * ROW_BYTES;                           // one column block of a block's keys
     static constexpr int TILE = E4M3 ? BLOCK : NH * BLOCK;
-    static constexpr int Q_BYTES = PA_ROWS * 128 * NH;
-    static constexpr int O_SCALE = 2 * TILE, O_Q = O_SCALE + (E4M3 ? 2 * PA_KEYS * 4 : 0), O_WHAT = O_Q + Q_BYTES;
-    static constexpr int STAGE = (O_WHAT + 32 + 1023) / 1024 * 1024;
-    static constexpr int STAGES = E4M3 ? (NH == 1 ? 5 : 3) : (NH == 1 ? 4 : 3);
+    static constexpr int STAGES = NH == 2 ? (E4M3 ? 3 : 2) : (E4M3 ? 2 : 4);
+    static constexpr int Q_BYTES = PA_ROWS * 128 * NH, WHAT = 32, SCALES = E4M3 ? 2 * KEYS * 4 : 0;
     static constexpr int LD = 64 * NH + 4;                                   // floats per row of a warp's result
-    static constexpr int O_OUT = STAGES * STAGE;
+    // ring of keys and values | scales | queries of an item's first block | what a block is | scale parts of a warp | results | barriers
+    static constexpr int STAGE = 2 * TILE;
+    static constexpr int O_SCALE = STAGES * STAGE, O_Q = O_SCALE + STAGES * SCALES, O_WHAT = O_Q + STAGES * Q_BYTES;
+    static constexpr int O_PARTS = O_WHAT + STAGES * WHAT;
+    static constexpr int O_OUT = O_PARTS + (E4M3 ? KEYS * 16 : 0);
     static constexpr int O_BARS = O_OUT + PA_WARPS * PA_ROWS * (LD + 2) * 4;
     static constexpr int SMEM = 1024 + O_BARS + 2 * STAGES * 8 + 16;
     static constexpr int PER_SM = SMEM <= 75 * 1024 ? 3 : SMEM <= 113 * 1024 ? 2 : 1;
@@ -124,12 +134,9 @@ __device__ __forceinline__ bool all_of(bool mine, int barrier, int threads) {
 }
 
 // blocks of one head of a sequence that the kernel for few rows takes
+template <int KEYS>
 __device__ __forceinline__ int row_blocks(const PagedAttParams& p, bool ok, int n, int kv) {
-    return ok && n > 0 && n * p.group <= PA_ROWS ? max(1, (kv + PA_KEYS - 1) / PA_KEYS) : 0;
-}
-__device__ __forceinline__ long long run_length(const PagedAttParams& p, long long total) {
-    const long long per = (total + p.grid - 1) / p.grid;
-    return per < PA_LEAST ? PA_LEAST : per;
+    return ok && n > 0 && n * p.group <= PA_ROWS ? max(1, (kv + KEYS - 1) / KEYS) : 0;
 }
 
 template <int NH, bool E4M3>
@@ -137,12 +144,15 @@ __global__ void __launch_bounds__(PA_THREADS, (RowsShape<NH, E4M3>::PER_SM))
 paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedAttParams p) {
     typedef RowsShape<NH, E4M3> Sh;
     typedef std::integral_constant<bool, E4M3> Kind;
-    constexpr int STAGES = Sh::STAGES;
+    constexpr int STAGES = Sh::STAGES, KEYS = Sh::KEYS, KW = Sh::KW, NT = KW / 8;
+    constexpr int KEYS_LOG2 = KEYS == 128 ? 7 : 6;
+    static_assert(KEYS == 1 << KEYS_LOG2, "");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sh::O_BARS);
     uint64_t* empty = full + STAGES;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + STAGES);
+    volatile int* is_last = abort_flag + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -156,57 +166,68 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     if (warp == PA_WARPS) {
         // ---- producer: finds this CTA's items, and fills the ring with their blocks.  A lane per piece of a page.
         const int heads = p.v.heads, seqs = p.v.seqs;
-        const int piece_shift = min(p.v.page_shift, 6), pieces = PA_KEYS >> piece_shift;      // keys per copy, copies per block
+        const int piece_shift = min(p.v.page_shift, KEYS_LOG2), pieces = KEYS >> piece_shift;   // keys per copy, copies per block
         const int piece_keys = 1 << piece_shift, per_page_shift = p.v.page_shift - piece_shift;
         int s = 0, h = 0, b = 0;              // the next block: of sequence s, head h
-        long long left = 0;                   // blocks of this CTA's run that are still to come
+        long long left = 0, at_block = 0, per = 1;      // blocks of this CTA's run that are still to come; the next one's number; a run
         if (p.whole) {
             s = (int)(blockIdx.x / (unsigned)heads);
             h = (int)(blockIdx.x % (unsigned)heads);
         } else {
-            // all sequences' blocks, a sequence per lane
-            long long total = 0;
-            for (int s0 = 0; s0 < seqs; s0 += 32) {
-                int q0, n, kv, nb = 0;
-                if (s0 + lane < seqs) {
-                    const bool ok = batch_of(p, s0 + lane, q0, n, kv);
-                    if (!ok) atomicExch(p.err, 76);
-                    nb = row_blocks(p, ok, n, kv);
+            // all sequences' blocks: lane i looks at PA_SCAN sequences in a row
+            int nb[PA_SCAN];
+            auto look = [&](int s0, long long& mine) {
+                int q[PA_SCAN + 1], kv[PA_SCAN];
+                const int a = s0 + lane * PA_SCAN;
+#pragma unroll
+                for (int i = 0; i <= PA_SCAN; ++i) q[i] = p.q_start[min(a + i, seqs)];
+#pragma unroll
+                for (int i = 0; i < PA_SCAN; ++i) kv[i] = p.kv_len[min(a + i, seqs - 1)];
+                mine = 0;
+#pragma unroll
+                for (int i = 0; i < PA_SCAN; ++i) {
+                    const bool ok = batch_ok(p, q[i], q[i + 1], kv[i]);
+                    if (!ok && a + i < seqs) atomicExch(p.err, 76);
+                    nb[i] = a + i < seqs ? row_blocks<KEYS>(p, ok, q[i + 1] - q[i], kv[i]) : 0;
+                    mine += nb[i];
                 }
-                long long incl = nb;
+                long long incl = mine;
                 for (int o = 1; o < 32; o <<= 1) {
                     const long long x = __shfl_up_sync(0xffffffffu, incl, o);
                     if (lane >= o) incl += x;
                 }
-                if (blockIdx.x == 0 && s0 + lane < seqs) p.before[s0 + lane] = total + incl - nb;
+                return incl;
+            };
+            long long total = 0, mine, incl = 0;
+            for (int s0 = 0; s0 < seqs; s0 += 32 * PA_SCAN) {
+                incl = look(s0, mine);
                 total += __shfl_sync(0xffffffffu, incl, 31);
             }
-            if (blockIdx.x == 0 && lane == 0) p.before[seqs] = total;
             total *= heads;
-            const long long per = run_length(p, total), first = per * blockIdx.x;
-            left = min(per, total - first);
+            per = max((total + p.grid - 1) / p.grid, (long long)(PA_LEAST >> KEYS_LOG2));
+            at_block = per * blockIdx.x;
+            left = min(per, total - at_block);
             if (left > 0) {
-                long long at = 0;
-                for (int s0 = 0; s0 < seqs; s0 += 32) {
-                    int q0, n, kv, nb = 0;
-                    if (s0 + lane < seqs) {
-                        const bool ok = batch_of(p, s0 + lane, q0, n, kv);
-                        nb = row_blocks(p, ok, n, kv);
-                    }
-                    long long incl = nb;
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-                        if (lane >= o) incl += x;
-                    }
-                    const unsigned ends_behind = __ballot_sync(0xffffffffu, (at + incl) * heads > first);
+                long long before = 0;
+                for (int s0 = 0; s0 < seqs; s0 += 32 * PA_SCAN) {
+                    if (seqs > 32 * PA_SCAN) incl = look(s0, mine);
+                    const unsigned ends_behind = __ballot_sync(0xffffffffu, (before + incl) * heads > at_block);
                     if (ends_behind) {
                         const int who = __ffs(ends_behind) - 1;
-                        const long long rest = first - (at + __shfl_sync(0xffffffffu, incl - nb, who)) * heads;
-                        const int blocks = __shfl_sync(0xffffffffu, nb, who);
-                        s = s0 + who; h = (int)(rest / blocks); b = (int)(rest - (long long)h * blocks);
+                        long long rest = at_block - (before + incl - mine) * heads;      // (of the lane that has it)
+                        int i = 0;
+#pragma unroll
+                        for (int x = 0; x < PA_SCAN - 1; ++x)
+                            if (i == x && rest >= (long long)nb[x] * heads) { rest -= (long long)nb[x] * heads; ++i; }
+                        int blocks = nb[0];
+#pragma unroll
+                        for (int x = 1; x < PA_SCAN; ++x) blocks = i == x ? nb[x] : blocks;
+                        blocks = max(blocks, 1);
+                        h = (int)(rest / blocks); b = (int)(rest - (long long)h * blocks); s = s0 + lane * PA_SCAN + i;
+                        s = __shfl_sync(0xffffffffu, s, who); h = __shfl_sync(0xffffffffu, h, who); b = __shfl_sync(0xffffffffu, b, who);
                         break;
                     }
-                    at += __shfl_sync(0xffffffffu, incl, 31);
+                    before += __shfl_sync(0xffffffffu, incl, 31);
                 }
             }
         }
@@ -217,12 +238,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             ok = __all_sync(0xffffffffu, ok);
             return ok;
         };
-        while (ok && (p.whole ? s < seqs : left > 0)) {
+        while (ok && s < seqs && (p.whole || left > 0)) {
             int q0, n, kv;
             const bool fine = batch_of(p, s, q0, n, kv);
             if (!fine && p.whole && lane == 0) atomicExch(p.err, 76);
-            const int nb = row_blocks(p, fine, n, kv);
-            const int b_end = p.whole ? nb : (int)min((long long)nb, b + left);
+            const int blocks = row_blocks<KEYS>(p, fine, n, kv);
+            const int b_end = p.whole ? blocks : (int)min((long long)blocks, b + left);
             const int* table = p.v.table + (long long)s * p.v.table_ld;
             const int last_piece = (kv + piece_keys - 1) >> piece_shift;
             auto page_at = [&](int piece) -> int {
@@ -235,7 +256,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             // the table is read 32 pieces at a time, one round ahead
             int held = b * pieces, now = 0, next = 0;
             if (b < b_end) { now = page_at(held + lane); next = page_at(held + 32 + lane); }
-            const int flags = p.whole || (b == 0 && b_end == nb) ? PA_FINAL : b == 0 ? PA_SLOT : 0;
+            int c0 = 0, runs = 1;             // the run that the item begins in, and how many it lies in
+            if (!p.whole && b < b_end) {
+                c0 = (int)((at_block - b) / per);
+                runs = (int)((at_block - b + blocks - 1) / per) - c0 + 1;
+            }
             const int b_begin = b;
             for (; b < b_end; ++b) {
                 const int at = b * pieces;
@@ -243,33 +268,33 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
                 const int count = max(0, min(pieces, last_piece - at));      // copies of this block
                 if (!slot_free()) break;
-                uint8_t* st = smem + (i % STAGES) * Sh::STAGE;
-                uint64_t* bar = &full[i % STAGES];
+                const int st = i % STAGES;
+                uint8_t* tile = smem + st * Sh::STAGE;
+                uint64_t* bar = &full[st];
                 const bool first = b == b_begin;
                 if (lane == 0) {
-                    int* what = reinterpret_cast<int*>(st + Sh::O_WHAT);
-                    what[0] = flags | (first ? PA_FIRST : 0) | (b == b_end - 1 ? PA_LAST : 0);
-                    what[1] = b * PA_KEYS; what[2] = q0; what[3] = n; what[4] = kv; what[5] = h;
-                    mbar_expect_tx(bar, (uint32_t)(count * piece_keys * (2 * Sh::TILE / PA_KEYS + (E4M3 ? 8 : 0)) +
-                                                   (first ? n * p.group * p.v.hd * 2 : 0)));
+                    int4* what = reinterpret_cast<int4*>(smem + Sh::O_WHAT + st * Sh::WHAT);
+                    what[0] = make_int4((first ? PA_FIRST : 0) | (b == b_end - 1 ? PA_LAST : 0) | (runs == 1 ? PA_FINAL : 0), b * KEYS, q0, n);
+                    what[1] = make_int4(kv, h, c0, runs);
+                    mbar_expect_tx(bar, (uint32_t)(count * piece_keys * (2 * Sh::TILE / KEYS + (E4M3 ? 8 : 0)) + (first ? n * p.group * p.v.hd * 2 : 0)));
                 }
                 __syncwarp();
                 if (first && lane < n)
-                    bulk_load(st + Sh::O_Q + lane * p.group * p.v.hd * 2, p.Q + (long long)(q0 + lane) * p.ld_q + (long long)h * p.group * p.v.hd,
-                              (uint32_t)(p.group * p.v.hd * 2), bar);
+                    bulk_load(smem + Sh::O_Q + st * Sh::Q_BYTES + lane * p.group * p.v.hd * 2,
+                              p.Q + (long long)(q0 + lane) * p.ld_q + (long long)h * p.group * p.v.hd, (uint32_t)(p.group * p.v.hd * 2), bar);
                 if (lane < count) {
                     const int block = pg * heads + h, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift;
                     const int o = lane << piece_shift;
 #pragma unroll
                     for (int c = 0; c < (E4M3 ? 1 : NH); ++c) {
-                        tma_load_3d(st + c * Sh::BLOCK + o * Sh::ROW_BYTES, &tmK, bar, c * 64, r0, block);
-                        tma_load_3d(st + Sh::TILE + c * Sh::BLOCK + o * Sh::ROW_BYTES, &tmV, bar, c * 64, r0, block);
+                        tma_load_3d(tile + c * Sh::BLOCK + o * Sh::ROW_BYTES, &tmK, bar, c * 64, r0, block);
+                        tma_load_3d(tile + Sh::TILE + c * Sh::BLOCK + o * Sh::ROW_BYTES, &tmV, bar, c * 64, r0, block);
                     }
                     if (E4M3) {
-                        float* sc = reinterpret_cast<float*>(st + Sh::O_SCALE);
+                        float* sc = reinterpret_cast<float*>(smem + Sh::O_SCALE + st * Sh::SCALES);
                         const long long row = ((long long)block << p.v.page_shift) + r0;
                         bulk_load(sc + o, p.ks + row, (uint32_t)piece_keys * 4u, bar);
-                        bulk_load(sc + PA_KEYS + o, p.vs + row, (uint32_t)piece_keys * 4u, bar);
+                        bulk_load(sc + KEYS + o, p.vs + row, (uint32_t)piece_keys * 4u, bar);
                     }
                 }
                 __syncwarp();
@@ -282,14 +307,15 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 if (h >= heads) { h -= heads; ++s; }
             } else {
                 left -= b - b_begin;
-                if (b >= nb) {
+                at_block += b - b_begin;
+                if (b >= blocks) {
                     b = 0;
-                    if (nb == 0 || ++h == heads) { h = 0; ++s; }
+                    if (blocks == 0 || ++h == heads) { h = 0; ++s; }
                 }
             }
         }
         if (ok && slot_free() && lane == 0) {
-            *reinterpret_cast<int*>(smem + (i % STAGES) * Sh::STAGE + Sh::O_WHAT) = PA_END;
+            *reinterpret_cast<int*>(smem + Sh::O_WHAT + (i % STAGES) * Sh::WHAT) = PA_END;
             mbar_arrive(&full[i % STAGES]);
         }
         pdl_launch_dependents_now();
@@ -301,15 +327,17 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const int r = lane >> 2, c = lane & 3;
     float* so = reinterpret_cast<float*>(smem + Sh::O_OUT);
     float2* sml = reinterpret_cast<float2*>(so + PA_WARPS * PA_ROWS * Sh::LD);
+    float4* parts = reinterpret_cast<float4*>(smem + Sh::O_PARTS) + warp * KW;     // (8 bits) of this warp's keys
     // query fragments: elements 16 c .. of rows r and r + 8, head-dimension block by block
     uint32_t qf[NH][4][4];
     float row_factor[2] = {p.scale_log2, p.scale_log2};
     int pos[2] = {0, 0}, first_pos = 0, last_pos = 0, nrows = 0;
     float o[8 * NH][4], m[2], l[2];
     bool ok = true;
-    for (int i = 0;; ++i) {
-        const int st = i % STAGES;
-        if (!mbar_wait(&full[st], (uint32_t)((i / STAGES) & 1), abort_flag)) {
+    int st = 0;
+    uint32_t phase = 0;
+    for (;;) {
+        if (!mbar_wait(&full[st], phase, abort_flag)) {
             if (lane == 0) *abort_flag = 1;
             all_of(false, 1, 128);
             ok = false;
@@ -317,10 +345,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         const uint8_t* sK = smem + st * Sh::STAGE;
         const uint8_t* sV = sK + Sh::TILE;
-        const float* sc = reinterpret_cast<const float*>(sK + Sh::O_SCALE);
-        const int4 what = *reinterpret_cast<const int4*>(sK + Sh::O_WHAT);             // flags, first key, first row, new rows
-        const int2 more = *reinterpret_cast<const int2*>(sK + Sh::O_WHAT + 16);        // keys, head
+        const int4 what = *reinterpret_cast<const int4*>(smem + Sh::O_WHAT + st * Sh::WHAT);           // flags, first key, first row, new rows
         if (what.x & PA_END) { all_of(true, 1, 128); break; }
+        const int4 more = *reinterpret_cast<const int4*>(smem + Sh::O_WHAT + st * Sh::WHAT + 16);      // keys, head, first run, runs
         const int kv = more.x, n = what.w;
         if (what.x & PA_FIRST) {
             nrows = n * p.group;
@@ -329,7 +356,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             for (int x = 0; x < 2; ++x) {
                 const int rr = r + 8 * x;
                 pos[x] = kv - n + min(rr, nrows - 1) / p.group;
-                const uint8_t* q = sK + Sh::O_Q + rr * p.v.hd * 2;
+                const uint8_t* q = smem + Sh::O_Q + st * Sh::Q_BYTES + rr * p.v.hd * 2;
                 uint32_t big = 0u;
 #pragma unroll
                 for (int b = 0; b < NH; ++b)
@@ -341,7 +368,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                         qf[b][2 * g][x] = w.x; qf[b][2 * g][2 + x] = w.y; qf[b][2 * g + 1][x] = w.z; qf[b][2 * g + 1][2 + x] = w.w;
                         if (E4M3) {
                             const uint32_t a = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
-                            big = max(big & 0xffffu, max(a & 0xffffu, a >> 16));
+                            big = max(big, max(a & 0xffffu, a >> 16));
                         }
                     }
                 if (E4M3) {
@@ -368,13 +395,22 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
             for (int e = 0; e < 8 * NH; ++e) { o[e][0] = 0.f; o[e][1] = 0.f; o[e][2] = 0.f; o[e][3] = 0.f; }
         }
-        const int kk = 16 * warp, k0 = what.y + kk;                        // this warp's 16 keys
-        if (k0 <= last_pos) {
-            // ---- scores of two tiles of 8 keys
-            float z[2][4];
-            ScaleParts vs[2][2];
+        const int kk = KW * warp, k0 = what.y + kk;                        // this warp's keys
+        // One step: this warp's keys of the block.  at_edge: some row does not see all of them.
+        auto step = [&](auto at_edge) {
+            constexpr bool edge = decltype(at_edge)::value;
+            if (E4M3) {
+                // a lane per key: what the scales do to scores, probabilities and sums
+                const float* sc = reinterpret_cast<const float*>(smem + Sh::O_SCALE + st * Sh::SCALES) + kk;
+                if (lane < KW) {
+                    const ScaleParts x = scale_parts(sc[KEYS + lane]);
+                    parts[lane] = make_float4(sc[lane], x.exponent, x.part, x.down);
+                }
+                __syncwarp();
+            }
+            float z[NT][4];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < NT; ++t) {
                 z[t][0] = z[t][1] = z[t][2] = z[t][3] = 0.f;
                 const int key = kk + 8 * t + r;
 #pragma unroll
@@ -395,34 +431,32 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
                     for (int e = 0; e < 4; ++e) mma_16816(z[t], qf[b][e], w[2 * e], w[2 * e + 1], Kind());
                 }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
                 if (E4M3) {
                     // the key's scale on the score; the value's scale, but for a factor below 2, in the exponent of the probability
-                    const float2 f = *reinterpret_cast<const float2*>(sc + kk + 8 * t + 2 * c);
-                    const float2 g = *reinterpret_cast<const float2*>(sc + PA_KEYS + kk + 8 * t + 2 * c);
-                    vs[t][0] = scale_parts(g.x); vs[t][1] = scale_parts(g.y);
-                    z[t][0] = fmaf(z[t][0], f.x * row_factor[0], vs[t][0].exponent);
-                    z[t][1] = fmaf(z[t][1], f.y * row_factor[0], vs[t][1].exponent);
-                    z[t][2] = fmaf(z[t][2], f.x * row_factor[1], vs[t][0].exponent);
-                    z[t][3] = fmaf(z[t][3], f.y * row_factor[1], vs[t][1].exponent);
+                    const float4 f = parts[8 * t + 2 * c], g = parts[8 * t + 2 * c + 1];
+                    z[t][0] = fmaf(z[t][0], f.x * row_factor[0], f.y); z[t][1] = fmaf(z[t][1], g.x * row_factor[0], g.y);
+                    z[t][2] = fmaf(z[t][2], f.x * row_factor[1], f.y); z[t][3] = fmaf(z[t][3], g.x * row_factor[1], g.y);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) z[t][e] *= p.scale_log2;
                 }
-            }
-            const bool edge = k0 + 15 > first_pos;                         // some row does not see all of these keys
-            if (edge) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
+                if (edge) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (k0 + 8 * t + 2 * c + (e & 1) > pos[e >> 1]) z[t][e] = -INFINITY;
+                }
             }
             // ---- running maximum and sum
             bool moved = false;
             float alpha[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float mx = fmaxf(fmaxf(z[0][2 * h], z[0][2 * h + 1]), fmaxf(z[1][2 * h], z[1][2 * h + 1]));
+                float mx = fmaxf(z[0][2 * h], z[0][2 * h + 1]);
+#pragma unroll
+                for (int t = 1; t < NT; ++t) mx = fmaxf(mx, fmaxf(z[t][2 * h], z[t][2 * h + 1]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float mn = fmaxf(m[h], mx);
@@ -436,75 +470,91 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
                 for (int t = 0; t < 8 * NH; ++t) { o[t][0] *= alpha[0]; o[t][1] *= alpha[0]; o[t][2] *= alpha[1]; o[t][3] *= alpha[1]; }
             }
-            uint32_t pa[4];
+            uint32_t pa[NT / 2][4];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < NT; ++t) {
+                float4 f = make_float4(0.f, 0.f, 1.f, 1.f), g = f;
+                if (E4M3) { f = parts[8 * t + 2 * c]; g = parts[8 * t + 2 * c + 1]; }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     // (a row that has seen no key yet: its maximum is -infinity, and so are its scores)
-                    const float base = m[h] == -INFINITY ? 0.f : m[h];
-                    const float p0 = ex2_approx(z[t][2 * h] - base), p1 = ex2_approx(z[t][2 * h + 1] - base);
+                    const float base = edge && m[h] == -INFINITY ? 0.f : m[h];
+                    float p0 = ex2_approx(z[t][2 * h] - base), p1 = ex2_approx(z[t][2 * h + 1] - base);
                     if (E4M3) {
                         // (a key that the row does not see may have any scale)
                         const bool no0 = edge && z[t][2 * h] == -INFINITY, no1 = edge && z[t][2 * h + 1] == -INFINITY;
-                        l[h] += (no0 ? 0.f : p0 * vs[t][0].down) + (no1 ? 0.f : p1 * vs[t][1].down);
-                        pa[2 * t + h] = f16_pair(no0 ? 0.f : p0 * vs[t][0].part, no1 ? 0.f : p1 * vs[t][1].part);
+                        l[h] += (no0 ? 0.f : p0 * f.w) + (no1 ? 0.f : p1 * g.w);
+                        p0 = no0 ? 0.f : p0 * f.z;
+                        p1 = no1 ? 0.f : p1 * g.z;
+                        pa[t / 2][2 * (t & 1) + h] = f16_pair(p0, p1);
                     } else {
                         l[h] += p0 + p1;
-                        pa[2 * t + h] = bf16_pair(p0, p1);
+                        pa[t / 2][2 * (t & 1) + h] = bf16_pair(p0, p1);
                     }
                 }
             }
             // ---- values
-            // keys behind position `last` count as zeros; at an edge, only the rows of that position take the product
-            auto values = [&](const uint32_t (&a)[4], int last, auto at_edge) {
+            // at an edge: keys behind position `last` count as zeros, and only the rows of that position take the product
+            auto values = [&](int last) {
 #pragma unroll
-                for (int b = 0; b < NH; ++b) {
-                    uint32_t w[4][4];
+                for (int half = 0; half < NT / 2; ++half) {
+                    uint32_t a[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int key = kk + 2 * c + (j & 1) + 8 * (j >> 1);
-                        const bool seen = !at_edge.value || k0 - kk + key <= last;
-                        if (E4M3) {
-                            uint2 x = *reinterpret_cast<const uint2*>(sV + key * Sh::ROW_BYTES + 64 * b + 8 * r);
-                            if (!seen) x = make_uint2(0u, 0u);
-                            w[j][0] = x.x; w[j][1] = x.y;
-                        } else {
-                            uint4 x = *reinterpret_cast<const uint4*>(sV + b * Sh::BLOCK + key * 128 + ((r ^ (key & 7)) << 4));
-                            if (!seen) x = make_uint4(0u, 0u, 0u, 0u);
-                            w[j][0] = x.x; w[j][1] = x.y; w[j][2] = x.z; w[j][3] = x.w;
+                    for (int j = 0; j < 4; ++j) a[j] = !edge || pos[j & 1] == last ? pa[half][j] : 0u;
+#pragma unroll
+                    for (int b = 0; b < NH; ++b) {
+                        uint32_t w[4][4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int key = kk + 16 * half + 2 * c + (j & 1) + 8 * (j >> 1);
+                            const bool seen = !edge || what.y + key <= last;
+                            if (E4M3) {
+                                uint2 x = *reinterpret_cast<const uint2*>(sV + key * Sh::ROW_BYTES + 64 * b + 8 * r);
+                                if (!seen) x = make_uint2(0u, 0u);
+                                w[j][0] = x.x; w[j][1] = x.y;
+                            } else {
+                                uint4 x = *reinterpret_cast<const uint4*>(sV + b * Sh::BLOCK + key * 128 + ((r ^ (key & 7)) << 4));
+                                if (!seen) x = make_uint4(0u, 0u, 0u, 0u);
+                                w[j][0] = x.x; w[j][1] = x.y; w[j][2] = x.z; w[j][3] = x.w;
+                            }
                         }
-                    }
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        uint32_t b0, b1;
-                        if (E4M3) {
-                            // byte e of two keys side by side
-                            const uint32_t sel = 0x0040u + 0x0011u * (e & 3);
-                            b0 = e4m3_f16(__byte_perm(w[0][e >> 2], w[1][e >> 2], sel));
-                            b1 = e4m3_f16(__byte_perm(w[2][e >> 2], w[3][e >> 2], sel));
-                        } else {
-                            const uint32_t sel = e & 1 ? 0x7632u : 0x5410u;
-                            b0 = __byte_perm(w[0][e >> 1], w[1][e >> 1], sel);
-                            b1 = __byte_perm(w[2][e >> 1], w[3][e >> 1], sel);
-                        }
-                        if (!at_edge.value) {
-                            mma_16816(o[8 * b + e], a, b0, b1, Kind());
-                        } else {
-                            float d[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_16816(d, a, b0, b1, Kind());
-                            if (pos[0] == last) { o[8 * b + e][0] += d[0]; o[8 * b + e][1] += d[1]; }
-                            if (pos[1] == last) { o[8 * b + e][2] += d[2]; o[8 * b + e][3] += d[3]; }
+                        for (int e = 0; e < 8; ++e) {
+                            uint32_t b0, b1;
+                            if (E4M3) {
+                                // byte e of two keys side by side
+                                const uint32_t sel = 0x0040u + 0x0011u * (e & 3);
+                                b0 = e4m3_f16(__byte_perm(w[0][e >> 2], w[1][e >> 2], sel));
+                                b1 = e4m3_f16(__byte_perm(w[2][e >> 2], w[3][e >> 2], sel));
+                            } else {
+                                const uint32_t sel = e & 1 ? 0x7632u : 0x5410u;
+                                b0 = __byte_perm(w[0][e >> 1], w[1][e >> 1], sel);
+                                b1 = __byte_perm(w[2][e >> 1], w[3][e >> 1], sel);
+                            }
+                            if (!edge) {
+                                mma_16816(o[8 * b + e], a, b0, b1, Kind());
+                            } else {
+                                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma_16816(d, a, b0, b1, Kind());
+                                if (pos[0] == last) { o[8 * b + e][0] += d[0]; o[8 * b + e][1] += d[1]; }
+                                if (pos[1] == last) { o[8 * b + e][2] += d[2]; o[8 * b + e][3] += d[3]; }
+                            }
                         }
                     }
                 }
             };
-            if (!edge) values(pa, 0, std::false_type());
+            if (!edge) values(0);
             else       // token by token: what a token does not see must not reach it, not even as 0 * infinity
-                for (int last = first_pos; last <= last_pos; ++last) values(pa, last, std::true_type());
+#pragma unroll 1
+                for (int last = max(first_pos, 0); last <= last_pos; ++last) values(last);
+        };
+        if (k0 <= last_pos) {
+            if (k0 + KW - 1 > first_pos) step(std::true_type());
+            else step(std::false_type());
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
+        if (++st == STAGES) { st = 0; phase ^= 1u; }
         if (!(what.x & PA_LAST)) continue;
 
         // ---- the item's end: the four warps' results, [warp][16 rows][LD] floats, maxima and sums behind
@@ -525,41 +575,94 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             if (c == 0) sml[warp * PA_ROWS + r + 8 * h] = make_float2(m[h], l[h]);
         }
         if (!all_of(true, 1, 128)) { ok = false; break; }
-        const int chunks = p.v.hd >> 3;                                    // eight elements per thread
-        for (int x = threadIdx.x; x < nrows * chunks; x += PA_WARPS * 32) {
-            const int rr = x / chunks, e = (x - rr * chunks) * 8;
-            float M = -INFINITY, L = 0.f;
+        const int chunks = p.v.hd >> 3, points = nrows * chunks;           // eight elements per thread
+        auto finish = [&](int rr, int e, float M, float L, const float (&acc)[8]) {
+            const int tok = rr / p.group, hq = more.y * p.group + (rr - tok * p.group), row = what.z + tok;
+            const bool none = kv - n + tok < 0;                            // a row without a key
+            const float inv = none ? 0.f : 1.0f / L;
+            *reinterpret_cast<uint4*>(p.att + (long long)row * p.ld_att + (long long)hq * p.v.hd + e) =
+                make_uint4(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv),
+                           bf16_pair(acc[4] * inv, acc[5] * inv), bf16_pair(acc[6] * inv, acc[7] * inv));
+            if (p.lse && e == 0) p.lse[(long long)row * p.H + hq] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+        };
+        auto add = [](float& M, float& L, float (&acc)[8], float2 ml, const float4& a, const float4& d) {
+            if (ml.y == 0.f) return;                                       // (no key of this part was visible)
+            const float mn = L == 0.f ? ml.x : fmaxf(M, ml.x);
+            const float f = L == 0.f ? 0.f : ex2_approx(M - mn), g = ex2_approx(ml.x - mn);
+            L = L * f + ml.y * g;
+            M = mn;
+            const float x[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
 #pragma unroll
-            for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, sml[w * PA_ROWS + rr].x);
-            float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 8; ++i) acc[i] = (f == 0.f ? 0.f : acc[i] * f) + x[i] * g;
+        };
+        for (int x = threadIdx.x; x < points; x += PA_WARPS * 32) {
+            const int rr = x / chunks, e = (x - rr * chunks) * 8;
+            float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < PA_WARPS; ++w) {
-                const float2 ml = sml[w * PA_ROWS + rr];
-                if (ml.y == 0.f) continue;                                 // (no key of this warp's was visible)
-                const float f = ex2_approx(ml.x - M);
-                L += ml.y * f;
                 const float4* src = reinterpret_cast<const float4*>(so + (w * PA_ROWS + rr) * Sh::LD + e);
-                const float4 a = src[0], d = src[1];
-                acc[0] += a.x * f; acc[1] += a.y * f; acc[2] += a.z * f; acc[3] += a.w * f;
-                acc[4] += d.x * f; acc[5] += d.y * f; acc[6] += d.z * f; acc[7] += d.w * f;
+                add(M, L, acc, sml[w * PA_ROWS + rr], src[0], src[1]);
             }
-            const int tok = rr / p.group, hq = more.y * p.group + (rr - tok * p.group), row = what.z + tok;
             if (what.x & PA_FINAL) {
-                const bool none = kv - n + tok < 0;                        // a row without a key
-                const float inv = none ? 0.f : 1.0f / L;
-                *reinterpret_cast<uint4*>(p.att + (long long)row * p.ld_att + (long long)hq * p.v.hd + e) =
-                    make_uint4(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv),
-                               bf16_pair(acc[4] * inv, acc[5] * inv), bf16_pair(acc[6] * inv, acc[7] * inv));
-                if (p.lse && e == 0) p.lse[(long long)row * p.H + hq] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+                finish(rr, e, M, L, acc);
             } else {
-                const int slot = (2 * blockIdx.x + (what.x & PA_SLOT ? 1 : 0)) * PA_ROWS + rr;
+                const int slot = (2 * blockIdx.x + ((int)blockIdx.x == more.z ? 1 : 0)) * PA_ROWS + rr;
                 float4* dst = reinterpret_cast<float4*>(p.part_o + (long long)slot * p.v.hd + e);
-                dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-                if (e == 0) p.part_ml[slot] = make_float2(M, L);
+                __stcg(dst, make_float4(acc[0], acc[1], acc[2], acc[3]));
+                __stcg(dst + 1, make_float4(acc[4], acc[5], acc[6], acc[7]));
+                if (e == 0) __stcg(p.part_ml + slot, make_float2(M, L));
             }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");                     // the buffer is read
+        if (what.x & PA_FINAL) {
+            asm volatile("bar.sync 1, 128;" ::: "memory");                 // the buffer is read
+            continue;
+        }
+        // ---- an item of several runs: whoever is last with its piece adds them, in the order of the runs.  The run that the item begins
+        // in has it in slot 1 of its CTA, the others in slot 0.
+        __threadfence();
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (threadIdx.x == 0) {
+            const unsigned int before = atomicAdd(p.arrived + more.z, 1u);
+            *is_last = before == (unsigned int)more.w - 1u ? 1 : 0;
+            if (*is_last) p.arrived[more.z] = 0u;                          // ready for the next launch
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (!*is_last) continue;
+        __threadfence();
+        // threads in groups, each with every groups-th piece; then the groups' results
+        const int groups = points <= 128 ? 128 / points : 1;
+        for (int x0 = threadIdx.x; x0 < (points <= 128 ? groups * points : points); x0 += PA_WARPS * 32) {
+            const int g = points <= 128 ? x0 / points : 0, x = x0 - g * points, rr = x / chunks, e = (x - rr * chunks) * 8;
+            float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+            for (int i = g; i < more.w; i += groups) {
+                const int slot = (2 * (more.z + i) + (i == 0 ? 1 : 0)) * PA_ROWS + rr;
+                const float4* src = reinterpret_cast<const float4*>(p.part_o + (long long)slot * p.v.hd + e);
+                add(M, L, acc, __ldcg(p.part_ml + slot), __ldcg(src), __ldcg(src + 1));
+            }
+            if (groups == 1) {
+                finish(rr, e, M, L, acc);
+            } else {
+                float* to = so + x0 * 10;
+                to[0] = M; to[1] = L;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) to[2 + i] = acc[i];
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (groups > 1) {
+            for (int x = threadIdx.x; x < points; x += PA_WARPS * 32) {
+                const int rr = x / chunks, e = (x - rr * chunks) * 8;
+                float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                for (int g = 0; g < groups; ++g) {
+                    const float* from = so + (g * points + x) * 10;
+                    add(M, L, acc, make_float2(from[0], from[1]), make_float4(from[2], from[3], from[4], from[5]),
+                        make_float4(from[6], from[7], from[8], from[9]));
+                }
+                finish(rr, e, M, L, acc);
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
     }
     if (!ok) {
         // (what was asked for may still arrive: the block keeps its memory a little longer)
@@ -568,57 +671,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
 }
 
-// ------------------------------------------------------------------------------- items of several runs, in the order of the runs
-// A warp per (row, head); items that lie in one run are final already.  The run that an item starts in has it as its last one
-// (slot 1 of that CTA), the others as their first (slot 0).
-constexpr int PC_WARPS = 8;
-__global__ void __launch_bounds__(PC_WARPS * 32)
-paged_combine_kernel(const PagedAttParams p) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const long long at = (long long)blockIdx.x * PC_WARPS + (threadIdx.x >> 5);
-    if (at >= (long long)p.rows * p.H) return;
-    const int row = (int)(at / p.H), hq = (int)(at - (long long)row * p.H), h = hq / p.group;
-    const int s = sequence_of(p.q_start, p.v.seqs, row);
-    if (s < 0) return;
-    int q0, n, kv;
-    const bool fine = batch_of(p, s, q0, n, kv);
-    const int nb = row_blocks(p, fine, n, kv);
-    if (nb == 0 || row >= q0 + n) return;
-    const long long per = run_length(p, p.before[p.v.seqs] * p.v.heads), first = p.before[s] * p.v.heads + (long long)h * nb;
-    const int c0 = (int)(first / per), c1 = (int)((first + nb - 1) / per);
-    if (c0 == c1) return;
-    const int rr = (row - q0) * p.group + hq - h * p.group;
-    auto slot = [&](int c) { return (2 * c + (c == c0 ? 1 : 0)) * PA_ROWS + rr; };
-    float M = -INFINITY, L = 0.f;
-    for (int c = c0; c <= c1; ++c) M = fmaxf(M, p.part_ml[slot(c)].x);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const int e = lane * 4;
-    for (int c = c0; c <= c1; ++c) {
-        const float2 ml = p.part_ml[slot(c)];
-        if (ml.y == 0.f) continue;
-        const float f = ex2_approx(ml.x - M);
-        L += ml.y * f;
-        if (e < p.v.hd) {
-            const float4 a = *reinterpret_cast<const float4*>(p.part_o + (long long)slot(c) * p.v.hd + e);
-            acc[0] += a.x * f; acc[1] += a.y * f; acc[2] += a.z * f; acc[3] += a.w * f;
-        }
-    }
-    const bool none = kv - n + row - q0 < 0;
-    const float inv = none ? 0.f : 1.0f / L;
-    if (e < p.v.hd)
-        *reinterpret_cast<uint2*>(p.att + (long long)row * p.ld_att + (long long)hq * p.v.hd + e) =
-            make_uint2(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv));
-    if (p.lse && lane == 0) p.lse[at] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-}
-
 template <int NH, bool E4M3>
 int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cudaStream_t st) {
     typedef RowsShape<NH, E4M3> Sh;
     static_assert(Sh::PER_SM == paged_per_sm(NH, E4M3), "the plan counts on as many CTAs per SM");
     CUtensorMap tmK, tmV;
-    const int box_rows = std::min(c->page_size, PA_KEYS);
+    const int box_rows = std::min(c->page_size, Sh::KEYS);
     TB_TRY(make_cache_map(&tmK, c->K, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
     TB_TRY(make_cache_map(&tmV, c->V, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
     static bool attr_set[64] = {false};
@@ -1098,6 +1156,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         int reference = 0;
         float f_next = 0.f, f = 0.f;                                        // the factor of this key's value, of the next block and of this one
         bool fin_next = true, fin = true;
+        // a row's 16-byte pieces in an order that differs from thread to thread: eight of them read 128 different bytes of banks
+        auto piece = [&](int x) { return NH == 2 ? (x + t) & 7 : (x + (t >> 1)) & 3; };
         auto keys = [&](int j) -> bool {
             const int st = j & 1;
             ok = ok && mbar_wait(&raw_full[0], (uint32_t)(j & 1), abort_flag);
@@ -1125,11 +1185,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
             for (int c = 0; c < NH; ++c)
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(rk + 64 * c + 16 * d);
-                    *reinterpret_cast<uint4*>(row + c * PT_TILE + (((2 * d) ^ (t & 7)) << 4)) =
+                for (int x = 0; x < 4; ++x) {
+                    const int y = piece(4 * c + x), d = y & 3;
+                    uint8_t* to = row + (y >> 2) * PT_TILE;
+                    const uint4 w = *reinterpret_cast<const uint4*>(rk + 16 * y);
+                    *reinterpret_cast<uint4*>(to + (((2 * d) ^ (t & 7)) << 4)) =
                         make_uint4(e4m3_f16(w.x), e4m3_f16(w.x >> 16), e4m3_f16(w.y), e4m3_f16(w.y >> 16));
-                    *reinterpret_cast<uint4*>(row + c * PT_TILE + (((2 * d + 1) ^ (t & 7)) << 4)) =
+                    *reinterpret_cast<uint4*>(to + (((2 * d + 1) ^ (t & 7)) << 4)) =
                         make_uint4(e4m3_f16(w.z), e4m3_f16(w.z >> 16), e4m3_f16(w.w), e4m3_f16(w.w >> 16));
                 }
             fence_proxy_async();
@@ -1167,8 +1229,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
             for (int c = 0; c < NH; ++c)
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    uint4 w = *reinterpret_cast<const uint4*>(rv + 64 * c + 16 * d);
+                for (int x = 0; x < 4; ++x) {
+                    const int y = piece(4 * c + x), d = y & 3;
+                    uint8_t* to = row + (y >> 2) * PT_TILE;
+                    uint4 w = *reinterpret_cast<const uint4*>(rv + 16 * y);
                     if (zero) w = make_uint4(0u, 0u, 0u, 0u);
                     if (bad) {                                              // NaN codes to zero
                         w.x &= ~((nan_codes(w.x) >> 7) * 255u); w.y &= ~((nan_codes(w.y) >> 7) * 255u);
@@ -1177,8 +1241,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     uint32_t u[8] = {w.x, w.x >> 16, w.y, w.y >> 16, w.z, w.z >> 16, w.w, w.w >> 16};
 #pragma unroll
                     for (int i = 0; i < 8; ++i) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(u[i]) : "r"(e4m3_f16(u[i])), "r"(f2));
-                    *reinterpret_cast<uint4*>(row + c * PT_TILE + (((2 * d) ^ (t & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
-                    *reinterpret_cast<uint4*>(row + c * PT_TILE + (((2 * d + 1) ^ (t & 7)) << 4)) = make_uint4(u[4], u[5], u[6], u[7]);
+                    *reinterpret_cast<uint4*>(to + (((2 * d) ^ (t & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+                    *reinterpret_cast<uint4*>(to + (((2 * d + 1) ^ (t & 7)) << 4)) = make_uint4(u[4], u[5], u[6], u[7]);
                 }
             fence_proxy_async();
             __syncwarp();
@@ -1233,9 +1297,9 @@ int launch_attention_paged(DeviceCtx* ctx, const TbKvCache* c, const int* q_star
     p.v = paged_view(c);
     p.q_start = q_start; p.kv_len = kv_len; p.Q = Q; p.ld_q = ld_q; p.ks = c->k_scale; p.vs = c->v_scale;
     p.att = att; p.ld_att = ld_att; p.lse = lse;
-    p.part_o = static_cast<float*>(ws);
+    p.part_o = static_cast<float*>(ws) + round_up(pl.grid, 4);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + 2LL * pl.grid * PA_ROWS * c->head_dim);
-    p.before = reinterpret_cast<long long*>(p.part_ml + 2LL * pl.grid * PA_ROWS);
+    p.arrived = static_cast<unsigned int*>(ws);
     p.rows = rows; p.H = H; p.group = group; p.max_q = max_q; p.max_kv = max_kv; p.grid = pl.grid; p.whole = pl.whole ? 1 : 0;
     p.scale_log2 = scale * 1.4426950408889634f; p.err = ctx->d_err;
     const bool wide = c->head_dim > 64;
@@ -1245,13 +1309,6 @@ int launch_attention_paged(DeviceCtx* ctx, const TbKvCache* c, const int* q_star
     }
     if (c->type == TB_KV_E4M3) TB_TRY(wide ? (launch_rows<2, true>(ctx, c, p, st)) : (launch_rows<1, true>(ctx, c, p, st)));
     else TB_TRY(wide ? (launch_rows<2, false>(ctx, c, p, st)) : (launch_rows<1, false>(ctx, c, p, st)));
-    if (!pl.whole) {
-        const long long blocks = ((long long)rows * H + PC_WARPS - 1) / PC_WARPS;
-        prof_mark(ctx, "paged_combine", 0.0, 0.0, st);
-        TB_CUDA(launch_kernel(paged_combine_kernel, dim3((unsigned)blocks), dim3(PC_WARPS * 32), 0, st, p));
-        ctx->launches++;
-        prof_close(ctx, st);
-    }
     return 0;
 }
 

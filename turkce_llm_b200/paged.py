@@ -96,7 +96,7 @@ class PagedCache:
         lib.init(self.device.index)
         n = self._lib.tb_attention_paged_workspace(self._ref, rows, q_heads, max_q, max_kv)
         lib.check(-1 if n < 0 else 0)
-        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        return torch.zeros(n, dtype=torch.uint8, device=self.device) if n else None
 
     def attend(self, q, att, q_start, kv_len, max_q, max_kv, scale=None, lse=None, workspace=None):
         """att = causal attention of q over the cache (both bfloat16 [rows, query heads * head_dim]); lse: optional float32
