@@ -692,6 +692,7 @@ int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cud
 }
 
 // ------------------------------------------------------------------------------- chunks: tcgen05
+// (constants of the tiles: paged_plan.h)
 // CTA = one tile of 128 query rows of a sequence: 128 / group tokens with the heads that share a key head side by side, so that
 // every key and value that comes in is used by all of them.  The roles are those of attention_fwd_kernel: a producer warp, one that
 // issues the products, and two groups of four softmax warps (thread = query row) that take the half blocks of 64 keys in turn,
@@ -703,7 +704,6 @@ int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cud
 //  * 8-bit rows: four more warps turn codes into f16 tiles, a key per thread.  A value's scale goes into its tile against the largest
 //    scale so far (a power of two, which the accumulators follow as they follow the maximum): 11 bits of every value whose scale is
 //    within 2^-21 of the largest, and an absolute error below 2^-31 of the largest value behind that.
-constexpr int PT_ROWS = 128, PT_KEYS = 128;
 constexpr int PT_TILE = 128 * 128;                      // bytes of a [128][64] 16-bit tile
 
 template <int NH, bool E4M3>
@@ -722,10 +722,110 @@ struct ChunkShape {
     static constexpr int TMEM = NH == 1 ? 256 : 512;
 };
 
+// A piece of a tile's keys, [blocks from, to): what one CTA does.  first, pieces: the tile's pieces are units first .. first + pieces - 1.
+struct ChunkUnit { int s, head, tile, from, to, first, pieces, unused; };
+
 struct PagedChunkParams {
     PagedAttParams a;
     int tokens, tiles;                // tokens per tile; tiles of max_q
+    int planned;                      // units come from paged_plan_kernel; else a CTA per tile
+    int most_units, slots;            // room for units; CTAs that the chip holds
+    int* count;                       // units there are
+    unsigned int* arrived;            // [most_units]: pieces written, by the tile's first unit
+    int* bad;                         // [most_units]: a piece has left out a value that is not finite
+    ChunkUnit* units;
+    float2* part_ml;                  // [most_units][128]
+    float4* part_o;                   // [most_units][NH 64 / 4][128]: a row per thread side by side
 };
+
+// blocks of keys that a tile's last token sees (at least one: a tile of rows without a key)
+__device__ __forceinline__ int tile_blocks(int n, int kv, int tile, int tokens) {
+    const int last = kv - n + min(n, (tile + 1) * tokens) - 1;
+    return last >= 0 ? last / PT_KEYS + 1 : 1;
+}
+
+// How few tiles are cut into pieces: by the number of pieces of the longest one for which (rounds of CTAs) * (blocks of a piece and what a
+// piece costs beside them) is least.  One block of threads, some microseconds; where there are tiles enough (the host's bound), they are
+// not cut and this does not run.
+constexpr int PL_THREADS = 512, PL_TILES = 1024;
+__global__ void __launch_bounds__(PL_THREADS)
+paged_plan_kernel(const PagedChunkParams pp) {
+    __shared__ int seq[PL_TILES], idx[PL_TILES], nb[PL_TILES], off[PL_TILES];
+    __shared__ int count, longest, best_cap, cost[PL_THREADS / 32], caps[PL_THREADS / 32], total;
+    const PagedAttParams& p = pp.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) { count = 0; longest = 1; total = 0; }
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
+    // ---- the tiles of one head, in the order of the sequences
+    for (int s0 = 0; s0 < p.v.seqs; s0 += 32) {
+        if (warp != 0) break;
+        int q0, n = 0, kv = 0, tiles = 0;
+        if (s0 + lane < p.v.seqs && batch_of(p, s0 + lane, q0, n, kv) && n * p.group > PA_ROWS) tiles = (n + pp.tokens - 1) / pp.tokens;
+        int incl = tiles;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        const int at = count + incl - tiles;
+        for (int t = 0; t < tiles && at + t < PL_TILES; ++t) { seq[at + t] = s0 + lane; idx[at + t] = t; nb[at + t] = tile_blocks(n, kv, t, pp.tokens); }
+        if (tiles > 0) atomicMax(&longest, tile_blocks(n, kv, tiles - 1, pp.tokens));
+        __syncwarp();
+        if (lane == 31) count += incl;
+        __syncwarp();
+    }
+    __syncthreads();
+    const int tiles = min(count, PL_TILES);                  // (no more than the host's bound, which is below)
+    // ---- a warp per number of pieces
+    {
+        const int pieces = warp < 8 ? warp + 1 : (warp - 5) * 4;      // 1 .. 8, 12, 16, .. 40
+        const int cap = (longest + pieces - 1) / pieces;
+        int units = 0;
+        for (int t = lane; t < tiles; t += 32) units += (nb[t] + cap - 1) / cap;
+        units = __reduce_add_sync(0xffffffffu, units) * p.v.heads;
+        if (lane == 0) {
+            caps[warp] = cap;
+            // (three blocks: the start of a piece, its result to memory and back)
+            cost[warp] = (pieces == 1 || units <= pp.most_units) ? (units + pp.slots - 1) / pp.slots * (cap + 3) : 0x7fffffff;
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int w = 0;
+        for (int i = 1; i < PL_THREADS / 32; ++i) if (cost[i] < cost[w]) w = i;
+        best_cap = caps[w];
+    }
+    __syncthreads();
+    const int cap = best_cap;
+    if (warp == 0) {
+        int before = 0;
+        for (int t0 = 0; t0 < tiles; t0 += 32) {
+            const int pieces = t0 + lane < tiles ? (nb[t0 + lane] + cap - 1) / cap * p.v.heads : 0;
+            int incl = pieces;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += x;
+            }
+            if (t0 + lane < tiles) off[t0 + lane] = before + incl - pieces;
+            before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) { total = min(before, pp.most_units); *pp.count = total; }
+    }
+    __syncthreads();
+    for (int t = warp; t < tiles; t += PL_THREADS / 32) {
+        const int pieces = (nb[t] + cap - 1) / cap, per = (nb[t] + pieces - 1) / pieces;
+        for (int x = lane; x < pieces * p.v.heads; x += 32) {
+            const int head = x / pieces, i = x - head * pieces, u = off[t] + x;
+            if (u >= pp.most_units) continue;
+            ChunkUnit c;
+            c.s = seq[t]; c.head = head; c.tile = idx[t]; c.from = min(i * per, nb[t]); c.to = min((i + 1) * per, nb[t]);
+            c.first = u - i; c.pieces = pieces; c.unused = 0;
+            pp.units[u] = c;
+            pp.arrived[u] = 0u;
+        }
+    }
+}
 
 __device__ __forceinline__ bool not_finite_16(uint32_t two) {            // either bf16 of a pair
     return (two & 0x7f80u) == 0x7f80u || (two & 0x7f800000u) == 0x7f800000u;
@@ -781,19 +881,29 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* bad_value = abort_flag + 1;                              // a value that is not finite has been set to zero
     volatile int* v_exponent = abort_flag + 2;                             // (8 bits) the last block's reference
-    float* v_moved = reinterpret_cast<float*>(tmem_slot + 4);              // (8 bits) [4]: 2^(reference before - reference) of a block
-    uint32_t* warp_most = tmem_slot + 8;                                   // (8 bits) [2][4]
+    volatile int* is_last = abort_flag + 3;                                // this CTA was the last with its piece of a tile
+    float* v_moved = reinterpret_cast<float*>(tmem_slot + 6);              // (8 bits) [4]: 2^(reference before - reference) of a block
+    uint32_t* warp_most = tmem_slot + 10;                                  // (8 bits) [2][4]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.x, s = blockIdx.z, tile = pp.tiles - 1 - (int)blockIdx.y;
     pdl_wait();
+    int s, head, tile, from = 0, to = 0x7fffffff, pieces = 1, first_unit = 0;
+    if (pp.planned) {
+        if ((int)blockIdx.x >= *pp.count) return;
+        const int4* u = reinterpret_cast<const int4*>(pp.units + blockIdx.x);
+        const int4 a = u[0], b = u[1];
+        s = a.x; head = a.y; tile = a.z; from = a.w; to = b.x; first_unit = b.y; pieces = b.z;
+    } else {
+        // the heaviest tiles of all sequences first
+        s = (int)(blockIdx.x / (unsigned)p.v.heads); head = (int)(blockIdx.x % (unsigned)p.v.heads); tile = pp.tiles - 1 - (int)blockIdx.y;
+    }
     int q0, n, kv;
     if (!batch_of(p, s, q0, n, kv)) return;                                // (paged_rows_kernel reports it)
     const int tok0 = tile * pp.tokens;
     if (n * p.group <= PA_ROWS || tok0 >= n) return;
     const int tokens = min(pp.tokens, n - tok0);
     const int first_pos = kv - n + tok0, last_pos = first_pos + tokens - 1;
-    const int nkv = last_pos >= 0 ? last_pos / PT_KEYS + 1 : 0;            // blocks of keys
+    const int nkv = min(to, last_pos >= 0 ? last_pos / PT_KEYS + 1 : 0) - from;      // blocks of keys, from block `from` on
     const int edge0 = max(0, first_pos + 1) / PT_KEYS;                     // the first block with a key that some row does not see
 
     if (threadIdx.x == 0) {
@@ -816,7 +926,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 
     if (warp == 0) {
         // ---- producer: a lane per piece of a page
-        const int piece_shift = min(p.v.page_shift, 7), pieces = PT_KEYS >> piece_shift, piece_keys = 1 << piece_shift;
+        const int piece_shift = min(p.v.page_shift, 7), page_pieces = PT_KEYS >> piece_shift, piece_keys = 1 << piece_shift;
         const int per_page_shift = p.v.page_shift - piece_shift;
         const int* table = p.v.table + (long long)s * p.v.table_ld;
         const int last_piece = (last_pos + piece_keys) >> piece_shift;
@@ -832,12 +942,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             mbar_expect_tx(q_full, (uint32_t)(NH * pp.tokens * p.group * 128));
             for (int c = 0; c < NH; ++c) tma_load_3d(sQ + c * PT_TILE, &tmQ, q_full, c * 64, head * p.group, q0 + tok0);
         }
-        int held = 0, now = nkv > 0 ? page_at(lane) : 0, next = nkv > 0 ? page_at(32 + lane) : 0, landed = 0;
+        const int piece0 = from * page_pieces;
+        int held = piece0, now = nkv > 0 ? page_at(piece0 + lane) : 0, next = nkv > 0 ? page_at(piece0 + 32 + lane) : 0, landed = 0;
         for (int j = 0; j < nkv && ok; ++j) {
-            const int at = j * pieces;
+            const int at = piece0 + j * page_pieces;
             if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
             const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
-            const int count = min(pieces, last_piece - at);
+            const int count = min(page_pieces, last_piece - at);
             const int block = pg * p.v.heads + head, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift, o = lane << piece_shift;
             const int st = j & 1;
             if (!E4M3) {
@@ -852,7 +963,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 ok = mbar_wait(&v_empty[vst], (uint32_t)((j / VST) & 1) ^ 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                const bool edge = j >= edge0;
+                const bool edge = from + j >= edge0;
                 uint64_t* bar = edge ? v_land : &v_full[vst];
                 uint8_t* tile_v = sV + vst * NH * PT_TILE;
                 if (lane == 0) mbar_expect_tx(bar, (uint32_t)(count * piece_keys * 128 * NH));
@@ -864,7 +975,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     ++landed;
-                    const int seen = last_pos + 1 - j * PT_KEYS;           // rows of the tile that some query sees
+                    const int seen = last_pos + 1 - (from + j) * PT_KEYS;           // rows of the tile that some query sees
                     bool bad = false;
                     for (int c = 0; c < NH; ++c)
 #pragma unroll 2
@@ -990,8 +1101,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free[b]);
-            const bool edge = j >= edge0;
-            const int lim = edge ? pos - j * PT_KEYS - b * 64 : 64;         // columns e <= lim are allowed
+            const bool edge = from + j >= edge0;
+            const int lim = edge ? pos - (from + j) * PT_KEYS - b * 64 : 64;         // columns e <= lim are allowed
             float mx = -INFINITY;
             if (edge) {
 #pragma unroll
@@ -1068,28 +1179,96 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         float2* stat = reinterpret_cast<float2*>(sP);
         if (ok) stat[b * PT_ROWS + r] = make_float2(m, l);
         asm volatile("bar.sync 1, 256;" ::: "memory");
+        const bool none = pos < 0;                                          // a row without a key
+        float M = -INFINITY, L = 0.f, w0 = 0.f, w1 = 0.f;
+        int last = 1;                                                       // this CTA has the tile's result
         if (ok) {
-            const bool none = pos < 0;                                      // a row without a key
             const float2 s0 = stat[r], s1 = stat[PT_ROWS + r];
-            const float M = fmaxf(s0.x, s1.x);
+            M = fmaxf(s0.x, s1.x);
             const float e0 = s0.y == 0.f ? 0.f : ex2_approx(s0.x - M), e1 = s1.y == 0.f ? 0.f : ex2_approx(s1.x - M);
-            const float lt = s0.y * e0 + s1.y * e1;
-            float inv = none ? 0.f : 1.0f / lt;
+            L = s0.y * e0 + s1.y * e1;
             const float unit = E4M3 ? exp2f((float)(*v_exponent - 127 - 6)) : 1.f;
-            const float w0 = e0 * inv * unit, w1 = e1 * inv * unit;
+            w0 = e0 * unit; w1 = e1 * unit;
+        }
+        tc_fence_after();
+        // columns 64 c + 32 b .. of this row, against M
+        auto own = [&](int c) {
+            if (nkv > 0) {
+                tmem_ld32(tO + lane_base + (uint32_t)(64 * c + 32 * b), v[0]);
+                tmem_ld32(tO + lane_base + (uint32_t)(64 * NH + 64 * c + 32 * b), v[1]);
+                tmem_ld_wait();
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                v[0][e] = __float_as_uint((w0 == 0.f ? 0.f : __uint_as_float(v[0][e]) * w0) + (w1 == 0.f ? 0.f : __uint_as_float(v[1][e]) * w1));
+        };
+        if (pieces > 1) {
+            // this piece's result to memory, a float4 of every row side by side; whoever is last adds them in their order
+            if (ok) {
+                float4* to16 = pp.part_o + ((long long)blockIdx.x * (16 * NH)) * PT_ROWS + r;
+#pragma unroll 1
+                for (int c = 0; c < NH; ++c) {
+                    own(c);
+#pragma unroll
+                    for (int d = 0; d < 8; ++d)
+                        __stcg(to16 + (16 * c + 8 * b + d) * PT_ROWS, make_float4(__uint_as_float(v[0][4 * d]), __uint_as_float(v[0][4 * d + 1]),
+                                                                                  __uint_as_float(v[0][4 * d + 2]), __uint_as_float(v[0][4 * d + 3])));
+                }
+                if (b == 0) __stcg(pp.part_ml + (long long)blockIdx.x * PT_ROWS + r, make_float2(M, L));
+                if (warp == 2 && lane == 0) pp.bad[blockIdx.x] = *bad_value;
+                __threadfence();
+            }
+            if (all_of(ok, 1, 256)) {
+                if (warp == 2 && lane == 0) *is_last = atomicAdd(pp.arrived + first_unit, 1u) == (unsigned int)pieces - 1u ? 1 : 0;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                last = *is_last;
+            } else {
+                ok = false;
+            }
+            if (ok && last) {
+                __threadfence();
+                M = -INFINITY;
+                L = 0.f;
+                bool any = false;
+                for (int i = 0; i < pieces; ++i) {
+                    const float2 ml = __ldcg(pp.part_ml + (long long)(first_unit + i) * PT_ROWS + r);
+                    if (__ldcg(pp.bad + first_unit + i)) any = true;
+                    if (ml.y == 0.f) continue;
+                    const float mn = L == 0.f ? ml.x : fmaxf(M, ml.x);
+                    L = (L == 0.f ? 0.f : L * ex2_approx(M - mn)) + ml.y * ex2_approx(ml.x - mn);
+                    M = mn;
+                }
+                if (any) *bad_value = 1;
+            }
+        }
+        if (ok && last) {
+            const float inv = none ? 0.f : 1.0f / L;
             // as bf16 through the query tile, so that whole rows leave side by side
             uint8_t* row = sQ + r * 128;
-            tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < NH; ++c) {
-                if (nkv > 0) {
-                    tmem_ld32(tO + lane_base + (uint32_t)(64 * c + 32 * b), v[0]);
-                    tmem_ld32(tO + lane_base + (uint32_t)(64 * NH + 64 * c + 32 * b), v[1]);
-                    tmem_ld_wait();
+                if (pieces == 1) {
+                    own(c);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[0][e] = 0u;
+#pragma unroll 1
+                    for (int i = 0; i < pieces; ++i) {
+                        const float2 ml = __ldcg(pp.part_ml + (long long)(first_unit + i) * PT_ROWS + r);
+                        if (ml.y == 0.f) continue;
+                        const float f = ex2_approx(ml.x - M);
+                        const float4* from16 = pp.part_o + ((long long)(first_unit + i) * (16 * NH) + 16 * c + 8 * b) * PT_ROWS + r;
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) {
+                            const float4 x = __ldcg(from16 + d * PT_ROWS);
+                            v[0][4 * d] = __float_as_uint(fmaf(x.x, f, __uint_as_float(v[0][4 * d])));
+                            v[0][4 * d + 1] = __float_as_uint(fmaf(x.y, f, __uint_as_float(v[0][4 * d + 1])));
+                            v[0][4 * d + 2] = __float_as_uint(fmaf(x.z, f, __uint_as_float(v[0][4 * d + 2])));
+                            v[0][4 * d + 3] = __float_as_uint(fmaf(x.w, f, __uint_as_float(v[0][4 * d + 3])));
+                        }
+                    }
                 }
-                auto out = [&](int e) {
-                    return none ? 0.f : (e0 == 0.f ? 0.f : __uint_as_float(v[0][e]) * w0) + (e1 == 0.f ? 0.f : __uint_as_float(v[1][e]) * w1);
-                };
+                auto out = [&](int e) { return none ? 0.f : __uint_as_float(v[0][e]) * inv; };
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
                     *reinterpret_cast<uint4*>(row + c * PT_TILE + (((4 * b + d) ^ (r & 7)) << 4)) =
@@ -1099,9 +1278,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (*bad_value && mine && !none) add_what_is_not_finite<NH, E4M3>(p, pool_v, s, head, edge0 * PT_KEYS, pos, b, r, row);
             if (p.lse && b == 0 && mine)
                 p.lse[(long long)(q0 + tok0 + r / p.group) * p.H + head * p.group + r % p.group] =
-                    none ? -INFINITY : (M + log2f(lt)) * 0.6931471805599453f;
+                    none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
         }
-        if (all_of(ok, 1, 256)) {
+        if (all_of(ok, 1, 256) && last) {
             const int per_row = p.v.hd >> 3;                                // 16-byte pieces of a row
             for (int x = threadIdx.x - 64; x < tokens * p.group * per_row; x += 256) {
                 const int rr = x / per_row, e = x - rr * per_row, t = rr / p.group, g = rr - t * p.group;
@@ -1161,7 +1340,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         auto keys = [&](int j) -> bool {
             const int st = j & 1;
             ok = ok && mbar_wait(&raw_full[0], (uint32_t)(j & 1), abort_flag);
-            const float vs = j * PT_KEYS + t <= last_pos ? sc[PT_KEYS + t] : 0.f;
+            const float vs = (from + j) * PT_KEYS + t <= last_pos ? sc[PT_KEYS + t] : 0.f;
             const uint32_t ve = (__float_as_uint(vs) >> 23) & 255u;
             fin_next = ve != 255u;
             // the block's reference: the largest exponent of a value's scale so far
@@ -1211,7 +1390,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 if (j + 2 < nkv) all_of(false, 2, 128);                     // (where the others meet in keys(j + 2))
                 break;
             }
-            const bool seen = j * PT_KEYS + t <= last_pos, looked = j >= edge0 && seen;
+            const bool seen = (from + j) * PT_KEYS + t <= last_pos, looked = from + j >= edge0 && seen;
             bool bad = looked && !fin;
             if (looked && fin) {
                 uint32_t has = 0u;
@@ -1259,13 +1438,21 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 }
 
 template <int NH, bool E4M3>
-int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cudaStream_t st) {
+int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, const PagedPlan& pl, uint8_t* ws, cudaStream_t st) {
     typedef ChunkShape<NH, E4M3> Sh;
+    static_assert(Sh::PER_SM == paged_tiles_per_sm(NH, E4M3), "the plan counts on as many CTAs per SM");
     PagedChunkParams pp;
     pp.a = p;
     pp.tokens = PT_ROWS / p.group;
     pp.tiles = (p.max_q + pp.tokens - 1) / pp.tokens;
-    TB_CHECK(pp.tiles <= 65535, "tb_attention_paged: max_q %d is too much for one launch", p.max_q);
+    pp.planned = pl.most_units > 0 ? 1 : 0; pp.most_units = pl.most_units; pp.slots = Sh::PER_SM * ctx->sm_count;
+    // (see paged_plan.h for the room)
+    pp.count = reinterpret_cast<int*>(ws);
+    pp.arrived = reinterpret_cast<unsigned int*>(ws + 16);
+    pp.bad = reinterpret_cast<int*>(pp.arrived + pl.most_units);
+    pp.units = reinterpret_cast<ChunkUnit*>(pp.bad + pl.most_units);
+    pp.part_ml = reinterpret_cast<float2*>(pp.units + pl.most_units);
+    pp.part_o = reinterpret_cast<float4*>(pp.part_ml + (size_t)pl.most_units * PT_ROWS);
     CUtensorMap tmQ, tmK, tmV;
     TB_TRY(make_query_map(&tmQ, p.Q, c->head_dim, p.H, p.rows, p.ld_q, p.group, pp.tokens));
     const int box_rows = std::min(c->page_size, PT_KEYS);
@@ -1276,9 +1463,17 @@ int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, c
         TB_CUDA(cudaFuncSetAttribute(paged_chunk_kernel<NH, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
         attr_set[ctx->device & 63] = true;
     }
+    if (pp.planned) {
+        prof_mark(ctx, "paged_plan", 0.0, 0.0, st);
+        TB_CUDA(launch_kernel(paged_plan_kernel, dim3(1), dim3(PL_THREADS), 0, st, pp));
+        ctx->launches++;
+        prof_close(ctx, st);
+    } else {
+        TB_CHECK(pp.tiles <= 65535, "tb_attention_paged: max_q %d is too much for one launch", p.max_q);
+    }
     prof_mark(ctx, "paged_chunk", 4.0 * p.rows * p.H * (double)p.max_kv * c->head_dim, 0.0, st);
-    TB_CUDA(launch_kernel(paged_chunk_kernel<NH, E4M3>, dim3(c->heads, pp.tiles, c->seqs), dim3(Sh::THREADS), Sh::SMEM, st, tmQ, tmK, tmV,
-                          static_cast<const uint8_t*>(c->V), pp));
+    const dim3 grid = pp.planned ? dim3(pl.most_units) : dim3((unsigned)c->heads * (unsigned)c->seqs, pp.tiles);
+    TB_CUDA(launch_kernel(paged_chunk_kernel<NH, E4M3>, grid, dim3(Sh::THREADS), Sh::SMEM, st, tmQ, tmK, tmV, static_cast<const uint8_t*>(c->V), pp));
     ctx->launches++;
     prof_close(ctx, st);
     return 0;
@@ -1290,7 +1485,7 @@ int launch_attention_paged(DeviceCtx* ctx, const TbKvCache* c, const int* q_star
                            int H, int max_q, int max_kv, float scale, bf16* att, long long ld_att, float* lse, void* ws, int64_t ws_bytes,
                            cudaStream_t st) {
     const int group = H / c->heads;
-    const PagedPlan pl = paged_plan(c->seqs, c->heads, c->head_dim, c->type == TB_KV_E4M3, max_kv, ctx->sm_count);
+    const PagedPlan pl = paged_plan(c->seqs, c->heads, group, c->head_dim, c->type == TB_KV_E4M3, rows, max_q, max_kv, ctx->sm_count);
     TB_CHECK(pl.workspace == 0 || (ws != nullptr && ws_bytes >= pl.workspace), "tb_attention_paged: the workspace has %lld bytes, %lld are needed",
              (long long)(ws ? ws_bytes : 0), (long long)pl.workspace);
     PagedAttParams p;
@@ -1304,8 +1499,9 @@ int launch_attention_paged(DeviceCtx* ctx, const TbKvCache* c, const int* q_star
     p.scale_log2 = scale * 1.4426950408889634f; p.err = ctx->d_err;
     const bool wide = c->head_dim > 64;
     if (max_q * (long long)group > PA_ROWS) {
-        if (c->type == TB_KV_E4M3) TB_TRY(wide ? (launch_chunks<2, true>(ctx, c, p, st)) : (launch_chunks<1, true>(ctx, c, p, st)));
-        else TB_TRY(wide ? (launch_chunks<2, false>(ctx, c, p, st)) : (launch_chunks<1, false>(ctx, c, p, st)));
+        uint8_t* more = static_cast<uint8_t*>(ws) + pl.rows_bytes;
+        if (c->type == TB_KV_E4M3) TB_TRY(wide ? (launch_chunks<2, true>(ctx, c, p, pl, more, st)) : (launch_chunks<1, true>(ctx, c, p, pl, more, st)));
+        else TB_TRY(wide ? (launch_chunks<2, false>(ctx, c, p, pl, more, st)) : (launch_chunks<1, false>(ctx, c, p, pl, more, st)));
     }
     if (c->type == TB_KV_E4M3) TB_TRY(wide ? (launch_rows<2, true>(ctx, c, p, st)) : (launch_rows<1, true>(ctx, c, p, st)));
     else TB_TRY(wide ? (launch_rows<2, false>(ctx, c, p, st)) : (launch_rows<1, false>(ctx, c, p, st)));
@@ -1330,7 +1526,8 @@ extern "C" {
 int64_t tb_attention_paged_workspace(const TbKvCache* cache, int rows, int q_heads, int max_q, int max_kv) {
     DeviceCtx* ctx;
     if (check_attention(cache, rows, q_heads, max_q, max_kv) != 0 || get_ctx(&ctx) != 0) return -1;
-    return paged_plan(cache->seqs, cache->heads, cache->head_dim, cache->type == TB_KV_E4M3, max_kv, ctx->sm_count).workspace;
+    return paged_plan(cache->seqs, cache->heads, q_heads / cache->heads, cache->head_dim, cache->type == TB_KV_E4M3, rows, std::min(max_q, rows),
+                      max_kv, ctx->sm_count).workspace;
 }
 
 int tb_attention_paged(const TbKvCache* cache, const int32_t* d_q_start, const int32_t* d_kv_len, const void* d_Q, int64_t ld_q, int rows,
