@@ -30,6 +30,8 @@ struct PagedAttParams {
     float* part_o; float2* part_ml;  // [2 grid][16][hd], [2 grid][16]: results of items that a CTA shares with its neighbours
     unsigned int* arrived;           // [grid], zero between launches: pieces written of the item that begins in a CTA's run and goes on
     int rows, H, group, max_q, max_kv, grid, whole;
+    int behind_plan;                 // few rows: the kernel in front is paged_plan_kernel, whose results concern the next one
+    uint32_t group_magic;            // x / group = x * group_magic >> 16 for x < 128
     float scale_log2;
     int* err;
 };
@@ -161,7 +163,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         fence_mbar_init();
     }
     __syncthreads();
-    pdl_wait();
+    if (!p.behind_plan) pdl_wait();      // (the plan has waited itself before it let this kernel start)
 
     if (warp == PA_WARPS) {
         // ---- producer: finds this CTA's items, and fills the ring with their blocks.  A lane per piece of a page.
@@ -318,6 +320,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             *reinterpret_cast<int*>(smem + Sh::O_WHAT + (i % STAGES) * Sh::WHAT) = PA_END;
             mbar_arrive(&full[i % STAGES]);
         }
+        if (p.behind_plan) pdl_wait();       // the next kernel reads the plan
         pdl_launch_dependents_now();
         if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 73); }
         // (the consumers wait for everything that has been asked for)
@@ -355,7 +358,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int rr = r + 8 * x;
-                pos[x] = kv - n + min(rr, nrows - 1) / p.group;
+                pos[x] = kv - n + (int)((uint32_t)min(rr, nrows - 1) * p.group_magic >> 16);
                 const uint8_t* q = smem + Sh::O_Q + st * Sh::Q_BYTES + rr * p.v.hd * 2;
                 uint32_t big = 0u;
 #pragma unroll
@@ -619,9 +622,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         // ---- an item of several runs: whoever is last with its piece adds them, in the order of the runs.  The run that the item begins
         // in has it in slot 1 of its CTA, the others in slot 0.
-        __threadfence();
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (threadIdx.x == 0) {
+            __threadfence();                                               // (everyone's piece, before the count)
             const unsigned int before = atomicAdd(p.arrived + more.z, 1u);
             *is_last = before == (unsigned int)more.w - 1u ? 1 : 0;
             if (*is_last) p.arrived[more.z] = 0u;                          // ready for the next launch
@@ -669,26 +672,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (lane == 0) { *abort_flag = 1; atomicExch(p.err, 74); }
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
     }
-}
-
-template <int NH, bool E4M3>
-int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cudaStream_t st) {
-    typedef RowsShape<NH, E4M3> Sh;
-    static_assert(Sh::PER_SM == paged_per_sm(NH, E4M3), "the plan counts on as many CTAs per SM");
-    CUtensorMap tmK, tmV;
-    const int box_rows = std::min(c->page_size, Sh::KEYS);
-    TB_TRY(make_cache_map(&tmK, c->K, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
-    TB_TRY(make_cache_map(&tmV, c->V, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
-    static bool attr_set[64] = {false};
-    if (!attr_set[ctx->device & 63]) {
-        TB_CUDA(cudaFuncSetAttribute(paged_rows_kernel<NH, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
-        attr_set[ctx->device & 63] = true;
-    }
-    prof_mark(ctx, "paged_rows", 4.0 * p.rows * p.H * (double)p.max_kv * c->head_dim, 0.0, st);
-    TB_CUDA(launch_kernel(paged_rows_kernel<NH, E4M3>, dim3(p.grid), dim3(PA_THREADS), Sh::SMEM, st, tmK, tmV, p));
-    ctx->launches++;
-    prof_close(ctx, st);
-    return 0;
 }
 
 // ------------------------------------------------------------------------------- chunks: tcgen05
@@ -786,8 +769,8 @@ paged_plan_kernel(const PagedChunkParams pp) {
         units = __reduce_add_sync(0xffffffffu, units) * p.v.heads;
         if (lane == 0) {
             caps[warp] = cap;
-            // (three blocks: the start of a piece, its result to memory and back)
-            cost[warp] = (pieces == 1 || units <= pp.most_units) ? (units + pp.slots - 1) / pp.slots * (cap + 3) : 0x7fffffff;
+            // (in blocks: three for the start of a piece and its result to memory, one for a piece's result on its way back)
+            cost[warp] = (pieces == 1 || units <= pp.most_units) ? (units + pp.slots - 1) / pp.slots * (cap + 3) + pieces : 0x7fffffff;
         }
     }
     __syncthreads();
@@ -886,10 +869,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     uint32_t* warp_most = tmem_slot + 10;                                  // (8 bits) [2][4]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_wait();
+    // No wait for the kernel in front (paged_rows_kernel writes other rows): it has let this one start after what both read was there,
+    // the plan included.  Every CTA waits for it at its end, so that what follows finds both kernels' rows.
     int s, head, tile, from = 0, to = 0x7fffffff, pieces = 1, first_unit = 0;
     if (pp.planned) {
-        if ((int)blockIdx.x >= *pp.count) return;
+        if ((int)blockIdx.x >= *pp.count) {
+            pdl_wait();
+            return;
+        }
         const int4* u = reinterpret_cast<const int4*>(pp.units + blockIdx.x);
         const int4 a = u[0], b = u[1];
         s = a.x; head = a.y; tile = a.z; from = a.w; to = b.x; first_unit = b.y; pieces = b.z;
@@ -898,15 +885,31 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         s = (int)(blockIdx.x / (unsigned)p.v.heads); head = (int)(blockIdx.x % (unsigned)p.v.heads); tile = pp.tiles - 1 - (int)blockIdx.y;
     }
     int q0, n, kv;
-    if (!batch_of(p, s, q0, n, kv)) return;                                // (paged_rows_kernel reports it)
+    const bool fine = batch_of(p, s, q0, n, kv);                           // (paged_rows_kernel reports it)
     const int tok0 = tile * pp.tokens;
-    if (n * p.group <= PA_ROWS || tok0 >= n) return;
+    if (!fine || n * p.group <= PA_ROWS || tok0 >= n) {
+        pdl_wait();
+        return;
+    }
     const int tokens = min(pp.tokens, n - tok0);
     const int first_pos = kv - n + tok0, last_pos = first_pos + tokens - 1;
     const int nkv = min(to, last_pos >= 0 ? last_pos / PT_KEYS + 1 : 0) - from;      // blocks of keys, from block `from` on
     const int edge0 = max(0, first_pos + 1) / PT_KEYS;                     // the first block with a key that some row does not see
+    // the producer's first pages, on their way while the block sets itself up
+    const int piece_shift = min(p.v.page_shift, 7), page_pieces = PT_KEYS >> piece_shift, piece_keys = 1 << piece_shift;
+    const int per_page_shift = p.v.page_shift - piece_shift, last_piece = (last_pos + piece_keys) >> piece_shift, piece0 = from * page_pieces;
+    const int* table = p.v.table + (long long)s * p.v.table_ld;
+    auto page_at = [&](int piece) -> int {
+        if (piece >= last_piece) return 0;
+        const int pg = table[piece >> per_page_shift];
+        if ((unsigned)pg < (unsigned)p.v.pages) return pg;
+        atomicExch(p.err, 75);
+        return 0;
+    };
+    int held = piece0, now = 0, next = 0;
+    if (warp == 0 && nkv > 0) { now = page_at(piece0 + lane); next = page_at(piece0 + 32 + lane); }
 
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 32 * 2) {
         mbar_init(q_full, 1); mbar_init(q_ready, 4); mbar_init(v_land, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], E4M3 ? 4 : 1); mbar_init(&v_full[i], E4M3 ? 4 : 1);
@@ -926,24 +929,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 
     if (warp == 0) {
         // ---- producer: a lane per piece of a page
-        const int piece_shift = min(p.v.page_shift, 7), page_pieces = PT_KEYS >> piece_shift, piece_keys = 1 << piece_shift;
-        const int per_page_shift = p.v.page_shift - piece_shift;
-        const int* table = p.v.table + (long long)s * p.v.table_ld;
-        const int last_piece = (last_pos + piece_keys) >> piece_shift;
-        auto page_at = [&](int piece) -> int {
-            if (piece >= last_piece) return 0;
-            const int pg = table[piece >> per_page_shift];
-            if ((unsigned)pg < (unsigned)p.v.pages) return pg;
-            atomicExch(p.err, 75);
-            return 0;
-        };
         bool ok = true;
         if (lane == 0 && nkv > 0) {
             mbar_expect_tx(q_full, (uint32_t)(NH * pp.tokens * p.group * 128));
             for (int c = 0; c < NH; ++c) tma_load_3d(sQ + c * PT_TILE, &tmQ, q_full, c * 64, head * p.group, q0 + tok0);
         }
-        const int piece0 = from * page_pieces;
-        int held = piece0, now = nkv > 0 ? page_at(piece0 + lane) : 0, next = nkv > 0 ? page_at(piece0 + 32 + lane) : 0, landed = 0;
+        int landed = 0;
         for (int j = 0; j < nkv && ok; ++j) {
             const int at = piece0 + j * page_pieces;
             if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
@@ -1064,7 +1055,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     } else if (warp < 10) {
         // ---- softmax
         const int q = warp & 3, b = (warp - 2) >> 2, r = q * 32 + lane;
-        const int tok = min(r / p.group, tokens - 1);
+        const int tok = min((int)((uint32_t)r * p.group_magic >> 16), tokens - 1);
         const int pos = first_pos + tok;
         const bool mine = r < tokens * p.group;
         const uint32_t lane_base = (uint32_t)(q * 32) << 16;
@@ -1216,9 +1207,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
                 if (b == 0) __stcg(pp.part_ml + (long long)blockIdx.x * PT_ROWS + r, make_float2(M, L));
                 if (warp == 2 && lane == 0) pp.bad[blockIdx.x] = *bad_value;
-                __threadfence();
             }
             if (all_of(ok, 1, 256)) {
+                if (warp == 2 && lane == 0) __threadfence();                // (everyone's piece, before the count)
                 if (warp == 2 && lane == 0) *is_last = atomicAdd(pp.arrived + first_unit, 1u) == (unsigned int)pieces - 1u ? 1 : 0;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 last = *is_last;
@@ -1252,11 +1243,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[0][e] = 0u;
-#pragma unroll 1
+#pragma unroll 2
                     for (int i = 0; i < pieces; ++i) {
                         const float2 ml = __ldcg(pp.part_ml + (long long)(first_unit + i) * PT_ROWS + r);
-                        if (ml.y == 0.f) continue;
-                        const float f = ex2_approx(ml.x - M);
+                        const float f = ml.y == 0.f ? 0.f : ex2_approx(ml.x - M);        // (a piece without a key for this row holds zeros)
                         const float4* from16 = pp.part_o + ((long long)(first_unit + i) * (16 * NH) + 16 * c + 8 * b) * PT_ROWS + r;
 #pragma unroll
                         for (int d = 0; d < 8; ++d) {
@@ -1277,15 +1267,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             if (*bad_value && mine && !none) add_what_is_not_finite<NH, E4M3>(p, pool_v, s, head, edge0 * PT_KEYS, pos, b, r, row);
             if (p.lse && b == 0 && mine)
-                p.lse[(long long)(q0 + tok0 + r / p.group) * p.H + head * p.group + r % p.group] =
+                p.lse[(long long)(q0 + tok0 + tok) * p.H + head * p.group + r - tok * p.group] =
                     none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
         }
         if (all_of(ok, 1, 256) && last) {
-            const int per_row = p.v.hd >> 3;                                // 16-byte pieces of a row
-            for (int x = threadIdx.x - 64; x < tokens * p.group * per_row; x += 256) {
-                const int rr = x / per_row, e = x - rr * per_row, t = rr / p.group, g = rr - t * p.group;
-                const uint4 w = *reinterpret_cast<const uint4*>(sQ + (e >> 3) * PT_TILE + rr * 128 + (((e & 7) ^ (rr & 7)) << 4));
-                *reinterpret_cast<uint4*>(p.att + (long long)(q0 + tok0 + t) * p.ld_att + (long long)(head * p.group + g) * p.v.hd + e * 8) = w;
+            // 8 NH lanes per row, each with 16 bytes
+            const int e = lane & (8 * NH - 1), rows_of_tile = tokens * p.group;
+            const uint8_t* src = sQ + (e >> 3) * PT_TILE;
+#pragma unroll
+            for (int i = 0; i < 4 * NH; ++i) {
+                const int rr = (warp - 2) * 16 + i * (4 / NH) + (lane >> (NH == 1 ? 3 : 4));
+                const int t = (int)((uint32_t)rr * p.group_magic >> 16), g = rr - t * p.group;
+                if (rr < rows_of_tile && e * 8 < p.v.hd)
+                    *reinterpret_cast<uint4*>(p.att + (long long)(q0 + tok0 + t) * p.ld_att + (long long)(head * p.group + g) * p.v.hd + e * 8) =
+                        *reinterpret_cast<const uint4*>(src + rr * 128 + (((e & 7) ^ (rr & 7)) << 4));
             }
         }
         if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 79); }
@@ -1432,27 +1427,62 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 
     __syncwarp();
     if (*abort_flag) for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    pdl_wait();
     tc_fence_before();
     __syncthreads();
     if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, Sh::TMEM); }
 }
 
 template <int NH, bool E4M3>
-int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, const PagedPlan& pl, uint8_t* ws, cudaStream_t st) {
+int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cudaStream_t st) {
+    typedef RowsShape<NH, E4M3> Sh;
+    static_assert(Sh::PER_SM == paged_per_sm(NH, E4M3), "the plan counts on as many CTAs per SM");
+    CUtensorMap tmK, tmV;
+    const int box_rows = std::min(c->page_size, Sh::KEYS);
+    TB_TRY(make_cache_map(&tmK, c->K, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
+    TB_TRY(make_cache_map(&tmV, c->V, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
+    static bool attr_set[64] = {false};
+    if (!attr_set[ctx->device & 63]) {
+        TB_CUDA(cudaFuncSetAttribute(paged_rows_kernel<NH, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+        attr_set[ctx->device & 63] = true;
+    }
+    prof_mark(ctx, "paged_rows", 4.0 * p.rows * p.H * (double)p.max_kv * c->head_dim, 0.0, st);
+    TB_CUDA(launch_kernel_early(paged_rows_kernel<NH, E4M3>, dim3(p.grid), dim3(PA_THREADS), Sh::SMEM, st, tmK, tmV, p));
+    ctx->launches++;
+    prof_close(ctx, st);
+    return 0;
+}
+
+template <int NH, bool E4M3>
+int plan_chunks(DeviceCtx* ctx, const PagedAttParams& p, const PagedPlan& pl, uint8_t* ws, PagedChunkParams* pp, cudaStream_t st) {
     typedef ChunkShape<NH, E4M3> Sh;
     static_assert(Sh::PER_SM == paged_tiles_per_sm(NH, E4M3), "the plan counts on as many CTAs per SM");
-    PagedChunkParams pp;
-    pp.a = p;
-    pp.tokens = PT_ROWS / p.group;
-    pp.tiles = (p.max_q + pp.tokens - 1) / pp.tokens;
-    pp.planned = pl.most_units > 0 ? 1 : 0; pp.most_units = pl.most_units; pp.slots = Sh::PER_SM * ctx->sm_count;
+    pp->a = p;
+    pp->tokens = PT_ROWS / p.group;
+    pp->tiles = (p.max_q + pp->tokens - 1) / pp->tokens;
+    pp->planned = p.behind_plan; pp->most_units = pl.most_units; pp->slots = Sh::PER_SM * ctx->sm_count;
     // (see paged_plan.h for the room)
-    pp.count = reinterpret_cast<int*>(ws);
-    pp.arrived = reinterpret_cast<unsigned int*>(ws + 16);
-    pp.bad = reinterpret_cast<int*>(pp.arrived + pl.most_units);
-    pp.units = reinterpret_cast<ChunkUnit*>(pp.bad + pl.most_units);
-    pp.part_ml = reinterpret_cast<float2*>(pp.units + pl.most_units);
-    pp.part_o = reinterpret_cast<float4*>(pp.part_ml + (size_t)pl.most_units * PT_ROWS);
+    pp->count = reinterpret_cast<int*>(ws);
+    pp->arrived = reinterpret_cast<unsigned int*>(ws + 16);
+    pp->bad = reinterpret_cast<int*>(pp->arrived + pl.most_units);
+    pp->units = reinterpret_cast<ChunkUnit*>(pp->bad + pl.most_units);
+    pp->part_ml = reinterpret_cast<float2*>(pp->units + pl.most_units);
+    pp->part_o = reinterpret_cast<float4*>(pp->part_ml + (size_t)pl.most_units * PT_ROWS);
+    if (!pp->planned) {
+        TB_CHECK(pp->tiles <= 65535, "tb_attention_paged: max_q %d is too much for one launch", p.max_q);
+        return 0;
+    }
+    prof_mark(ctx, "paged_plan", 0.0, 0.0, st);
+    TB_CUDA(launch_kernel(paged_plan_kernel, dim3(1), dim3(PL_THREADS), 0, st, *pp));
+    ctx->launches++;
+    prof_close(ctx, st);
+    return 0;
+}
+
+template <int NH, bool E4M3>
+int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedChunkParams& pp, cudaStream_t st) {
+    typedef ChunkShape<NH, E4M3> Sh;
+    const PagedAttParams& p = pp.a;
     CUtensorMap tmQ, tmK, tmV;
     TB_TRY(make_query_map(&tmQ, p.Q, c->head_dim, p.H, p.rows, p.ld_q, p.group, pp.tokens));
     const int box_rows = std::min(c->page_size, PT_KEYS);
@@ -1463,19 +1493,22 @@ int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, c
         TB_CUDA(cudaFuncSetAttribute(paged_chunk_kernel<NH, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
         attr_set[ctx->device & 63] = true;
     }
-    if (pp.planned) {
-        prof_mark(ctx, "paged_plan", 0.0, 0.0, st);
-        TB_CUDA(launch_kernel(paged_plan_kernel, dim3(1), dim3(PL_THREADS), 0, st, pp));
-        ctx->launches++;
-        prof_close(ctx, st);
-    } else {
-        TB_CHECK(pp.tiles <= 65535, "tb_attention_paged: max_q %d is too much for one launch", p.max_q);
-    }
     prof_mark(ctx, "paged_chunk", 4.0 * p.rows * p.H * (double)p.max_kv * c->head_dim, 0.0, st);
-    const dim3 grid = pp.planned ? dim3(pl.most_units) : dim3((unsigned)c->heads * (unsigned)c->seqs, pp.tiles);
-    TB_CUDA(launch_kernel(paged_chunk_kernel<NH, E4M3>, grid, dim3(Sh::THREADS), Sh::SMEM, st, tmQ, tmK, tmV, static_cast<const uint8_t*>(c->V), pp));
+    const dim3 grid = pp.planned ? dim3(pp.most_units) : dim3((unsigned)c->heads * (unsigned)c->seqs, pp.tiles);
+    TB_CUDA(launch_kernel_early(paged_chunk_kernel<NH, E4M3>, grid, dim3(Sh::THREADS), Sh::SMEM, st, tmQ, tmK, tmV, static_cast<const uint8_t*>(c->V), pp));
     ctx->launches++;
     prof_close(ctx, st);
+    return 0;
+}
+
+// The kernel for few rows goes first: its CTAs leave the SMs one after the other, and tiles start where they do.
+template <int NH, bool E4M3>
+int launch_both(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, const PagedPlan& pl, uint8_t* more, cudaStream_t st) {
+    const bool chunks = p.max_q * (long long)p.group > PA_ROWS;
+    PagedChunkParams pp;
+    if (chunks) TB_TRY((plan_chunks<NH, E4M3>(ctx, p, pl, more, &pp, st)));
+    TB_TRY((launch_rows<NH, E4M3>(ctx, c, p, st)));
+    if (chunks) TB_TRY((launch_chunks<NH, E4M3>(ctx, c, pp, st)));
     return 0;
 }
 
@@ -1497,15 +1530,11 @@ int launch_attention_paged(DeviceCtx* ctx, const TbKvCache* c, const int* q_star
     p.arrived = static_cast<unsigned int*>(ws);
     p.rows = rows; p.H = H; p.group = group; p.max_q = max_q; p.max_kv = max_kv; p.grid = pl.grid; p.whole = pl.whole ? 1 : 0;
     p.scale_log2 = scale * 1.4426950408889634f; p.err = ctx->d_err;
-    const bool wide = c->head_dim > 64;
-    if (max_q * (long long)group > PA_ROWS) {
-        uint8_t* more = static_cast<uint8_t*>(ws) + pl.rows_bytes;
-        if (c->type == TB_KV_E4M3) TB_TRY(wide ? (launch_chunks<2, true>(ctx, c, p, pl, more, st)) : (launch_chunks<1, true>(ctx, c, p, pl, more, st)));
-        else TB_TRY(wide ? (launch_chunks<2, false>(ctx, c, p, pl, more, st)) : (launch_chunks<1, false>(ctx, c, p, pl, more, st)));
-    }
-    if (c->type == TB_KV_E4M3) TB_TRY(wide ? (launch_rows<2, true>(ctx, c, p, st)) : (launch_rows<1, true>(ctx, c, p, st)));
-    else TB_TRY(wide ? (launch_rows<2, false>(ctx, c, p, st)) : (launch_rows<1, false>(ctx, c, p, st)));
-    return 0;
+    p.group_magic = (65536u + group - 1) / group; p.behind_plan = pl.most_units > 0 ? 1 : 0;
+    const bool wide = c->head_dim > 64, e4m3 = c->type == TB_KV_E4M3;
+    uint8_t* more = static_cast<uint8_t*>(ws) + pl.rows_bytes;
+    return e4m3 ? (wide ? launch_both<2, true>(ctx, c, p, pl, more, st) : launch_both<1, true>(ctx, c, p, pl, more, st))
+                : (wide ? launch_both<2, false>(ctx, c, p, pl, more, st) : launch_both<1, false>(ctx, c, p, pl, more, st));
 }
 
 }  // namespace tb

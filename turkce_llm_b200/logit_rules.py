@@ -8,6 +8,7 @@ import ctypes as C
 import torch
 
 from . import lib
+from .paged import _F32, _device_of, _ld, _stream_of
 
 
 class LogitRules:
@@ -48,15 +49,17 @@ class LogitRules:
         self._struct = lib.LogitRulesStruct(*[lib._ptr(t) if t is not None and t.numel() else None for t in self._kept], width(prompt),
                                             width(output), mask.shape[0] if mask is not None else 0, width(mask), entries)
         self._ref = C.addressof(self._struct)
+        self._index = self.device.index
 
     def apply(self, logits, out=None):
         """out = the rules on logits (float32 [rows, vocab], rows contiguous); out None: in place."""
         out = logits if out is None else out
-        for t in (logits, out):
-            if t.dtype != torch.float32 or tuple(t.shape) != (self.rows, self.vocab) or (t.stride(1) != 1 and self.vocab > 1) or \
-                    t.device != self.device:
-                raise lib.TbError("logits have to be float32 [%d, %d] on %s with contiguous rows" % (self.rows, self.vocab, self.device))
-        if torch.cuda.current_device() != self.device.index:
+        rows, vocab = self.rows, self.vocab
+        a, b = _ld(logits, _F32, vocab, self._index), _ld(out, _F32, vocab, self._index)
+        if a == 0 or b == 0 or logits.shape[0] != rows or out.shape[0] != rows:
+            raise lib.TbError("logits have to be float32 [%d, %d] on %s with contiguous rows" % (rows, vocab, self.device))
+        if _device_of() != self._index:
             raise lib.TbError("the rules are on %s, which is not the current device" % self.device)
-        lds = [t.stride(0) if self.rows > 1 else self.vocab for t in (logits, out)]
-        lib.check(self._lib.tb_logits_adjust(self._ref, logits.data_ptr(), lds[0], out.data_ptr(), lds[1], self.rows, self.vocab, lib._stream()))
+        rc = self._lib.tb_logits_adjust(self._ref, logits.data_ptr(), a, out.data_ptr(), b, rows, vocab, _stream_of(self._index))
+        if rc:
+            lib.check(rc)
