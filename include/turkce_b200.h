@@ -288,7 +288,7 @@ typedef struct TbLogitRules {
     int32_t prompt_ld, output_ld, masks, mask_ld, bias_entries;
 } TbLogitRules;
 
-/* d_out may be d_logits (in place) or another matrix that does not overlap it.  Ids of a row number less than 2^30; a length or an
+/* d_out may be d_logits (in place) or another matrix that does not overlap it.  Ids of a row number less than 2^29; a length or an
  * index outside its array is cut to it or left out, and reported by the next tb_check (code 81). */
 int tb_logits_adjust(const TbLogitRules* rules, const float* d_logits, int64_t ld_logits, float* d_out, int64_t ld_out, int rows,
                      int vocab, void* stream);

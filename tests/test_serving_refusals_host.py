@@ -88,7 +88,7 @@ def rules(**over):
     ({}, dict(z=None), "NULL logits"), ({}, dict(out=None), "NULL logits"), ({}, dict(ld=99), "leading dimensions"),
     ({}, dict(ld_out=99), "leading dimensions"), ({}, dict(out=A, ld_out=104), "in place"), ({}, dict(out=A + 64), "overlaps"),
     ({}, dict(out=A - 64), "overlaps"), (dict(prompt=A), {}, "prompt ids need"), (dict(prompt=A, prompt_len=A), {}, "prompt ids need"),
-    (dict(output=A, output_len=A, output_ld=1 << 30), {}, "output ids need"), (dict(bias_start=A, bias_entries=3), {}, "bias entries need"),
+    (dict(output=A, output_len=A, output_ld=1 << 29), {}, "output ids need"), (dict(bias_start=A, bias_entries=3), {}, "bias entries need"),
     (dict(bias_entries=-1), {}, "negative"), (dict(mask=A, masks=4, mask_ld=3), {}, "need 4 words"), (dict(mask=A, masks=3, mask_ld=4), {}, "need mask_row")])
 def test_rules_on_logits_refuse(over, call, match):
     a = dict(z=A, ld=100, out=2 * A, ld_out=100, rows=4, vocab=100)

@@ -814,6 +814,12 @@ __device__ __forceinline__ bool not_finite_16(uint32_t two) {            // eith
     return (two & 0x7f80u) == 0x7f80u || (two & 0x7f800000u) == 0x7f800000u;
 }
 
+__device__ __forceinline__ uint32_t finite_16(uint32_t two) {             // zeros for what is not
+    if ((two & 0x7f80u) == 0x7f80u) two &= 0xffff0000u;
+    if ((two & 0x7f800000u) == 0x7f800000u) two &= 0xffffu;
+    return two;
+}
+
 // What the product left out: values that are not finite, of the keys from k0 on that the row sees, added to the row's columns 32 b ..
 // of every 64 in the staged result (bf16, 128-byte swizzle).  Rare; straight from the pool.
 template <int NH, bool E4M3>
@@ -968,23 +974,26 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     ++landed;
                     const int seen = last_pos + 1 - (from + j) * PT_KEYS;           // rows of the tile that some query sees
                     bool bad = false;
-                    for (int c = 0; c < NH; ++c)
-#pragma unroll 2
-                        for (int x = lane; x < PT_KEYS * 8; x += 32) {
-                            uint4* at16 = reinterpret_cast<uint4*>(tile_v + c * PT_TILE + x * 16);
-                            const uint4 w = *at16;
-                            if ((x >> 3) >= seen) {
-                                *at16 = make_uint4(0u, 0u, 0u, 0u);
-                            } else if (not_finite_16(w.x) || not_finite_16(w.y) || not_finite_16(w.z) || not_finite_16(w.w)) {
-                                bad = true;
-                                uint32_t u[4] = {w.x, w.y, w.z, w.w};
-                                for (int e = 0; e < 4; ++e) {
-                                    if ((u[e] & 0x7f80u) == 0x7f80u) u[e] &= 0xffff0000u;
-                                    if ((u[e] & 0x7f800000u) == 0x7f800000u) u[e] &= 0xffffu;
-                                }
-                                *at16 = make_uint4(u[0], u[1], u[2], u[3]);
-                            }
+#pragma unroll 1
+                    for (int x0 = 0; x0 < PT_KEYS * 8 * NH; x0 += 32 * 8) {             // eight 16-byte pieces per lane side by side
+                        uint4 w[8];
+                        bool any = false;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const uint4*>(tile_v + (x0 + i * 32 + lane) * 16);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            any |= not_finite_16(w[i].x) || not_finite_16(w[i].y) || not_finite_16(w[i].z) || not_finite_16(w[i].w);
+                        if (!any) continue;
+#pragma unroll 1
+                        for (int i = 0; i < 8; ++i) {
+                            uint4* at16 = reinterpret_cast<uint4*>(tile_v + (x0 + i * 32 + lane) * 16);
+                            uint4 y = *at16;
+                            // (behind the last row that some query sees: whatever a page holds, or an earlier block)
+                            if (((x0 + i * 32 + lane) >> 3) % PT_KEYS < seen &&
+                                (not_finite_16(y.x) || not_finite_16(y.y) || not_finite_16(y.z) || not_finite_16(y.w))) bad = true;
+                            *at16 = make_uint4(finite_16(y.x), finite_16(y.y), finite_16(y.z), finite_16(y.w));
                         }
+                    }
                     if (bad) *bad_value = 1;
                     fence_proxy_async();
                     __syncwarp();

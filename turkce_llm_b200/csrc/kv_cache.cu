@@ -43,7 +43,7 @@ struct AppendParams {
     PagedView v;
     const int *q_start, *kv_len;
     const void* x; long long ld_x;
-    int rows, H, parts, threads_log2;                 // warps per row; threads per head: 1 << threads_log2
+    int rows, H, per_warp, parts, threads_log2;       // rows per warp, or warps per row; threads per head: 1 << threads_log2
     const float *cos_t, *sin_t;
     int positions, half;                              // rot_dim / 2
     bf16* Q; long long ld_q;
@@ -72,8 +72,35 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
     return make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
 }
 
+// Where the rows row0 .. row0 + count - 1 (count <= 32) of a warp belong: lane i has row row0 + i's sequence (-1: none), the end of that
+// sequence's rows and a number of it (lens[s]).  Rows of one sequence, the usual case, take one look at the starts.
+struct RowsOf { int s, end, len; };
+__device__ __forceinline__ RowsOf rows_of(const int* __restrict__ start, const int* __restrict__ lens, int seqs, int row0, int count) {
+    const int lane = threadIdx.x & 31, row = row0 + min(lane, count - 1);
+    RowsOf r;
+    r.s = sequence_of(start, seqs, row0);
+    r.end = r.s >= 0 ? start[r.s + 1] : row0;
+    if (row0 + count > r.end) {                                  // (the same for all lanes)
+        int lo = 0, hi = seqs;                                   // the last start at or before this lane's row is in [lo, hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        r.s = start[lo] <= row ? lo : -1;
+        r.end = r.s >= 0 ? start[r.s + 1] : row;
+        if (row >= r.end) r.s = -1;                              // behind the last sequence
+    }
+    r.len = r.s >= 0 && lens ? lens[r.s] : 0;
+    return r;
+}
+__device__ __forceinline__ long long shfl64(long long x, int lane) {
+    return (long long)__shfl_sync(0xffffffffu, (unsigned long long)x, lane);
+}
+
 // Rotated elements are a cos - b sin and a sin + b cos with every product rounded, the same sums whichever thread forms them.
-// A warp takes every `parts`-th group of heads of its row, the next group's elements on their way while it works on one.
+// A warp has p.per_warp rows, or a row's every `parts`-th group of heads; the next group's elements are on their way while it works on
+// one.  Bound: instructions about as much as bytes with an 8-bit cache (XX of 12,600 rows of 12 + 8 heads of 64), else bytes.
 template <bool BF16_IN, bool HALVES, bool E4M3>
 __global__ void __launch_bounds__(KV_THREADS)
 kv_append_kernel(const AppendParams p) {
@@ -82,117 +109,145 @@ kv_append_kernel(const AppendParams p) {
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned w = blockIdx.x * KV_WARPS + warp;
-    const int row = (int)(w / (unsigned)p.parts), part = (int)(w - (unsigned)row * (unsigned)p.parts);
-    if (row >= p.rows) return;                                   // (whole warps)
+    const int part = (int)(w % (unsigned)p.parts), row0 = (int)(w / (unsigned)p.parts) * p.per_warp;
+    if (row0 >= p.rows) return;                                  // (whole warps)
+    const int count = min(p.per_warp, p.rows - row0);
     const int hd = p.v.hd, G = p.v.heads, all = p.H + 2 * G;
-    const int per_warp = 32 >> p.threads_log2, step = per_warp * p.parts;
+    const int heads_of_warp = 32 >> p.threads_log2, step = heads_of_warp * p.parts;
     const int e0 = (lane & ((1 << p.threads_log2) - 1)) * 8;     // first of this thread's elements
-    const long long x_row = (long long)row * p.ld_x + e0;
-    int group = part * per_warp, head = group + (lane >> p.threads_log2);
+    const int first_group = part * heads_of_warp, in_group = lane >> p.threads_log2;
     const bool lane_in = e0 < hd;
     float x[8], nx[8];
-    auto fetch = [&](float (&f)[8], int h) {
+    auto fetch = [&](float (&f)[8], int row, int h) {
         if (lane_in && h < all) {
-            load8<BF16_IN>(p.x, x_row + (long long)h * hd, f);
+            load8<BF16_IN>(p.x, (long long)row * p.ld_x + e0 + (long long)h * hd, f);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = 0.f;
         }
     };
-    fetch(x, head);                                              // (needs nothing of the batch)
-    const int s = sequence_of(p.q_start, p.v.seqs, row);
-    if (s < 0) return;
-    const int end = p.q_start[s + 1], len = p.kv_len[s];
-    if (row >= end) return;                                      // behind the last sequence
-    const long long pos = (long long)len - end + row;
-    if (pos < 0 || pos >= (long long)p.v.table_ld << p.v.page_shift || (p.half > 0 && pos >= p.positions)) {
-        if (lane == 0) atomicExch(p.err, 72);
-        return;
+    fetch(x, row0, first_group + in_group);                      // (needs nothing of the batch)
+    // ---- lane i: position and place in the cache of row row0 + i
+    const RowsOf mine_of = rows_of(p.q_start, p.kv_len, p.v.seqs, row0, count);
+    long long my_pos = (long long)mine_of.len - mine_of.end + row0 + lane, my_slot = -1;
+    if (mine_of.s < 0 || lane >= count) {
+        my_pos = -1;
+    } else if (my_pos < 0 || my_pos >= (long long)p.v.table_ld << p.v.page_shift || (p.half > 0 && my_pos >= p.positions)) {
+        atomicExch(p.err, 72);
+        my_pos = -1;
+    } else {
+        const int page = p.v.table[(long long)mine_of.s * p.v.table_ld + (my_pos >> p.v.page_shift)];
+        if ((unsigned)page < (unsigned)p.v.pages) my_slot = ((long long)page * G << p.v.page_shift) + (my_pos & ((1 << p.v.page_shift) - 1));
+        else atomicExch(p.err, 71);
     }
-    const int page = p.v.table[(long long)s * p.v.table_ld + (pos >> p.v.page_shift)];
-    const bool page_ok = (unsigned)page < (unsigned)p.v.pages;
-    if (!page_ok && lane == 0) atomicExch(p.err, 71);
-    const long long slot = ((long long)page * G << p.v.page_shift) + (pos & ((1 << p.v.page_shift) - 1));
-    // this thread's angles are the same in every head
-    float c[HALVES ? 8 : 4], d[HALVES ? 8 : 4];
-    if (p.half > 0) {
-#pragma unroll
-        for (int i = 0; i < (HALVES ? 8 : 4); ++i) {
-            const int e = HALVES ? e0 + i : (e0 >> 1) + i, k = HALVES && e >= p.half ? e - p.half : e;
-            const bool turns = HALVES ? e < 2 * p.half : e < p.half;
-            c[i] = turns ? p.cos_t[pos * p.half + k] : 1.f;
-            d[i] = turns ? p.sin_t[pos * p.half + k] : 0.f;
+    // partners a whole number of threads apart change hands in registers, others through shared memory
+    const bool by_lane = HALVES && (p.half & 7) == 0;
+    const int other_lane = e0 < p.half ? lane + (p.half >> 3) : lane - (p.half >> 3);
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+        const int row = row0 + i;
+        const long long pos = shfl64(my_pos, i), slot = shfl64(my_slot, i);
+        if (pos < 0) {                                           // not of the batch, or out of range
+            if (i + 1 < count) fetch(x, row + 1, first_group + in_group);
+            continue;
         }
-    }
-    for (; group < all; group += step, head += step) {
-        const bool mine = lane_in && head < all;
-        if (group + step < all) fetch(nx, head + step);
-        if (p.half > 0 && group < p.H + G) {                     // (a group of values alone has nothing to rotate)
-            const bool turns = head < p.H + G;
-            if (!HALVES) {
+        // this thread's angles are the same in every head
+        float c[HALVES ? 8 : 4], d[HALVES ? 8 : 4];
+        if (p.half > 0) {
+            const float* ct = p.cos_t + pos * p.half;
+            const float* st = p.sin_t + pos * p.half;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (turns && (e0 >> 1) + i < p.half) {
-                        const float a = x[2 * i], b = x[2 * i + 1];
-                        x[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, d[i]));
-                        x[2 * i + 1] = __fadd_rn(__fmul_rn(a, d[i]), __fmul_rn(b, c[i]));
-                    }
-                }
-            } else {
-                // the partner's elements through shared memory: element e of this head at (e / 8) * 9 + e % 8 from the head's first
-                float* sw = swap[warp];
-                const int base = (lane >> p.threads_log2 << p.threads_log2) * 9;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sw[lane * 9 + i] = x[i];
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int e = e0 + i;
-                    if (mine && turns && e < 2 * p.half) {
-                        const bool low = e < p.half;
-                        const int o = low ? e + p.half : e - p.half;
-                        const float other = sw[base + (o >> 3) * 9 + (o & 7)];
-                        x[i] = low ? __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(other, d[i]))
-                                   : __fadd_rn(__fmul_rn(other, d[i]), __fmul_rn(x[i], c[i]));
-                    }
-                }
-                __syncwarp();
+            for (int k = 0; k < (HALVES ? 8 : 4); ++k) {
+                const int e = HALVES ? e0 + k : (e0 >> 1) + k, at = HALVES && e >= p.half ? e - p.half : e;
+                const bool turns = HALVES ? e < 2 * p.half : e < p.half;
+                c[k] = turns ? __ldg(ct + at) : 1.f;
+                d[k] = turns ? __ldg(st + at) : 0.f;
             }
         }
-        // largest magnitude of the row: as integers, so that NaN is larger than infinity and infinity than the rest
-        uint32_t big = 0u;
-        if (E4M3 && group + per_warp > p.H) {
+#pragma unroll 1
+        for (int group = first_group; group < all; group += step) {
+            const int head = group + in_group;
+            const bool mine = lane_in && head < all;
+            if (group + step < all) fetch(nx, row, head + step);
+            else if (i + 1 < count) fetch(nx, row + 1, first_group + in_group);
+            if (p.half > 0 && group < p.H + G) {                 // (a group of values alone has nothing to rotate)
+                const bool turns = head < p.H + G;
+                if (!HALVES) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
-            for (int o = (1 << p.threads_log2) >> 1; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-        }
-        if (mine && head < p.H) {
-            *reinterpret_cast<uint4*>(p.Q + (long long)row * p.ld_q + (long long)head * hd + e0) = pack8(x);
-        } else if (mine && page_ok) {
-            const bool key = head < p.H + G;
-            const long long at = slot + ((long long)(head - p.H - (key ? 0 : G)) << p.v.page_shift);
-            if (!E4M3) {
-                *reinterpret_cast<uint4*>(static_cast<bf16*>(key ? p.K : p.V) + at * hd + e0) = pack8(x);
-            } else {
-                float scale = __fdiv_rn(__uint_as_float(big), 448.0f);
-                if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;          // (stays NaN where it is)
-                uint32_t q[4];
+                    for (int k = 0; k < 4; ++k) {
+                        if (turns && (e0 >> 1) + k < p.half) {
+                            const float a = x[2 * k], b = x[2 * k + 1];
+                            x[2 * k] = __fsub_rn(__fmul_rn(a, c[k]), __fmul_rn(b, d[k]));
+                            x[2 * k + 1] = __fadd_rn(__fmul_rn(a, d[k]), __fmul_rn(b, c[k]));
+                        }
+                    }
+                } else if (by_lane) {
+                    const bool low = e0 < p.half, rotated = turns && e0 < 2 * p.half;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) q[i] = e4m3_pair(quotient_to_odd(x[2 * i], scale), quotient_to_odd(x[2 * i + 1], scale));
-                *reinterpret_cast<uint2*>(static_cast<uint8_t*>(key ? p.K : p.V) + at * hd + e0) =
-                    make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
-                if (e0 == 0) (key ? p.ks : p.vs)[at] = scale;
+                    for (int k = 0; k < 8; ++k) {
+                        const float other = __shfl_sync(0xffffffffu, x[k], other_lane);
+                        const float y = low ? __fsub_rn(__fmul_rn(x[k], c[k]), __fmul_rn(other, d[k]))
+                                            : __fadd_rn(__fmul_rn(other, d[k]), __fmul_rn(x[k], c[k]));
+                        if (rotated) x[k] = y;
+                    }
+                } else {
+                    // element e of this head at (e / 8) * 9 + e % 8 from the head's first
+                    float* sw = swap[warp];
+                    const int base = (lane >> p.threads_log2 << p.threads_log2) * 9;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sw[lane * 9 + k] = x[k];
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int e = e0 + k;
+                        if (mine && turns && e < 2 * p.half) {
+                            const bool low = e < p.half;
+                            const int o = low ? e + p.half : e - p.half;
+                            const float other = sw[base + (o >> 3) * 9 + (o & 7)];
+                            x[k] = low ? __fsub_rn(__fmul_rn(x[k], c[k]), __fmul_rn(other, d[k]))
+                                       : __fadd_rn(__fmul_rn(other, d[k]), __fmul_rn(x[k], c[k]));
+                        }
+                    }
+                    __syncwarp();
+                }
             }
-        }
+            // largest magnitude of the row: as integers, so that NaN is larger than infinity and infinity than the rest
+            uint32_t big = 0u;
+            if (E4M3 && group + heads_of_warp > p.H) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = nx[i];
+                for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(x[k]) & 0x7fffffffu);
+                for (int o = (1 << p.threads_log2) >> 1; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+            }
+            if (mine && head < p.H) {
+                *reinterpret_cast<uint4*>(p.Q + (long long)row * p.ld_q + (long long)head * hd + e0) = pack8(x);
+            } else if (mine && slot >= 0) {
+                const bool key = head < p.H + G;
+                const long long at = slot + ((long long)(head - p.H - (key ? 0 : G)) << p.v.page_shift);
+                if (!E4M3) {
+                    *reinterpret_cast<uint4*>(static_cast<bf16*>(key ? p.K : p.V) + at * hd + e0) = pack8(x);
+                } else {
+                    float scale = __fdiv_rn(__uint_as_float(big), 448.0f);
+                    if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;          // (stays NaN where it is)
+                    const float inverse = __frcp_rn(scale);
+                    uint32_t q[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        q[k] = e4m3_pair(quotient_to_odd(x[2 * k], scale, inverse), quotient_to_odd(x[2 * k + 1], scale, inverse));
+                    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(key ? p.K : p.V) + at * hd + e0) =
+                        make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+                    if (e0 == 0) (key ? p.ks : p.vs)[at] = scale;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = nx[k];
+        }
     }
 }
 
 struct ReadParams {
     PagedView v;
     const int *start, *first;
-    int rows, parts, threads_log2, kinds;             // warps per row, threads per head, 1 or 2 of K and V
+    int rows, per_warp, parts, threads_log2, kinds;   // rows per warp, or warps per row; threads per head; 1 or 2 of K and V
     const void *A, *B;                                // the pools read (B: the second one)
     const float *as, *bs;
     bf16 *oA, *oB;
@@ -207,59 +262,83 @@ kv_read_kernel(const ReadParams p) {
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned w = blockIdx.x * KV_WARPS + warp;
-    const int row = (int)(w / (unsigned)p.parts), part = (int)(w - (unsigned)row * (unsigned)p.parts);
-    if (row >= p.rows) return;
+    const int part = (int)(w % (unsigned)p.parts), row0 = (int)(w / (unsigned)p.parts) * p.per_warp;
+    if (row0 >= p.rows) return;
+    const int count = min(p.per_warp, p.rows - row0);
     const int hd = p.v.hd, G = p.v.heads, all = p.kinds * G;
-    const int step = (32 >> p.threads_log2) * p.parts;
+    const int heads_of_warp = 32 >> p.threads_log2, step = heads_of_warp * p.parts;
     const int e0 = (lane & ((1 << p.threads_log2) - 1)) * 8;
-    const int s = sequence_of(p.start, p.v.seqs, row);
-    if (s < 0 || row >= p.start[s + 1]) return;
-    const long long t = (long long)row - p.start[s] + (p.first ? p.first[s] : 0);
-    if (t < 0 || t >= (long long)p.v.table_ld << p.v.page_shift) {
-        if (lane == 0) atomicExch(p.err, 72);
-        return;
-    }
-    const int page = p.v.table[(long long)s * p.v.table_ld + (t >> p.v.page_shift)];
-    if ((unsigned)page >= (unsigned)p.v.pages) {
-        if (lane == 0) atomicExch(p.err, 71);
-        return;
-    }
-    if (e0 >= hd) return;
-    const long long slot = ((long long)page * G << p.v.page_shift) + (t & ((1 << p.v.page_shift) - 1));
-#pragma unroll 4
-    for (int head = part * (32 >> p.threads_log2) + (lane >> p.threads_log2); head < all; head += step) {
-        const bool first = head < G;
-        const int h = first ? head : head - G;
-        const long long at = slot + ((long long)h << p.v.page_shift);
-        uint4 out;
-        if (!E4M3) {
-            out = __ldg(reinterpret_cast<const uint4*>(static_cast<const bf16*>(first ? p.A : p.B) + at * hd + e0));
+    // ---- lane i: the place in the cache of row row0 + i
+    const RowsOf mine_of = rows_of(p.start, p.first, p.v.seqs, row0, count);
+    long long my_slot = -1;
+    if (mine_of.s >= 0 && lane < count) {
+        const long long t = (long long)row0 + lane - p.start[mine_of.s] + mine_of.len;
+        if (t < 0 || t >= (long long)p.v.table_ld << p.v.page_shift) {
+            atomicExch(p.err, 72);
         } else {
-            const uint2 c = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(first ? p.A : p.B) + at * hd + e0));
-            const float scale = __ldg((first ? p.as : p.bs) + at);
-            const uint32_t u[4] = {c.x & 0xffffu, c.x >> 16, c.y & 0xffffu, c.y >> 16};
-            uint32_t o[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = e4m3_floats(u[i]);
-                o[i] = bf16_pair(f.x * scale, f.y * scale);
-            }
-            out = make_uint4(o[0], o[1], o[2], o[3]);
+            const int page = p.v.table[(long long)mine_of.s * p.v.table_ld + (t >> p.v.page_shift)];
+            if ((unsigned)page < (unsigned)p.v.pages) my_slot = ((long long)page * G << p.v.page_shift) + (t & ((1 << p.v.page_shift) - 1));
+            else atomicExch(p.err, 71);
         }
-        *reinterpret_cast<uint4*>((first ? p.oA : p.oB) + (long long)row * p.ld_row + h * p.ld_head + e0) = out;
+    }
+    // All (row, group of heads) pairs of the warp, four of them on their way at a time
+    const int groups = (all - part * heads_of_warp + step - 1) / step, total = count * groups;
+    constexpr int ROUND = 4;
+#pragma unroll 1
+    for (int k0 = 0; k0 < total; k0 += ROUND) {
+        uint4 in[ROUND];
+        float scale[ROUND];
+        long long to[ROUND];
+        bool second[ROUND];
+#pragma unroll
+        for (int j = 0; j < ROUND; ++j) {
+            const int k = min(k0 + j, total - 1), i = k / groups, head = part * heads_of_warp + (k - i * groups) * step + (lane >> p.threads_log2);
+            const long long slot = shfl64(my_slot, i);
+            second[j] = head >= G;
+            const int h = second[j] ? head - G : head;
+            to[j] = -1;
+            if (slot >= 0 && k0 + j < total && head < all && e0 < hd) {
+                to[j] = (long long)(row0 + i) * p.ld_row + h * p.ld_head + e0;
+                const long long at = slot + ((long long)h << p.v.page_shift);
+                if (!E4M3) {
+                    in[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const bf16*>(second[j] ? p.B : p.A) + at * hd + e0));
+                } else {
+                    const uint2 c = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(second[j] ? p.B : p.A) + at * hd + e0));
+                    in[j].x = c.x; in[j].y = c.y;
+                    scale[j] = __ldg((second[j] ? p.bs : p.as) + at);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < ROUND; ++j) {
+            if (to[j] < 0) continue;
+            uint4 out = in[j];
+            if (E4M3) {
+                const uint32_t u[4] = {in[j].x & 0xffffu, in[j].x >> 16, in[j].y & 0xffffu, in[j].y >> 16};
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = e4m3_floats(u[i]);
+                    o[i] = bf16_pair(f.x * scale[j], f.y * scale[j]);
+                }
+                out = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+            *reinterpret_cast<uint4*>((second[j] ? p.oB : p.oA) + to[j]) = out;
+        }
     }
 }
 
-// threads per head (a power of two that divides a warp), warps per row, and the blocks for all rows.  A warp takes its row's heads
-// one group after the other, and what it knows of the row once; where there are fewer rows than that keeps the chip busy with
-// (eight warps per SM), a row's groups go to different warps.
-void shape_of(const DeviceCtx* ctx, int hd, int heads, int rows, int* threads_log2, int* parts, long long* blocks) {
+// threads per head (a power of two that divides a warp), and how rows are dealt to warps: what a warp finds out about a sequence
+// serves up to four rows, where that leaves sixteen warps for every SM; where there are fewer rows than eight for every SM, a row's
+// groups of heads go to different warps.
+void shape_of(const DeviceCtx* ctx, int hd, int heads, int rows, int* threads_log2, int* per_warp, int* parts, long long* blocks) {
     int t = 0;
     while ((8 << t) < hd) ++t;
     *threads_log2 = t;
-    const int per_warp = 32 >> t, groups = (heads + per_warp - 1) / per_warp;
+    const int in_warp = 32 >> t, groups = (heads + in_warp - 1) / in_warp;
     *parts = (int)std::max<long long>(1, std::min<long long>(groups, 8LL * ctx->sm_count / rows));
-    *blocks = ((long long)rows * *parts + KV_WARPS - 1) / KV_WARPS;
+    *per_warp = (int)std::max<long long>(1, std::min<long long>(4, rows / (16LL * ctx->sm_count)));
+    *blocks = (((long long)rows + *per_warp - 1) / *per_warp * *parts + KV_WARPS - 1) / KV_WARPS;
 }
 
 }  // namespace
@@ -273,7 +352,7 @@ int launch_kv_append(DeviceCtx* ctx, const TbKvCache* c, const int* q_start, con
     p.cos_t = cos_t; p.sin_t = sin_t; p.positions = positions; p.half = rot_dim / 2;
     p.Q = Q; p.ld_q = ld_q; p.K = c->K; p.V = c->V; p.ks = c->k_scale; p.vs = c->v_scale; p.err = ctx->d_err;
     long long blocks;
-    shape_of(ctx, c->head_dim, H + 2 * c->heads, rows, &p.threads_log2, &p.parts, &blocks);
+    shape_of(ctx, c->head_dim, H + 2 * c->heads, rows, &p.threads_log2, &p.per_warp, &p.parts, &blocks);
     TB_CHECK(blocks < (1LL << 31) / KV_WARPS, "tb_kv_append: too many rows");
     typedef void (*Kernel)(AppendParams);
     const bool halves = form == TB_ROPE_HALVES && rot_dim > 0, e4m3 = c->type == TB_KV_E4M3;
@@ -298,7 +377,7 @@ int launch_kv_read(DeviceCtx* ctx, const TbKvCache* c, const int* start, const i
     p.B = c->V; p.bs = c->v_scale; p.oB = V;
     p.ld_row = ld_row; p.ld_head = ld_head; p.err = ctx->d_err;
     long long blocks;
-    shape_of(ctx, c->head_dim, p.kinds * c->heads, rows, &p.threads_log2, &p.parts, &blocks);
+    shape_of(ctx, c->head_dim, p.kinds * c->heads, rows, &p.threads_log2, &p.per_warp, &p.parts, &blocks);
     TB_CHECK(blocks < (1LL << 31) / KV_WARPS, "tb_kv_read: too many rows");
     const bool e4m3 = c->type == TB_KV_E4M3;
     prof_mark(ctx, "kv_read", 0.0, (double)rows * p.kinds * c->heads * c->head_dim * (e4m3 ? 3 : 4), st);

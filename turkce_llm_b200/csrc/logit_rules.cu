@@ -15,8 +15,10 @@ namespace {
 
 constexpr int LR_THREADS = 256;
 constexpr uint32_t LR_PROMPT = 0x80000000u;      // bits of a token's word: among the prompt's ids
-constexpr uint32_t LR_TWICE = 0x40000000u;       // more than one bias entry; the rest counts the output ids
-constexpr uint32_t LR_COUNT = 0x3fffffffu;
+constexpr uint32_t LR_BIAS = 0x40000000u;        // a bias entry
+constexpr uint32_t LR_TWICE = 0x20000000u;       // more than one; the rest counts the output ids
+constexpr uint32_t LR_COUNT = 0x1fffffffu;
+constexpr int LR_IDS = 4;                        // ids of the prompt and of the output that a thread asks for at once
 constexpr uint32_t LR_NONE = 0xffffffffu;
 constexpr int LR_ROUNDS = kLogitSlice / (LR_THREADS * 4);
 
@@ -35,7 +37,7 @@ __global__ void __launch_bounds__(LR_THREADS)
 logit_rules_kernel(const LogitParams p) {
     extern __shared__ uint32_t lr_smem[];
     uint32_t* seen = lr_smem;                                    // [slice]
-    uint32_t* owner = lr_smem + p.slice;                         // [slice]: the token's first bias entry
+    uint32_t* owner = lr_smem + p.slice;                         // [slice]: the number of the token's first bias entry, or the value of its only one
     pdl_wait();
     pdl_launch_dependents();
     const int row = blockIdx.y, tid = threadIdx.x;
@@ -56,9 +58,17 @@ logit_rules_kernel(const LogitParams p) {
             for (int i = 0; i < 4; ++i) z[g][i] = t + i < n ? in[t + i] : 0.0f;
         }
     }
+    // The first ids of the row as well, before it is known how many count: lengths, ids and logits come in the same time.
+    uint32_t ids[2][LR_IDS];
+    auto early = [&](const uint32_t* at, int ld, uint32_t (&to)[LR_IDS]) {
+#pragma unroll
+        for (int i = 0; i < LR_IDS; ++i) to[i] = at && i * LR_THREADS + tid < ld ? at[(long long)row * ld + i * LR_THREADS + tid] : LR_NONE;
+    };
+    early(r.prompt, r.prompt_ld, ids[0]);
+    early(r.output, r.output_ld, ids[1]);
+    int lens[2] = {r.prompt ? r.prompt_len[row * r.prompt_len_stride] : 0, r.output ? r.output_len[row * r.output_len_stride] : 0};
     const float rep = r.repetition ? r.repetition[row] : 1.0f, freq = r.frequency ? r.frequency[row] : 0.0f,
                 pres = r.presence ? r.presence[row] : 0.0f;
-    const bool counts = rep != 1.0f || freq != 0.0f || pres != 0.0f;
     int b0 = 0, b1 = 0;
     if (r.bias_start) {
         b0 = r.bias_start[row]; b1 = r.bias_start[row + 1];
@@ -67,7 +77,11 @@ logit_rules_kernel(const LogitParams p) {
             b0 = b1 = 0;
         }
     }
-    const bool biased = b1 > b0;
+    // this thread's first bias entry
+    const int my_bias = b0 + tid;
+    const uint32_t bias_id = my_bias < b1 ? r.bias_id[my_bias] : LR_NONE;
+    const float bias_value = my_bias < b1 ? r.bias_value[my_bias] : 0.0f;
+    const bool counts = rep != 1.0f || freq != 0.0f || pres != 0.0f, biased = b1 > b0;
     const uint32_t* mask = nullptr;
     if (r.mask) {
         const int m = r.mask_row ? r.mask_row[row] : row;
@@ -84,35 +98,45 @@ logit_rules_kernel(const LogitParams p) {
         allowed[g] = mask && t < n ? mask[(v0 + t) >> 5] >> (t & 31) : 0xfu;
     }
     if (counts || biased) {
-        for (int i = tid * 4; i < p.slice; i += LR_THREADS * 4) {
-            *reinterpret_cast<uint4*>(seen + i) = make_uint4(0u, 0u, 0u, 0u);
-            if (biased) *reinterpret_cast<uint4*>(owner + i) = make_uint4(LR_NONE, LR_NONE, LR_NONE, LR_NONE);
-        }
+        for (int i = tid * 4; i < p.slice; i += LR_THREADS * 4) *reinterpret_cast<uint4*>(seen + i) = make_uint4(0u, 0u, 0u, 0u);
+        if (biased)
+            for (int i = tid * 4; i < p.slice; i += LR_THREADS * 4) *reinterpret_cast<uint4*>(owner + i) = make_uint4(LR_NONE, LR_NONE, LR_NONE, LR_NONE);
         __syncthreads();
+        auto place = [&](uint32_t id) -> uint32_t { return id >= (uint32_t)v0 ? id - (uint32_t)v0 : LR_NONE; };       // (of this slice where below n)
         if (counts) {
-            auto look = [&](const uint32_t* ids, const int* lens, int len_stride, int ld, bool prompt) {
-                if (!ids) return;
-                int len = lens[row * len_stride];
+            auto look = [&](int which, const uint32_t* at, int ld) {
+                if (!at || (which == 0 && rep == 1.0f)) return;
+                int len = lens[which];
                 if (len < 0 || len > ld) {
                     if (tid == 0) atomicExch(p.err, 81);
                     len = min(max(len, 0), ld);
                 }
-                const uint32_t* at = ids + (long long)row * ld;
+                auto one = [&](uint32_t id) {
+                    const uint32_t t = place(id);
+                    if (t >= (uint32_t)n) return;
+                    if (which == 0) atomicOr(&seen[t], LR_PROMPT);
+                    else atomicAdd(&seen[t], 1u);
+                };
+#pragma unroll
+                for (int i = 0; i < LR_IDS; ++i)
+                    if (i * LR_THREADS + tid < len) one(ids[which][i]);
 #pragma unroll 4
-                for (int i = tid; i < len; i += LR_THREADS) {
-                    const uint32_t id = at[i], t = id - (uint32_t)v0;
-                    if (id >= (uint32_t)v0 && t < (uint32_t)n) {
-                        if (prompt) atomicOr(&seen[t], LR_PROMPT);
-                        else atomicAdd(&seen[t], 1u);
-                    }
-                }
+                for (int i = LR_IDS * LR_THREADS + tid; i < len; i += LR_THREADS) one(at[(long long)row * ld + i]);
             };
-            if (rep != 1.0f) look(r.prompt, r.prompt_len, r.prompt_len_stride, r.prompt_ld, true);
-            look(r.output, r.output_len, r.output_len_stride, r.output_ld, false);
+            look(0, r.prompt, r.prompt_ld);
+            look(1, r.output, r.output_ld);
         }
-        for (int i = b0 + tid; i < b1; i += LR_THREADS) {
-            const uint32_t id = r.bias_id[i], t = id - (uint32_t)v0;
-            if (id >= (uint32_t)v0 && t < (uint32_t)n && atomicMin(&owner[t], (uint32_t)i) != LR_NONE) atomicOr(&seen[t], LR_TWICE);
+        if (biased) {
+            for (int i = my_bias; i < b1; i += LR_THREADS) {
+                const uint32_t t = place(i == my_bias ? bias_id : r.bias_id[i]);
+                if (t < (uint32_t)n) atomicOr(&seen[t], atomicMin(&owner[t], (uint32_t)i) != LR_NONE ? LR_TWICE : LR_BIAS);
+            }
+            __syncthreads();
+            // a token's only entry leaves its value in the place of its number
+            for (int i = my_bias; i < b1; i += LR_THREADS) {
+                const uint32_t t = place(i == my_bias ? bias_id : r.bias_id[i]);
+                if (t < (uint32_t)n && !(seen[t] & LR_TWICE)) owner[t] = __float_as_uint(i == my_bias ? bias_value : r.bias_value[i]);
+            }
         }
         __syncthreads();
     }
@@ -136,11 +160,13 @@ logit_rules_kernel(const LogitParams p) {
                 const uint32_t o[4] = {o4.x, o4.y, o4.z, o4.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if (o[i] == LR_NONE) continue;
-                    float sum = r.bias_value[o[i]];
-                    if (w[i] & LR_TWICE)
+                    if (!(w[i] & LR_BIAS)) continue;
+                    float sum = __uint_as_float(o[i]);
+                    if (w[i] & LR_TWICE) {
+                        sum = r.bias_value[o[i]];
                         for (int j = (int)o[i] + 1; j < b1; ++j)
                             if (r.bias_id[j] == (uint32_t)(v0 + t + i)) sum += r.bias_value[j];
+                    }
                     z[g][i] += sum;
                 }
             }
@@ -193,8 +219,8 @@ extern "C" int tb_logits_adjust(const TbLogitRules* rules, const float* d_logits
         TB_CHECK(a1 <= b0 || b1 <= a0, "tb_logits_adjust: the output overlaps the logits");
     }
     const TbLogitRules& r = *rules;
-    TB_CHECK(!r.prompt || (r.prompt_len && r.prompt_ld > 0 && r.prompt_ld < (1 << 30)), "tb_logits_adjust: prompt ids need lengths and a leading dimension below 2^30");
-    TB_CHECK(!r.output || (r.output_len && r.output_ld > 0 && r.output_ld < (1 << 30)), "tb_logits_adjust: output ids need lengths and a leading dimension below 2^30");
+    TB_CHECK(!r.prompt || (r.prompt_len && r.prompt_ld > 0 && r.prompt_ld < (1 << 29)), "tb_logits_adjust: prompt ids need lengths and a leading dimension below 2^29");
+    TB_CHECK(!r.output || (r.output_len && r.output_ld > 0 && r.output_ld < (1 << 29)), "tb_logits_adjust: output ids need lengths and a leading dimension below 2^29");
     TB_CHECK(!r.bias_start || r.bias_entries == 0 || (r.bias_id && r.bias_value), "tb_logits_adjust: bias entries need ids and values");
     TB_CHECK(r.bias_entries >= 0, "tb_logits_adjust: bias_entries must not be negative");
     TB_CHECK(!r.mask || (r.masks > 0 && r.mask_ld >= (vocab + 31) / 32), "tb_logits_adjust: masks need %d words each", (vocab + 31) / 32);

@@ -45,18 +45,19 @@ __device__ __forceinline__ int sequence_of(const int* __restrict__ start, int se
     }
 }
 
-// x / scale as the nearest 8-bit float (4 exponent bits, 3 of significand), halves to the even one.  The quotient of float32
-// numbers is rounded already; where it was, its last bit is set instead (a number strictly between two floats keeps to its side
-// of every middle of two codes), so that the code is the one nearest to the true quotient.
-__device__ __forceinline__ float quotient_to_odd(float x, float scale) {
-    const float q = __fdiv_rn(x, scale);
+// x / scale on its way to the nearest 8-bit float (4 exponent bits, 3 of significand; halves to the even one): a float32 that lies on the
+// same side of every middle of two codes as the true quotient.  q is within a unit of its last place of that, its remainder tells on which
+// side, and a number strictly between two floats becomes the one of them whose last bit is set, which no middle has.
+__device__ __forceinline__ float quotient_to_odd(float x, float scale, float inverse) {
+    const float q0 = x * inverse;
+    const float q = __fmaf_rn(__fmaf_rn(-q0, scale, x), inverse, q0);
     const float rest = __fmaf_rn(-q, scale, x);
     uint32_t b = __float_as_uint(q);
-    if (rest != 0.0f && fabsf(q) < INFINITY) {
-        if ((rest < 0.0f) != (x < 0.0f) && (b & 0x7fffffffu) != 0u) b -= 1u;      // |q| was rounded up
+    if (rest != 0.0f) {
+        if ((__float_as_uint(rest) ^ __float_as_uint(x)) >> 31 && (b & 0x7fffffffu) != 0u) b -= 1u;      // |q| is too large
         b |= 1u;
     }
-    return __uint_as_float(b);
+    return __uint_as_float((b & 0x7fffffffu) | (__float_as_uint(x) & 0x80000000u));      // (zeros keep their sign)
 }
 __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
     uint16_t r;
