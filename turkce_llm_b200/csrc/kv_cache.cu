@@ -162,6 +162,7 @@ kv_append_kernel(const AppendParams p) {
                 const bool turns = HALVES ? e < 2 * p.half : e < p.half;
                 c[k] = turns ? __ldg(ct + at) : 1.f;
                 d[k] = turns ? __ldg(st + at) : 0.f;
+                if (HALVES && e < p.half) d[k] = -d[k];          // a cos - b sin as a cos + b (-sin): the same rounding
             }
         }
 #pragma unroll 1
@@ -182,12 +183,11 @@ kv_append_kernel(const AppendParams p) {
                         }
                     }
                 } else if (by_lane) {
-                    const bool low = e0 < p.half, rotated = turns && e0 < 2 * p.half;
+                    const bool rotated = turns && e0 < 2 * p.half;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const float other = __shfl_sync(0xffffffffu, x[k], other_lane);
-                        const float y = low ? __fsub_rn(__fmul_rn(x[k], c[k]), __fmul_rn(other, d[k]))
-                                            : __fadd_rn(__fmul_rn(other, d[k]), __fmul_rn(x[k], c[k]));
+                        const float y = __fadd_rn(__fmul_rn(x[k], c[k]), __fmul_rn(other, d[k]));
                         if (rotated) x[k] = y;
                     }
                 } else {
@@ -201,11 +201,9 @@ kv_append_kernel(const AppendParams p) {
                     for (int k = 0; k < 8; ++k) {
                         const int e = e0 + k;
                         if (mine && turns && e < 2 * p.half) {
-                            const bool low = e < p.half;
-                            const int o = low ? e + p.half : e - p.half;
+                            const int o = e < p.half ? e + p.half : e - p.half;
                             const float other = sw[base + (o >> 3) * 9 + (o & 7)];
-                            x[k] = low ? __fsub_rn(__fmul_rn(x[k], c[k]), __fmul_rn(other, d[k]))
-                                       : __fadd_rn(__fmul_rn(other, d[k]), __fmul_rn(x[k], c[k]));
+                            x[k] = __fadd_rn(__fmul_rn(x[k], c[k]), __fmul_rn(other, d[k]));
                         }
                     }
                     __syncwarp();
@@ -267,7 +265,8 @@ kv_read_kernel(const ReadParams p) {
     const int count = min(p.per_warp, p.rows - row0);
     const int hd = p.v.hd, G = p.v.heads, all = p.kinds * G;
     const int heads_of_warp = 32 >> p.threads_log2, step = heads_of_warp * p.parts;
-    const int e0 = (lane & ((1 << p.threads_log2) - 1)) * 8;
+    constexpr int EPT = E4M3 ? 16 : 8;                           // elements per thread: 16 bytes of the cache
+    const int e0 = (lane & ((1 << p.threads_log2) - 1)) * EPT;
     // ---- lane i: the place in the cache of row row0 + i
     const RowsOf mine_of = rows_of(p.start, p.first, p.v.seqs, row0, count);
     long long my_slot = -1;
@@ -300,30 +299,27 @@ kv_read_kernel(const ReadParams p) {
             if (slot >= 0 && k0 + j < total && head < all && e0 < hd) {
                 to[j] = (long long)(row0 + i) * p.ld_row + h * p.ld_head + e0;
                 const long long at = slot + ((long long)h << p.v.page_shift);
-                if (!E4M3) {
-                    in[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const bf16*>(second[j] ? p.B : p.A) + at * hd + e0));
-                } else {
-                    const uint2 c = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(second[j] ? p.B : p.A) + at * hd + e0));
-                    in[j].x = c.x; in[j].y = c.y;
-                    scale[j] = __ldg((second[j] ? p.bs : p.as) + at);
-                }
+                in[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(second[j] ? p.B : p.A) + (at * hd + e0) * (E4M3 ? 1 : 2)));
+                if (E4M3) scale[j] = __ldg((second[j] ? p.bs : p.as) + at);
             }
         }
 #pragma unroll
         for (int j = 0; j < ROUND; ++j) {
             if (to[j] < 0) continue;
-            uint4 out = in[j];
+            uint4* o16 = reinterpret_cast<uint4*>((second[j] ? p.oB : p.oA) + to[j]);
             if (E4M3) {
-                const uint32_t u[4] = {in[j].x & 0xffffu, in[j].x >> 16, in[j].y & 0xffffu, in[j].y >> 16};
-                uint32_t o[4];
+                const uint32_t u[4] = {in[j].x, in[j].y, in[j].z, in[j].w};
+                uint32_t o[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = e4m3_floats(u[i]);
+                for (int i = 0; i < 8; ++i) {
+                    const float2 f = e4m3_floats(i & 1 ? u[i >> 1] >> 16 : u[i >> 1] & 0xffffu);
                     o[i] = bf16_pair(f.x * scale[j], f.y * scale[j]);
                 }
-                out = make_uint4(o[0], o[1], o[2], o[3]);
+                o16[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                o16[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            } else {
+                o16[0] = in[j];
             }
-            *reinterpret_cast<uint4*>((second[j] ? p.oB : p.oA) + to[j]) = out;
         }
     }
 }
@@ -331,9 +327,9 @@ kv_read_kernel(const ReadParams p) {
 // threads per head (a power of two that divides a warp), and how rows are dealt to warps: what a warp finds out about a sequence
 // serves up to four rows, where that leaves sixteen warps for every SM; where there are fewer rows than eight for every SM, a row's
 // groups of heads go to different warps.
-void shape_of(const DeviceCtx* ctx, int hd, int heads, int rows, int* threads_log2, int* per_warp, int* parts, long long* blocks) {
+void shape_of(const DeviceCtx* ctx, int hd, int elements, int heads, int rows, int* threads_log2, int* per_warp, int* parts, long long* blocks) {
     int t = 0;
-    while ((8 << t) < hd) ++t;
+    while ((elements << t) < hd) ++t;
     *threads_log2 = t;
     const int in_warp = 32 >> t, groups = (heads + in_warp - 1) / in_warp;
     *parts = (int)std::max<long long>(1, std::min<long long>(groups, 8LL * ctx->sm_count / rows));
@@ -352,7 +348,7 @@ int launch_kv_append(DeviceCtx* ctx, const TbKvCache* c, const int* q_start, con
     p.cos_t = cos_t; p.sin_t = sin_t; p.positions = positions; p.half = rot_dim / 2;
     p.Q = Q; p.ld_q = ld_q; p.K = c->K; p.V = c->V; p.ks = c->k_scale; p.vs = c->v_scale; p.err = ctx->d_err;
     long long blocks;
-    shape_of(ctx, c->head_dim, H + 2 * c->heads, rows, &p.threads_log2, &p.per_warp, &p.parts, &blocks);
+    shape_of(ctx, c->head_dim, 8, H + 2 * c->heads, rows, &p.threads_log2, &p.per_warp, &p.parts, &blocks);
     TB_CHECK(blocks < (1LL << 31) / KV_WARPS, "tb_kv_append: too many rows");
     typedef void (*Kernel)(AppendParams);
     const bool halves = form == TB_ROPE_HALVES && rot_dim > 0, e4m3 = c->type == TB_KV_E4M3;
@@ -377,7 +373,7 @@ int launch_kv_read(DeviceCtx* ctx, const TbKvCache* c, const int* start, const i
     p.B = c->V; p.bs = c->v_scale; p.oB = V;
     p.ld_row = ld_row; p.ld_head = ld_head; p.err = ctx->d_err;
     long long blocks;
-    shape_of(ctx, c->head_dim, p.kinds * c->heads, rows, &p.threads_log2, &p.per_warp, &p.parts, &blocks);
+    shape_of(ctx, c->head_dim, c->type == TB_KV_E4M3 ? 16 : 8, p.kinds * c->heads, rows, &p.threads_log2, &p.per_warp, &p.parts, &blocks);
     TB_CHECK(blocks < (1LL << 31) / KV_WARPS, "tb_kv_read: too many rows");
     const bool e4m3 = c->type == TB_KV_E4M3;
     prof_mark(ctx, "kv_read", 0.0, (double)rows * p.kinds * c->heads * c->head_dim * (e4m3 ? 3 : 4), st);

@@ -20,6 +20,7 @@ constexpr uint32_t LR_TWICE = 0x20000000u;       // more than one; the rest coun
 constexpr uint32_t LR_COUNT = 0x1fffffffu;
 constexpr int LR_IDS = 4;                        // ids of the prompt and of the output that a thread asks for at once
 constexpr uint32_t LR_NONE = 0xffffffffu;
+constexpr int LR_AGAIN = 64;
 constexpr int LR_ROUNDS = kLogitSlice / (LR_THREADS * 4);
 
 struct LogitParams {
@@ -31,31 +32,39 @@ struct LogitParams {
 };
 
 // The logits of a slice are asked for first and held in registers while the ids are counted: the two share the time of one trip
-// to memory.  (Counting first and reading then: 49 us for 256 rows of 31,769 with 750 ids and 150 biases each, against XX.)
+// to memory.  (Counting first and reading then: 49 us for 256 rows of 31,769 with 750 ids and 150 biases each.)
+// WIDE: rows of logits and result that begin at the same place of a 16-byte piece, whatever it is: a CTA's slice begins at a whole piece, up
+// to three columns in front of a multiple of the slice, and a thread has four neighbours.  Else a thread has every 256th column.  (Rows of
+// 31,769 begin at another place each: four neighbours in single accesses took 31.6 us.)
 template <bool WIDE>
 __global__ void __launch_bounds__(LR_THREADS)
 logit_rules_kernel(const LogitParams p) {
     extern __shared__ uint32_t lr_smem[];
     uint32_t* seen = lr_smem;                                    // [slice]
-    uint32_t* owner = lr_smem + p.slice;                         // [slice]: the number of the token's first bias entry, or the value of its only one
+    float* bias = reinterpret_cast<float*>(lr_smem + p.slice);   // [slice], where LR_BIAS is set
+    __shared__ int again, again_at[LR_AGAIN];                    // tokens with more than one bias entry
     pdl_wait();
     pdl_launch_dependents();
     const int row = blockIdx.y, tid = threadIdx.x;
-    const int v0 = blockIdx.x * p.slice, n = min(p.slice, p.V - v0);
     const LogitRuleArgs& r = p.r;
-    const float* in = p.in + (long long)row * p.ld_in + v0;
-    float* out = p.out + (long long)row * p.ld_out + v0;
-    // four columns per thread and round: slices start at multiples of 32, so that they share a mask word
+    const float* in = p.in + (long long)row * p.ld_in;
+    float* out = p.out + (long long)row * p.ld_out;
+    // columns v0 .. v0 + slice - 1, those that exist
+    const int v0 = (int)blockIdx.x * p.slice - (WIDE ? (int)(reinterpret_cast<uintptr_t>(in) >> 2 & 3u) : 0);
+    const int lo = max(-v0, 0), n = min(p.slice, p.V - v0);
+    if (n <= 0) return;
+    in += v0; out += v0;
+    auto column = [&](int g, int i) { return WIDE ? (g * LR_THREADS + tid) * 4 + i : (g * 4 + i) * LR_THREADS + tid; };
+    auto whole = [&](int t) { return WIDE && t >= lo && t + 4 <= n; };       // four columns that all exist
     float z[LR_ROUNDS][4];
 #pragma unroll
     for (int g = 0; g < LR_ROUNDS; ++g) {
-        const int t = (g * LR_THREADS + tid) * 4;
-        if (WIDE && t + 4 <= n) {
-            const float4 w = *reinterpret_cast<const float4*>(in + t);
+        if (whole(column(g, 0))) {
+            const float4 w = *reinterpret_cast<const float4*>(in + column(g, 0));
             z[g][0] = w.x; z[g][1] = w.y; z[g][2] = w.z; z[g][3] = w.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[g][i] = t + i < n ? in[t + i] : 0.0f;
+            for (int i = 0; i < 4; ++i) z[g][i] = column(g, i) >= lo && column(g, i) < n ? in[column(g, i)] : 0.0f;
         }
     }
     // The first ids of the row as well, before it is known how many count: lengths, ids and logits come in the same time.
@@ -91,18 +100,29 @@ logit_rules_kernel(const LogitParams p) {
             mask = r.mask + (long long)m * r.mask_ld;
         }
     }
-    uint32_t allowed[LR_ROUNDS];
+    uint32_t allowed = 0xffffffffu;                              // bit 4 g + i
+    if (mask) {
+        allowed = 0u;
 #pragma unroll
-    for (int g = 0; g < LR_ROUNDS; ++g) {
-        const int t = (g * LR_THREADS + tid) * 4;
-        allowed[g] = mask && t < n ? mask[(v0 + t) >> 5] >> (t & 31) : 0xfu;
+        for (int g = 0; g < LR_ROUNDS; ++g) {
+            if (whole(column(g, 0))) {
+                const int v = v0 + column(g, 0), bit = v & 31;
+                const uint32_t a = mask[v >> 5], b = bit > 28 ? mask[(v >> 5) + 1] : 0u;
+                allowed |= (__funnelshift_r(a, b, bit) & 0xfu) << (4 * g);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = column(g, i);
+                    if (t >= lo && t < n) allowed |= (mask[(v0 + t) >> 5] >> ((v0 + t) & 31) & 1u) << (4 * g + i);
+                }
+            }
+        }
     }
     if (counts || biased) {
         for (int i = tid * 4; i < p.slice; i += LR_THREADS * 4) *reinterpret_cast<uint4*>(seen + i) = make_uint4(0u, 0u, 0u, 0u);
-        if (biased)
-            for (int i = tid * 4; i < p.slice; i += LR_THREADS * 4) *reinterpret_cast<uint4*>(owner + i) = make_uint4(LR_NONE, LR_NONE, LR_NONE, LR_NONE);
+        if (tid == 0) again = 0;
         __syncthreads();
-        auto place = [&](uint32_t id) -> uint32_t { return id >= (uint32_t)v0 ? id - (uint32_t)v0 : LR_NONE; };       // (of this slice where below n)
+        auto place = [&](uint32_t id) -> uint32_t { return id < (uint32_t)p.V ? id - (uint32_t)v0 : LR_NONE; };       // (of this slice where below n)
         if (counts) {
             auto look = [&](int which, const uint32_t* at, int ld) {
                 if (!at || (which == 0 && rep == 1.0f)) return;
@@ -126,60 +146,77 @@ logit_rules_kernel(const LogitParams p) {
             look(0, r.prompt, r.prompt_ld);
             look(1, r.output, r.output_ld);
         }
-        if (biased) {
-            for (int i = my_bias; i < b1; i += LR_THREADS) {
-                const uint32_t t = place(i == my_bias ? bias_id : r.bias_id[i]);
-                if (t < (uint32_t)n) atomicOr(&seen[t], atomicMin(&owner[t], (uint32_t)i) != LR_NONE ? LR_TWICE : LR_BIAS);
-            }
-            __syncthreads();
-            // a token's only entry leaves its value in the place of its number
-            for (int i = my_bias; i < b1; i += LR_THREADS) {
-                const uint32_t t = place(i == my_bias ? bias_id : r.bias_id[i]);
-                if (t < (uint32_t)n && !(seen[t] & LR_TWICE)) owner[t] = __float_as_uint(i == my_bias ? bias_value : r.bias_value[i]);
+        // a token's only entry leaves its value; who finds that there is one already makes a note
+        for (int i = my_bias; i < b1; i += LR_THREADS) {
+            const uint32_t t = place(i == my_bias ? bias_id : r.bias_id[i]);
+            if (t >= (uint32_t)n) continue;
+            const uint32_t before = atomicOr(&seen[t], LR_BIAS);
+            if (!(before & LR_BIAS)) {
+                bias[t] = i == my_bias ? bias_value : r.bias_value[i];
+            } else if (!(atomicOr(&seen[t], LR_TWICE) & LR_TWICE)) {
+                const int k = atomicAdd(&again, 1);
+                if (k < LR_AGAIN) again_at[k] = (int)t;
             }
         }
         __syncthreads();
+        if (again > 0) {
+            // those tokens' entries in the order of the list, a warp per token.  (More of them than there is room for: every token is looked at.)
+            const int lane = tid & 31, count = again <= LR_AGAIN ? again : p.slice;
+            for (int k = tid >> 5; k < count; k += LR_THREADS / 32) {
+                const int t = again <= LR_AGAIN ? again_at[k] : k;
+                if (t >= n || !(seen[t] & LR_TWICE)) continue;
+                float sum = 0.0f;
+                for (int j0 = b0; j0 < b1; j0 += 32) {
+                    const bool same = j0 + lane < b1 && r.bias_id[j0 + lane] == (uint32_t)(v0 + t);
+                    const float value = same ? r.bias_value[j0 + lane] : 0.0f;
+                    for (uint32_t left = __ballot_sync(0xffffffffu, same); left != 0u; left &= left - 1u)
+                        sum += __shfl_sync(0xffffffffu, value, __ffs(left) - 1);
+                }
+                if (lane == 0) bias[t] = sum;
+            }
+            __syncthreads();
+        }
     }
+    const float inverse = __frcp_rn(rep);
+    auto rule = [&](float x, uint32_t w, int t) -> float {
+        if (counts && (w & (LR_COUNT | LR_PROMPT)) != 0u) {
+            // x / rep in two steps (the second one corrects the first by its remainder), x * rep of what is not positive
+            const float q = x * inverse, y = __fmaf_rn(__fmaf_rn(-q, rep, x), inverse, q);
+            x = x > 0.0f ? (q < INFINITY ? y : q) : x * rep;
+            if ((w & LR_COUNT) != 0u) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)(w & LR_COUNT))), pres);
+        }
+        if (w & LR_BIAS) x += bias[t];
+        return x;
+    };
 #pragma unroll
     for (int g = 0; g < LR_ROUNDS; ++g) {
-        const int t = (g * LR_THREADS + tid) * 4;
-        if (t >= n) break;
+        const int t = column(g, 0);
         if (counts || biased) {
-            const uint4 w4 = *reinterpret_cast<const uint4*>(seen + t);
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t c = w[i] & LR_COUNT;
-                if (counts && (w[i] & (LR_COUNT | LR_PROMPT)) != 0u) {
-                    if (rep != 1.0f) z[g][i] = z[g][i] > 0.0f ? __fdiv_rn(z[g][i], rep) : z[g][i] * rep;
-                    if (c != 0u) z[g][i] = __fsub_rn(__fsub_rn(z[g][i], __fmul_rn(freq, (float)c)), pres);
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+            if (WIDE) {
+                if (t < n) {
+                    const uint4 w4 = *reinterpret_cast<const uint4*>(seen + t);
+                    w[0] = w4.x; w[1] = w4.y; w[2] = w4.z; w[3] = w4.w;
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if (column(g, i) < n) w[i] = seen[column(g, i)];
             }
-            if (biased) {
-                const uint4 o4 = *reinterpret_cast<const uint4*>(owner + t);
-                const uint32_t o[4] = {o4.x, o4.y, o4.z, o4.w};
+            // (most columns are touched by no rule)
+            if ((w[0] | w[1] | w[2] | w[3]) != 0u) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (!(w[i] & LR_BIAS)) continue;
-                    float sum = __uint_as_float(o[i]);
-                    if (w[i] & LR_TWICE) {
-                        sum = r.bias_value[o[i]];
-                        for (int j = (int)o[i] + 1; j < b1; ++j)
-                            if (r.bias_id[j] == (uint32_t)(v0 + t + i)) sum += r.bias_value[j];
-                    }
-                    z[g][i] += sum;
-                }
+                for (int i = 0; i < 4; ++i) z[g][i] = rule(z[g][i], w[i], column(g, i));
             }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (!(allowed[g] >> i & 1u)) z[g][i] = -INFINITY;
-        if (WIDE && t + 4 <= n) {
+            if (!(allowed >> (4 * g + i) & 1u)) z[g][i] = -INFINITY;
+        if (whole(t)) {
             *reinterpret_cast<float4*>(out + t) = make_float4(z[g][0], z[g][1], z[g][2], z[g][3]);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (t + i < n) out[t + i] = z[g][i];
+                if (column(g, i) >= lo && column(g, i) < n) out[column(g, i)] = z[g][i];
         }
     }
 }
@@ -191,10 +228,10 @@ int launch_logit_rules(DeviceCtx* ctx, const LogitRuleArgs& r, const float* in, 
     LogitParams p;
     p.r = r; p.in = in; p.ld_in = ld_in; p.out = out; p.ld_out = ld_out; p.V = V; p.err = ctx->d_err;
     p.slice = logit_rules_slice(rows, V, ctx->sm_count);
-    const bool wide = ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0 && ld_in % 4 == 0 && ld_out % 4 == 0;
+    const bool wide = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0 && (rows == 1 || (ld_in - ld_out) % 4 == 0);
     const size_t smem = (size_t)p.slice * 8;
     prof_mark(ctx, "logit_rules", 0.0, 8.0 * rows * V, st);
-    TB_CUDA(launch_kernel(wide ? logit_rules_kernel<true> : logit_rules_kernel<false>, dim3((V + p.slice - 1) / p.slice, rows), dim3(LR_THREADS),
+    TB_CUDA(launch_kernel(wide ? logit_rules_kernel<true> : logit_rules_kernel<false>, dim3((V + (wide ? 3 : 0) + p.slice - 1) / p.slice, rows), dim3(LR_THREADS),
                           smem, st, p));
     ctx->launches++;
     prof_close(ctx, st);
