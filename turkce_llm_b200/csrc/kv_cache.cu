@@ -38,6 +38,8 @@ namespace {
 
 constexpr int KV_THREADS = 256;
 constexpr int KV_WARPS = KV_THREADS / 32;
+constexpr int KV_ROUND = 4;          // (read) groups of heads that a warp asks for at a time
+constexpr int KV_AHEAD = 3;          // (append) groups of heads on their way to a warp
 
 struct AppendParams {
     PagedView v;
@@ -52,20 +54,30 @@ struct AppendParams {
     int* err;
 };
 
+// eight elements as they lie in memory, and as float32
+template <bool BF16_IN> struct Raw8 { uint4 w[BF16_IN ? 1 : 2]; };
+__device__ __forceinline__ void copy_async16(void* to_shared, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to_shared)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 template <bool BF16_IN>
-__device__ __forceinline__ void load8(const void* x, long long at, float (&f)[8]) {
+__device__ __forceinline__ void widen8(const Raw8<BF16_IN>& r, float (&f)[8]) {
     if (BF16_IN) {
-        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(x) + at);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 p = bf16_floats(u[i]);
             f[2 * i] = p.x; f[2 * i + 1] = p.y;
         }
     } else {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
-        const float4 a = p[0], b = p[1];
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint4 w = r.w[BF16_IN ? 0 : i];
+            f[4 * i] = __uint_as_float(w.x); f[4 * i + 1] = __uint_as_float(w.y);
+            f[4 * i + 2] = __uint_as_float(w.z); f[4 * i + 3] = __uint_as_float(w.w);
+        }
     }
 }
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
@@ -99,12 +111,14 @@ __device__ __forceinline__ long long shfl64(long long x, int lane) {
 }
 
 // Rotated elements are a cos - b sin and a sin + b cos with every product rounded, the same sums whichever thread forms them.
-// A warp has p.per_warp rows, or a row's every `parts`-th group of heads; the next group's elements are on their way while it works on
-// one.  Bound: instructions about as much as bytes with an 8-bit cache (XX of 12,600 rows of 12 + 8 heads of 64), else bytes.
+// A warp has p.per_warp rows, or a row's every `parts`-th group of heads.  The groups come through a ring in shared memory, KV_AHEAD of them
+// on their way while it works on one, a thread reading what it asked for itself: with the next group alone on its way, in registers, an SM
+// had 12 KB in flight, and 12,600 rows of 12 + 8 heads of 64 into an 8-bit cache took 31 us.
 template <bool BF16_IN, bool HALVES, bool E4M3>
 __global__ void __launch_bounds__(KV_THREADS)
 kv_append_kernel(const AppendParams p) {
     __shared__ float swap[HALVES ? KV_WARPS : 1][HALVES ? 32 * 9 : 1];
+    __shared__ Raw8<BF16_IN> ring[KV_WARPS][KV_AHEAD + 1][32];
     pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -115,18 +129,30 @@ kv_append_kernel(const AppendParams p) {
     const int hd = p.v.hd, G = p.v.heads, all = p.H + 2 * G;
     const int heads_of_warp = 32 >> p.threads_log2, step = heads_of_warp * p.parts;
     const int e0 = (lane & ((1 << p.threads_log2) - 1)) * 8;     // first of this thread's elements
-    const int first_group = part * heads_of_warp, in_group = lane >> p.threads_log2;
+    const int first_head = part * heads_of_warp + (lane >> p.threads_log2);
+    const int groups = (all - part * heads_of_warp + step - 1) / step, total = count * groups;
     const bool lane_in = e0 < hd;
-    float x[8], nx[8];
-    auto fetch = [&](float (&f)[8], int row, int h) {
-        if (lane_in && h < all) {
-            load8<BF16_IN>(p.x, (long long)row * p.ld_x + e0 + (long long)h * hd, f);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    // the next (row, group of heads) to be asked for, and its place in the ring
+    int next_row = row0, next_head = first_head, asked = 0, place = 0;
+    auto ask = [&]() {
+        if (asked < total && lane_in && next_head < all) {
+            Raw8<BF16_IN>& to = ring[warp][place][lane];
+            if (BF16_IN) {
+                copy_async16(&to, static_cast<const bf16*>(p.x) + (long long)next_row * p.ld_x + (next_head * hd + e0));
+            } else {
+                const float* from = static_cast<const float*>(p.x) + (long long)next_row * p.ld_x + (next_head * hd + e0);
+                copy_async16(&to, from);
+                copy_async16(reinterpret_cast<uint4*>(&to) + 1, from + 4);
+            }
         }
+        copy_async_commit();
+        ++asked;
+        place = place == KV_AHEAD ? 0 : place + 1;
+        next_head += step;
+        if (next_head - first_head >= groups * step) { next_head = first_head; ++next_row; }
     };
-    fetch(x, row0, first_group + in_group);                      // (needs nothing of the batch)
+#pragma unroll
+    for (int j = 0; j < KV_AHEAD; ++j) ask();                    // (needs nothing of the batch)
     // ---- lane i: position and place in the cache of row row0 + i
     const RowsOf mine_of = rows_of(p.q_start, p.kv_len, p.v.seqs, row0, count);
     long long my_pos = (long long)mine_of.len - mine_of.end + row0 + lane, my_slot = -1;
@@ -143,35 +169,45 @@ kv_append_kernel(const AppendParams p) {
     // partners a whole number of threads apart change hands in registers, others through shared memory
     const bool by_lane = HALVES && (p.half & 7) == 0;
     const int other_lane = e0 < p.half ? lane + (p.half >> 3) : lane - (p.half >> 3);
+    // this thread's angles of the row at hand; they are the same in every head
+    float c[HALVES ? 8 : 4], d[HALVES ? 8 : 4];
+    long long pos = -1, slot = -1;
+    int i = -1, group = groups - 1, at_ring = KV_AHEAD;
 #pragma unroll 1
-    for (int i = 0; i < count; ++i) {
-        const int row = row0 + i;
-        const long long pos = shfl64(my_pos, i), slot = shfl64(my_slot, i);
-        if (pos < 0) {                                           // not of the batch, or out of range
-            if (i + 1 < count) fetch(x, row + 1, first_group + in_group);
-            continue;
-        }
-        // this thread's angles are the same in every head
-        float c[HALVES ? 8 : 4], d[HALVES ? 8 : 4];
-        if (p.half > 0) {
-            const float* ct = p.cos_t + pos * p.half;
-            const float* st = p.sin_t + pos * p.half;
+    for (int k0 = 0; k0 < total; ++k0) {
+        ask();
+        copy_async_wait<KV_AHEAD>();
+        at_ring = at_ring == KV_AHEAD ? 0 : at_ring + 1;
+        if (++group == groups) {
+            group = 0;
+            ++i;
+            pos = shfl64(my_pos, i); slot = shfl64(my_slot, i);
+            if (p.half > 0 && pos >= 0) {
+                const float* ct = p.cos_t + pos * p.half;
+                const float* st = p.sin_t + pos * p.half;
 #pragma unroll
-            for (int k = 0; k < (HALVES ? 8 : 4); ++k) {
-                const int e = HALVES ? e0 + k : (e0 >> 1) + k, at = HALVES && e >= p.half ? e - p.half : e;
-                const bool turns = HALVES ? e < 2 * p.half : e < p.half;
-                c[k] = turns ? __ldg(ct + at) : 1.f;
-                d[k] = turns ? __ldg(st + at) : 0.f;
-                if (HALVES && e < p.half) d[k] = -d[k];          // a cos - b sin as a cos + b (-sin): the same rounding
+                for (int k = 0; k < (HALVES ? 8 : 4); ++k) {
+                    const int e = HALVES ? e0 + k : (e0 >> 1) + k, at = HALVES && e >= p.half ? e - p.half : e;
+                    const bool turns = HALVES ? e < 2 * p.half : e < p.half;
+                    c[k] = turns ? __ldg(ct + at) : 1.f;
+                    d[k] = turns ? __ldg(st + at) : 0.f;
+                    if (HALVES && e < p.half) d[k] = -d[k];      // a cos - b sin as a cos + b (-sin): the same rounding
+                }
             }
         }
-#pragma unroll 1
-        for (int group = first_group; group < all; group += step) {
-            const int head = group + in_group;
+        if (pos < 0) continue;                                   // not of the batch, or out of range
+        {
+            const int head = first_head + group * step, row = row0 + i;
             const bool mine = lane_in && head < all;
-            if (group + step < all) fetch(nx, row, head + step);
-            else if (i + 1 < count) fetch(nx, row + 1, first_group + in_group);
-            if (p.half > 0 && group < p.H + G) {                 // (a group of values alone has nothing to rotate)
+            const int warp_head = head - (lane >> p.threads_log2);   // the warp's first head
+            float x[8];
+            if (mine) {
+                widen8<BF16_IN>(ring[warp][at_ring][lane], x);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = 0.f;
+            }
+            if (p.half > 0 && warp_head < p.H + G) {             // (a group of values alone has nothing to rotate)
                 const bool turns = head < p.H + G;
                 if (!HALVES) {
 #pragma unroll
@@ -202,42 +238,37 @@ kv_append_kernel(const AppendParams p) {
                         const int e = e0 + k;
                         if (mine && turns && e < 2 * p.half) {
                             const int o = e < p.half ? e + p.half : e - p.half;
-                            const float other = sw[base + (o >> 3) * 9 + (o & 7)];
-                            x[k] = __fadd_rn(__fmul_rn(x[k], c[k]), __fmul_rn(other, d[k]));
+                            x[k] = __fadd_rn(__fmul_rn(x[k], c[k]), __fmul_rn(sw[base + (o >> 3) * 9 + (o & 7)], d[k]));
                         }
                     }
                     __syncwarp();
                 }
             }
+            if (warp_head < p.H && mine && head < p.H) *reinterpret_cast<uint4*>(p.Q + (long long)row * p.ld_q + (head * hd + e0)) = pack8(x);
+            if (warp_head + heads_of_warp <= p.H) continue;      // (queries alone)
             // largest magnitude of the row: as integers, so that NaN is larger than infinity and infinity than the rest
             uint32_t big = 0u;
-            if (E4M3 && group + heads_of_warp > p.H) {
+            if (E4M3) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(x[k]) & 0x7fffffffu);
                 for (int o = (1 << p.threads_log2) >> 1; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
             }
-            if (mine && head < p.H) {
-                *reinterpret_cast<uint4*>(p.Q + (long long)row * p.ld_q + (long long)head * hd + e0) = pack8(x);
-            } else if (mine && slot >= 0) {
-                const bool key = head < p.H + G;
-                const long long at = slot + ((long long)(head - p.H - (key ? 0 : G)) << p.v.page_shift);
-                if (!E4M3) {
-                    *reinterpret_cast<uint4*>(static_cast<bf16*>(key ? p.K : p.V) + at * hd + e0) = pack8(x);
-                } else {
-                    float scale = __fdiv_rn(__uint_as_float(big), 448.0f);
-                    if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;          // (stays NaN where it is)
-                    const float inverse = __frcp_rn(scale);
-                    uint32_t q[4];
+            if (!mine || head < p.H || slot < 0) continue;
+            const bool key = head < p.H + G;
+            const long long at = slot + ((head - p.H - (key ? 0 : G)) << p.v.page_shift);
+            if (!E4M3) {
+                *reinterpret_cast<uint4*>(static_cast<bf16*>(key ? p.K : p.V) + at * hd + e0) = pack8(x);
+            } else {
+                float scale = __fdiv_rn(__uint_as_float(big), 448.0f);
+                if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;          // (stays NaN where it is)
+                const float inverse = __frcp_rn(scale);
+                uint32_t q[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        q[k] = e4m3_pair(quotient_to_odd(x[2 * k], scale, inverse), quotient_to_odd(x[2 * k + 1], scale, inverse));
-                    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(key ? p.K : p.V) + at * hd + e0) =
-                        make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
-                    if (e0 == 0) (key ? p.ks : p.vs)[at] = scale;
-                }
+                for (int k = 0; k < 4; ++k)
+                    q[k] = e4m3_pair(quotient_to_odd(x[2 * k], scale, inverse), quotient_to_odd(x[2 * k + 1], scale, inverse));
+                *reinterpret_cast<uint2*>(static_cast<uint8_t*>(key ? p.K : p.V) + at * hd + e0) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+                if (e0 == 0) (key ? p.ks : p.vs)[at] = scale;
             }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = nx[k];
         }
     }
 }
@@ -282,15 +313,14 @@ kv_read_kernel(const ReadParams p) {
     }
     // All (row, group of heads) pairs of the warp, four of them on their way at a time
     const int groups = (all - part * heads_of_warp + step - 1) / step, total = count * groups;
-    constexpr int ROUND = 4;
 #pragma unroll 1
-    for (int k0 = 0; k0 < total; k0 += ROUND) {
-        uint4 in[ROUND];
-        float scale[ROUND];
-        long long to[ROUND];
-        bool second[ROUND];
+    for (int k0 = 0; k0 < total; k0 += KV_ROUND) {
+        uint4 in[KV_ROUND];
+        float scale[KV_ROUND];
+        long long to[KV_ROUND];
+        bool second[KV_ROUND];
 #pragma unroll
-        for (int j = 0; j < ROUND; ++j) {
+        for (int j = 0; j < KV_ROUND; ++j) {
             const int k = min(k0 + j, total - 1), i = k / groups, head = part * heads_of_warp + (k - i * groups) * step + (lane >> p.threads_log2);
             const long long slot = shfl64(my_slot, i);
             second[j] = head >= G;
@@ -304,7 +334,7 @@ kv_read_kernel(const ReadParams p) {
             }
         }
 #pragma unroll
-        for (int j = 0; j < ROUND; ++j) {
+        for (int j = 0; j < KV_ROUND; ++j) {
             if (to[j] < 0) continue;
             uint4* o16 = reinterpret_cast<uint4*>((second[j] ? p.oB : p.oA) + to[j]);
             if (E4M3) {

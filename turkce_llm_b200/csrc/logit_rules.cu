@@ -13,12 +13,12 @@ namespace tb {
 
 namespace {
 
-constexpr int LR_THREADS = 256;
+constexpr int LR_THREADS = 512;
 constexpr uint32_t LR_PROMPT = 0x80000000u;      // bits of a token's word: among the prompt's ids
 constexpr uint32_t LR_BIAS = 0x40000000u;        // a bias entry
 constexpr uint32_t LR_TWICE = 0x20000000u;       // more than one; the rest counts the output ids
 constexpr uint32_t LR_COUNT = 0x1fffffffu;
-constexpr int LR_IDS = 4;                        // ids of the prompt and of the output that a thread asks for at once
+constexpr int LR_IDS = 2;                        // ids of the prompt and of the output that a thread asks for at once
 constexpr uint32_t LR_NONE = 0xffffffffu;
 constexpr int LR_AGAIN = 64;
 constexpr int LR_ROUNDS = kLogitSlice / (LR_THREADS * 4);
@@ -34,7 +34,7 @@ struct LogitParams {
 // The logits of a slice are asked for first and held in registers while the ids are counted: the two share the time of one trip
 // to memory.  (Counting first and reading then: 49 us for 256 rows of 31,769 with 750 ids and 150 biases each.)
 // WIDE: rows of logits and result that begin at the same place of a 16-byte piece, whatever it is: a CTA's slice begins at a whole piece, up
-// to three columns in front of a multiple of the slice, and a thread has four neighbours.  Else a thread has every 256th column.  (Rows of
+// to three columns in front of a multiple of the slice, and a thread has four neighbours.  Else a thread has every 512th column.  (Rows of
 // 31,769 begin at another place each: four neighbours in single accesses took 31.6 us.)
 template <bool WIDE>
 __global__ void __launch_bounds__(LR_THREADS)

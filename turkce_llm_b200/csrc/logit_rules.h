@@ -5,7 +5,7 @@
 
 namespace tb {
 
-constexpr int kLogitSlice = 4096;         // most columns per CTA: four per thread in four rounds
+constexpr int kLogitSlice = 4096;         // most columns per CTA: four per thread in two rounds
 
 // Columns of the vocabulary per CTA: a multiple of 32 (a mask word belongs to one CTA) up to 4096.  As many as give every SM
 // four CTAs, so that few rows spread over the chip and many rows do not read their ids more often than needed.

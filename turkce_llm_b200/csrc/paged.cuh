@@ -52,12 +52,9 @@ __device__ __forceinline__ float quotient_to_odd(float x, float scale, float inv
     const float q0 = x * inverse;
     const float q = __fmaf_rn(__fmaf_rn(-q0, scale, x), inverse, q0);
     const float rest = __fmaf_rn(-q, scale, x);
-    uint32_t b = __float_as_uint(q);
-    if (rest != 0.0f) {
-        if ((__float_as_uint(rest) ^ __float_as_uint(x)) >> 31 && (b & 0x7fffffffu) != 0u) b -= 1u;      // |q| is too large
-        b |= 1u;
-    }
-    return __uint_as_float((b & 0x7fffffffu) | (__float_as_uint(x) & 0x80000000u));      // (zeros keep their sign)
+    const uint32_t b = __float_as_uint(q) & 0x7fffffffu, sign = __float_as_uint(x) & 0x80000000u;
+    const uint32_t too_large = (__float_as_uint(rest) ^ __float_as_uint(x)) >> 31 & (b != 0u ? 1u : 0u);
+    return __uint_as_float((rest != 0.0f ? (b - too_large) | 1u : b) | sign);            // (zeros keep their sign)
 }
 __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
     uint16_t r;
