@@ -115,10 +115,10 @@ __device__ __forceinline__ long long shfl64(long long x, int lane) {
 // on their way while it works on one, a thread reading what it asked for itself: with the next group alone on its way, in registers, an SM
 // had 12 KB in flight, and 12,600 rows of 12 + 8 heads of 64 into an 8-bit cache took 31 us.
 template <bool BF16_IN, bool HALVES, bool E4M3>
-__global__ void __launch_bounds__(KV_THREADS)
+__global__ void __launch_bounds__(KV_THREADS, 3)
 kv_append_kernel(const AppendParams p) {
-    __shared__ float swap[HALVES ? KV_WARPS : 1][HALVES ? 32 * 9 : 1];
     __shared__ Raw8<BF16_IN> ring[KV_WARPS][KV_AHEAD + 1][32];
+    __shared__ float4 angles[KV_WARPS][2][32];                   // cosines, then sines, of this row and the next
     pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -133,23 +133,26 @@ kv_append_kernel(const AppendParams p) {
     const int groups = (all - part * heads_of_warp + step - 1) / step, total = count * groups;
     const bool lane_in = e0 < hd;
     // the next (row, group of heads) to be asked for, and its place in the ring
-    int next_row = row0, next_head = first_head, asked = 0, place = 0;
+    constexpr int SIZE = BF16_IN ? 2 : 4;
+    const char* next = static_cast<const char*>(p.x) + ((long long)row0 * p.ld_x + (first_head * hd + e0)) * SIZE;
+    const int to_next_group = step * hd * SIZE;
+    const long long to_next_row = p.ld_x * SIZE - (long long)(groups - 1) * to_next_group;
+    int next_group = 0, left = total, place = 0;
+    const int last_group = lane_in ? groups - (first_head + (groups - 1) * step < all ? 0 : 1) : 0;      // groups that have this lane's head
     auto ask = [&]() {
-        if (asked < total && lane_in && next_head < all) {
-            Raw8<BF16_IN>& to = ring[warp][place][lane];
-            if (BF16_IN) {
-                copy_async16(&to, static_cast<const bf16*>(p.x) + (long long)next_row * p.ld_x + (next_head * hd + e0));
-            } else {
-                const float* from = static_cast<const float*>(p.x) + (long long)next_row * p.ld_x + (next_head * hd + e0);
-                copy_async16(&to, from);
-                copy_async16(reinterpret_cast<uint4*>(&to) + 1, from + 4);
+        if (left > 0) {
+            if (next_group < last_group) {
+                Raw8<BF16_IN>& to = ring[warp][place][lane];
+                copy_async16(&to, next);
+                if (!BF16_IN) copy_async16(reinterpret_cast<uint4*>(&to) + 1, next + 16);
             }
+            --left;
+            const bool wrap = ++next_group == groups;
+            next += wrap ? to_next_row : (long long)to_next_group;
+            next_group = wrap ? 0 : next_group;
+            place = place == KV_AHEAD ? 0 : place + 1;
         }
         copy_async_commit();
-        ++asked;
-        place = place == KV_AHEAD ? 0 : place + 1;
-        next_head += step;
-        if (next_head - first_head >= groups * step) { next_head = first_head; ++next_row; }
     };
 #pragma unroll
     for (int j = 0; j < KV_AHEAD; ++j) ask();                    // (needs nothing of the batch)
@@ -166,32 +169,56 @@ kv_append_kernel(const AppendParams p) {
         if ((unsigned)page < (unsigned)p.v.pages) my_slot = ((long long)page * G << p.v.page_shift) + (my_pos & ((1 << p.v.page_shift) - 1));
         else atomicExch(p.err, 71);
     }
-    // partners a whole number of threads apart change hands in registers, others through shared memory
+    // (halves) partners are read from the other thread's place in the ring, all eight at once where they are a whole number of threads apart
     const bool by_lane = HALVES && (p.half & 7) == 0;
-    const int other_lane = e0 < p.half ? lane + (p.half >> 3) : lane - (p.half >> 3);
+    const int other_lane = !by_lane || e0 >= 2 * p.half ? lane : e0 < p.half ? lane + (p.half >> 3) : lane - (p.half >> 3);
+    // A row's angles: with the groups of the row before it, where these are enough for them to have arrived.
+    const bool wide_angles = (p.half & 3) == 0, angles_ahead = wide_angles && groups >= KV_AHEAD && p.half > 0;
+    auto ask_angles = [&](int i) {
+        const long long next_pos = shfl64(my_pos, i);
+        const int quads = p.half >> 2;
+        if (next_pos >= 0 && lane < 2 * quads)
+            copy_async16(&angles[warp][i & 1][lane], (lane < quads ? p.cos_t : p.sin_t) + next_pos * p.half + (lane < quads ? lane : lane - quads) * 4);
+    };
     // this thread's angles of the row at hand; they are the same in every head
     float c[HALVES ? 8 : 4], d[HALVES ? 8 : 4];
     long long pos = -1, slot = -1;
     int i = -1, group = groups - 1, at_ring = KV_AHEAD;
 #pragma unroll 1
     for (int k0 = 0; k0 < total; ++k0) {
+        __syncwarp();                                            // (other lanes' elements and angles are read)
+        if (group == groups - 1 && angles_ahead && i + 2 < count) ask_angles(i + 2);
         ask();
         copy_async_wait<KV_AHEAD>();
+        __syncwarp();
         at_ring = at_ring == KV_AHEAD ? 0 : at_ring + 1;
         if (++group == groups) {
             group = 0;
             ++i;
             pos = shfl64(my_pos, i); slot = shfl64(my_slot, i);
             if (p.half > 0 && pos >= 0) {
-                const float* ct = p.cos_t + pos * p.half;
-                const float* st = p.sin_t + pos * p.half;
-#pragma unroll
-                for (int k = 0; k < (HALVES ? 8 : 4); ++k) {
-                    const int e = HALVES ? e0 + k : (e0 >> 1) + k, at = HALVES && e >= p.half ? e - p.half : e;
+                // (the same angles in memory and in the ring: generic addresses)
+                const float* ct = angles_ahead && i > 0 ? reinterpret_cast<const float*>(angles[warp][i & 1]) : p.cos_t + pos * p.half;
+                const float* st = angles_ahead && i > 0 ? ct + p.half : p.sin_t + pos * p.half;
+                if (HALVES ? by_lane : wide_angles) {
+                    const int e = HALVES ? e0 : e0 >> 1, at = HALVES && e >= p.half ? e - p.half : e;
                     const bool turns = HALVES ? e < 2 * p.half : e < p.half;
-                    c[k] = turns ? __ldg(ct + at) : 1.f;
-                    d[k] = turns ? __ldg(st + at) : 0.f;
-                    if (HALVES && e < p.half) d[k] = -d[k];      // a cos - b sin as a cos + b (-sin): the same rounding
+                    const float flip = HALVES && e < p.half ? -1.f : 1.f;        // a cos - b sin as a cos + b (-sin): the same rounding
+#pragma unroll
+                    for (int k = 0; k < (HALVES ? 8 : 4); k += 4) {
+                        const float4 x = turns ? *reinterpret_cast<const float4*>(ct + at + k) : make_float4(1.f, 1.f, 1.f, 1.f);
+                        const float4 y = turns ? *reinterpret_cast<const float4*>(st + at + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        c[k] = x.x; c[k + 1] = x.y; c[k + 2] = x.z; c[k + 3] = x.w;
+                        d[k] = y.x * flip; d[k + 1] = y.y * flip; d[k + 2] = y.z * flip; d[k + 3] = y.w * flip;
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < (HALVES ? 8 : 4); ++k) {
+                        const int e = HALVES ? e0 + k : (e0 >> 1) + k, at = HALVES && e >= p.half ? e - p.half : e;
+                        const bool turns = HALVES ? e < 2 * p.half : e < p.half;
+                        c[k] = turns ? ct[at] : 1.f;
+                        d[k] = turns ? (HALVES && e < p.half ? -st[at] : st[at]) : 0.f;
+                    }
                 }
             }
         }
@@ -219,29 +246,24 @@ kv_append_kernel(const AppendParams p) {
                         }
                     }
                 } else if (by_lane) {
-                    const bool rotated = turns && e0 < 2 * p.half;
+                    if (mine && turns && e0 < 2 * p.half) {
+                        float other[8];
+                        widen8<BF16_IN>(ring[warp][at_ring][other_lane], other);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float other = __shfl_sync(0xffffffffu, x[k], other_lane);
-                        const float y = __fadd_rn(__fmul_rn(x[k], c[k]), __fmul_rn(other, d[k]));
-                        if (rotated) x[k] = y;
+                        for (int k = 0; k < 8; ++k) x[k] = __fadd_rn(__fmul_rn(x[k], c[k]), __fmul_rn(other[k], d[k]));
                     }
                 } else {
-                    // element e of this head at (e / 8) * 9 + e % 8 from the head's first
-                    float* sw = swap[warp];
-                    const int base = (lane >> p.threads_log2 << p.threads_log2) * 9;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) sw[lane * 9 + k] = x[k];
-                    __syncwarp();
+                    const int first_lane = lane >> p.threads_log2 << p.threads_log2;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int e = e0 + k;
                         if (mine && turns && e < 2 * p.half) {
                             const int o = e < p.half ? e + p.half : e - p.half;
-                            x[k] = __fadd_rn(__fmul_rn(x[k], c[k]), __fmul_rn(sw[base + (o >> 3) * 9 + (o & 7)], d[k]));
+                            const Raw8<BF16_IN>* from = &ring[warp][at_ring][first_lane + (o >> 3)];
+                            const float other = BF16_IN ? __bfloat162float(reinterpret_cast<const bf16*>(from)[o & 7]) : reinterpret_cast<const float*>(from)[o & 7];
+                            x[k] = __fadd_rn(__fmul_rn(x[k], c[k]), __fmul_rn(other, d[k]));
                         }
                     }
-                    __syncwarp();
                 }
             }
             if (warp_head < p.H && mine && head < p.H) *reinterpret_cast<uint4*>(p.Q + (long long)row * p.ld_q + (head * hd + e0)) = pack8(x);
@@ -259,9 +281,8 @@ kv_append_kernel(const AppendParams p) {
             if (!E4M3) {
                 *reinterpret_cast<uint4*>(static_cast<bf16*>(key ? p.K : p.V) + at * hd + e0) = pack8(x);
             } else {
-                float scale = __fdiv_rn(__uint_as_float(big), 448.0f);
-                if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;          // (stays NaN where it is)
-                const float inverse = __frcp_rn(scale);
+                float inverse;
+                const float scale = e4m3_scale(__uint_as_float(big), &inverse);
                 uint32_t q[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)

@@ -52,9 +52,22 @@ __device__ __forceinline__ float quotient_to_odd(float x, float scale, float inv
     const float q0 = x * inverse;
     const float q = __fmaf_rn(__fmaf_rn(-q0, scale, x), inverse, q0);
     const float rest = __fmaf_rn(-q, scale, x);
-    const uint32_t b = __float_as_uint(q) & 0x7fffffffu, sign = __float_as_uint(x) & 0x80000000u;
-    const uint32_t too_large = (__float_as_uint(rest) ^ __float_as_uint(x)) >> 31 & (b != 0u ? 1u : 0u);
-    return __uint_as_float((rest != 0.0f ? (b - too_large) | 1u : b) | sign);            // (zeros keep their sign)
+    // (|q| too large: the remainder has the other sign.  Where q is 0 the remainder is x.)
+    const uint32_t b = __float_as_uint(q), too_large = (__float_as_uint(rest) ^ __float_as_uint(x)) >> 31;
+    const uint32_t odd = rest != 0.0f ? (b - too_large) | 1u : b;
+    return __uint_as_float((odd & 0x7fffffffu) | (__float_as_uint(x) & 0x80000000u));      // (zeros keep their sign)
+}
+// the scale of an 8-bit row from its largest magnitude: the nearest float32 to big / 448, at least the smallest normal number, and about its
+// inverse (quotient_to_odd corrects what that is off)
+__device__ __forceinline__ float e4m3_scale(float big, float* inverse) {
+    const float one = 1.0f / 448.0f;                             // rounded; a quotient by it corrected by its remainder is the nearest
+    const float q = big * one;
+    float scale = __fmaf_rn(__fmaf_rn(-q, 448.0f, big), one, q);
+    if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;        // (stays NaN where it is)
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
+    *inverse = r;
+    return scale;
 }
 __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
     uint16_t r;
