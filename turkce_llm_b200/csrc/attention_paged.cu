@@ -692,15 +692,16 @@ constexpr int PT_TILE = 128 * 128;                      // bytes of a [128][64] 
 template <int NH, bool E4M3>
 struct ChunkShape {
     static constexpr int THREADS = E4M3 ? 448 : 320;
-    static constexpr int VST = NH == 2 && E4M3 ? 1 : 2;                  // stages of values
+    static constexpr int KST = NH == 2 && E4M3 ? 1 : 2, VST = KST;       // stages of keys and of values
     static constexpr int RAW = PT_KEYS * 64 * NH;                        // bytes of a block's codes
-    static constexpr int O_K = NH * PT_TILE, O_V = O_K + 2 * NH * PT_TILE, O_P = O_V + VST * NH * PT_TILE, O_RAW = O_P + 2 * PT_TILE;
-    static constexpr int O_SCALE = O_RAW + (E4M3 ? 2 * RAW : 0);         // scales as they come in: keys' and values', [2][128]
-    static constexpr int O_KS = O_SCALE + (E4M3 ? 2 * PT_KEYS * 4 : 0);  // [4][128] key scales * scale_log2
+    static constexpr int O_K = NH * PT_TILE, O_V = O_K + KST * NH * PT_TILE, O_P = O_V + VST * NH * PT_TILE, O_RAW = O_P + 2 * PT_TILE;
+    // (8 bits) codes as they come in: two stages of keys and two of values; their scales, [2][2][128]
+    static constexpr int O_SCALE = O_RAW + (E4M3 ? 4 * RAW : 0);
+    static constexpr int O_KS = O_SCALE + (E4M3 ? 4 * PT_KEYS * 4 : 0);  // [4][128] key scales * scale_log2
     static constexpr int O_RF = O_KS + (E4M3 ? 4 * PT_KEYS * 4 : 0);     // [128] row factors
     static constexpr int O_BARS = O_RF + (E4M3 ? PT_ROWS * 4 : 0);
     // (bf16 heads of 64: exactly what lets two CTAs share an SM; 256 bytes of barriers behind the tiles or in the alignment's pad)
-    static constexpr int SMEM = 1024 + O_BARS + (NH == 1 && !E4M3 ? 0 : 256);
+    static constexpr int SMEM = 1024 + O_BARS + (NH == 1 && !E4M3 ? 0 : E4M3 ? 384 : 256);
     static constexpr int PER_SM = SMEM <= 113 * 1024 ? 2 : 1;
     static constexpr int TMEM = NH == 1 ? 256 : 512;
 };
@@ -847,7 +848,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                    const uint8_t* __restrict__ pool_v, const PagedChunkParams pp) {
     typedef ChunkShape<NH, E4M3> Sh;
     const PagedAttParams& p = pp.a;
-    constexpr int VST = Sh::VST;
+    constexpr int KST = Sh::KST, VST = Sh::VST;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
     uint8_t* smem = smem_raw + pad;
@@ -864,9 +865,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     uint64_t* s_free = bars + 13;     // 2
     uint64_t* p_full = bars + 15;     // 2
     uint64_t* o_full = bars + 17;     // 2
-    uint64_t* raw_full = bars + 19;   // (8 bits) 2: codes of keys with all scales, codes of values
-    uint64_t* raw_empty = bars + 21;  // 2
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+    uint64_t* raw_full = bars + 32;   // (8 bits) 2 x 2: codes of keys with all scales, codes of values; behind the 256 bytes of the rest
+    uint64_t* raw_empty = bars + 36;  // 2 x 2
+    uint64_t* ks_full = bars + 40;    // 4: what the softmax warps read of a block's scales.  (Not k_full, which may be a whole round ahead of them.)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* bad_value = abort_flag + 1;                              // a value that is not finite has been set to zero
     volatile int* v_exponent = abort_flag + 2;                             // (8 bits) the last block's reference
@@ -921,8 +923,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             mbar_init(&k_full[i], E4M3 ? 4 : 1); mbar_init(&v_full[i], E4M3 ? 4 : 1);
             mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1);
-            mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4);
+            if (E4M3)
+                for (int x = 0; x < 2; ++x) { mbar_init(&raw_full[2 * i + x], 1); mbar_init(&raw_empty[2 * i + x], 4); }
         }
+        if (E4M3)
+            for (int i = 0; i < 4; ++i) mbar_init(&ks_full[i], 4);
         *abort_flag = 0; *bad_value = 0; *v_exponent = 0;
         fence_mbar_init();
     }
@@ -1001,18 +1006,19 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
             } else {
                 for (int x = 0; x < 2 && ok; ++x) {
-                    ok = mbar_wait(&raw_empty[x], (uint32_t)(j & 1) ^ 1u, abort_flag);
+                    uint64_t* bar = &raw_full[2 * x + st];
+                    ok = mbar_wait(&raw_empty[2 * x + st], (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    if (lane == 0) mbar_expect_tx(&raw_full[x], (uint32_t)(count * piece_keys * (64 * NH + (x == 0 ? 8 : 0))));
+                    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(count * piece_keys * (64 * NH + (x == 0 ? 8 : 0))));
                     __syncwarp();
                     if (lane < count) {
-                        tma_load_3d(smem + Sh::O_RAW + x * Sh::RAW + o * 64 * NH, x == 0 ? &tmK : &tmV, &raw_full[x], 0, r0, block);
+                        tma_load_3d(smem + Sh::O_RAW + (2 * x + st) * Sh::RAW + o * 64 * NH, x == 0 ? &tmK : &tmV, bar, 0, r0, block);
                         if (x == 0) {
-                            float* sc = reinterpret_cast<float*>(smem + Sh::O_SCALE) + o;
+                            float* sc = reinterpret_cast<float*>(smem + Sh::O_SCALE) + st * 2 * PT_KEYS + o;
                             const long long row = ((long long)block << p.v.page_shift) + r0;
-                            bulk_load(sc, p.ks + row, (uint32_t)piece_keys * 4u, &raw_full[0]);
-                            bulk_load(sc + PT_KEYS, p.vs + row, (uint32_t)piece_keys * 4u, &raw_full[0]);
+                            bulk_load(sc, p.ks + row, (uint32_t)piece_keys * 4u, bar);
+                            bulk_load(sc + PT_KEYS, p.vs + row, (uint32_t)piece_keys * 4u, bar);
                         }
                     }
                     __syncwarp();
@@ -1032,8 +1038,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const int nsub = 2 * nkv;
             bool ok = mbar_wait(E4M3 ? q_ready : q_full, 0, abort_flag);
             auto issue_scores = [&](int i) -> bool {
-                const int j = i >> 1, st = j & 1, b = i & 1;
-                if (b == 0 && !mbar_wait(&k_full[st], (uint32_t)((j >> 1) & 1), abort_flag)) return false;
+                const int j = i >> 1, st = j % KST, b = i & 1;
+                if (b == 0 && !mbar_wait(&k_full[st], (uint32_t)((j / KST) & 1), abort_flag)) return false;
                 if (!mbar_wait(&s_free[b], (uint32_t)((i >> 1) & 1) ^ 1u, abort_flag)) return false;
                 tc_fence_after();
                 const uint64_t dK = dK0 + (uint64_t)(st * NH) * TILE + (uint64_t)b * (TILE / 2);
@@ -1048,7 +1054,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (ok) ok = issue_scores(0) && issue_scores(1);
             for (int i = 0; i < nsub && ok; ++i) {
                 const int j = i >> 1, b = i & 1, vst = j % VST;
-                if (i + 2 < nsub && !issue_scores(i + 2)) { ok = false; break; }
+                // (with one stage of keys the next block's are still being turned into f16: this product first)
+                if (KST > 1 && i + 2 < nsub && !issue_scores(i + 2)) { ok = false; break; }
                 if (!mbar_wait(&p_full[b], (uint32_t)(j & 1), abort_flag)) { ok = false; break; }
                 if (b == 0 && !mbar_wait(&v_full[vst], (uint32_t)((j / VST) & 1), abort_flag)) { ok = false; break; }
                 tc_fence_after();
@@ -1058,6 +1065,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     umma_bf16(tO + (uint32_t)(b * 64 * NH), dP + k * KSTEP, dV + k * MNSTEP, idesc_o, (i > 1 || k > 0) ? 1u : 0u);
                 umma_commit(&o_full[b]);
                 if (b == 1) umma_commit(&v_empty[vst]);
+                if (KST == 1 && i + 2 < nsub && !issue_scores(i + 2)) { ok = false; break; }
             }
             if (!ok) { *abort_flag = 1; atomicExch(p.err, 78); }
         }
@@ -1077,7 +1085,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             c1 = reinterpret_cast<const float*>(smem + Sh::O_RF)[r];
         }
         for (int j = 0; j < nkv && ok; ++j) {
-            if (E4M3 && !mbar_wait(&k_full[j & 1], (uint32_t)((j >> 1) & 1), abort_flag)) { ok = false; break; }
+            if (E4M3 && !mbar_wait(&ks_full[j & 3], (uint32_t)((j >> 2) & 1), abort_flag)) { ok = false; break; }
             if (!mbar_wait(&s_full[b], (uint32_t)(j & 1), abort_flag)) { ok = false; break; }
             tc_fence_after();
             tmem_ld32(ts, v[0]);
@@ -1333,23 +1341,22 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (lane == 0) mbar_arrive(q_ready);
         }
         // Keys go one block ahead of the values, so that the next scores do not wait for this block's product.
-        const uint8_t* rk = smem + Sh::O_RAW + t * 64 * NH;
-        const uint8_t* rv = rk + Sh::RAW;
-        const float* sc = reinterpret_cast<const float*>(smem + Sh::O_SCALE);
         int reference = 0;
         float f_next = 0.f, f = 0.f;                                        // the factor of this key's value, of the next block and of this one
         bool fin_next = true, fin = true;
         // a row's 16-byte pieces in an order that differs from thread to thread: eight of them read 128 different bytes of banks
         auto piece = [&](int x) { return NH == 2 ? (x + t) & 7 : (x + (t >> 1)) & 3; };
         auto keys = [&](int j) -> bool {
-            const int st = j & 1;
-            ok = ok && mbar_wait(&raw_full[0], (uint32_t)(j & 1), abort_flag);
+            const int st = j % KST;
+            const uint8_t* rk = smem + Sh::O_RAW + (j & 1) * Sh::RAW + t * 64 * NH;
+            const float* sc = reinterpret_cast<const float*>(smem + Sh::O_SCALE) + (j & 1) * 2 * PT_KEYS;
+            ok = ok && mbar_wait(&raw_full[j & 1], (uint32_t)((j >> 1) & 1), abort_flag);
             const float vs = (from + j) * PT_KEYS + t <= last_pos ? sc[PT_KEYS + t] : 0.f;
             const uint32_t ve = (__float_as_uint(vs) >> 23) & 255u;
             fin_next = ve != 255u;
             // the block's reference: the largest exponent of a value's scale so far
             const uint32_t most = __reduce_max_sync(0xffffffffu, fin_next ? ve : 0u);
-            ok = ok && mbar_wait(&k_empty[st], (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag);
+            ok = ok && mbar_wait(&k_empty[st], (uint32_t)((j / KST) & 1) ^ 1u, abort_flag);
             uint32_t* w4 = warp_most + (j & 1) * 4;
             if (lane == 0) w4[q] = most;
             if (!all_of(ok, 2, 128)) return false;
@@ -1379,7 +1386,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(&k_full[st]); mbar_arrive(&raw_empty[0]); }
+            if (lane == 0) { mbar_arrive(&ks_full[j & 3]); mbar_arrive(&k_full[st]); mbar_arrive(&raw_empty[j & 1]); }
             return true;
         };
         auto nan_codes = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
@@ -1388,7 +1395,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const int vst = j % VST;
             f = f_next; fin = fin_next;
             if (j + 1 < nkv && !keys(j + 1)) { ok = false; break; }
-            ok = mbar_wait(&raw_full[1], (uint32_t)(j & 1), abort_flag) && mbar_wait(&v_empty[vst], (uint32_t)((j / VST) & 1) ^ 1u, abort_flag);
+            const uint8_t* rv = smem + Sh::O_RAW + (2 + (j & 1)) * Sh::RAW + t * 64 * NH;
+            ok = mbar_wait(&raw_full[2 + (j & 1)], (uint32_t)((j >> 1) & 1), abort_flag) && mbar_wait(&v_empty[vst], (uint32_t)((j / VST) & 1) ^ 1u, abort_flag);
             if (!ok) {
                 if (lane == 0) *abort_flag = 1;
                 if (j + 2 < nkv) all_of(false, 2, 128);                     // (where the others meet in keys(j + 2))
@@ -1429,7 +1437,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(&v_full[vst]); mbar_arrive(&raw_empty[1]); }
+            if (lane == 0) { mbar_arrive(&v_full[vst]); mbar_arrive(&raw_empty[2 + (j & 1)]); }
         }
         if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 80); }
     }
