@@ -692,11 +692,11 @@ constexpr int PT_TILE = 128 * 128;                      // bytes of a [128][64] 
 template <int NH, bool E4M3>
 struct ChunkShape {
     static constexpr int THREADS = E4M3 ? 448 : 320;
-    static constexpr int KST = NH == 2 && E4M3 ? 1 : 2, VST = KST;       // stages of keys and of values
+    static constexpr int KST = 2, VST = NH == 2 && E4M3 ? 1 : 2;         // stages of keys and of values
     static constexpr int RAW = PT_KEYS * 64 * NH;                        // bytes of a block's codes
     static constexpr int O_K = NH * PT_TILE, O_V = O_K + KST * NH * PT_TILE, O_P = O_V + VST * NH * PT_TILE, O_RAW = O_P + 2 * PT_TILE;
-    // (8 bits) codes as they come in: two stages of keys and two of values; their scales, [2][2][128]
-    static constexpr int O_SCALE = O_RAW + (E4M3 ? 4 * RAW : 0);
+    // (8 bits) codes as they come in: two stages of keys, then as many of values as there are of f16 values; their scales, [2][2][128]
+    static constexpr int O_SCALE = O_RAW + (E4M3 ? (2 + VST) * RAW : 0);
     static constexpr int O_KS = O_SCALE + (E4M3 ? 4 * PT_KEYS * 4 : 0);  // [4][128] key scales * scale_log2
     static constexpr int O_RF = O_KS + (E4M3 ? 4 * PT_KEYS * 4 : 0);     // [128] row factors
     static constexpr int O_BARS = O_RF + (E4M3 ? PT_ROWS * 4 : 0);
@@ -946,14 +946,49 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             for (int c = 0; c < NH; ++c) tma_load_3d(sQ + c * PT_TILE, &tmQ, q_full, c * 64, head * p.group, q0 + tok0);
         }
         int landed = 0;
-        for (int j = 0; j < nkv && ok; ++j) {
+        if (E4M3) {
+            // codes: keys two blocks ahead of values, as they are turned into f16
+            struct Place { int block, r0; } k_at = {0, 0}, v_at = {0, 0}, v_next = {0, 0};
+            auto load = [&](int x, int j, const Place& at) -> bool {      // x: keys with all scales, or values
+                const int of = x == 0 ? 2 : VST, rs = 2 * x + j % of, count = min(page_pieces, last_piece - (piece0 + j * page_pieces)), o = lane << piece_shift;
+                uint64_t* bar = &raw_full[rs];
+                if (!__all_sync(0xffffffffu, mbar_wait(&raw_empty[rs], (uint32_t)((j / of) & 1) ^ 1u, abort_flag))) return false;
+                if (lane == 0) mbar_expect_tx(bar, (uint32_t)(count * piece_keys * (64 * NH + (x == 0 ? 8 : 0))));
+                __syncwarp();
+                if (lane < count) {
+                    tma_load_3d(smem + Sh::O_RAW + rs * Sh::RAW + o * 64 * NH, x == 0 ? &tmK : &tmV, bar, 0, at.r0, at.block);
+                    if (x == 0) {
+                        float* sc = reinterpret_cast<float*>(smem + Sh::O_SCALE) + (j & 1) * 2 * PT_KEYS + o;
+                        const long long row = ((long long)at.block << p.v.page_shift) + at.r0;
+                        bulk_load(sc, p.ks + row, (uint32_t)piece_keys * 4u, bar);
+                        bulk_load(sc + PT_KEYS, p.vs + row, (uint32_t)piece_keys * 4u, bar);
+                    }
+                }
+                __syncwarp();
+                return true;
+            };
+            for (int j = -2; j < nkv && ok; ++j) {
+                if (j + 2 < nkv) {
+                    const int at = piece0 + (j + 2) * page_pieces;
+                    if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
+                    const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
+                    k_at.block = pg * p.v.heads + head;
+                    k_at.r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift;
+                }
+                // (values first: the keys two blocks on wait for a stage that this block's scores free)
+                if (j >= 0) ok = load(1, j, v_at);
+                if (ok && j + 2 < nkv) ok = load(0, j + 2, k_at);
+                v_at = v_next; v_next = k_at;
+            }
+        }
+        for (int j = 0; j < nkv && ok && !E4M3; ++j) {
             const int at = piece0 + j * page_pieces;
             if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
             const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
             const int count = min(page_pieces, last_piece - at);
             const int block = pg * p.v.heads + head, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift, o = lane << piece_shift;
             const int st = j & 1;
-            if (!E4M3) {
+            {
                 const int vst = j % VST;
                 ok = mbar_wait(&k_empty[st], (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -1004,25 +1039,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&v_full[vst]);
                 }
-            } else {
-                for (int x = 0; x < 2 && ok; ++x) {
-                    uint64_t* bar = &raw_full[2 * x + st];
-                    ok = mbar_wait(&raw_empty[2 * x + st], (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(count * piece_keys * (64 * NH + (x == 0 ? 8 : 0))));
-                    __syncwarp();
-                    if (lane < count) {
-                        tma_load_3d(smem + Sh::O_RAW + (2 * x + st) * Sh::RAW + o * 64 * NH, x == 0 ? &tmK : &tmV, bar, 0, r0, block);
-                        if (x == 0) {
-                            float* sc = reinterpret_cast<float*>(smem + Sh::O_SCALE) + st * 2 * PT_KEYS + o;
-                            const long long row = ((long long)block << p.v.page_shift) + r0;
-                            bulk_load(sc, p.ks + row, (uint32_t)piece_keys * 4u, bar);
-                            bulk_load(sc + PT_KEYS, p.vs + row, (uint32_t)piece_keys * 4u, bar);
-                        }
-                    }
-                    __syncwarp();
-                }
             }
             __syncwarp();
         }
@@ -1054,8 +1070,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (ok) ok = issue_scores(0) && issue_scores(1);
             for (int i = 0; i < nsub && ok; ++i) {
                 const int j = i >> 1, b = i & 1, vst = j % VST;
-                // (with one stage of keys the next block's are still being turned into f16: this product first)
-                if (KST > 1 && i + 2 < nsub && !issue_scores(i + 2)) { ok = false; break; }
+                if (i + 2 < nsub && !issue_scores(i + 2)) { ok = false; break; }
                 if (!mbar_wait(&p_full[b], (uint32_t)(j & 1), abort_flag)) { ok = false; break; }
                 if (b == 0 && !mbar_wait(&v_full[vst], (uint32_t)((j / VST) & 1), abort_flag)) { ok = false; break; }
                 tc_fence_after();
@@ -1065,7 +1080,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     umma_bf16(tO + (uint32_t)(b * 64 * NH), dP + k * KSTEP, dV + k * MNSTEP, idesc_o, (i > 1 || k > 0) ? 1u : 0u);
                 umma_commit(&o_full[b]);
                 if (b == 1) umma_commit(&v_empty[vst]);
-                if (KST == 1 && i + 2 < nsub && !issue_scores(i + 2)) { ok = false; break; }
             }
             if (!ok) { *abort_flag = 1; atomicExch(p.err, 78); }
         }
@@ -1340,10 +1354,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
         }
-        // Keys go one block ahead of the values, so that the next scores do not wait for this block's product.
+        // Keys go two blocks ahead of the values, so that neither the scores nor the products wait for them.
         int reference = 0;
-        float f_next = 0.f, f = 0.f;                                        // the factor of this key's value, of the next block and of this one
-        bool fin_next = true, fin = true;
+        float f = 0.f, f_next = 0.f, f_new = 0.f;                           // the factor of this key's value, in this block, the next and the one after
+        bool fin = true, fin_next = true, fin_new = true;                   // its scale is finite
         // a row's 16-byte pieces in an order that differs from thread to thread: eight of them read 128 different bytes of banks
         auto piece = [&](int x) { return NH == 2 ? (x + t) & 7 : (x + (t >> 1)) & 3; };
         auto keys = [&](int j) -> bool {
@@ -1353,9 +1367,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             ok = ok && mbar_wait(&raw_full[j & 1], (uint32_t)((j >> 1) & 1), abort_flag);
             const float vs = (from + j) * PT_KEYS + t <= last_pos ? sc[PT_KEYS + t] : 0.f;
             const uint32_t ve = (__float_as_uint(vs) >> 23) & 255u;
-            fin_next = ve != 255u;
+            fin_new = ve != 255u;
             // the block's reference: the largest exponent of a value's scale so far
-            const uint32_t most = __reduce_max_sync(0xffffffffu, fin_next ? ve : 0u);
+            const uint32_t most = __reduce_max_sync(0xffffffffu, fin_new ? ve : 0u);
             ok = ok && mbar_wait(&k_empty[st], (uint32_t)((j / KST) & 1) ^ 1u, abort_flag);
             uint32_t* w4 = warp_most + (j & 1) * 4;
             if (lane == 0) w4[q] = most;
@@ -1370,7 +1384,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             reference = now;
             // code * scale * 2^(6 - reference), in two steps: 2^(127 - reference) alone may be no normal number
             const int half_way = (127 - now) / 2;
-            f_next = fin_next ? vs * __uint_as_float((uint32_t)(127 + half_way) << 23) * __uint_as_float((uint32_t)(133 + 127 - now - half_way) << 23) : vs;
+            f_new = fin_new ? vs * __uint_as_float((uint32_t)(127 + half_way) << 23) * __uint_as_float((uint32_t)(133 + 127 - now - half_way) << 23) : vs;
             uint8_t* row = sK + st * NH * PT_TILE + t * 128;
 #pragma unroll
             for (int c = 0; c < NH; ++c)
@@ -1391,12 +1405,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         };
         auto nan_codes = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
         if (nkv > 0) ok = keys(0);
+        f = f_new; fin = fin_new;
+        if (nkv > 1 && ok) ok = keys(1);
+        f_next = f_new; fin_next = fin_new;
         for (int j = 0; j < nkv && ok; ++j) {
             const int vst = j % VST;
-            f = f_next; fin = fin_next;
-            if (j + 1 < nkv && !keys(j + 1)) { ok = false; break; }
-            const uint8_t* rv = smem + Sh::O_RAW + (2 + (j & 1)) * Sh::RAW + t * 64 * NH;
-            ok = mbar_wait(&raw_full[2 + (j & 1)], (uint32_t)((j >> 1) & 1), abort_flag) && mbar_wait(&v_empty[vst], (uint32_t)((j / VST) & 1) ^ 1u, abort_flag);
+            const uint8_t* rv = smem + Sh::O_RAW + (2 + vst) * Sh::RAW + t * 64 * NH;
+            ok = mbar_wait(&raw_full[2 + vst], (uint32_t)((j / VST) & 1), abort_flag) && mbar_wait(&v_empty[vst], (uint32_t)((j / VST) & 1) ^ 1u, abort_flag);
             if (!ok) {
                 if (lane == 0) *abort_flag = 1;
                 if (j + 2 < nkv) all_of(false, 2, 128);                     // (where the others meet in keys(j + 2))
@@ -1437,7 +1452,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(&v_full[vst]); mbar_arrive(&raw_empty[2 + (j & 1)]); }
+            if (lane == 0) { mbar_arrive(&v_full[vst]); mbar_arrive(&raw_empty[2 + vst]); }
+            if (j + 2 < nkv && !keys(j + 2)) { ok = false; break; }
+            f = f_next; fin = fin_next;
+            f_next = f_new; fin_next = fin_new;
         }
         if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 80); }
     }
