@@ -108,6 +108,12 @@ __device__ __forceinline__ uint32_t e4m3_f16(uint32_t two) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
     return h;
 }
+__device__ __forceinline__ uint32_t e5m2_pair(float lo, float hi) {
+    uint16_t h;
+    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(h) : "f"(hi), "f"(lo));
+    return h;
+}
+__device__ __forceinline__ float2 f16_floats(uint32_t two) { return __half22float2(*reinterpret_cast<const __half2*>(&two)); }
 __device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
     uint32_t h;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(hi), "f"(lo));
@@ -687,21 +693,25 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 //  * 8-bit rows: four more warps turn codes into f16 tiles, a key per thread.  A value's scale goes into its tile against the largest
 //    scale so far (a power of two, which the accumulators follow as they follow the maximum): 11 bits of every value whose scale is
 //    within 2^-21 of the largest, and an absolute error below 2^-31 of the largest value behind that.
+// A row's reference m follows its largest score only when that lies more than this above it (log2): every sum and product is against the
+// same m, so the result is the same, probabilities reach 2^8 at most, and the accumulators are seldom scaled.
+constexpr float PT_SLACK = 8.f;
 constexpr int PT_TILE = 128 * 128;                      // bytes of a [128][64] 16-bit tile
 
 template <int NH, bool E4M3>
 struct ChunkShape {
     static constexpr int THREADS = E4M3 ? 448 : 320;
-    static constexpr int KST = 2, VST = NH == 2 && E4M3 ? 1 : 2;         // stages of keys and of values
-    static constexpr int RAW = PT_KEYS * 64 * NH;                        // bytes of a block's codes
-    static constexpr int O_K = NH * PT_TILE, O_V = O_K + KST * NH * PT_TILE, O_P = O_V + VST * NH * PT_TILE, O_RAW = O_P + 2 * PT_TILE;
-    // (8 bits) codes as they come in: two stages of keys, then as many of values as there are of f16 values; their scales, [2][2][128]
-    static constexpr int O_SCALE = O_RAW + (E4M3 ? (2 + VST) * RAW : 0);
-    static constexpr int O_KS = O_SCALE + (E4M3 ? 4 * PT_KEYS * 4 : 0);  // [4][128] key scales * scale_log2
+    static constexpr int KST = E4M3 ? 3 : 2, VST = 2;                    // stages of keys and of values
+    static constexpr int K_TILE = E4M3 ? PT_TILE : NH * PT_TILE;         // bytes of a stage of keys: bf16, or codes (rows of 128 bytes)
+    static constexpr int RAW = PT_KEYS * 64 * NH;                        // bytes of a block's codes of values
+    static constexpr int O_K = NH * PT_TILE, O_V = O_K + KST * K_TILE, O_P = O_V + VST * NH * PT_TILE, O_RAW = O_P + 2 * PT_TILE;
+    // (8 bits) stages of codes of values as they come in
+    static constexpr int RST = 2;
+    static constexpr int O_KS = O_RAW + (E4M3 ? RST * RAW : 0);          // [4][128] key scales * scale_log2
     static constexpr int O_RF = O_KS + (E4M3 ? 4 * PT_KEYS * 4 : 0);     // [128] row factors
     static constexpr int O_BARS = O_RF + (E4M3 ? PT_ROWS * 4 : 0);
     // (bf16 heads of 64: exactly what lets two CTAs share an SM; 256 bytes of barriers behind the tiles or in the alignment's pad)
-    static constexpr int SMEM = 1024 + O_BARS + (NH == 1 && !E4M3 ? 0 : E4M3 ? 384 : 256);
+    static constexpr int SMEM = 1024 + O_BARS + (NH == 1 && !E4M3 ? 0 : E4M3 ? 512 : 256);
     static constexpr int PER_SM = SMEM <= 113 * 1024 ? 2 : 1;
     static constexpr int TMEM = NH == 1 ? 256 : 512;
 };
@@ -855,9 +865,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     uint8_t *sQ = smem, *sK = smem + Sh::O_K, *sV = smem + Sh::O_V, *sP = smem + Sh::O_P;
     uint64_t* bars = reinterpret_cast<uint64_t*>(pad <= 768u ? smem + Sh::O_BARS : smem_raw);
     uint64_t* q_full = bars;          // 1: the query tile has come
-    uint64_t* q_ready = bars + 1;     // (8 bits) and is f16
-    uint64_t* k_full = bars + 2;      // 2
-    uint64_t* k_empty = bars + 4;     // 2: the scores of both halves have been formed
+    uint64_t* q_ready = bars + 1;     // (8 bits) and is two terms of 8 bits
+    uint64_t* k_full = bars + (E4M3 ? 44 : 2);       // KST
+    uint64_t* k_empty = bars + (E4M3 ? 48 : 4);      // KST: the scores of both halves have been formed
     uint64_t* v_full = bars + 6;      // 2
     uint64_t* v_empty = bars + 8;     // 2
     uint64_t* v_land = bars + 10;     // 1: values of a block that is looked through first
@@ -866,8 +876,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     uint64_t* p_full = bars + 15;     // 2
     uint64_t* o_full = bars + 17;     // 2
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
-    uint64_t* raw_full = bars + 32;   // (8 bits) 2 x 2: codes of keys with all scales, codes of values; behind the 256 bytes of the rest
-    uint64_t* raw_empty = bars + 36;  // 2 x 2
+    uint64_t* raw_full = bars + 32;   // (8 bits) RST: codes of values; behind the 256 bytes of the rest
+    uint64_t* raw_empty = bars + 36;  // RST
     uint64_t* ks_full = bars + 40;    // 4: what the softmax warps read of a block's scales.  (Not k_full, which may be a whole round ahead of them.)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* bad_value = abort_flag + 1;                              // a value that is not finite has been set to zero
@@ -920,12 +930,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     if (threadIdx.x == 32 * 2) {
         mbar_init(q_full, 1); mbar_init(q_ready, 4); mbar_init(v_land, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], E4M3 ? 4 : 1); mbar_init(&v_full[i], E4M3 ? 4 : 1);
-            mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1);
+            mbar_init(&v_full[i], E4M3 ? 4 : 1); mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1);
-            if (E4M3)
-                for (int x = 0; x < 2; ++x) { mbar_init(&raw_full[2 * i + x], 1); mbar_init(&raw_empty[2 * i + x], 4); }
         }
+        if (E4M3)
+            for (int i = 0; i < Sh::RST; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
+        for (int i = 0; i < KST; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
         if (E4M3)
             for (int i = 0; i < 4; ++i) mbar_init(&ks_full[i], 4);
         *abort_flag = 0; *bad_value = 0; *v_exponent = 0;
@@ -947,38 +957,24 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         int landed = 0;
         if (E4M3) {
-            // codes: keys two blocks ahead of values, as they are turned into f16
-            struct Place { int block, r0; } k_at = {0, 0}, v_at = {0, 0}, v_next = {0, 0};
-            auto load = [&](int x, int j, const Place& at) -> bool {      // x: keys with all scales, or values
-                const int of = x == 0 ? 2 : VST, rs = 2 * x + j % of, count = min(page_pieces, last_piece - (piece0 + j * page_pieces)), o = lane << piece_shift;
-                uint64_t* bar = &raw_full[rs];
-                if (!__all_sync(0xffffffffu, mbar_wait(&raw_empty[rs], (uint32_t)((j / of) & 1) ^ 1u, abort_flag))) return false;
-                if (lane == 0) mbar_expect_tx(bar, (uint32_t)(count * piece_keys * (64 * NH + (x == 0 ? 8 : 0))));
+            for (int j = 0; j < nkv; ++j) {
+                const int at = piece0 + j * page_pieces, st = j % KST, rs = j % Sh::RST, o = lane << piece_shift;
+                if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
+                const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
+                const int count = min(page_pieces, last_piece - at);
+                const int block = pg * p.v.heads + head, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift;
+                ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], (uint32_t)((j / KST) & 1) ^ 1u, abort_flag));
+                if (!ok) break;
+                if (lane == 0) mbar_expect_tx(&k_full[st], (uint32_t)(count * piece_keys * 128));
                 __syncwarp();
-                if (lane < count) {
-                    tma_load_3d(smem + Sh::O_RAW + rs * Sh::RAW + o * 64 * NH, x == 0 ? &tmK : &tmV, bar, 0, at.r0, at.block);
-                    if (x == 0) {
-                        float* sc = reinterpret_cast<float*>(smem + Sh::O_SCALE) + (j & 1) * 2 * PT_KEYS + o;
-                        const long long row = ((long long)at.block << p.v.page_shift) + at.r0;
-                        bulk_load(sc, p.ks + row, (uint32_t)piece_keys * 4u, bar);
-                        bulk_load(sc + PT_KEYS, p.vs + row, (uint32_t)piece_keys * 4u, bar);
-                    }
-                }
+                if (lane < count) tma_load_3d(sK + st * Sh::K_TILE + o * 128, &tmK, &k_full[st], 0, r0, block);
                 __syncwarp();
-                return true;
-            };
-            for (int j = -2; j < nkv && ok; ++j) {
-                if (j + 2 < nkv) {
-                    const int at = piece0 + (j + 2) * page_pieces;
-                    if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
-                    const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
-                    k_at.block = pg * p.v.heads + head;
-                    k_at.r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift;
-                }
-                // (values first: the keys two blocks on wait for a stage that this block's scores free)
-                if (j >= 0) ok = load(1, j, v_at);
-                if (ok && j + 2 < nkv) ok = load(0, j + 2, k_at);
-                v_at = v_next; v_next = k_at;
+                ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[rs], (uint32_t)((j / Sh::RST) & 1) ^ 1u, abort_flag));
+                if (!ok) break;
+                if (lane == 0) mbar_expect_tx(&raw_full[rs], (uint32_t)(count * piece_keys * 64 * NH));
+                __syncwarp();
+                if (lane < count) tma_load_3d(smem + Sh::O_RAW + rs * Sh::RAW + o * 64 * NH, &tmV, &raw_full[rs], 0, r0, block);
+                __syncwarp();
             }
         }
         for (int j = 0; j < nkv && ok && !E4M3; ++j) {
@@ -1047,7 +1043,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     } else if (warp == 1) {
         if (elect_one() && nkv > 0) {
             const uint32_t fmt = E4M3 ? 0u : 1u;
-            const uint32_t idesc_s = umma_idesc(fmt, 0u, 0u, PT_ROWS, 64), idesc_o = umma_idesc(fmt, 0u, 1u, PT_ROWS, 64 * NH);
+            // (8 bits: the row's first term is e5m2)
+            const uint32_t idesc_s = umma_idesc(fmt, 0u, 0u, PT_ROWS, 64), idesc_s1 = idesc_s | 1u << 7, idesc_o = umma_idesc(fmt, 0u, 1u, PT_ROWS, 64 * NH);
             const uint64_t dQ = umma_desc_sw128(smem_u32(sQ), 16, 1024), dK0 = umma_desc_sw128(smem_u32(sK), 16, 1024);
             const uint64_t dP0 = umma_desc_sw128(smem_u32(sP), 16, 1024), dV0 = umma_desc_sw128(smem_u32(sV), PT_TILE, 1024);
             constexpr uint64_t TILE = PT_TILE >> 4, KSTEP = 32 >> 4, MNSTEP = 2048 >> 4;
@@ -1058,9 +1055,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 if (b == 0 && !mbar_wait(&k_full[st], (uint32_t)((j / KST) & 1), abort_flag)) return false;
                 if (!mbar_wait(&s_free[b], (uint32_t)((i >> 1) & 1) ^ 1u, abort_flag)) return false;
                 tc_fence_after();
-                const uint64_t dK = dK0 + (uint64_t)(st * NH) * TILE + (uint64_t)b * (TILE / 2);
+                const uint64_t dK = dK0 + (uint64_t)st * (Sh::K_TILE >> 4) + (uint64_t)b * (TILE / 2);
 #pragma unroll
-                for (int k = 0; k < 4 * NH; ++k)
+                for (int k = 0; k < 4 * NH && E4M3; ++k) {                  // both terms of the rows with the same codes
+                    const int term = k / (2 * NH), e = k % (2 * NH);
+                    umma_f8(tS + (uint32_t)(b * 64), dQ + (NH == 2 ? term * TILE : (uint64_t)(2 * term) * KSTEP) + e * KSTEP, dK + e * KSTEP,
+                            term == 0 ? idesc_s1 : idesc_s, k > 0 ? 1u : 0u);
+                }
+#pragma unroll
+                for (int k = 0; k < 4 * NH && !E4M3; ++k)
                     umma_bf16(tS + (uint32_t)(b * 64), dQ + (k >> 2) * TILE + (k & 3) * KSTEP, dK + (k >> 2) * TILE + (k & 3) * KSTEP, idesc_s,
                               k > 0 ? 1u : 0u);
                 umma_commit(&s_full[b]);
@@ -1145,7 +1148,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             const float m_new = fmaxf(m, mx * c1);
             float alpha = 1.0f;
-            if (m_new > m) {
+            if (m_new > m + PT_SLACK) {
                 alpha = ex2_approx(m - m_new);
                 l *= alpha;
                 m = m_new;
@@ -1316,105 +1319,114 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 79); }
     } else if (E4M3) {
-        // ---- codes to f16: thread = query row once, then a key of every block
+        // ---- thread = query row once, which becomes two terms of 8 bits; then a key of every block, whose value becomes f16
         const int t = threadIdx.x - 320, q = warp - 10;
         bool ok = true;
         if (nkv > 0) ok = mbar_wait(q_full, 0, abort_flag);
         if (nkv > 0 && ok) {
             uint32_t most = 0u;
             uint8_t* row = sQ + t * 128;
+            uint4 w[8 * NH];
 #pragma unroll
-            for (int c = 0; c < NH; ++c)
-#pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(row + c * PT_TILE + (d << 4));
-                    const uint32_t a = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
-                    most = max(most, max(a & 0xffffu, a >> 16));
-                }
-            // scaled by a power of two so that the row's largest magnitude lies in [1, 2): exact but for what is less than 2^-24 of it
-            const int e = max((int)(most >> 7), 1);
-            const bool odd = e >= 254;
-            const float down = odd ? 1.f : __uint_as_float((uint32_t)(254 - e) << 23), up = odd ? 1.f : __uint_as_float((uint32_t)e << 23);
+            for (int d = 0; d < 8 * NH; ++d) {
+                w[d] = *reinterpret_cast<const uint4*>(row + (d >> 3) * PT_TILE + (((d & 7) ^ (t & 7)) << 4));
+                const uint32_t a = __vmaxu2(__vmaxu2(w[d].x & 0x7fff7fffu, w[d].y & 0x7fff7fffu), __vmaxu2(w[d].z & 0x7fff7fffu, w[d].w & 0x7fff7fffu));
+                most = max(most, max(a & 0xffffu, a >> 16));
+            }
+            // Scaled by a power of two so that the row's largest magnitude lies in [2^11, 2^12).  Three bits of an element are its e5m2
+            // term, and what is left of its eight fits four bits, an e4m3 term of at most 2^8: exact but for what lies below 2^-10, which
+            // is 2^-21 of the row's largest.  (Both with the same codes of the keys, as they lie in the cache: no key is converted.)
+            const int e = max((int)(most >> 7), 12);
+            const bool odd = e == 255;                                      // (an infinity or NaN: no score of this row is a number)
+            const float down = odd ? 1.f : __uint_as_float((uint32_t)(265 - e) << 23), up = odd ? 1.f : __uint_as_float((uint32_t)(e - 11) << 23);
             reinterpret_cast<float*>(smem + Sh::O_RF)[t] = up;
 #pragma unroll
-            for (int c = 0; c < NH; ++c)
+            for (int d = 0; d < 4 * NH; ++d) {
+                const uint32_t u[8] = {w[2 * d].x, w[2 * d].y, w[2 * d].z, w[2 * d].w, w[2 * d + 1].x, w[2 * d + 1].y, w[2 * d + 1].z, w[2 * d + 1].w};
+                uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    uint4* at = reinterpret_cast<uint4*>(row + c * PT_TILE + (d << 4));
-                    uint4 w = *at;
-                    uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t a[2], b[2];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 f = bf16_floats(u[i]);
-                        u[i] = f16_pair(f.x * down, f.y * down);
+                    for (int x = 0; x < 2; ++x) {
+                        float2 f = bf16_floats(u[2 * i + x]);
+                        f.x *= down; f.y *= down;
+                        a[x] = e5m2_pair(f.x, f.y);
+                        const float2 g = f16_floats((a[x] & 0xffu) << 8 | (a[x] & 0xff00u) << 16);
+                        b[x] = e4m3_pair(f.x - g.x, f.y - g.y);
                     }
-                    *at = make_uint4(u[0], u[1], u[2], u[3]);
+                    hi[i] = odd ? 0x7f7f7f7fu : a[0] | a[1] << 16;
+                    lo[i] = odd ? 0x7f7f7f7fu : b[0] | b[1] << 16;
                 }
+                uint8_t* second = NH == 2 ? row + PT_TILE + ((d ^ (t & 7)) << 4) : row + (((d + 4) ^ (t & 7)) << 4);
+                *reinterpret_cast<uint4*>(row + ((d ^ (t & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(second) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
         }
-        // Keys go two blocks ahead of the values, so that neither the scores nor the products wait for them.
+        // Scales by plain loads, a block ahead, and the pages they are found by another one.  (Bulk copies of 64 bytes and more beside the
+        // codes are as fast, but make the values wait for them.)
+        auto page_of = [&](int j) -> int {                                  // of this thread's key of a block; -1: none
+            const int key = (from + j) * PT_KEYS + t;
+            if (j >= nkv || key > last_pos) return -1;
+            const int pg = table[key >> p.v.page_shift];
+            return (unsigned)pg < (unsigned)p.v.pages ? pg : 0;             // (the producer reports it)
+        };
+        float ks_new = 0.f, vs_new = 0.f;
+        auto load_scales = [&](int j, int pg) {
+            const long long row = (((long long)pg * p.v.heads + head) << p.v.page_shift) + (((from + j) * PT_KEYS + t) & ((1 << p.v.page_shift) - 1));
+            ks_new = pg < 0 ? 0.f : p.ks[row];
+            vs_new = pg < 0 ? 0.f : p.vs[row];
+        };
         int reference = 0;
-        float f = 0.f, f_next = 0.f, f_new = 0.f;                           // the factor of this key's value, in this block, the next and the one after
-        bool fin = true, fin_next = true, fin_new = true;                   // its scale is finite
-        // a row's 16-byte pieces in an order that differs from thread to thread: eight of them read 128 different bytes of banks
-        auto piece = [&](int x) { return NH == 2 ? (x + t) & 7 : (x + (t >> 1)) & 3; };
-        auto keys = [&](int j) -> bool {
-            const int st = j % KST;
-            const uint8_t* rk = smem + Sh::O_RAW + (j & 1) * Sh::RAW + t * 64 * NH;
-            const float* sc = reinterpret_cast<const float*>(smem + Sh::O_SCALE) + (j & 1) * 2 * PT_KEYS;
-            ok = ok && mbar_wait(&raw_full[j & 1], (uint32_t)((j >> 1) & 1), abort_flag);
-            const float vs = (from + j) * PT_KEYS + t <= last_pos ? sc[PT_KEYS + t] : 0.f;
+        float f = 0.f, f_next = 0.f;                                        // the factor of this key's value, in this block and the next
+        bool fin = true, fin_next = true;                                   // its scale is finite
+        // What the softmax warps need of a block's scales, a block ahead of the values and so three blocks ahead of their product at
+        // most: the ring of four holds what is still read.
+        auto scales = [&](int j) -> bool {
+            const float vs = vs_new;
             const uint32_t ve = (__float_as_uint(vs) >> 23) & 255u;
-            fin_new = ve != 255u;
+            fin_next = ve != 255u;
             // the block's reference: the largest exponent of a value's scale so far
-            const uint32_t most = __reduce_max_sync(0xffffffffu, fin_new ? ve : 0u);
-            ok = ok && mbar_wait(&k_empty[st], (uint32_t)((j / KST) & 1) ^ 1u, abort_flag);
+            const uint32_t most = __reduce_max_sync(0xffffffffu, fin_next ? ve : 0u);
             uint32_t* w4 = warp_most + (j & 1) * 4;
             if (lane == 0) w4[q] = most;
             if (!all_of(ok, 2, 128)) return false;
             const int now = max(reference, (int)max(max(w4[0], w4[1]), max(w4[2], w4[3])));
-            reinterpret_cast<float*>(smem + Sh::O_KS)[(j & 3) * PT_KEYS + t] = sc[t] * p.scale_log2;
+            reinterpret_cast<float*>(smem + Sh::O_KS)[(j & 3) * PT_KEYS + t] = ks_new * p.scale_log2;
             if (t == 0) {
                 const int d = now - reference;                              // (an accumulator that is still empty may be scaled by anything)
                 v_moved[j & 3] = d == 0 ? 1.f : d > 126 ? 0.f : __uint_as_float((uint32_t)(127 - d) << 23);
                 *v_exponent = now;
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ks_full[j & 3]);
             reference = now;
             // code * scale * 2^(6 - reference), in two steps: 2^(127 - reference) alone may be no normal number
             const int half_way = (127 - now) / 2;
-            f_new = fin_new ? vs * __uint_as_float((uint32_t)(127 + half_way) << 23) * __uint_as_float((uint32_t)(133 + 127 - now - half_way) << 23) : vs;
-            uint8_t* row = sK + st * NH * PT_TILE + t * 128;
-#pragma unroll
-            for (int c = 0; c < NH; ++c)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int y = piece(4 * c + x), d = y & 3;
-                    uint8_t* to = row + (y >> 2) * PT_TILE;
-                    const uint4 w = *reinterpret_cast<const uint4*>(rk + 16 * y);
-                    *reinterpret_cast<uint4*>(to + (((2 * d) ^ (t & 7)) << 4)) =
-                        make_uint4(e4m3_f16(w.x), e4m3_f16(w.x >> 16), e4m3_f16(w.y), e4m3_f16(w.y >> 16));
-                    *reinterpret_cast<uint4*>(to + (((2 * d + 1) ^ (t & 7)) << 4)) =
-                        make_uint4(e4m3_f16(w.z), e4m3_f16(w.z >> 16), e4m3_f16(w.w), e4m3_f16(w.w >> 16));
-                }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) { mbar_arrive(&ks_full[j & 3]); mbar_arrive(&k_full[st]); mbar_arrive(&raw_empty[j & 1]); }
+            f_next = fin_next ? vs * __uint_as_float((uint32_t)(127 + half_way) << 23) * __uint_as_float((uint32_t)(133 + 127 - now - half_way) << 23) : vs;
             return true;
         };
+        // a row's 16-byte pieces in an order that differs from thread to thread: eight of them read 128 different bytes of banks
+        auto piece = [&](int x) { return NH == 2 ? (x + t) & 7 : (x + (t >> 1)) & 3; };
         auto nan_codes = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
-        if (nkv > 0) ok = keys(0);
-        f = f_new; fin = fin_new;
-        if (nkv > 1 && ok) ok = keys(1);
-        f_next = f_new; fin_next = fin_new;
+        load_scales(0, page_of(0));
+        if (nkv > 0) ok = scales(0);
+        load_scales(1, page_of(1));
+        int page = page_of(2);
         for (int j = 0; j < nkv && ok; ++j) {
-            const int vst = j % VST;
-            const uint8_t* rv = smem + Sh::O_RAW + (2 + vst) * Sh::RAW + t * 64 * NH;
-            ok = mbar_wait(&raw_full[2 + vst], (uint32_t)((j / VST) & 1), abort_flag) && mbar_wait(&v_empty[vst], (uint32_t)((j / VST) & 1) ^ 1u, abort_flag);
+            const int vst = j % VST, rs = j % Sh::RST;
+            const uint8_t* rv = smem + Sh::O_RAW + rs * Sh::RAW + t * 64 * NH;
+            f = f_next; fin = fin_next;
+            if (j + 1 < nkv && !scales(j + 1)) { ok = false; break; }
+            load_scales(j + 2, page);
+            page = page_of(j + 3);
+            ok = mbar_wait(&raw_full[rs], (uint32_t)((j / Sh::RST) & 1), abort_flag) && mbar_wait(&v_empty[vst], (uint32_t)((j / VST) & 1) ^ 1u, abort_flag);
             if (!ok) {
                 if (lane == 0) *abort_flag = 1;
-                if (j + 2 < nkv) all_of(false, 2, 128);                     // (where the others meet in keys(j + 2))
+                if (j + 2 < nkv) all_of(false, 2, 128);                     // (where the others meet in scales(j + 2))
                 break;
             }
             const bool seen = (from + j) * PT_KEYS + t <= last_pos, looked = from + j >= edge0 && seen;
@@ -1452,10 +1464,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(&v_full[vst]); mbar_arrive(&raw_empty[2 + vst]); }
-            if (j + 2 < nkv && !keys(j + 2)) { ok = false; break; }
-            f = f_next; fin = fin_next;
-            f_next = f_new; fin_next = fin_new;
+            if (lane == 0) { mbar_arrive(&v_full[vst]); mbar_arrive(&raw_empty[rs]); }
         }
         if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 80); }
     }
@@ -1474,8 +1483,8 @@ int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cud
     static_assert(Sh::PER_SM == paged_per_sm(NH, E4M3), "the plan counts on as many CTAs per SM");
     CUtensorMap tmK, tmV;
     const int box_rows = std::min(c->page_size, Sh::KEYS);
-    TB_TRY(make_cache_map(&tmK, c->K, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
-    TB_TRY(make_cache_map(&tmV, c->V, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
+    TB_TRY(make_cache_map(&tmK, c->K, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows, !E4M3));
+    TB_TRY(make_cache_map(&tmV, c->V, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows, !E4M3));
     static bool attr_set[64] = {false};
     if (!attr_set[ctx->device & 63]) {
         TB_CUDA(cudaFuncSetAttribute(paged_rows_kernel<NH, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
@@ -1521,8 +1530,8 @@ int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedChunkParams& pp
     CUtensorMap tmQ, tmK, tmV;
     TB_TRY(make_query_map(&tmQ, p.Q, c->head_dim, p.H, p.rows, p.ld_q, p.group, pp.tokens));
     const int box_rows = std::min(c->page_size, PT_KEYS);
-    TB_TRY(make_cache_map(&tmK, c->K, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
-    TB_TRY(make_cache_map(&tmV, c->V, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows));
+    TB_TRY(make_cache_map(&tmK, c->K, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, E4M3 ? 128 : 64, box_rows, true));
+    TB_TRY(make_cache_map(&tmV, c->V, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows, !E4M3));
     static bool attr_set[64] = {false};
     if (!attr_set[ctx->device & 63]) {
         TB_CUDA(cudaFuncSetAttribute(paged_chunk_kernel<NH, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));

@@ -198,10 +198,10 @@ int make_operand_map_f32(CUtensorMap* map, const float* ptr, long long inner, lo
 int make_operand_map4(CUtensorMap* map, const bf16* ptr, long long inner, long long rows, long long ld,
                       long long n0, long long stride0, long long n1, long long stride1, int box_rows);
 
-// a pool of cache pages seen as [blocks][rows][inner], blocks of one head of a page.  es = 2: bf16, box of 64 elements (128-byte
-// swizzle), es = 1: bytes, box of box_inner (as they lie)
+// a pool of cache pages seen as [blocks][rows][inner], blocks of one head of a page.  es = 2: bf16, es = 1: bytes; a box of
+// box_inner by box_rows as it lies, or with the 128-byte swizzle (128 bytes wide; what is wider than the row reads zeros)
 int make_cache_map(CUtensorMap* map, const void* ptr, int es, long long inner, long long rows, long long blocks, int box_inner,
-                   int box_rows);
+                   int box_rows, bool swizzled);
 
 // rows of heads, [rows][heads][hd] with leading dimension ld: a box of 64 elements of box_heads heads of box_rows rows
 int make_query_map(CUtensorMap* map, const bf16* ptr, int hd, int heads, int rows, long long ld, int box_heads, int box_rows);

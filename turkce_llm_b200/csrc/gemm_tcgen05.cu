@@ -1508,7 +1508,7 @@ int make_operand_map_f32(CUtensorMap* map, const float* ptr, long long inner, lo
 }
 
 int make_cache_map(CUtensorMap* map, const void* ptr, int es, long long inner, long long rows, long long blocks, int box_inner,
-                   int box_rows) {
+                   int box_rows, bool swizzled) {
     EncodeTiledFn enc = get_encode_fn();
     TB_CHECK(enc != nullptr, "cuTensorMapEncodeTiled entry point not available");
     cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)blocks};
@@ -1516,7 +1516,7 @@ int make_cache_map(CUtensorMap* map, const void* ptr, int es, long long inner, l
     cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, 1u};
     cuuint32_t estr[3] = {1u, 1u, 1u};
     CUresult r = enc(map, es == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims,
-                     strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, es == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                     strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     TB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code %d (inner=%lld rows=%lld blocks=%lld)", (int)r, inner, rows, blocks);
     return 0;
