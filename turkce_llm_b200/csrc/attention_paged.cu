@@ -702,9 +702,12 @@ template <int NH, bool E4M3>
 struct ChunkShape {
     static constexpr int THREADS = E4M3 ? 448 : 320;
     static constexpr int KST = E4M3 ? 3 : 2, VST = 2;                    // stages of keys and of values
+    // Query rows and probabilities in tensor memory, where it has room for them: what the tensor cores read of shared memory is then keys and
+    // values alone.
+    static constexpr bool TS = NH == 2 || E4M3;
     static constexpr int K_TILE = E4M3 ? PT_TILE : NH * PT_TILE;         // bytes of a stage of keys: bf16, or codes (rows of 128 bytes)
     static constexpr int RAW = PT_KEYS * 64 * NH;                        // bytes of a block's codes of values
-    static constexpr int O_K = NH * PT_TILE, O_V = O_K + KST * K_TILE, O_P = O_V + VST * NH * PT_TILE, O_RAW = O_P + 2 * PT_TILE;
+    static constexpr int O_K = NH * PT_TILE, O_V = O_K + KST * K_TILE, O_P = O_V + VST * NH * PT_TILE, O_RAW = O_P + (TS ? 2 * PT_ROWS * 8 : 2 * PT_TILE);
     // (8 bits) stages of codes of values as they come in
     static constexpr int RST = 2;
     static constexpr int O_KS = O_RAW + (E4M3 ? RST * RAW : 0);          // [4][128] key scales * scale_log2
@@ -712,8 +715,9 @@ struct ChunkShape {
     static constexpr int O_BARS = O_RF + (E4M3 ? PT_ROWS * 4 : 0);
     // (bf16 heads of 64: exactly what lets two CTAs share an SM; 256 bytes of barriers behind the tiles or in the alignment's pad)
     static constexpr int SMEM = 1024 + O_BARS + (NH == 1 && !E4M3 ? 0 : E4M3 ? 512 : 256);
-    static constexpr int PER_SM = SMEM <= 113 * 1024 ? 2 : 1;
-    static constexpr int TMEM = NH == 1 ? 256 : 512;
+    static constexpr int PER_SM = TS ? 1 : 2;
+    static_assert(SMEM <= (TS ? 227 : 113) * 1024, "shared memory of an SM");
+    static constexpr int TMEM = TS ? 512 : 256;
 };
 
 // A piece of a tile's keys, [blocks from, to): what one CTA does.  first, pieces: the tile's pieces are units first .. first + pieces - 1.
@@ -865,7 +869,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     uint8_t *sQ = smem, *sK = smem + Sh::O_K, *sV = smem + Sh::O_V, *sP = smem + Sh::O_P;
     uint64_t* bars = reinterpret_cast<uint64_t*>(pad <= 768u ? smem + Sh::O_BARS : smem_raw);
     uint64_t* q_full = bars;          // 1: the query tile has come
-    uint64_t* q_ready = bars + 1;     // (8 bits) and is two terms of 8 bits
+    uint64_t* q_ready = bars + 1;     // and is in tensor memory (8 bits: as two terms of 8 bits)
     uint64_t* k_full = bars + (E4M3 ? 44 : 2);       // KST
     uint64_t* k_empty = bars + (E4M3 ? 48 : 4);      // KST: the scores of both halves have been formed
     uint64_t* v_full = bars + 6;      // 2
@@ -946,7 +950,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const uint32_t tS = tmem_base, tO = tmem_base + 128;                   // two score buffers of 64, two accumulators of 64 NH columns
+    const uint32_t tS = tmem_base, tO = tmem_base + 128;                   // two score buffers of 64, two accumulators of 64 NH columns,
+    const uint32_t tP = tO + 128 * NH, tQ = tP + 64;                       // two of probabilities, 64 16-bit values each, the rows
 
     if (warp == 0) {
         // ---- producer: a lane per piece of a page
@@ -1049,7 +1054,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const uint64_t dP0 = umma_desc_sw128(smem_u32(sP), 16, 1024), dV0 = umma_desc_sw128(smem_u32(sV), PT_TILE, 1024);
             constexpr uint64_t TILE = PT_TILE >> 4, KSTEP = 32 >> 4, MNSTEP = 2048 >> 4;
             const int nsub = 2 * nkv;
-            bool ok = mbar_wait(E4M3 ? q_ready : q_full, 0, abort_flag);
+            bool ok = mbar_wait(Sh::TS ? q_ready : q_full, 0, abort_flag);
             auto issue_scores = [&](int i) -> bool {
                 const int j = i >> 1, st = j % KST, b = i & 1;
                 if (b == 0 && !mbar_wait(&k_full[st], (uint32_t)((j / KST) & 1), abort_flag)) return false;
@@ -1057,15 +1062,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 tc_fence_after();
                 const uint64_t dK = dK0 + (uint64_t)st * (Sh::K_TILE >> 4) + (uint64_t)b * (TILE / 2);
 #pragma unroll
-                for (int k = 0; k < 4 * NH && E4M3; ++k) {                  // both terms of the rows with the same codes
-                    const int term = k / (2 * NH), e = k % (2 * NH);
-                    umma_f8(tS + (uint32_t)(b * 64), dQ + (NH == 2 ? term * TILE : (uint64_t)(2 * term) * KSTEP) + e * KSTEP, dK + e * KSTEP,
-                            term == 0 ? idesc_s1 : idesc_s, k > 0 ? 1u : 0u);
+                for (int k = 0; k < 4 * NH; ++k) {
+                    if (E4M3) {                                             // both terms of the rows with the same codes
+                        umma_f8_ts(tS + (uint32_t)(b * 64), tQ + (uint32_t)(8 * k), dK + (k % (2 * NH)) * KSTEP, k < 2 * NH ? idesc_s1 : idesc_s, k > 0 ? 1u : 0u);
+                    } else if (Sh::TS) {
+                        umma_bf16_ts(tS + (uint32_t)(b * 64), tQ + (uint32_t)(8 * k), dK + (k >> 2) * TILE + (k & 3) * KSTEP, idesc_s, k > 0 ? 1u : 0u);
+                    } else {
+                        umma_bf16(tS + (uint32_t)(b * 64), dQ + (k >> 2) * TILE + (k & 3) * KSTEP, dK + (k >> 2) * TILE + (k & 3) * KSTEP, idesc_s,
+                                  k > 0 ? 1u : 0u);
+                    }
                 }
-#pragma unroll
-                for (int k = 0; k < 4 * NH && !E4M3; ++k)
-                    umma_bf16(tS + (uint32_t)(b * 64), dQ + (k >> 2) * TILE + (k & 3) * KSTEP, dK + (k >> 2) * TILE + (k & 3) * KSTEP, idesc_s,
-                              k > 0 ? 1u : 0u);
                 umma_commit(&s_full[b]);
                 if (b == 1) umma_commit(&k_empty[st]);
                 return true;
@@ -1079,8 +1085,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 tc_fence_after();
                 const uint64_t dP = dP0 + (uint64_t)b * TILE, dV = dV0 + (uint64_t)(vst * NH) * TILE + (uint64_t)b * (4 * MNSTEP);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_bf16(tO + (uint32_t)(b * 64 * NH), dP + k * KSTEP, dV + k * MNSTEP, idesc_o, (i > 1 || k > 0) ? 1u : 0u);
+                for (int k = 0; k < 4; ++k) {
+                    if (Sh::TS)
+                        umma_bf16_ts(tO + (uint32_t)(b * 64 * NH), tP + (uint32_t)(b * 32 + 8 * k), dV + k * MNSTEP, idesc_o, (i > 1 || k > 0) ? 1u : 0u);
+                    else
+                        umma_bf16(tO + (uint32_t)(b * 64 * NH), dP + k * KSTEP, dV + k * MNSTEP, idesc_o, (i > 1 || k > 0) ? 1u : 0u);
+                }
                 umma_commit(&o_full[b]);
                 if (b == 1) umma_commit(&v_empty[vst]);
             }
@@ -1097,6 +1107,22 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         float m = -INFINITY, l = 0.f, c1 = p.scale_log2;
         bool ok = true;
         uint32_t v[2][32];
+        if (Sh::TS && !E4M3 && nkv > 0 && b == 0) {                         // the rows to tensor memory
+            ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag));
+#pragma unroll
+            for (int c = 0; c < NH; ++c) {
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(sQ + c * PT_TILE + r * 128 + ((d ^ (r & 7)) << 4));
+                    v[0][4 * d] = w.x; v[0][4 * d + 1] = w.y; v[0][4 * d + 2] = w.z; v[0][4 * d + 3] = w.w;
+                }
+                tmem_st32(tQ + lane_base + (uint32_t)(c * 32), v[0]);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0 && ok) mbar_arrive(q_ready);
+        }
         if (E4M3 && nkv > 0) {
             ok = mbar_wait(q_ready, 0, abort_flag);
             c1 = reinterpret_cast<const float*>(smem + Sh::O_RF)[r];
@@ -1159,6 +1185,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const float2 c2 = make_float2(c1, c1), nm2 = make_float2(-m, -m);
             float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             uint8_t* prow = sP + b * PT_TILE + r * 128;
+            uint32_t all[32];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
 #pragma unroll
@@ -1176,9 +1203,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         ls[h & 1] = __fadd2_rn(ls[h & 1], pr);
                         w[h] = E4M3 ? f16_pair(pr.x, pr.y) : bf16_pair(pr.x, pr.y);
                     }
-                    *reinterpret_cast<uint4*>(prow + (((4 * c + g) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (Sh::TS) {
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) all[16 * c + 4 * g + h] = w[h];
+                    } else {
+                        *reinterpret_cast<uint4*>(prow + (((4 * c + g) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
                 }
             }
+            if (Sh::TS) tmem_st32(tP + lane_base + (uint32_t)(b * 32), all);
             l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
             if (move && j > 0) {
                 tc_fence_after();
@@ -1190,10 +1223,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     for (int e = 0; e < 32; ++e) v[0][e] = __float_as_uint(__uint_as_float(v[0][e]) * alpha);
                     tmem_st32(to + (uint32_t)(h2 * 32), v[0]);
                 }
-                tmem_st_wait();
             }
+            if (Sh::TS || (move && j > 0)) tmem_st_wait();
             tc_fence_before();
-            fence_proxy_async();
+            if (!Sh::TS) fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[b]);
         }
@@ -1322,15 +1355,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         // ---- thread = query row once, which becomes two terms of 8 bits; then a key of every block, whose value becomes f16
         const int t = threadIdx.x - 320, q = warp - 10;
         bool ok = true;
-        if (nkv > 0) ok = mbar_wait(q_full, 0, abort_flag);
+        if (nkv > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag));
         if (nkv > 0 && ok) {
+            const int r = (warp & 3) * 32 + lane;                           // (the lanes of tensor memory that this warp reaches)
             uint32_t most = 0u;
-            uint8_t* row = sQ + t * 128;
-            uint4 w[8 * NH];
+            const uint8_t* row = sQ + r * 128;
+            auto eight = [&](int d) { return *reinterpret_cast<const uint4*>(row + (d >> 3) * PT_TILE + (((d & 7) ^ (r & 7)) << 4)); };
 #pragma unroll
             for (int d = 0; d < 8 * NH; ++d) {
-                w[d] = *reinterpret_cast<const uint4*>(row + (d >> 3) * PT_TILE + (((d & 7) ^ (t & 7)) << 4));
-                const uint32_t a = __vmaxu2(__vmaxu2(w[d].x & 0x7fff7fffu, w[d].y & 0x7fff7fffu), __vmaxu2(w[d].z & 0x7fff7fffu, w[d].w & 0x7fff7fffu));
+                const uint4 w = eight(d);
+                const uint32_t a = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
                 most = max(most, max(a & 0xffffu, a >> 16));
             }
             // Scaled by a power of two so that the row's largest magnitude lies in [2^11, 2^12).  Three bits of an element are its e5m2
@@ -1339,30 +1373,35 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const int e = max((int)(most >> 7), 12);
             const bool odd = e == 255;                                      // (an infinity or NaN: no score of this row is a number)
             const float down = odd ? 1.f : __uint_as_float((uint32_t)(265 - e) << 23), up = odd ? 1.f : __uint_as_float((uint32_t)(e - 11) << 23);
-            reinterpret_cast<float*>(smem + Sh::O_RF)[t] = up;
+            reinterpret_cast<float*>(smem + Sh::O_RF)[r] = up;
+            const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+#pragma unroll 1
+            for (int c = 0; c < NH; ++c) {                                  // 64 elements: 16 columns of first terms, 16 of second ones
+                uint32_t hi[16], lo[16];
 #pragma unroll
-            for (int d = 0; d < 4 * NH; ++d) {
-                const uint32_t u[8] = {w[2 * d].x, w[2 * d].y, w[2 * d].z, w[2 * d].w, w[2 * d + 1].x, w[2 * d + 1].y, w[2 * d + 1].z, w[2 * d + 1].w};
-                uint32_t hi[4], lo[4];
+                for (int d = 0; d < 8; ++d) {
+                    const uint4 w = eight(8 * c + d);
+                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t a[2], b[2];
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t a[2], b[2];
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float2 f = bf16_floats(u[2 * i + x]);
-                        f.x *= down; f.y *= down;
-                        a[x] = e5m2_pair(f.x, f.y);
-                        const float2 g = f16_floats((a[x] & 0xffu) << 8 | (a[x] & 0xff00u) << 16);
-                        b[x] = e4m3_pair(f.x - g.x, f.y - g.y);
+                        for (int x = 0; x < 2; ++x) {
+                            float2 f = bf16_floats(u[2 * i + x]);
+                            f.x *= down; f.y *= down;
+                            a[x] = e5m2_pair(f.x, f.y);
+                            const float2 g = f16_floats((a[x] & 0xffu) << 8 | (a[x] & 0xff00u) << 16);
+                            b[x] = e4m3_pair(f.x - g.x, f.y - g.y);
+                        }
+                        hi[2 * d + i] = odd ? 0x7f7f7f7fu : a[0] | a[1] << 16;
+                        lo[2 * d + i] = odd ? 0x7f7f7f7fu : b[0] | b[1] << 16;
                     }
-                    hi[i] = odd ? 0x7f7f7f7fu : a[0] | a[1] << 16;
-                    lo[i] = odd ? 0x7f7f7f7fu : b[0] | b[1] << 16;
                 }
-                uint8_t* second = NH == 2 ? row + PT_TILE + ((d ^ (t & 7)) << 4) : row + (((d + 4) ^ (t & 7)) << 4);
-                *reinterpret_cast<uint4*>(row + ((d ^ (t & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(second) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                tmem_st16(tQ + lane_base + (uint32_t)(16 * c), hi);
+                tmem_st16(tQ + lane_base + (uint32_t)(16 * (NH + c)), lo);
             }
-            fence_proxy_async();
+            tmem_st_wait();
+            tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
         }
