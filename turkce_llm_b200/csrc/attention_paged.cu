@@ -701,20 +701,20 @@ constexpr int PT_TILE = 128 * 128;                      // bytes of a [128][64] 
 template <int NH, bool E4M3>
 struct ChunkShape {
     static constexpr int THREADS = E4M3 ? 448 : 320;
-    static constexpr int KST = E4M3 ? 3 : 2, VST = 2;                    // stages of keys and of values
+    static constexpr int KST = NH == 2 || E4M3 ? 3 : 2, VST = E4M3 ? 2 : KST;        // stages of keys and of values
     // Query rows and probabilities in tensor memory, where it has room for them: what the tensor cores read of shared memory is then keys and
     // values alone.
     static constexpr bool TS = NH == 2 || E4M3;
     static constexpr int K_TILE = E4M3 ? PT_TILE : NH * PT_TILE;         // bytes of a stage of keys: bf16, or codes (rows of 128 bytes)
     static constexpr int RAW = PT_KEYS * 64 * NH;                        // bytes of a block's codes of values
-    static constexpr int O_K = NH * PT_TILE, O_V = O_K + KST * K_TILE, O_P = O_V + VST * NH * PT_TILE, O_RAW = O_P + (TS ? 2 * PT_ROWS * 8 : 2 * PT_TILE);
+    static constexpr int O_K = NH * PT_TILE, O_V = O_K + KST * K_TILE, O_P = O_V + VST * NH * PT_TILE, O_RAW = O_P + (TS ? 0 : 2 * PT_TILE);
     // (8 bits) stages of codes of values as they come in
     static constexpr int RST = 2;
-    static constexpr int O_KS = O_RAW + (E4M3 ? RST * RAW : 0);          // [4][128] key scales * scale_log2
-    static constexpr int O_RF = O_KS + (E4M3 ? 4 * PT_KEYS * 4 : 0);     // [128] row factors
+    static constexpr int O_KS = O_RAW + (E4M3 ? RST * RAW : 0);          // [8][128] key scales * scale_log2
+    static constexpr int O_RF = O_KS + (E4M3 ? 8 * PT_KEYS * 4 : 0);     // [128] row factors
     static constexpr int O_BARS = O_RF + (E4M3 ? PT_ROWS * 4 : 0);
     // (bf16 heads of 64: exactly what lets two CTAs share an SM; 256 bytes of barriers behind the tiles or in the alignment's pad)
-    static constexpr int SMEM = 1024 + O_BARS + (NH == 1 && !E4M3 ? 0 : E4M3 ? 512 : 256);
+    static constexpr int SMEM = 1024 + O_BARS + (TS ? 640 : 0);
     static constexpr int PER_SM = TS ? 1 : 2;
     static_assert(SMEM <= (TS ? 227 : 113) * 1024, "shared memory of an SM");
     static constexpr int TMEM = TS ? 512 : 256;
@@ -870,10 +870,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     uint64_t* bars = reinterpret_cast<uint64_t*>(pad <= 768u ? smem + Sh::O_BARS : smem_raw);
     uint64_t* q_full = bars;          // 1: the query tile has come
     uint64_t* q_ready = bars + 1;     // and is in tensor memory (8 bits: as two terms of 8 bits)
-    uint64_t* k_full = bars + (E4M3 ? 44 : 2);       // KST
-    uint64_t* k_empty = bars + (E4M3 ? 48 : 4);      // KST: the scores of both halves have been formed
-    uint64_t* v_full = bars + 6;      // 2
-    uint64_t* v_empty = bars + 8;     // 2
+    uint64_t* k_full = bars + (Sh::TS ? 44 : 2);       // KST
+    uint64_t* k_empty = bars + (Sh::TS ? 48 : 4);      // KST: the scores of both halves have been formed
+    uint64_t* v_full = bars + (Sh::TS ? 52 : 6);     // VST
+    uint64_t* v_empty = bars + (Sh::TS ? 56 : 8);    // VST
     uint64_t* v_land = bars + 10;     // 1: values of a block that is looked through first
     uint64_t* s_full = bars + 11;     // 2
     uint64_t* s_free = bars + 13;     // 2
@@ -882,13 +882,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
     uint64_t* raw_full = bars + 32;   // (8 bits) RST: codes of values; behind the 256 bytes of the rest
     uint64_t* raw_empty = bars + 36;  // RST
-    uint64_t* ks_full = bars + 40;    // 4: what the softmax warps read of a block's scales.  (Not k_full, which may be a whole round ahead of them.)
+    uint64_t* ks_full = bars + 60;    // 8: what the softmax warps read of a block's scales.  (Not k_full, which may be a whole round ahead of them.)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* bad_value = abort_flag + 1;                              // a value that is not finite has been set to zero
     volatile int* v_exponent = abort_flag + 2;                             // (8 bits) the last block's reference
     volatile int* is_last = abort_flag + 3;                                // this CTA was the last with its piece of a tile
-    float* v_moved = reinterpret_cast<float*>(tmem_slot + 6);              // (8 bits) [4]: 2^(reference before - reference) of a block
-    uint32_t* warp_most = tmem_slot + 10;                                  // (8 bits) [2][4]
+    float* v_moved = reinterpret_cast<float*>(tmem_slot + 6);              // (8 bits) [8]: 2^(reference before - reference) of a block
+    uint32_t* warp_most = tmem_slot + 14;                                  // (8 bits) [2][4]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // No wait for the kernel in front (paged_rows_kernel writes other rows): it has let this one start after what both read was there,
@@ -934,14 +934,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     if (threadIdx.x == 32 * 2) {
         mbar_init(q_full, 1); mbar_init(q_ready, 4); mbar_init(v_land, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&v_full[i], E4M3 ? 4 : 1); mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1);
         }
         if (E4M3)
             for (int i = 0; i < Sh::RST; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
         for (int i = 0; i < KST; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
+        for (int i = 0; i < VST; ++i) { mbar_init(&v_full[i], E4M3 ? 4 : 1); mbar_init(&v_empty[i], 1); }
         if (E4M3)
-            for (int i = 0; i < 4; ++i) mbar_init(&ks_full[i], 4);
+            for (int i = 0; i < 8; ++i) mbar_init(&ks_full[i], 4);
         *abort_flag = 0; *bad_value = 0; *v_exponent = 0;
         fence_mbar_init();
     }
@@ -988,10 +988,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
             const int count = min(page_pieces, last_piece - at);
             const int block = pg * p.v.heads + head, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift, o = lane << piece_shift;
-            const int st = j & 1;
+            const int st = j % KST;
             {
                 const int vst = j % VST;
-                ok = mbar_wait(&k_empty[st], (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag);
+                ok = mbar_wait(&k_empty[st], (uint32_t)((j / KST) & 1) ^ 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (lane == 0) mbar_expect_tx(&k_full[st], (uint32_t)(count * piece_keys * 128 * NH));
@@ -1128,7 +1128,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             c1 = reinterpret_cast<const float*>(smem + Sh::O_RF)[r];
         }
         for (int j = 0; j < nkv && ok; ++j) {
-            if (E4M3 && !mbar_wait(&ks_full[j & 3], (uint32_t)((j >> 2) & 1), abort_flag)) { ok = false; break; }
+            if (E4M3 && !mbar_wait(&ks_full[j & 7], (uint32_t)((j >> 3) & 1), abort_flag)) { ok = false; break; }
             if (!mbar_wait(&s_full[b], (uint32_t)(j & 1), abort_flag)) { ok = false; break; }
             tc_fence_after();
             tmem_ld32(ts, v[0]);
@@ -1136,7 +1136,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             tmem_ld_wait();
             float moved = 1.f;
             if (E4M3) {
-                const float4* ks = reinterpret_cast<const float4*>(smem + Sh::O_KS) + (j & 3) * (PT_KEYS / 4) + b * 16;
+                const float4* ks = reinterpret_cast<const float4*>(smem + Sh::O_KS) + (j & 7) * (PT_KEYS / 4) + b * 16;
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -1147,7 +1147,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         v[c][e] = __float_as_uint(x.x); v[c][e + 1] = __float_as_uint(x.y);
                         v[c][e + 2] = __float_as_uint(y.x); v[c][e + 3] = __float_as_uint(y.y);
                     }
-                moved = v_moved[j & 3];
+                moved = v_moved[j & 7];
             }
             tc_fence_before();
             __syncwarp();
@@ -1234,7 +1234,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (ok && nkv > 0)
             ok = mbar_wait(&o_full[0], (uint32_t)((nkv - 1) & 1), abort_flag) && mbar_wait(&o_full[1], (uint32_t)((nkv - 1) & 1), abort_flag) &&
                  mbar_wait(&v_full[(nkv - 1) % VST], (uint32_t)(((nkv - 1) / VST) & 1), abort_flag);        // (for bad_value)
-        float2* stat = reinterpret_cast<float2*>(sP);
+        float2* stat = reinterpret_cast<float2*>(Sh::TS ? sK : sP);        // (nothing reads keys any more)
         if (ok) stat[b * PT_ROWS + r] = make_float2(m, l);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const bool none = pos < 0;                                          // a row without a key
@@ -1422,8 +1422,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         int reference = 0;
         float f = 0.f, f_next = 0.f;                                        // the factor of this key's value, in this block and the next
         bool fin = true, fin_next = true;                                   // its scale is finite
-        // What the softmax warps need of a block's scales, a block ahead of the values and so three blocks ahead of their product at
-        // most: the ring of four holds what is still read.
+        // What the softmax warps need of a block's scales, a block ahead of the values and so four blocks ahead of those that are still
+        // read at most: a ring of eight.
         auto scales = [&](int j) -> bool {
             const float vs = vs_new;
             const uint32_t ve = (__float_as_uint(vs) >> 23) & 255u;
@@ -1434,14 +1434,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (lane == 0) w4[q] = most;
             if (!all_of(ok, 2, 128)) return false;
             const int now = max(reference, (int)max(max(w4[0], w4[1]), max(w4[2], w4[3])));
-            reinterpret_cast<float*>(smem + Sh::O_KS)[(j & 3) * PT_KEYS + t] = ks_new * p.scale_log2;
+            reinterpret_cast<float*>(smem + Sh::O_KS)[(j & 7) * PT_KEYS + t] = ks_new * p.scale_log2;
             if (t == 0) {
                 const int d = now - reference;                              // (an accumulator that is still empty may be scaled by anything)
-                v_moved[j & 3] = d == 0 ? 1.f : d > 126 ? 0.f : __uint_as_float((uint32_t)(127 - d) << 23);
+                v_moved[j & 7] = d == 0 ? 1.f : d > 126 ? 0.f : __uint_as_float((uint32_t)(127 - d) << 23);
                 *v_exponent = now;
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ks_full[j & 3]);
+            if (lane == 0) mbar_arrive(&ks_full[j & 7]);
             reference = now;
             // code * scale * 2^(6 - reference), in two steps: 2^(127 - reference) alone may be no normal number
             const int half_way = (127 - now) / 2;
