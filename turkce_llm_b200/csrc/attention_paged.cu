@@ -30,7 +30,8 @@ struct PagedAttParams {
     float* part_o; float2* part_ml;  // [2 grid][16][hd], [2 grid][16]: results of items that a CTA shares with its neighbours
     unsigned int* arrived;           // [grid], zero between launches: pieces written of the item that begins in a CTA's run and goes on
     int rows, H, group, max_q, max_kv, grid, whole;
-    int behind_plan;                 // few rows: the kernel in front is paged_plan_kernel, whose results concern the next one
+    const int* runs;                 // few rows: CTAs that share the work, as the plan says; nullptr: all
+    int behind_chunks;               // few rows: the kernel in front is paged_chunk_kernel, which writes other rows
     uint32_t group_magic;            // x / group = x * group_magic >> 16 for x < 128
     float scale_log2;
     int* err;
@@ -169,7 +170,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         fence_mbar_init();
     }
     __syncthreads();
-    if (!p.behind_plan) pdl_wait();      // (the plan has waited itself before it let this kernel start)
+    if (!p.behind_chunks) pdl_wait();    // (the tiles' kernel has waited itself before it let this one start)
 
     if (warp == PA_WARPS) {
         // ---- producer: finds this CTA's items, and fills the ring with their blocks.  A lane per piece of a page.
@@ -212,7 +213,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 total += __shfl_sync(0xffffffffu, incl, 31);
             }
             total *= heads;
-            per = max((total + p.grid - 1) / p.grid, (long long)(PA_LEAST >> KEYS_LOG2));
+            const int runs = p.runs ? min(max(__ldcg(p.runs), 1), p.grid) : p.grid;
+            per = max((total + runs - 1) / runs, (long long)(PA_LEAST >> KEYS_LOG2));
             at_block = per * blockIdx.x;
             left = min(per, total - at_block);
             if (left > 0) {
@@ -326,7 +328,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             *reinterpret_cast<int*>(smem + Sh::O_WHAT + (i % STAGES) * Sh::WHAT) = PA_END;
             mbar_arrive(&full[i % STAGES]);
         }
-        if (p.behind_plan) pdl_wait();       // the next kernel reads the plan
+        if (p.behind_chunks) pdl_wait();     // what follows finds the tiles' rows as well
         pdl_launch_dependents_now();
         if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 73); }
         // (the consumers wait for everything that has been asked for)
@@ -728,7 +730,9 @@ struct PagedChunkParams {
     int tokens, tiles;                // tokens per tile; tiles of max_q
     int planned;                      // units come from paged_plan_kernel; else a CTA per tile
     int most_units, slots;            // room for units; CTAs that the chip holds
-    int* count;                       // units there are
+    int* count;                       // units there are; CTAs of paged_rows_kernel that have work
+    int rows_keys_log2, rows_cost;    // keys of its blocks; what one costs, in quarters of a tile's block
+    int rows_slots, rows_lost;        // CTAs of it that the chip holds; how many fewer for a CTA with a tile
     unsigned int* arrived;            // [most_units]: pieces written, by the tile's first unit
     int* bad;                         // [most_units]: a piece has left out a value that is not finite
     ChunkUnit* units;
@@ -749,18 +753,24 @@ constexpr int PL_THREADS = 512, PL_TILES = 1024;
 __global__ void __launch_bounds__(PL_THREADS)
 paged_plan_kernel(const PagedChunkParams pp) {
     __shared__ int seq[PL_TILES], idx[PL_TILES], nb[PL_TILES], off[PL_TILES];
-    __shared__ int count, longest, best_cap, cost[PL_THREADS / 32], caps[PL_THREADS / 32], total;
+    __shared__ int count, longest, best_cap, cost[PL_THREADS / 32], caps[PL_THREADS / 32], runs[PL_THREADS / 32], total;
+    __shared__ long long few;                                // blocks of paged_rows_kernel
     const PagedAttParams& p = pp.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) { count = 0; longest = 1; total = 0; }
+    if (tid == 0) { count = 0; longest = 1; total = 0; few = 0; }
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
     // ---- the tiles of one head, in the order of the sequences
     for (int s0 = 0; s0 < p.v.seqs; s0 += 32) {
         if (warp != 0) break;
-        int q0, n = 0, kv = 0, tiles = 0;
-        if (s0 + lane < p.v.seqs && batch_of(p, s0 + lane, q0, n, kv) && n * p.group > PA_ROWS) tiles = (n + pp.tokens - 1) / pp.tokens;
+        int q0, n = 0, kv = 0, tiles = 0, blocks = 0;
+        if (s0 + lane < p.v.seqs && batch_of(p, s0 + lane, q0, n, kv)) {
+            if (n * p.group > PA_ROWS) tiles = (n + pp.tokens - 1) / pp.tokens;
+            else if (n > 0) blocks = max(1, (kv + (1 << pp.rows_keys_log2) - 1) >> pp.rows_keys_log2);
+        }
+        blocks = __reduce_add_sync(0xffffffffu, blocks);
+        if (lane == 0) few += blocks;
         int incl = tiles;
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(0xffffffffu, incl, o);
@@ -784,8 +794,20 @@ paged_plan_kernel(const PagedChunkParams pp) {
         units = __reduce_add_sync(0xffffffffu, units) * p.v.heads;
         if (lane == 0) {
             caps[warp] = cap;
-            // (in blocks: three for the start of a piece and its result to memory, one for a piece's result on its way back)
-            cost[warp] = (pieces == 1 || units <= pp.most_units) ? (units + pp.slots - 1) / pp.slots * (cap + 3) + pieces : 0x7fffffff;
+            // (in quarters of a block: three blocks for the start of a piece and its result to memory, one for a piece's result on its way
+            // back, four for the start of the few rows' kernel.)  Both kernels side by side, or one after the other.
+            const long long tile_cost = 4 * ((long long)(units + pp.slots - 1) / pp.slots * (cap + 3) + pieces), blocks = few * p.v.heads;
+            const int beside = pp.rows_slots - pp.rows_lost * units;
+            long long best = tile_cost;
+            runs[warp] = pp.rows_slots;
+            if (blocks > 0) {
+                best += pp.rows_cost * blocks / pp.rows_slots + 16;
+                if (beside > 0) {
+                    const long long both = max(tile_cost, pp.rows_cost * blocks / beside + 16);
+                    if (both < best) { best = both; runs[warp] = beside; }
+                }
+            }
+            cost[warp] = (pieces == 1 || units <= pp.most_units) ? (int)min(best, 0x7ffffffeLL) : 0x7fffffff;
         }
     }
     __syncthreads();
@@ -793,6 +815,7 @@ paged_plan_kernel(const PagedChunkParams pp) {
         int w = 0;
         for (int i = 1; i < PL_THREADS / 32; ++i) if (cost[i] < cost[w]) w = i;
         best_cap = caps[w];
+        pp.count[1] = runs[w];
     }
     __syncthreads();
     const int cap = best_cap;
@@ -891,14 +914,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     uint32_t* warp_most = tmem_slot + 14;                                  // (8 bits) [2][4]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // No wait for the kernel in front (paged_rows_kernel writes other rows): it has let this one start after what both read was there,
-    // the plan included.  Every CTA waits for it at its end, so that what follows finds both kernels' rows.
+    pdl_wait();
+    pdl_launch_dependents_now();         // paged_rows_kernel reads nothing of this kernel's: it starts where there is room
     int s, head, tile, from = 0, to = 0x7fffffff, pieces = 1, first_unit = 0;
     if (pp.planned) {
-        if ((int)blockIdx.x >= *pp.count) {
-            pdl_wait();
-            return;
-        }
+        if ((int)blockIdx.x >= *pp.count) return;
         const int4* u = reinterpret_cast<const int4*>(pp.units + blockIdx.x);
         const int4 a = u[0], b = u[1];
         s = a.x; head = a.y; tile = a.z; from = a.w; to = b.x; first_unit = b.y; pieces = b.z;
@@ -909,10 +929,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     int q0, n, kv;
     const bool fine = batch_of(p, s, q0, n, kv);                           // (paged_rows_kernel reports it)
     const int tok0 = tile * pp.tokens;
-    if (!fine || n * p.group <= PA_ROWS || tok0 >= n) {
-        pdl_wait();
-        return;
-    }
+    if (!fine || n * p.group <= PA_ROWS || tok0 >= n) return;
     const int tokens = min(pp.tokens, n - tok0);
     const int first_pos = kv - n + tok0, last_pos = first_pos + tokens - 1;
     const int nkv = min(to, last_pos >= 0 ? last_pos / PT_KEYS + 1 : 0) - from;      // blocks of keys, from block `from` on
@@ -1043,7 +1060,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             __syncwarp();
         }
-        pdl_launch_dependents_now();
         if (!ok && lane == 0) { *abort_flag = 1; atomicExch(p.err, 77); }
     } else if (warp == 1) {
         if (elect_one() && nkv > 0) {
@@ -1510,7 +1526,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 
     __syncwarp();
     if (*abort_flag) for (int i = 0; i < 64; ++i) __nanosleep(1000);
-    pdl_wait();
     tc_fence_before();
     __syncthreads();
     if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, Sh::TMEM); }
@@ -1543,7 +1558,10 @@ int plan_chunks(DeviceCtx* ctx, const PagedAttParams& p, const PagedPlan& pl, ui
     pp->a = p;
     pp->tokens = PT_ROWS / p.group;
     pp->tiles = (p.max_q + pp->tokens - 1) / pp->tokens;
-    pp->planned = p.behind_plan; pp->most_units = pl.most_units; pp->slots = Sh::PER_SM * ctx->sm_count;
+    pp->planned = pl.most_units > 0 ? 1 : 0; pp->most_units = pl.most_units; pp->slots = Sh::PER_SM * ctx->sm_count;
+    // a CTA with a tile takes the place of one of the two that an SM holds for few rows, or of all
+    pp->rows_keys_log2 = paged_keys(NH, E4M3) == 128 ? 7 : 6; pp->rows_cost = NH == 2 && !E4M3 ? 6 : 3;
+    pp->rows_slots = paged_per_sm(NH, E4M3) * ctx->sm_count; pp->rows_lost = Sh::TS ? paged_per_sm(NH, E4M3) : 1;
     // (see paged_plan.h for the room)
     pp->count = reinterpret_cast<int*>(ws);
     pp->arrived = reinterpret_cast<unsigned int*>(ws + 16);
@@ -1584,15 +1602,15 @@ int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedChunkParams& pp
     return 0;
 }
 
-// The kernel for few rows goes first: its CTAs leave the SMs one after the other, and tiles start where they do.
 template <int NH, bool E4M3>
-int launch_both(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, const PagedPlan& pl, uint8_t* more, cudaStream_t st) {
-    const bool chunks = p.max_q * (long long)p.group > PA_ROWS;
-    PagedChunkParams pp;
-    if (chunks) TB_TRY((plan_chunks<NH, E4M3>(ctx, p, pl, more, &pp, st)));
-    TB_TRY((launch_rows<NH, E4M3>(ctx, c, p, st)));
-    if (chunks) TB_TRY((launch_chunks<NH, E4M3>(ctx, c, pp, st)));
-    return 0;
+int launch_both(DeviceCtx* ctx, const TbKvCache* c, PagedAttParams& p, const PagedPlan& pl, uint8_t* more, cudaStream_t st) {
+    if (p.behind_chunks) {
+        PagedChunkParams pp;
+        TB_TRY((plan_chunks<NH, E4M3>(ctx, p, pl, more, &pp, st)));
+        TB_TRY((launch_chunks<NH, E4M3>(ctx, c, pp, st)));
+        if (pp.planned) p.runs = pp.count + 1;
+    }
+    return launch_rows<NH, E4M3>(ctx, c, p, st);
 }
 
 }  // namespace
@@ -1613,7 +1631,8 @@ int launch_attention_paged(DeviceCtx* ctx, const TbKvCache* c, const int* q_star
     p.arrived = static_cast<unsigned int*>(ws);
     p.rows = rows; p.H = H; p.group = group; p.max_q = max_q; p.max_kv = max_kv; p.grid = pl.grid; p.whole = pl.whole ? 1 : 0;
     p.scale_log2 = scale * 1.4426950408889634f; p.err = ctx->d_err;
-    p.group_magic = (65536u + group - 1) / group; p.behind_plan = pl.most_units > 0 ? 1 : 0;
+    p.group_magic = (65536u + group - 1) / group; p.behind_chunks = max_q * (long long)group > PA_ROWS ? 1 : 0;
+    p.runs = nullptr;
     const bool wide = c->head_dim > 64, e4m3 = c->type == TB_KV_E4M3;
     uint8_t* more = static_cast<uint8_t*>(ws) + pl.rows_bytes;
     return e4m3 ? (wide ? launch_both<2, true>(ctx, c, p, pl, more, st) : launch_both<1, true>(ctx, c, p, pl, more, st))

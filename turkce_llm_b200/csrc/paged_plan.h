@@ -43,7 +43,7 @@ inline PagedPlan paged_plan(int seqs, int heads, int group, int hd, bool e4m3, i
         const int64_t tokens = PT_ROWS / group, least_rows = PA_ROWS / group + 1;
         const int64_t tiles = heads * (rows / tokens + std::min<int64_t>(seqs, rows / least_rows)), slots = (int64_t)paged_tiles_per_sm(wide, e4m3) * sms;
         if (tiles < 2 * slots && max_kv > PT_KEYS) {
-            p.most_units = (int)(3 * slots + 3) / 4 * 4;
+            p.most_units = (int)(std::max(slots, tiles) + 3) / 4 * 4;
             // header, then for every unit: a counter, a flag, what it is, and [128] (maximum, sum) and [128][64 wide] float32
             p.workspace += 16 + (int64_t)p.most_units * (4 + 4 + 32 + PT_ROWS * (8 + 64 * wide * 4));
         }
