@@ -258,9 +258,12 @@ int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_
  * scale positive.  d_lse (optional): float [rows, q_heads], natural
  * log of the row's sum of exponentials.  Keys behind a row's position have no influence on it, whatever they hold.  A row without
  * any key (kv_len below the number of new rows) gets zeros and lse -infinity.
+ * 8-bit rows: scores are exact but for 2^-21 of a row's largest query element; next to a row's largest probability those of 2^-32 of it
+ * and more count, and values of 2^-31 of the sequence's largest scale and more.
  * max_q and max_kv bound the new rows and the keys of any one sequence (host numbers: they size the launch, and a captured
- * call may be replayed with any lengths within them).  d_workspace: tb_attention_paged_workspace(..) bytes, 16-byte aligned
- * (NULL where that is 0), zero before its first use; every call leaves it ready for the next one, of any batch that needs no more.
+ * call may be replayed with any lengths within them).  d_workspace: 16-byte aligned (NULL where the call needs none), zero before its
+ * first use; every call leaves it ready for the next one, of whatever sizes and types.  tb_attention_paged_workspace(..): bytes that no
+ * batch of the cache's sequences with no more rows, new rows and keys needs more than; a larger one is refused.
  * Calls that can overlap on the GPU need one each.  (After a call that reported a failed wait: zero it again.) */
 int64_t tb_attention_paged_workspace(const TbKvCache* cache, int rows, int q_heads, int max_q, int max_kv);
 int tb_attention_paged(const TbKvCache* cache, const int32_t* d_q_start, const int32_t* d_kv_len, const void* d_Q, int64_t ld_q,

@@ -278,6 +278,156 @@ def test_two_calls_side_by_side(tb):
     tb.sync_check()
 
 
+def test_one_workspace_for_calls_of_all_sizes_and_types(tb):
+    """Single tokens of many and of few CTAs, whole items, chunks in pieces and tiles that are not cut, one after the other."""
+    cases = [(False, [1, 1, 1], [5000, 4000, 3000], 64), (True, [1], [9000], 64), (False, [60, 1], [900, 40], 64), (False, [1, 1], [30, 500], 64),
+             (True, [1, 1, 1], [5000, 4000, 3000], 128), (False, [200], [3000], 128), (True, [1, 1], [2100, 700], 64), (True, [90, 1], [2000, 1500], 64)]
+    bs = [Batch(e, new, kv, 2, dim, 16, seed=i) for i, (e, new, kv, dim) in enumerate(cases)]
+    ws = max((b.cache.workspace(4, b.rows, max(b.new), max(b.kv)) for b in bs), key=lambda w: 0 if w is None else w.nbytes)
+    for _ in range(2):
+        for b in bs:
+            q = torch.randn(b.rows, 4 * b.dim, device="cuda").to(torch.bfloat16)
+            att, lse = torch.zeros_like(q), torch.zeros(b.rows, 4, device="cuda")
+            b.cache.attend(q, att, b.q_start, b.kv_len, max(b.new), max(b.kv), lse=lse, workspace=ws)
+            compare(b, 4, q.float().cpu().numpy().reshape(b.rows, 4, b.dim), att.float().cpu().numpy().reshape(b.rows, 4, b.dim), lse.cpu().numpy())
+    tb.sync_check()
+
+
+@pytest.mark.parametrize("e4m3,dim", [(False, 64), (True, 64), (False, 128), (True, 128)])
+def test_many_sequences_of_all_kinds(tb, e4m3, dim):
+    """More sequences than a warp has lanes and than one look of the single tokens' kernel takes; chunks among them, empty ones too."""
+    rng = np.random.default_rng(dim + e4m3)
+    new = [int(rng.choice([0, 1, 1, 1, 1, 2, 9])) for _ in range(300)]
+    new[17], new[200], new[299] = 150, 40, 33
+    kv = [n + int(rng.integers(0, 200)) for n in new]
+    kv[0], kv[150], kv[17], kv[31] = new[0] + 2500, new[150] + 3000, 1200, new[31]
+    b = Batch(e4m3, new, kv, 2, dim, 32, seed=dim)
+    compare(b, 4, *attend(b, 4, seed=10))
+
+
+@pytest.mark.parametrize("e4m3,dim,G", [(False, 64, 16), (True, 64, 8), (True, 128, 8), (False, 128, 8)])
+def test_more_tiles_than_the_chip_holds_at_once(tb, e4m3, dim, G):
+    new = [130] * 19 + [3]
+    kv = [130 + 7 * s for s in range(19)] + [1]
+    b = Batch(e4m3, new, kv, G, dim, 64, seed=G)
+    compare(b, G, *attend(b, G, seed=11))
+
+
+def test_replayed_chunks_follow_the_lengths(tb):
+    """Two graphs of one workspace, replayed in turn: other chunks, other tiles, other pieces than those of the capture."""
+    H, G, rows, bound = 4, 2, 260, 2048
+    for e4m3 in (False, True):
+        a = Batch(e4m3, [200, 1, 2], [1900, 700, 60], G, 64, 32, seed=1, width=bound // 32)
+        b = Batch(e4m3, [17, 1, 240], [30, 2000, 1000], G, 64, 32, seed=2, width=bound // 32)
+        ws = a.cache.workspace(H, rows, rows, bound)
+        held = []
+        for x in (a, b):
+            q = torch.randn(rows, H * 64, device="cuda").to(torch.bfloat16)
+            att, lse = torch.zeros_like(q), torch.zeros(rows, H, device="cuda")
+            lens, starts = torch.tensor([1, 1, 1], dtype=torch.int32, device="cuda"), torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda")
+            graph = torch.cuda.CUDAGraph()
+            x.cache.attend(q, att, starts, lens, rows, bound, lse=lse, workspace=ws)
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                x.cache.attend(q, att, starts, lens, rows, bound, lse=lse, workspace=ws)
+            lens.copy_(x.kv_len)
+            starts.copy_(x.q_start)
+            held.append((x, graph, q, att, lse, lens, starts))
+        for _ in range(3):
+            for x, graph, q, att, lse, _, _ in held:
+                att.zero_()
+                graph.replay()
+                torch.cuda.synchronize()
+                compare(x, H, *(t[:x.rows].float().cpu().numpy().reshape(x.rows, H, -1) for t in (q, att)), lse[:x.rows].cpu().numpy())
+                assert (att[x.rows:] == 0).all()
+    tb.sync_check()
+
+
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_8_bit_rows_of_very_different_sizes(tb, new, dim):
+    """Scales of values over 2^90, of keys over 2^20; queries with one element that is 2^9 times the others."""
+    b = Batch(True, [new, 1], [500 + new, 300], 1, dim, 16, seed=dim)
+    rng = np.random.default_rng(4)
+    b.host["v_scale"][:] = np.ldexp(b.host["v_scale"], rng.integers(-60, 30, b.host["v_scale"].shape))
+    b.host["k_scale"][:] = np.ldexp(b.host["k_scale"], rng.integers(-20, 1, b.host["k_scale"].shape))
+    b.host["v_scale"][b.table[0, 3], 0, 2] = 0.0
+    for n in ("k", "v"):
+        b.dev[n + "_scale"].copy_(torch.from_numpy(b.host[n + "_scale"]))
+    q = torch.randn(b.rows + 3, 2 * dim).to(torch.bfloat16)
+    q[:, 5] *= 512
+    q[:, dim + 9] *= 512
+    rows, got, lse = attend(b, 2, seed=12, q=q)
+    # Beside the bound of other batches: rows go to the tensor cores exact but for 2^-21 of their largest element, against every key.
+    # Probabilities are f16.  In chunks, at least 2^7 for a row's largest: off by 2^-25 at most where they are small, which is 2^-32 of the
+    # largest, times every value; and values are f16 against the largest scale s, 64 s and more, off by 2^-25 of that 64th: 2^-31 s.  For
+    # single tokens, at least 2^13 for the largest product p s: off by 2^-38 of it per key, times a code of 448 at most (2^-29).
+    # The logarithm: exponents of up to 2^7 are added to scores of single tokens in float32, half a unit in the last place is 2^-18.
+    for s in range(2):
+        at = slice(b.starts[s], b.starts[s + 1])
+        k, v = b.sequence("k", s), b.sequence("v", s)
+        want, want_lse, spread, size = plain.attention(rows[at], k, v, np.arange(b.kv[s] - b.new[s], b.kv[s]), dim ** -0.5)
+        more = 2.0 ** -21 * np.abs(rows[at]).max(axis=2) * np.abs(k[:, 0]).sum(axis=1).max() * dim ** -0.5
+        score = (dim + 4) * 2.0 ** -24 * size + more
+        scales = np.stack([b.host["v_scale"][b.table[s, t // 16], 0, t % 16] for t in range(b.kv[s])]).astype(np.float64)
+        if b.new[s] > 16 // 2:
+            lost = 2.0 ** -32 * np.abs(v[:, 0]).sum(axis=0)[None, None] + 2.0 ** -31 * scales.max()
+        else:
+            p = np.exp(np.einsum("td,rhd->rht", k[:, 0], rows[at].astype(np.float64)) * dim ** -0.5 - want_lse[..., None])
+            lost = 2.0 ** -29 * b.kv[s] * (p * scales).max(axis=2)[..., None]
+        bound = 2.0 ** -8 * np.abs(want) + (2.0 ** -8 * 1.01 + 2 * score[..., None] + 2.0 ** -17) * spread + lost + 1e-30
+        assert (np.abs(got[at] - want) <= bound).all(), np.nanmax(np.abs(got[at] - want) / bound)
+        assert (np.abs(lse[at] - want_lse) <= score + 2.0 ** -18 + 2.0 ** -20 * (1 + np.abs(want_lse))).all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_8_bit_values_of_zeros(tb, new):
+    """Rows of zeros have the smallest scale there is: many of them, alone, in front of and behind others."""
+    for zeros in (slice(0, 400), slice(0, 150), slice(100, 400)):
+        b = Batch(True, [new], [300 + new], 1, 64, 16, seed=6)
+        for t in range(*zeros.indices(300 + new)):
+            b.host["v"][b.table[0, t // 16], 0, t % 16] = 0
+            b.host["v_scale"][b.table[0, t // 16], 0, t % 16] = 2.0 ** -126
+        b.dev["v"].copy_(torch.from_numpy(b.host["v"]).cuda().view(torch.float8_e4m3fn))
+        b.dev["v_scale"].copy_(torch.from_numpy(b.host["v_scale"]))
+        compare(b, 2, *attend(b, 2, seed=15))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_codes_that_are_no_numbers(tb, new):
+    """A NaN code in a key takes its rows along, one in a value its column, and neither reaches a row that does not see it."""
+    for name in ("k", "v"):
+        b = Batch(True, [new, 1], [200 + new, 100], 2, 64, 16, seed=3)
+        t = 200 + new // 2                                      # rows new // 2 and later see it
+        b.host[name][b.table[0, t // 16], 1, t % 16, 7] = 0xff
+        b.dev[name].copy_(torch.from_numpy(b.host[name]).cuda().view(torch.float8_e4m3fn))
+        q, got, lse = attend(b, 4, seed=13)
+        sees = np.zeros((b.rows, 4), bool)
+        sees[new // 2:new, 2:] = True                           # query heads 2, 3 read key head 1
+        if name == "k":
+            assert np.isnan(got[sees]).all() and np.isnan(lse[sees]).all()
+        else:
+            assert np.isnan(got[sees][:, 7]).all() and np.isfinite(np.delete(got[sees], 7, axis=1)).all() and np.isfinite(lse).all()
+        assert np.isfinite(got[~sees]).all() and np.isfinite(lse[~sees]).all()
+        clean = Batch(True, [new, 1], [200 + new, 100], 2, 64, 16, seed=3)
+        _, other, _ = attend(clean, 4, seed=13)
+        assert (got[~sees] == other[~sees]).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_a_query_that_is_not_finite_spoils_its_own_row_alone(tb, e4m3, bad):
+    b = Batch(e4m3, [40, 1], [100, 60], 1, 64, 16, seed=5)
+    q = torch.randn(b.rows + 3, 2 * 64).to(torch.bfloat16)
+    clean = attend(b, 2, seed=14, q=q)[1]
+    q[7, 64 + 3] = bad
+    q[40, 5] = bad
+    got = attend(b, 2, seed=14, q=q)[1]
+    spoilt = np.zeros((b.rows, 2), bool)
+    spoilt[7, 1] = spoilt[40, 0] = True
+    assert np.isnan(got[spoilt]).all() and (got[~spoilt] == clean[~spoilt]).all()
+
+
 # ---------------------------------------------------------------------------------------------- writing and reading
 
 def tables(positions, half, seed=0):

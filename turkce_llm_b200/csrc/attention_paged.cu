@@ -69,6 +69,9 @@ __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0
 // with byte permutes; accumulator tile i then holds elements 8 (2c) + i and 8 (2c + 1) + i of rows r and r + 8.
 //
 // 8-bit rows of up to 64: as many bytes are twice the keys, and a step of a warp is 32 of them.
+// (8 bits) Probabilities, which become f16, are against 2^-13 of the largest: at most 2^15 with what is left of a value's scale, and those
+// down to 2^-38 of it count.
+constexpr float PA_UP = 13.f;
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = (PA_WARPS + 1) * 32;
 constexpr int PA_SCAN = 4;               // sequences per lane of one look at the batch
@@ -120,15 +123,15 @@ __device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(hi), "f"(lo));
     return h;
 }
-// a value's scale as 2^exponent * part, |part| < 2, and 2^-exponent.  (Infinity and NaN are their own part.)
+// a value's scale as 2^exponent * part, and 2^-exponent: |part| < 2, but less for scales below 2^-80 (a sum of many probabilities times
+// 2^80 stays finite) and below 4 for those above 2^126.  (Infinity and NaN are their own part.)
 struct ScaleParts { float exponent, part, down; };
 __device__ __forceinline__ ScaleParts scale_parts(float s) {
-    const uint32_t b = __float_as_uint(s), e = (b >> 23) & 255u;
+    const uint32_t b = __float_as_uint(s), e = (b >> 23) & 255u, x = min(max(e, 47u), 253u);
     ScaleParts r;
-    r.exponent = __uint_as_float(0x4b000000u | e) - 8388735.0f;                        // e - 127
-    r.part = __uint_as_float((b & 0x807fffffu) | 0x3f800000u);
-    r.down = __uint_as_float((254u - min(e, 253u)) << 23);
-    if (e == 0u) { r.exponent = -126.f; r.part = s * 8.507059173e37f; r.down = 8.507059173e37f; }      // 2^126
+    r.exponent = __uint_as_float(0x4b000000u | x) - 8388735.0f;                        // x - 127
+    r.down = __uint_as_float((254u - x) << 23);
+    r.part = s * r.down;
     if (e == 255u) { r.exponent = 0.f; r.part = s; r.down = 1.f; }
     return r;
 }
@@ -470,7 +473,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 for (int t = 1; t < NT; ++t) mx = fmaxf(mx, fmaxf(z[t][2 * h], z[t][2 * h + 1]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float mn = fmaxf(m[h], mx);
+                const float mn = fmaxf(m[h], E4M3 ? mx - PA_UP : mx);
                 alpha[h] = mn > m[h] ? ex2_approx(m[h] - mn) : 1.0f;
                 moved |= mn > m[h];
                 m[h] = mn;
@@ -697,7 +700,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 //    within 2^-21 of the largest, and an absolute error below 2^-31 of the largest value behind that.
 // A row's reference m follows its largest score only when that lies more than this above it (log2): every sum and product is against the
 // same m, so the result is the same, probabilities reach 2^8 at most, and the accumulators are seldom scaled.
-constexpr float PT_SLACK = 8.f;
+// (8 bits: probabilities are f16 there, against 2^-7 of that score: 2^15 at most, and those down to 2^-32 of the largest count.)
+constexpr float PT_SLACK = 8.f, PT_UP = 7.f;
 constexpr int PT_TILE = 128 * 128;                      // bytes of a [128][64] 16-bit tile
 
 template <int NH, bool E4M3>
@@ -1188,9 +1192,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
                 mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
             }
-            const float m_new = fmaxf(m, mx * c1);
+            float m_new = fmaxf(m, mx * c1);
             float alpha = 1.0f;
-            if (m_new > m + PT_SLACK) {
+            if (m_new > m + (E4M3 ? PT_SLACK + PT_UP : PT_SLACK)) {
+                if (E4M3) m_new -= PT_UP;
                 alpha = ex2_approx(m - m_new);
                 l *= alpha;
                 m = m_new;
@@ -1258,7 +1263,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         int last = 1;                                                       // this CTA has the tile's result
         if (ok) {
             const float2 s0 = stat[r], s1 = stat[PT_ROWS + r];
-            M = fmaxf(s0.x, s1.x);
+            M = fmaxf(s0.x, s1.x) + (E4M3 ? PT_SLACK + PT_UP : 0.f);         // (products and their scale within float32)
             const float e0 = s0.y == 0.f ? 0.f : ex2_approx(s0.x - M), e1 = s1.y == 0.f ? 0.f : ex2_approx(s1.x - M);
             L = s0.y * e0 + s1.y * e1;
             const float unit = E4M3 ? exp2f((float)(*v_exponent - 127 - 6)) : 1.f;
@@ -1534,7 +1539,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 template <int NH, bool E4M3>
 int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cudaStream_t st) {
     typedef RowsShape<NH, E4M3> Sh;
-    static_assert(Sh::PER_SM == paged_per_sm(NH, E4M3), "the plan counts on as many CTAs per SM");
+    static_assert(Sh::PER_SM == paged_per_sm(NH, E4M3) && Sh::PER_SM <= PA_MOST_PER_SM, "the plan counts on as many CTAs per SM");
     CUtensorMap tmK, tmV;
     const int box_rows = std::min(c->page_size, Sh::KEYS);
     TB_TRY(make_cache_map(&tmK, c->K, E4M3 ? 1 : 2, c->head_dim, c->page_size, (long long)c->pages * c->heads, 64 * (E4M3 ? NH : 1), box_rows, !E4M3));
@@ -1626,7 +1631,7 @@ int launch_attention_paged(DeviceCtx* ctx, const TbKvCache* c, const int* q_star
     p.v = paged_view(c);
     p.q_start = q_start; p.kv_len = kv_len; p.Q = Q; p.ld_q = ld_q; p.ks = c->k_scale; p.vs = c->v_scale;
     p.att = att; p.ld_att = ld_att; p.lse = lse;
-    p.part_o = static_cast<float*>(ws) + round_up(pl.grid, 4);
+    p.part_o = static_cast<float*>(ws) + paged_counters(ctx->sm_count);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + 2LL * pl.grid * PA_ROWS * c->head_dim);
     p.arrived = static_cast<unsigned int*>(ws);
     p.rows = rows; p.H = H; p.group = group; p.max_q = max_q; p.max_kv = max_kv; p.grid = pl.grid; p.whole = pl.whole ? 1 : 0;
@@ -1658,7 +1663,7 @@ int64_t tb_attention_paged_workspace(const TbKvCache* cache, int rows, int q_hea
     DeviceCtx* ctx;
     if (check_attention(cache, rows, q_heads, max_q, max_kv) != 0 || get_ctx(&ctx) != 0) return -1;
     return paged_plan(cache->seqs, cache->heads, q_heads / cache->heads, cache->head_dim, cache->type == TB_KV_E4M3, rows, std::min(max_q, rows),
-                      max_kv, ctx->sm_count).workspace;
+                      max_kv, ctx->sm_count).room;
 }
 
 int tb_attention_paged(const TbKvCache* cache, const int32_t* d_q_start, const int32_t* d_kv_len, const void* d_Q, int64_t ld_q, int rows,

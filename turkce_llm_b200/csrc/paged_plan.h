@@ -19,34 +19,42 @@ constexpr int PT_ROWS = 128, PT_KEYS = 128;      // query rows and keys of the k
 // CTAs of that kernel that an SM holds
 constexpr int paged_tiles_per_sm(int wide, bool e4m3) { return wide == 1 && !e4m3 ? 2 : 1; }
 
+// A workspace begins with a counter for every CTA of the kernel for few rows that the chip can hold, whatever the call: what a call leaves
+// there (zeros) is where the next one, of another size or type, looks for it.  Nothing else outlives a call.
+constexpr int PA_MOST_PER_SM = 3;
+constexpr int64_t paged_counters(int sms) { return ((int64_t)PA_MOST_PER_SM * sms + 3) / 4 * 4; }
+
 struct PagedPlan {
     bool whole;                      // few rows: every item is one CTA's
     int grid;                        // few rows: CTAs
     int most_units;                  // longer chunks: room for pieces of tiles; 0: a CTA per tile
-    int64_t rows_bytes, workspace;   // bytes of the kernel for few rows (a counter and two results per CTA); of both
+    int64_t rows_bytes, workspace;   // bytes of the counters and the kernel for few rows (two results per CTA); of both (0: none needed)
+    int64_t room;                    // bytes that no batch within these bounds needs more than
 };
 
 inline PagedPlan paged_plan(int seqs, int heads, int group, int hd, bool e4m3, int rows, int max_q, int max_kv, int sms) {
     PagedPlan p;
     const int wide = hd > 64 ? 2 : 1;
-    const int64_t items = (int64_t)seqs * heads, most = (int64_t)paged_per_sm(wide, e4m3) * sms;
+    const int64_t items = (int64_t)seqs * heads, most = (int64_t)paged_per_sm(wide, e4m3) * sms, counters = paged_counters(sms) * 4;
     p.whole = max_kv <= PA_WHOLE;
     const int64_t keys = paged_keys(wide, e4m3), blocks = items * (((int64_t)max_kv + keys - 1) / keys), least = PA_LEAST / keys;
     p.grid = (int)std::max<int64_t>(1, std::min(most, p.whole ? items : (blocks + least - 1) / least));
-    // a word per CTA (to a multiple of 16 bytes), then its two results
-    p.rows_bytes = p.whole ? 0 : (int64_t)(p.grid + 3) / 4 * 16 + 2LL * p.grid * PA_ROWS * (hd + 2) * 4;
+    const int64_t results = p.whole ? 0 : 2LL * p.grid * PA_ROWS * (hd + 2) * 4;
+    p.rows_bytes = counters + (results + 15) / 16 * 16;
     p.most_units = 0;
-    p.workspace = p.rows_bytes;
-    if ((int64_t)max_q * group > PA_ROWS) {
+    p.workspace = p.room = p.whole ? 0 : p.rows_bytes;
+    if ((int64_t)max_q * group > PA_ROWS && max_kv > PT_KEYS) {
         // No more tiles than this many: every sequence that has tiles at all has more than PA_ROWS rows per key head.  Where that is
-        // less than two for every CTA that the chip holds, tiles are cut into pieces (up to three for every CTA).
+        // less than two for every CTA that the chip holds, tiles are cut into pieces (no more of them than CTAs, or tiles).
         const int64_t tokens = PT_ROWS / group, least_rows = PA_ROWS / group + 1;
         const int64_t tiles = heads * (rows / tokens + std::min<int64_t>(seqs, rows / least_rows)), slots = (int64_t)paged_tiles_per_sm(wide, e4m3) * sms;
-        if (tiles < 2 * slots && max_kv > PT_KEYS) {
+        // header, then for every unit: a counter, a flag, what it is, and [128] (maximum, sum) and [128][64 wide] float32
+        auto bytes = [&](int64_t units) { return 16 + (units + 3) / 4 * 4 * (4 + 4 + 32 + PT_ROWS * (8 + 64 * wide * 4)); };
+        if (tiles < 2 * slots) {
             p.most_units = (int)(std::max(slots, tiles) + 3) / 4 * 4;
-            // header, then for every unit: a counter, a flag, what it is, and [128] (maximum, sum) and [128][64 wide] float32
-            p.workspace += 16 + (int64_t)p.most_units * (4 + 4 + 32 + PT_ROWS * (8 + 64 * wide * 4));
+            p.workspace = p.rows_bytes + bytes(p.most_units);
         }
+        p.room = p.rows_bytes + bytes(std::max(slots, std::min(tiles, 2 * slots - 1)));
     }
     return p;
 }

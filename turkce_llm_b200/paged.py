@@ -115,7 +115,8 @@ class PagedCache:
             lib.check(rc)
 
     def workspace(self, q_heads, rows, max_q, max_kv):
-        """The memory that `attend` needs for batches within these bounds (None: none).  One for every call that may run beside another."""
+        """The memory that `attend` needs for any batch of no more rows, new rows and keys (None: none).  One for every call that may run
+        beside another; those that follow one another may share it, whatever their sizes."""
         _need(_device_of() == self._index, "the cache is on %s, which is not the current device", self.device)
         lib.init(self._index)
         n = self._lib.tb_attention_paged_workspace(self._ref, rows, q_heads, max_q, max_kv)
