@@ -240,7 +240,7 @@ typedef struct TbKvCache {
  * contexts are the caller's; rot_dim 0: no rotation), q leaves as bf16 [rows, q_heads * head_dim] (leading dimension ld_q, a
  * multiple of 8), k and v go to their places in the cache.  Float32 arithmetic.  TB_KV_E4M3: scale = max(largest
  * magnitude of the row / 448, 2^-126), codes are the nearest to value / scale, halves to the even code; a row with an
- * infinity or NaN in it reads back as NaN.  q_heads a multiple of heads. */
+ * infinity or NaN in it reads back as NaN.  q_heads a multiple of heads.  d_Q must not lie over d_qkv. */
 int tb_kv_append(const TbKvCache* cache, const int32_t* d_q_start, const int32_t* d_kv_len, const void* d_qkv, int qkv_bf16,
                  int64_t ld_qkv, int rows, int q_heads, const float* d_cos, const float* d_sin, int positions, int rot_dim,
                  int rope_form, void* d_Q, int64_t ld_q, void* stream);

@@ -484,6 +484,28 @@ def test_append_writes_what_the_formula_says_and_nothing_else(tb, e4m3, bf16_in,
             assert torch.equal(b.dev[name].cpu().view(torch.int16), want[name].view(torch.int16))
 
 
+@pytest.mark.parametrize("form", [0, 1])
+@pytest.mark.parametrize("at", [1, 2, 3])
+def test_append_with_tables_that_begin_anywhere(tb, form, at):
+    """Rows of 32 angles are whole 16-byte pieces, the table's first byte need not be: the same result as from an aligned one."""
+    b = Batch(False, [1, 70, 30], [9, 100, 30], 2, 64, 16, seed=8)
+    x = torch.randn(b.rows, (4 + 4) * 64, device="cuda")
+    cos, sin = (torch.from_numpy(t).cuda() for t in tables(128, 32))
+    results = []
+    for shift in (0, at):
+        held = [torch.zeros(128 * 32 + 8, device="cuda") for _ in range(2)]
+        views = [h[shift:shift + 128 * 32].view(128, 32) for h in held]
+        views[0].copy_(cos)
+        views[1].copy_(sin)
+        q = torch.zeros(b.rows, 4 * 64, dtype=torch.bfloat16, device="cuda")
+        b.dev["k"].zero_()
+        b.cache.append(x, q, b.q_start, b.kv_len, *views, form=form)
+        tb.sync_check()
+        results.append((q, b.dev["k"].clone()))
+    for got, want in zip(results[1], results[0]):
+        assert torch.equal(got, want)
+
+
 def test_append_rotates_as_the_projection_epilogue_does(tb):
     """Pairs, whole head: the same angles and pairs as tb_gemm_qkv_rope_bf16 (there on the unrounded float32 product)."""
     T, H, dim = 64, 6, 64

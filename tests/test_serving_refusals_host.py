@@ -23,7 +23,7 @@ def refused(match, name, *args):
         lib.check(rc)
 
 
-def append(c, starts=A, lens=A, qkv=A, bf16=0, ld=512, rows=4, heads=4, cos=A, sin=A, positions=9, rot=64, form=0, q=A, ld_q=256):
+def append(c, starts=A, lens=A, qkv=A, bf16=0, ld=512, rows=4, heads=4, cos=A, sin=A, positions=9, rot=64, form=0, q=2 * A, ld_q=256):
     return ("tb_kv_append", C.byref(c), starts, lens, qkv, bf16, ld, rows, heads, cos, sin, positions, rot, form, q, ld_q, None)
 
 
@@ -31,7 +31,7 @@ def attend(c, starts=A, lens=A, q=A, ld_q=256, rows=4, heads=4, max_q=2, max_kv=
     return ("tb_attention_paged", C.byref(c), starts, lens, q, ld_q, rows, heads, max_q, max_kv, scale, att, ld_att, lse, ws, n, None)
 
 
-def read(c, starts=A, first=None, rows=4, k=A, v=A, ld_row=128, ld_head=64):
+def read(c, starts=A, first=None, rows=4, k=A, v=2 * A, ld_row=128, ld_head=64):
     return ("tb_kv_read", C.byref(c), starts, first, rows, k, v, ld_row, ld_head, None)
 
 
@@ -53,7 +53,7 @@ def test_caches_that_are_none(over, match):
     (dict(rows=-1), "negative"), (dict(heads=3), "cannot share"), (dict(heads=0), "cannot share"), (dict(ld=511), "ld_qkv"), (dict(ld=508), "ld_qkv"),
     (dict(ld=516, bf16=1), "ld_qkv"), (dict(ld_q=255), "ld_q"), (dict(ld_q=260), "ld_q"), (dict(qkv=A + 8), "aligned"), (dict(q=A + 2), "aligned"),
     (dict(rot=63), "rot_dim"), (dict(rot=66), "rot_dim"), (dict(rot=-2), "rot_dim"), (dict(form=2), "rotation form"), (dict(cos=None), "both tables"),
-    (dict(sin=None), "both tables"), (dict(positions=0), "both tables")])
+    (dict(sin=None), "both tables"), (dict(positions=0), "both tables"), (dict(q=A), "over the rows")])
 def test_append_refuses(over, match):
     refused(match, *append(struct(), **over))
 
@@ -70,7 +70,7 @@ def test_attention_refuses(over, match):
 
 @pytest.mark.parametrize("over,match", [
     (dict(starts=None), "row starts"), (dict(k=None, v=None), "both outputs"), (dict(rows=-1), "negative"), (dict(ld_row=60), "multiples of 8"),
-    (dict(ld_head=68), "multiples of 8"), (dict(ld_row=64, ld_head=64), "over one another"), (dict(k=A + 8), "aligned")])
+    (dict(ld_head=68), "multiples of 8"), (dict(ld_row=64, ld_head=64), "over one another"), (dict(k=A + 8), "aligned"), (dict(v=A), "over one another")])
 def test_read_refuses(over, match):
     refused(match, *read(struct(), **over))
 

@@ -47,7 +47,7 @@ struct AppendParams {
     const void* x; long long ld_x;
     int rows, H, per_warp, parts, threads_log2;       // rows per warp, or warps per row; threads per head: 1 << threads_log2
     const float *cos_t, *sin_t;
-    int positions, half;                              // rot_dim / 2
+    int positions, half, aligned;                     // rot_dim / 2; both tables begin on 16 bytes
     bf16* Q; long long ld_q;
     void *K, *V;
     float *ks, *vs;
@@ -173,7 +173,7 @@ kv_append_kernel(const AppendParams p) {
     const bool by_lane = HALVES && (p.half & 7) == 0;
     const int other_lane = !by_lane || e0 >= 2 * p.half ? lane : e0 < p.half ? lane + (p.half >> 3) : lane - (p.half >> 3);
     // A row's angles: with the groups of the row before it, where these are enough for them to have arrived.
-    const bool wide_angles = (p.half & 3) == 0, angles_ahead = wide_angles && groups >= KV_AHEAD && p.half > 0;
+    const bool wide_angles = p.aligned && (p.half & 3) == 0, angles_ahead = wide_angles && groups >= KV_AHEAD && p.half > 0;
     auto ask_angles = [&](int i) {
         const long long next_pos = shfl64(my_pos, i);
         const int quads = p.half >> 2;
@@ -200,7 +200,7 @@ kv_append_kernel(const AppendParams p) {
                 // (the same angles in memory and in the ring: generic addresses)
                 const float* ct = angles_ahead && i > 0 ? reinterpret_cast<const float*>(angles[warp][i & 1]) : p.cos_t + pos * p.half;
                 const float* st = angles_ahead && i > 0 ? ct + p.half : p.sin_t + pos * p.half;
-                if (HALVES ? by_lane : wide_angles) {
+                if (HALVES ? by_lane && wide_angles : wide_angles) {
                     const int e = HALVES ? e0 : e0 >> 1, at = HALVES && e >= p.half ? e - p.half : e;
                     const bool turns = HALVES ? e < 2 * p.half : e < p.half;
                     const float flip = HALVES && e < p.half ? -1.f : 1.f;        // a cos - b sin as a cos + b (-sin): the same rounding
@@ -397,6 +397,7 @@ int launch_kv_append(DeviceCtx* ctx, const TbKvCache* c, const int* q_start, con
     p.v = paged_view(c);
     p.q_start = q_start; p.kv_len = kv_len; p.x = x; p.ld_x = ld_x; p.rows = rows; p.H = H;
     p.cos_t = cos_t; p.sin_t = sin_t; p.positions = positions; p.half = rot_dim / 2;
+    p.aligned = ((reinterpret_cast<uintptr_t>(cos_t) | reinterpret_cast<uintptr_t>(sin_t)) & 15u) == 0;
     p.Q = Q; p.ld_q = ld_q; p.K = c->K; p.V = c->V; p.ks = c->k_scale; p.vs = c->v_scale; p.err = ctx->d_err;
     long long blocks;
     shape_of(ctx, c->head_dim, 8, H + 2 * c->heads, rows, &p.threads_log2, &p.per_warp, &p.parts, &blocks);
@@ -455,6 +456,7 @@ int tb_kv_append(const TbKvCache* cache, const int32_t* d_q_start, const int32_t
     TB_CHECK(ld_q >= (long long)q_heads * cache->head_dim && ld_q % 8 == 0, "tb_kv_append: ld_q must be a multiple of 8 and at least %lld (got %lld)",
              (long long)q_heads * cache->head_dim, (long long)ld_q);
     TB_CHECK(((reinterpret_cast<uintptr_t>(d_qkv) | reinterpret_cast<uintptr_t>(d_Q)) & 15u) == 0, "tb_kv_append: rows must be 16-byte aligned");
+    TB_CHECK(rows == 0 || d_Q != d_qkv, "tb_kv_append: the queries must not lie over the rows they come from");
     TB_CHECK(rot_dim >= 0 && rot_dim <= cache->head_dim && rot_dim % 2 == 0, "tb_kv_append: rot_dim must be even and at most head_dim (got %d)", rot_dim);
     TB_CHECK(rope_form == TB_ROPE_PAIRS || rope_form == TB_ROPE_HALVES, "tb_kv_append: unknown rotation form %d", rope_form);
     TB_CHECK(rot_dim == 0 || (d_cos && d_sin && positions > 0), "tb_kv_append: a rotation needs both tables");
@@ -471,6 +473,7 @@ int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_
     TB_CHECK(rows >= 0, "tb_kv_read: rows must not be negative");
     TB_CHECK(d_start, "tb_kv_read: NULL row starts");
     TB_CHECK(d_K || d_V, "tb_kv_read: both outputs are NULL");
+    TB_CHECK(rows == 0 || d_K != d_V, "tb_kv_read: the two outputs lie over one another");
     TB_CHECK(ld_row >= cache->head_dim && ld_row % 8 == 0 && ld_head >= cache->head_dim && ld_head % 8 == 0,
              "tb_kv_read: ld_row and ld_head must be multiples of 8 and at least head_dim (got %lld, %lld)", (long long)ld_row,
              (long long)ld_head);

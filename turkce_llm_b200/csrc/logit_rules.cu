@@ -180,7 +180,8 @@ logit_rules_kernel(const LogitParams p) {
     const float inverse = __frcp_rn(rep);
     auto rule = [&](float x, uint32_t w, int t) -> float {
         if (counts && (w & (LR_COUNT | LR_PROMPT)) != 0u) {
-            // x / rep in two steps (the second one corrects the first by its remainder), x * rep of what is not positive
+            // x / rep by Markstein's correction (a quotient by the correctly rounded reciprocal, and what its remainder adds, both fused),
+            // x * rep of what is not positive
             const float q = x * inverse, y = __fmaf_rn(__fmaf_rn(-q, rep, x), inverse, q);
             x = x > 0.0f ? (q < INFINITY ? y : q) : x * rep;
             if ((w & LR_COUNT) != 0u) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)(w & LR_COUNT))), pres);

@@ -46,7 +46,7 @@ __device__ __forceinline__ int sequence_of(const int* __restrict__ start, int se
 }
 
 // x / scale on its way to the nearest 8-bit float (4 exponent bits, 3 of significand; halves to the even one): a float32 that lies on the
-// same side of every middle of two codes as the true quotient.  q is within a unit of its last place of that, its remainder tells on which
+// same side of every middle of two codes as the true quotient.  By Markstein's correction of a quotient from its remainder, q is within a unit of its last place of that, its remainder tells on which
 // side, and a number strictly between two floats becomes the one of them whose last bit is set, which no middle has.
 __device__ __forceinline__ float quotient_to_odd(float x, float scale, float inverse) {
     const float q0 = x * inverse;
