@@ -1178,8 +1178,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (edge) {
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    mx = fmaxf(mx, e <= lim ? __uint_as_float(v[0][e]) : -INFINITY);
-                    mx = fmaxf(mx, e + 32 <= lim ? __uint_as_float(v[1][e]) : -INFINITY);
+                    if (e > lim) v[0][e] = 0xff800000u;                     // -infinity: no probability
+                    if (e + 32 > lim) v[1][e] = 0xff800000u;
+                    mx = fmaxf(mx, fmaxf(__uint_as_float(v[0][e]), __uint_as_float(v[1][e])));
                 }
             } else {
                 float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
@@ -1203,7 +1204,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (E4M3) alpha *= moved;
             const bool move = __any_sync(0xffffffffu, alpha != 1.0f);
             if (j > 0 && !mbar_wait(&o_full[b], (uint32_t)((j - 1) & 1), abort_flag)) { ok = false; break; }
-            const float2 c2 = make_float2(c1, c1), nm2 = make_float2(-m, -m);
+            // (a row that has seen no key yet, and sees none here)
+            const float nm = edge && lim < 0 && m == -INFINITY ? 0.f : -m;
+            const float2 c2 = make_float2(c1, c1), nm2 = make_float2(nm, nm);
             float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             uint8_t* prow = sP + b * PT_TILE + r * 128;
             uint32_t all[32];
@@ -1216,11 +1219,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     for (int h = 0; h < 4; ++h) {
                         const int e = 8 * g + 2 * h;
                         const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1])), c2, nm2);
-                        float2 pr = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                        if (edge) {
-                            pr.x = e + 32 * c <= lim ? pr.x : 0.0f;
-                            pr.y = e + 1 + 32 * c <= lim ? pr.y : 0.0f;
-                        }
+                        const float2 pr = make_float2(ex2_approx(x.x), ex2_approx(x.y));
                         ls[h & 1] = __fadd2_rn(ls[h & 1], pr);
                         w[h] = E4M3 ? f16_pair(pr.x, pr.y) : bf16_pair(pr.x, pr.y);
                     }
