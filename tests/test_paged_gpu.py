@@ -305,6 +305,15 @@ def test_many_sequences_of_all_kinds(tb, e4m3, dim):
     compare(b, 4, *attend(b, 4, seed=10))
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_a_chunk_among_hundreds_of_single_tokens(tb, e4m3):
+    new = [1] * 700
+    new[333] = 100
+    kv = [n + s % 40 for s, n in enumerate(new)]
+    b = Batch(e4m3, new, kv, 16, 64, 16, seed=21)
+    compare(b, 16, *attend(b, 16, seed=16))
+
+
 @pytest.mark.parametrize("e4m3,dim,G", [(False, 64, 16), (True, 64, 8), (True, 128, 8), (False, 128, 8)])
 def test_more_tiles_than_the_chip_holds_at_once(tb, e4m3, dim, G):
     new = [130] * 19 + [3]

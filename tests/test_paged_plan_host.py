@@ -33,7 +33,7 @@ int main() {
         if (!p.whole) CHECK(p.rows_bytes >= paged_counters(sms) * 4 + 2LL * p.grid * PA_ROWS * (hd + 2) * 4);
         // a batch within the bounds has no more tiles than there is room for units
         if (p.most_units > 0) {
-            CHECK(p.most_units % 4 == 0);
+            CHECK(p.most_units % 4 == 0 && p.most_pieces > 0 && p.most_pieces <= p.most_units && p.most_units <= (long long)heads * PL_TILES + 1024);
             for (int k = 0; k < 4; ++k) {
                 long long left = rows, tiles = 0;
                 const int tokens = PT_ROWS / group, least = PA_ROWS / group + 1;

@@ -3,11 +3,13 @@
 // For query row (token i, head h) of a sequence, with positions up to its own visible:
 //   o = sum_t p_t v_t / sum_t p_t,   p_t = 2^(s_t - m),   s_t = scale log2(e) <q, k_t>,   m = max s_t,
 // in one pass over the keys: a running maximum m, the sum l and the accumulator rescaled where m grows.  Pieces of the cache
-// are taken by different CTAs where there are few sequences; each leaves (o, m, l) and paged_combine_kernel adds them in the order
-// of the pieces.
+// are taken by different CTAs where there are few sequences; each leaves (o, m, l), and the CTA that is last with its piece adds them
+// in the order of the pieces.
 //
-// 8-bit codes enter the tensor cores as f16, which holds each of them, against queries in f16 (every bf16 row, scaled by a power of
-// two) and probabilities in f16.  A key's scale multiplies its score.
+// Sequences with at most 16 query rows per key head (new tokens times the heads that share it) are paged_rows_kernel's, the others
+// paged_chunk_kernel's.  Where tiles are few, paged_plan_kernel deals them out: tiles start first, single tokens beside them.
+//
+// 8-bit rows: a key's scale multiplies its score, a value's its probability (few rows) or its tile (chunks).  Probabilities are f16.
 #include "paged.cuh"
 #include "paged_plan.h"
 #include "ptx.cuh"
@@ -69,8 +71,13 @@ __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0
 // with byte permutes; accumulator tile i then holds elements 8 (2c) + i and 8 (2c + 1) + i of rows r and r + 8.
 //
 // 8-bit rows of up to 64: as many bytes are twice the keys, and a step of a warp is 32 of them.
-// (8 bits) Probabilities, which become f16, are against 2^-13 of the largest: at most 2^15 with what is left of a value's scale, and those
-// down to 2^-38 of it count.
+// Codes become f16, which holds each of them, against queries in f16 (a row scaled by a power of two).  The exponent of a value's scale is
+// added to the score before the maximum is taken, so that probabilities, which become f16, carry it; they are against 2^-13 of the
+// largest: at most 2^15 with what is left of the scale, and those down to 2^-38 of it count.
+//
+// Bound: memory; 64 sequences of 16,000 keys, 6 heads of 64: bf16 6.8 TB/s, 8 bits 5.1 TB/s, there by the instructions around the
+// conversions (43 % of the issue slots of 12 warps that wait for one another's loads).  A call of 40 us loses 4 us before its first block is
+// there and 2 to 4 us to the spread of its CTAs' ends.
 constexpr float PA_UP = 13.f;
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = (PA_WARPS + 1) * 32;
@@ -695,12 +702,23 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 //  * where a block holds keys that some row does not see (the chunk's own tokens, the rest of the last page), what is not finite
 //    among its values is set to zero before the product, because 0 * infinity would reach the rows that do not see it; a row that does
 //    see it gets it added at the end (add_what_is_not_finite);
-//  * 8-bit rows: four more warps turn codes into f16 tiles, a key per thread.  A value's scale goes into its tile against the largest
-//    scale so far (a power of two, which the accumulators follow as they follow the maximum): 11 bits of every value whose scale is
-//    within 2^-21 of the largest, and an absolute error below 2^-31 of the largest value behind that.
-// A row's reference m follows its largest score only when that lies more than this above it (log2): every sum and product is against the
-// same m, so the result is the same, probabilities reach 2^8 at most, and the accumulators are seldom scaled.
-// (8 bits: probabilities are f16 there, against 2^-7 of that score: 2^15 at most, and those down to 2^-32 of the largest count.)
+//  * heads of 128 and 8-bit rows (TS): queries and probabilities lie in tensor memory, so that the tensor cores read nothing but keys
+//    and values from shared memory (8-bit chunks of 128 behind 16,000 keys: 94.6 -> 84.9 us; heads of 64 have no room for it beside two
+//    CTAs per SM);
+//  * 8-bit rows: keys stay codes.  A query row becomes two 8-bit terms (below), and the products of both with the same codes are one
+//    sum (111 -> 102 us, where keys were turned into f16 before).  Four more warps turn values into f16 tiles, a key per thread.  A value's
+//    scale goes into its tile against the largest scale so far (a power of two, which the accumulators follow as they follow the
+//    maximum): 11 bits of every value whose scale is within 2^-21 of the largest, and an absolute error below 2^-31 of the largest
+//    value behind that.
+//
+// Bound: a group's way through a block.  Clocks per block of 64 keys, bf16 heads of 64 (two CTAs per SM) / of 128 / 8 bits of 128: scores to
+// come 510 / 570 / 630, from tensor memory 250 / 150 / 290, maximum 300, product before to end 270 / 190 / 290, exponentials and their way
+// back 1,680 / 1,140 / 1,250.  Neither fewer loads, nor a quarter of the products, nor no exponentials at all change the total by more than
+// 10 %.  2 x 512 rows of 8 heads of 128 behind 32,000 keys: bf16 158 us (856 TFLOP/s), 8 bits 196 us (690 TFLOP/s).
+//
+// A row's reference m follows its largest score only when that lies more than PT_SLACK above it (log2): every sum and product is against
+// the same m, so the result is the same, probabilities reach 2^8 at most, and the accumulators are seldom scaled (104 -> 94.6 us).
+// 8 bits: probabilities are f16 there, against 2^-PT_UP of that score: 2^15 at most, and those down to 2^-32 of the largest count.
 constexpr float PT_SLACK = 8.f, PT_UP = 7.f;
 constexpr int PT_TILE = 128 * 128;                      // bytes of a [128][64] 16-bit tile
 
@@ -733,15 +751,15 @@ struct PagedChunkParams {
     PagedAttParams a;
     int tokens, tiles;                // tokens per tile; tiles of max_q
     int planned;                      // units come from paged_plan_kernel; else a CTA per tile
-    int most_units, slots;            // room for units; CTAs that the chip holds
+    int most_units, most_pieces, slots;       // room for units, for pieces' results; CTAs that the chip holds
     int* count;                       // units there are; CTAs of paged_rows_kernel that have work
     int rows_keys_log2, rows_cost;    // keys of its blocks; what one costs, in quarters of a tile's block
     int rows_slots, rows_lost;        // CTAs of it that the chip holds; how many fewer for a CTA with a tile
     unsigned int* arrived;            // [most_units]: pieces written, by the tile's first unit
     int* bad;                         // [most_units]: a piece has left out a value that is not finite
     ChunkUnit* units;
-    float2* part_ml;                  // [most_units][128]
-    float4* part_o;                   // [most_units][NH 64 / 4][128]: a row per thread side by side
+    float2* part_ml;                  // [most_pieces][128]
+    float4* part_o;                   // [most_pieces][NH 64 / 4][128]: a row per thread side by side
 };
 
 // blocks of keys that a tile's last token sees (at least one: a tile of rows without a key)
@@ -753,41 +771,47 @@ __device__ __forceinline__ int tile_blocks(int n, int kv, int tile, int tokens) 
 // How few tiles are cut into pieces: by the number of pieces of the longest one for which (rounds of CTAs) * (blocks of a piece and what a
 // piece costs beside them) is least.  One block of threads, some microseconds; where there are tiles enough (the host's bound), they are
 // not cut and this does not run.
-constexpr int PL_THREADS = 512, PL_TILES = 1024;
+constexpr int PL_THREADS = 512;
 __global__ void __launch_bounds__(PL_THREADS)
 paged_plan_kernel(const PagedChunkParams pp) {
     __shared__ int seq[PL_TILES], idx[PL_TILES], nb[PL_TILES], off[PL_TILES];
     __shared__ int count, longest, best_cap, cost[PL_THREADS / 32], caps[PL_THREADS / 32], runs[PL_THREADS / 32], total;
-    __shared__ long long few;                                // blocks of paged_rows_kernel
+    __shared__ unsigned long long few;                       // blocks of paged_rows_kernel
+    __shared__ int of_warp[PL_THREADS / 32];
     const PagedAttParams& p = pp.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) { count = 0; longest = 1; total = 0; few = 0; }
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    // ---- the tiles of one head, in the order of the sequences
-    for (int s0 = 0; s0 < p.v.seqs; s0 += 32) {
-        if (warp != 0) break;
+    // ---- the tiles of one head, in the order of the sequences; a thread per sequence
+    for (int s0 = 0; s0 < p.v.seqs; s0 += PL_THREADS) {
         int q0, n = 0, kv = 0, tiles = 0, blocks = 0;
-        if (s0 + lane < p.v.seqs && batch_of(p, s0 + lane, q0, n, kv)) {
+        if (s0 + tid < p.v.seqs && batch_of(p, s0 + tid, q0, n, kv)) {
             if (n * p.group > PA_ROWS) tiles = (n + pp.tokens - 1) / pp.tokens;
             else if (n > 0) blocks = max(1, (kv + (1 << pp.rows_keys_log2) - 1) >> pp.rows_keys_log2);
         }
-        blocks = __reduce_add_sync(0xffffffffu, blocks);
-        if (lane == 0) few += blocks;
         int incl = tiles;
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += x;
         }
-        const int at = count + incl - tiles;
-        for (int t = 0; t < tiles && at + t < PL_TILES; ++t) { seq[at + t] = s0 + lane; idx[at + t] = t; nb[at + t] = tile_blocks(n, kv, t, pp.tokens); }
+        if (lane == 31) of_warp[warp] = incl;
+        for (int o = 16; o > 0; o >>= 1) blocks += __shfl_xor_sync(0xffffffffu, blocks, o);      // (32 times 2^26 at most)
+        if (lane == 0 && blocks > 0) atomicAdd(&few, (unsigned long long)blocks);
+        __syncthreads();
+        int at = count + incl - tiles, all = 0;
+#pragma unroll
+        for (int w = 0; w < PL_THREADS / 32; ++w) {
+            if (w < warp) at += of_warp[w];
+            all += of_warp[w];
+        }
+        for (int t = 0; t < tiles && at + t < PL_TILES; ++t) { seq[at + t] = s0 + tid; idx[at + t] = t; nb[at + t] = tile_blocks(n, kv, t, pp.tokens); }
         if (tiles > 0) atomicMax(&longest, tile_blocks(n, kv, tiles - 1, pp.tokens));
-        __syncwarp();
-        if (lane == 31) count += incl;
-        __syncwarp();
+        __syncthreads();
+        if (tid == 0) count += all;
+        __syncthreads();
     }
-    __syncthreads();
     const int tiles = min(count, PL_TILES);                  // (no more than the host's bound, which is below)
     // ---- a warp per number of pieces
     {
@@ -800,7 +824,7 @@ paged_plan_kernel(const PagedChunkParams pp) {
             caps[warp] = cap;
             // (in quarters of a block: three blocks for the start of a piece and its result to memory, one for a piece's result on its way
             // back, four for the start of the few rows' kernel.)  Both kernels side by side, or one after the other.
-            const long long tile_cost = 4 * ((long long)(units + pp.slots - 1) / pp.slots * (cap + 3) + pieces), blocks = few * p.v.heads;
+            const long long tile_cost = 4 * ((long long)(units + pp.slots - 1) / pp.slots * (cap + 3) + pieces), blocks = (long long)few * p.v.heads;
             const int beside = pp.rows_slots - pp.rows_lost * units;
             long long best = tile_cost;
             runs[warp] = pp.rows_slots;
@@ -811,7 +835,7 @@ paged_plan_kernel(const PagedChunkParams pp) {
                     if (both < best) { best = both; runs[warp] = beside; }
                 }
             }
-            cost[warp] = (pieces == 1 || units <= pp.most_units) ? (int)min(best, 0x7ffffffeLL) : 0x7fffffff;
+            cost[warp] = (pieces == 1 || units <= pp.most_pieces) ? (int)min(best, 0x7ffffffeLL) : 0x7fffffff;
         }
     }
     __syncthreads();
@@ -1425,8 +1449,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
         }
-        // Scales by plain loads, a block ahead, and the pages they are found by another one.  (Bulk copies of 64 bytes and more beside the
-        // codes are as fast, but make the values wait for them.)
+        // Scales by plain loads, a block ahead, and the pages they are found by another one.  (Bulk copies beside the codes are as fast, but
+        // cost a copy per piece of a page.)
         auto page_of = [&](int j) -> int {                                  // of this thread's key of a block; -1: none
             const int key = (from + j) * PT_KEYS + t;
             if (j >= nkv || key > last_pos) return -1;
@@ -1562,7 +1586,7 @@ int plan_chunks(DeviceCtx* ctx, const PagedAttParams& p, const PagedPlan& pl, ui
     pp->a = p;
     pp->tokens = PT_ROWS / p.group;
     pp->tiles = (p.max_q + pp->tokens - 1) / pp->tokens;
-    pp->planned = pl.most_units > 0 ? 1 : 0; pp->most_units = pl.most_units; pp->slots = Sh::PER_SM * ctx->sm_count;
+    pp->planned = pl.most_units > 0 ? 1 : 0; pp->most_units = pl.most_units; pp->most_pieces = pl.most_pieces; pp->slots = Sh::PER_SM * ctx->sm_count;
     // a CTA with a tile takes the place of one of the two that an SM holds for few rows, or of all
     pp->rows_keys_log2 = paged_keys(NH, E4M3) == 128 ? 7 : 6; pp->rows_cost = NH == 2 && !E4M3 ? 6 : 3;
     pp->rows_slots = paged_per_sm(NH, E4M3) * ctx->sm_count; pp->rows_lost = Sh::TS ? paged_per_sm(NH, E4M3) : 1;
@@ -1572,7 +1596,7 @@ int plan_chunks(DeviceCtx* ctx, const PagedAttParams& p, const PagedPlan& pl, ui
     pp->bad = reinterpret_cast<int*>(pp->arrived + pl.most_units);
     pp->units = reinterpret_cast<ChunkUnit*>(pp->bad + pl.most_units);
     pp->part_ml = reinterpret_cast<float2*>(pp->units + pl.most_units);
-    pp->part_o = reinterpret_cast<float4*>(pp->part_ml + (size_t)pl.most_units * PT_ROWS);
+    pp->part_o = reinterpret_cast<float4*>(pp->part_ml + (size_t)pl.most_pieces * PT_ROWS);
     if (!pp->planned) {
         TB_CHECK(pp->tiles <= 65535, "tb_attention_paged: max_q %d is too much for one launch", p.max_q);
         return 0;
