@@ -44,7 +44,7 @@ inline PagedPlan paged_plan(int seqs, int heads, int group, int hd, bool e4m3, i
     p.rows_bytes = counters + (results + 15) / 16 * 16;
     p.most_units = p.most_pieces = 0;
     p.workspace = p.room = p.whole ? 0 : p.rows_bytes;
-    if ((int64_t)max_q * group > PA_ROWS && max_kv > PT_KEYS) {
+    if ((int64_t)max_q * group > PA_ROWS) {
         // No more tiles than this many: every sequence that has tiles at all has more than PA_ROWS rows per key head.  Where that is
         // less than two for every CTA that the chip holds, tiles are cut into pieces (no more of them than CTAs).  Where it is less than
         // half of a CTA for every tile that a sequence may have, they are dealt out all the same: 4,096 single tokens and a chunk of 60
@@ -54,7 +54,7 @@ inline PagedPlan paged_plan(int seqs, int heads, int group, int hd, bool e4m3, i
         const int64_t slots = (int64_t)paged_tiles_per_sm(wide, e4m3) * sms;
         // header, then for every unit: a counter, a flag, what it is; for every piece [128] (maximum, sum) and [128][64 wide] float32
         auto bytes = [&](int64_t units) { return 16 + (units + 3) / 4 * 4 * (4 + 4 + 32) + (slots + 3) / 4 * 4 * PT_ROWS * (8 + 64 * wide * 4); };
-        if (per_head <= PL_TILES && (tiles < 2 * slots || 2 * tiles <= items * ((max_q + tokens - 1) / tokens))) {
+        if (per_head <= PL_TILES && ((max_kv > PT_KEYS && tiles < 2 * slots) || 2 * tiles <= items * ((max_q + tokens - 1) / tokens))) {
             p.most_units = (int)(std::max(slots, tiles) + 3) / 4 * 4;
             p.most_pieces = (int)(slots + 3) / 4 * 4;
             p.workspace = p.rows_bytes + bytes(p.most_units);
