@@ -75,7 +75,7 @@ __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0
 // added to the score before the maximum is taken, so that probabilities, which become f16, carry it; they are against 2^-13 of the
 // largest: at most 2^15 with what is left of the scale, and those down to 2^-38 of it count.
 //
-// Bound: memory; 64 sequences of 16,000 keys, 6 heads of 64: bf16 6.8 TB/s, 8 bits 5.1 TB/s, there by the instructions around the
+// Bound: memory; 64 sequences of 16,000 keys, 6 heads of 64: bf16 6.7 TB/s, 8 bits 5.2 TB/s, there by the instructions around the
 // conversions (43 % of the issue slots of 12 warps that wait for one another's loads).  A call of 40 us loses 4 us before its first block is
 // there and 2 to 4 us to the spread of its CTAs' ends.
 constexpr float PA_UP = 13.f;
