@@ -26,6 +26,7 @@ struct PagedAttParams {
     PagedView v;
     const int *q_start, *kv_len;
     const bf16* Q; long long ld_q;
+    const void* K;
     const float *ks, *vs;
     bf16* att; long long ld_att;
     float* lse;                      // [rows, H] or NULL
@@ -71,9 +72,12 @@ __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0
 // with byte permutes; accumulator tile i then holds elements 8 (2c) + i and 8 (2c + 1) + i of rows r and r + 8.
 //
 // 8-bit rows of up to 64: as many bytes are twice the keys, and a step of a warp is 32 of them.
-// Codes become f16, which holds each of them, against queries in f16 (a row scaled by a power of two).  The exponent of a value's scale is
-// added to the score before the maximum is taken, so that probabilities, which become f16, carry it; they are against 2^-13 of the
-// largest: at most 2^15 with what is left of the scale, and those down to 2^-38 of it count.
+// Codes become f16, which holds each of them, against queries in f16 (a row scaled by a power of two).  The exponent e of a value's scale is
+// added to the score before the maximum is taken, so that probabilities, which become f16, carry it: p' = 2^(s + e - m), against 2^-13 of
+// the largest: at most 2^15 with what is left of the scale, and products of probability and scale down to 2^-38 of the largest count.  The sum
+// takes the exponent back, l = sum of p' 2^(B - e) with B the exponent at the item's first key.  That holds while every e lies within NEAR of B;
+// behind it p' may be no number that float32 has, and the sum would lose a key whose value is small beside another.  (A row of zeros has
+// the smallest scale there is, 2^-126.)  Rows that have seen such a key get their sum at the item's end, from the keys once more.
 //
 // Bound: memory; 64 sequences of 16,000 keys, 6 heads of 64: bf16 6.7 TB/s, 8 bits 5.2 TB/s, there by the instructions around the
 // conversions (43 % of the issue slots of 12 warps that wait for one another's loads).  A call of 40 us loses 4 us before its first block is
@@ -130,17 +134,19 @@ __device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(hi), "f"(lo));
     return h;
 }
-// a value's scale as 2^exponent * part, and 2^-exponent: |part| < 2, but less for scales below 2^-80 (a sum of many probabilities times
-// 2^80 stays finite) and below 4 for those above 2^126.  (Infinity and NaN are their own part.)
-struct ScaleParts { float exponent, part, down; };
-__device__ __forceinline__ ScaleParts scale_parts(float s) {
-    const uint32_t b = __float_as_uint(s), e = (b >> 23) & 255u, x = min(max(e, 47u), 253u);
-    ScaleParts r;
-    r.exponent = __uint_as_float(0x4b000000u | x) - 8388735.0f;                        // x - 127
-    r.down = __uint_as_float((254u - x) << 23);
-    r.part = s * r.down;
-    if (e == 255u) { r.exponent = 0.f; r.part = s; r.down = 1.f; }
-    return r;
+// 2^n for n from -126 to 127
+__device__ __forceinline__ float power_of_two(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
+// The exponent of a value's scale as float32 keeps it: a scale is 2^(exponent - 127) * part with |part| < 2, below 4 where it is above 2^126.
+// 0: infinity or NaN, their own part with any exponent.
+constexpr int NEAR = 40;
+__device__ __forceinline__ int scale_exponent(float s) {
+    const int e = (int)(__float_as_uint(s) >> 23) & 255;
+    return e == 255 ? 0 : min(max(e, 1), 253);
+}
+// a sum of 2^x and the largest x, put together with another one
+__device__ __forceinline__ void add_sums(float2& to, float2 x) {
+    const float top = fmaxf(to.x, x.x), base = top == -INFINITY ? 0.f : top;
+    to = make_float2(top, to.y * ex2_approx(to.x - base) + x.y * ex2_approx(x.x - base));
 }
 
 __device__ __forceinline__ void copy_async16(void* to_shared, const void* from) {
@@ -303,7 +309,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 const bool first = b == b_begin;
                 if (lane == 0) {
                     int4* what = reinterpret_cast<int4*>(smem + Sh::O_WHAT + st * Sh::WHAT);
-                    what[0] = make_int4((first ? PA_FIRST : 0) | (b == b_end - 1 ? PA_LAST : 0) | (runs == 1 ? PA_FINAL : 0), b * KEYS, q0, n);
+                    what[0] = make_int4((first ? PA_FIRST : 0) | (b == b_end - 1 ? PA_LAST : 0) | (runs == 1 ? PA_FINAL : 0) | s << 16, b * KEYS, q0, n);
                     what[1] = make_int4(kv, h, c0, runs);
                     mbar_expect_tx(bar, (uint32_t)(count * piece_keys * (2 * Sh::TILE / KEYS) + (first ? n * p.group * p.v.hd * 2 : 0)));
                 }
@@ -374,6 +380,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     bool ok = true;
     int st = 0;
     uint32_t phase = 0;
+    // (8 bits) what a warp knows of its item lies where the item's result goes at its end: B, the first key, the first one with a value's scale
+    // far from B (which concerns the rows that see it)
+    int* known = reinterpret_cast<int*>(so + warp * PA_ROWS * Sh::LD);
+    enum { K_BASE, K_FIRST, K_FAR };
     for (;;) {
         if (!mbar_wait(&full[st], phase, abort_flag)) {
             if (lane == 0) *abort_flag = 1;
@@ -383,7 +393,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         const uint8_t* sK = smem + st * Sh::STAGE;
         const uint8_t* sV = sK + Sh::TILE;
-        const int4 what = *reinterpret_cast<const int4*>(smem + Sh::O_WHAT + st * Sh::WHAT);           // flags, first key, first row, new rows
+        const int4 what = *reinterpret_cast<const int4*>(smem + Sh::O_WHAT + st * Sh::WHAT);           // flags and sequence, first key, first row, new rows
         if (what.x & PA_END) { all_of(true, 1, 128); break; }
         const int4 more = *reinterpret_cast<const int4*>(smem + Sh::O_WHAT + st * Sh::WHAT + 16);      // keys, head, first run, runs
         const int kv = more.x, n = what.w;
@@ -430,6 +440,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 }
                 m[x] = -INFINITY; l[x] = 0.f;
             }
+            if (E4M3) {
+                const float vs = reinterpret_cast<const float*>(smem + Sh::O_SCALE + st * Sh::SCALES)[KEYS];
+                if (lane <= K_FAR) known[lane] = lane == K_BASE ? max(scale_exponent(vs), 1) : lane == K_FIRST ? what.y : 0x7fffffff;
+                __syncwarp();
+            }
 #pragma unroll
             for (int e = 0; e < 8 * NH; ++e) { o[e][0] = 0.f; o[e][1] = 0.f; o[e][2] = 0.f; o[e][3] = 0.f; }
         }
@@ -441,8 +456,14 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 // a lane per key: what the scales do to scores, probabilities and sums
                 const float* sc = reinterpret_cast<const float*>(smem + Sh::O_SCALE + st * Sh::SCALES) + kk;
                 if (lane < KW) {
-                    const ScaleParts x = scale_parts(sc[KEYS + lane]);
-                    parts[lane] = make_float4(sc[lane], x.exponent, x.part, x.down);
+                    const float vs = sc[KEYS + lane];
+                    const int B = known[K_BASE];
+                    int e = scale_exponent(vs);
+                    e = e == 0 ? B : e;
+                    const int off = e - B, near = min(max(off, -NEAR), NEAR);
+                    parts[lane] = make_float4(sc[lane], __uint_as_float(0x4b000000u | (uint32_t)e) - 8388735.0f /* e - 127 */, vs * power_of_two(127 - e),
+                                              power_of_two(-near));
+                    if (off != near) atomicMin(known + K_FAR, k0 + lane);
                 }
                 __syncwarp();
             }
@@ -595,7 +616,54 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (++st == STAGES) { st = 0; phase ^= 1u; }
         if (!(what.x & PA_LAST)) continue;
 
-        // ---- the item's end: the four warps' results, [warp][16 rows][LD] floats, maxima and sums behind
+        // ---- the item's end: the four warps' results, [warp][16 rows][LD] floats, maxima and sums behind.  (8 bits: what leaves the CTA, or the
+        // kernel, are means of values and sums in units of scores alone: other parts of the item have other B.)
+        int B = 0;
+        bool far[2] = {false, false};
+        float2 sum[2];                                                     // of rows that have seen a key far from B: the largest score and the sum
+        if (E4M3) {
+            B = known[K_BASE];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { far[h] = pos[h] >= known[K_FAR]; sum[h] = make_float2(-INFINITY, 0.f); }
+            if (__any_sync(0xffffffffu, far[0] || far[1])) {
+                const int first_key = known[K_FIRST];
+                const int* table = p.v.table + (long long)((uint32_t)what.x >> 16) * p.v.table_ld;
+#pragma unroll 1
+                for (int t0 = first_key + kk; t0 <= min(k0, last_pos); t0 += KEYS) {
+#pragma unroll 1
+                    for (int t = 0; t < KW; t += 8) {
+                        // (lane (r, c): elements 16 c .. of key t0 + t + r; products with keys t0 + t + 2 c and the next)
+                        auto row_of = [&](int key) -> long long {
+                            const int page = key <= last_pos ? table[key >> p.v.page_shift] : -1;
+                            if ((unsigned)page >= (unsigned)p.v.pages) return -1;
+                            return (((long long)page * p.v.heads + more.y) << p.v.page_shift) + (key & ((1 << p.v.page_shift) - 1));
+                        };
+                        const long long row = row_of(t0 + t + r);
+                        float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int b = 0; b < NH; ++b) {
+                            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                            if (row >= 0 && 64 * b + 16 * c < p.v.hd) x = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.K) + row * p.v.hd + 64 * b + 16 * c);
+                            const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) mma_16816(z, qf[b][e], e4m3_f16(u[e]), e4m3_f16(u[e] >> 16), Kind());
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = t0 + t + 2 * c + (e & 1);
+                            if (key > pos[e >> 1]) continue;
+                            const long long at = row_of(key);
+                            if (at >= 0) add_sums(sum[e >> 1], make_float2(z[e] * (p.ks[at] * row_factor[e >> 1]), 1.f));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int x = 1; x < 4; x <<= 1) add_sums(sum[h], make_float2(__shfl_xor_sync(0xffffffffu, sum[h].x, x), __shfl_xor_sync(0xffffffffu, sum[h].y, x)));
+                __syncwarp();
+            }
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -610,24 +678,40 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     *reinterpret_cast<float4*>(dst + 64 * b + 8 + e) =
                         make_float4(o[8 * b + e][2 * h + 1], o[8 * b + e + 1][2 * h + 1], o[8 * b + e + 2][2 * h + 1], o[8 * b + e + 3][2 * h + 1]);
                 }
-            if (c == 0) sml[warp * PA_ROWS + r + 8 * h] = make_float2(m[h], l[h]);
+            if (c == 0) {
+                float2 ml = make_float2(m[h], l[h]);
+                if (E4M3 && far[h]) {
+                    // behind the row, what makes a mean of its values where the sum is against another reference, in two factors; the sum's sign says so
+                    const float half = ex2_approx(0.5f * (m[h] - sum[h].x));
+                    *reinterpret_cast<float2*>(so + (warp * PA_ROWS + r + 8 * h) * Sh::LD + 64 * NH) = make_float2(half / sum[h].y, half);
+                    ml = make_float2(sum[h].x, -sum[h].y);
+                }
+                sml[warp * PA_ROWS + r + 8 * h] = ml;
+            }
         }
         if (!all_of(true, 1, 128)) { ok = false; break; }
         const int chunks = p.v.hd >> 3, points = nrows * chunks;           // eight elements per thread
         auto finish = [&](int rr, int e, float M, float L, const float (&acc)[8]) {
             const int tok = rr / p.group, hq = more.y * p.group + (rr - tok * p.group), row = what.z + tok;
             const bool none = kv - n + tok < 0;                            // a row without a key
-            const float inv = none ? 0.f : 1.0f / L;
+            const float inv = none ? 0.f : E4M3 ? (L == 0.f ? __uint_as_float(0x7fffffffu) : 1.0f) : 1.0f / L;        // (8 bits: means already)
             *reinterpret_cast<uint4*>(p.att + (long long)row * p.ld_att + (long long)hq * p.v.hd + e) =
                 make_uint4(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv),
                            bf16_pair(acc[4] * inv, acc[5] * inv), bf16_pair(acc[6] * inv, acc[7] * inv));
             if (p.lse && e == 0) p.lse[(long long)row * p.H + hq] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
         };
-        auto add = [](float& M, float& L, float (&acc)[8], float2 ml, const float4& a, const float4& d) {
+        auto add = [](auto means, float& M, float& L, float (&acc)[8], float2 ml, const float4& a, const float4& d) {
             if (ml.y == 0.f) return;                                       // (no key of this part was visible)
             const float mn = L == 0.f ? ml.x : fmaxf(M, ml.x);
-            const float f = L == 0.f ? 0.f : ex2_approx(M - mn), g = ex2_approx(ml.x - mn);
-            L = L * f + ml.y * g;
+            float f = L == 0.f ? 0.f : ex2_approx(M - mn), g = ex2_approx(ml.x - mn);
+            if (decltype(means)::value) {
+                f *= L; g *= ml.y;
+                L = f + g;
+                const float inv = __fdividef(1.0f, L);
+                f *= inv; g *= inv;
+            } else {
+                L = L * f + ml.y * g;
+            }
             M = mn;
             const float x[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
 #pragma unroll
@@ -636,10 +720,38 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         for (int x = threadIdx.x; x < points; x += PA_WARPS * 32) {
             const int rr = x / chunks, e = (x - rr * chunks) * 8;
             float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            float2 ml[PA_WARPS];
+            bool any_far = false;
 #pragma unroll
-            for (int w = 0; w < PA_WARPS; ++w) {
-                const float4* src = reinterpret_cast<const float4*>(so + (w * PA_ROWS + rr) * Sh::LD + e);
-                add(M, L, acc, sml[w * PA_ROWS + rr], src[0], src[1]);
+            for (int w = 0; w < PA_WARPS; ++w) { ml[w] = sml[w * PA_ROWS + rr]; any_far |= E4M3 && ml[w].y < 0.f; }
+            if (!any_far) {
+#pragma unroll
+                for (int w = 0; w < PA_WARPS; ++w) {
+                    const float4* src = reinterpret_cast<const float4*>(so + (w * PA_ROWS + rr) * Sh::LD + e);
+                    add(std::false_type(), M, L, acc, ml[w], src[0], src[1]);
+                }
+                if (E4M3) {
+                    const float a = L == 0.f ? 0.f : __fdividef(1.0f, L), b = power_of_two(B - 127);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[i] = acc[i] * a * b;
+                    M -= (float)(B - 127);
+                }
+            } else {
+#pragma unroll 1
+                for (int w = 0; w < PA_WARPS; ++w) {
+                    const float4* src = reinterpret_cast<const float4*>(so + (w * PA_ROWS + rr) * Sh::LD + e);
+                    float2 its = sml[w * PA_ROWS + rr], f;
+                    if (its.y < 0.f) {
+                        f = *reinterpret_cast<const float2*>(so + (w * PA_ROWS + rr) * Sh::LD + 64 * NH);
+                        its.y = -its.y;
+                    } else {
+                        f = make_float2(1.0f / its.y, power_of_two(B - 127));
+                        its.x -= (float)(B - 127);
+                    }
+                    const float4 x = src[0], y = src[1];
+                    add(std::true_type(), M, L, acc, its, make_float4(x.x * f.x * f.y, x.y * f.x * f.y, x.z * f.x * f.y, x.w * f.x * f.y),
+                        make_float4(y.x * f.x * f.y, y.y * f.x * f.y, y.z * f.x * f.y, y.w * f.x * f.y));
+                }
             }
             if (what.x & PA_FINAL) {
                 finish(rr, e, M, L, acc);
@@ -676,7 +788,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             for (int i = g; i < more.w; i += groups) {
                 const int slot = (2 * (more.z + i) + (i == 0 ? 1 : 0)) * PA_ROWS + rr;
                 const float4* src = reinterpret_cast<const float4*>(p.part_o + (long long)slot * p.v.hd + e);
-                add(M, L, acc, __ldcg(p.part_ml + slot), __ldcg(src), __ldcg(src + 1));
+                add(Kind(), M, L, acc, __ldcg(p.part_ml + slot), __ldcg(src), __ldcg(src + 1));
             }
             if (groups == 1) {
                 finish(rr, e, M, L, acc);
@@ -694,7 +806,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                 for (int g = 0; g < groups; ++g) {
                     const float* from = so + (g * points + x) * 10;
-                    add(M, L, acc, make_float2(from[0], from[1]), make_float4(from[2], from[3], from[4], from[5]),
+                    add(Kind(), M, L, acc, make_float2(from[0], from[1]), make_float4(from[2], from[3], from[4], from[5]),
                         make_float4(from[6], from[7], from[8], from[9]));
                 }
                 finish(rr, e, M, L, acc);
@@ -1669,7 +1781,7 @@ int launch_attention_paged(DeviceCtx* ctx, const TbKvCache* c, const int* q_star
              (long long)(ws ? ws_bytes : 0), (long long)pl.workspace);
     PagedAttParams p;
     p.v = paged_view(c);
-    p.q_start = q_start; p.kv_len = kv_len; p.Q = Q; p.ld_q = ld_q; p.ks = c->k_scale; p.vs = c->v_scale;
+    p.q_start = q_start; p.kv_len = kv_len; p.Q = Q; p.ld_q = ld_q; p.K = c->K; p.ks = c->k_scale; p.vs = c->v_scale;
     p.att = att; p.ld_att = ld_att; p.lse = lse;
     p.part_o = static_cast<float*>(ws) + paged_counters(ctx->sm_count);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + 2LL * pl.grid * PA_ROWS * c->head_dim);
