@@ -81,3 +81,71 @@ def test_a_row_of_zeros_halves_the_value_beside_it(tb, new, size):
     # (equal probabilities: f16 holds them, exponents are whole numbers; bf16 at the end)
     assert (np.abs(got / want[:, None, None] - 1) <= 2.0 ** -8 + 2.0 ** -15).all()
     assert (np.abs(lse - np.log(n)[:, None]) <= 2.0 ** -15).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("before", [0, 30, 200, 4000])
+@pytest.mark.parametrize("new", [6, 40, 200])
+@pytest.mark.parametrize("up", [3, 23, 40, 100])
+def test_scales_of_later_tokens_do_not_reach_earlier_rows(tb, dim, before, new, up):
+    """The values of some tokens of a chunk are 2^up times the others: rows in front of them have the same bits as without them, those that
+    see them are right."""
+    kv = before + new
+    b = Batch(True, [new, 1], [kv, 50], 1, dim, 16, seed=new)
+    clean = attend(b, 2, seed=23)
+    large = [before + (2 * new) // 3, kv - 1]
+    for t in large:
+        page, slot = at(b, 0, np.array(t))
+        b.host["v_scale"][page, 0, slot] *= np.float32(2.0 ** up)
+    upload(b)
+    q, got, lse = attend(b, 2, seed=23)
+    unseen = large[0] - before
+    others = np.r_[:unseen, new:b.rows]
+    assert (got[others] == clean[1][others]).all() and (lse[others] == clean[2][others]).all()
+    k, v = b.sequence("k", 0), b.sequence("v", 0)
+    positions = np.arange(before, kv)
+    want, want_lse, spread, size = plain.attention(q[:new], k, v, positions, dim ** -0.5)
+    # f16 probabilities (2^7 and more for a row's largest: off by 2^-25 of that where they are small, times a code of 448 and the largest scale
+    # that the row sees, twice a power of two) and f16 values (off by 2^-31 of that scale); single tokens: less
+    score = (dim + 4) * 2.0 ** -24 * size + 2.0 ** -21 * np.abs(q[:new]).max(axis=2) * np.abs(k[:, 0]).sum(axis=1).max() * dim ** -0.5
+    scales = b.host["v_scale"][at(b, 0, np.arange(kv))[0], 0, np.arange(kv) % 16].astype(np.float64)
+    most = np.maximum.accumulate(scales)[positions][:, None, None]
+    lost = positions[:, None, None] * (2.0 ** -32 * 448 * 2 + 2.0 ** -31) * most
+    bound = 2.0 ** -8 * np.abs(want) + (2 * 2.0 ** -11 * 1.01 + 2 * score[..., None] + 2.0 ** -15) * spread + lost + 1e-30
+    assert (np.abs(got[:new] - want) <= bound).all(), np.nanmax(np.abs(got[:new] - want) / bound)
+    assert (np.abs(lse[:new] - want_lse) <= score + 2.0 ** -15 + 2.0 ** -20 * (1 + np.abs(want_lse))).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scales_that_grow_along_a_chunk(tb, dim):
+    """Every token's value is 2^3 times the one before it, over a range of 2^120: each row is about its own last keys, and right."""
+    b = Batch(True, [40], [40], 1, dim, 16, seed=3)
+    page, slot = at(b, 0, np.arange(40))
+    b.host["v_scale"][page, 0, slot] = np.ldexp(np.float32(1.5), 3 * np.arange(40) - 80)
+    upload(b)
+    q, got, _ = attend(b, 2, seed=24)
+    k, v = b.sequence("k", 0), b.sequence("v", 0)
+    want, _, spread, size = plain.attention(q, k, v, np.arange(40), dim ** -0.5)
+    score = (dim + 4) * 2.0 ** -24 * size + 2.0 ** -21 * np.abs(q).max(axis=2) * np.abs(k[:, 0]).sum(axis=1).max() * dim ** -0.5
+    # (as above, with the row's own scale as the largest it sees)
+    lost = np.arange(1, 41)[:, None, None] * (2.0 ** -32 * 448 * 2 + 2.0 ** -31) * (1.5 * 2.0 ** (3 * np.arange(40) - 80))[:, None, None]
+    bound = 2.0 ** -8 * np.abs(want) + (2 * 2.0 ** -11 * 1.01 + 2 * score[..., None] + 2.0 ** -15) * spread + lost
+    assert (np.abs(got - want) <= bound).all(), np.nanmax(np.abs(got - want) / bound)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("exponent", [-126, -60, 118])
+def test_chunks_of_values_at_the_ends_of_their_range(tb, dim, exponent):
+    b = Batch(True, [40], [240], 1, dim, 16, seed=4)
+    page, slot = at(b, 0, np.arange(240))
+    b.host["v_scale"][page, 0, slot] = np.ldexp((1 + np.random.default_rng(5).random(240)).astype(np.float32), exponent)
+    upload(b)
+    q, got, lse = attend(b, 2, seed=27)
+    k, v = b.sequence("k", 0), b.sequence("v", 0)
+    want, want_lse, spread, size = plain.attention(q, k, v, np.arange(200, 240), dim ** -0.5)
+    score = (dim + 4) * 2.0 ** -24 * size + 2.0 ** -21 * np.abs(q).max(axis=2) * np.abs(k[:, 0]).sum(axis=1).max() * dim ** -0.5
+    # (as above; the smallest bf16 is 2^-133)
+    lost = 240 * (2.0 ** -32 * 448 * 2 + 2.0 ** -31) * 2.0 ** (exponent + 1)
+    bound = 2.0 ** -8 * np.abs(want) + (2 * 2.0 ** -11 * 1.01 + 2 * score[..., None] + 2.0 ** -15) * spread + lost + 2.0 ** -133
+    assert (np.abs(got - want) <= bound).all(), np.nanmax(np.abs(got - want) / bound)
+    assert (np.abs(lse - want_lse) <= score + 2.0 ** -15 + 2.0 ** -20 * (1 + np.abs(want_lse))).all()

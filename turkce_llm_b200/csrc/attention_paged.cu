@@ -838,7 +838,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 //    sum (111 -> 102 us, where keys were turned into f16 before).  Four more warps turn values into f16 tiles, a key per thread.  A value's
 //    scale goes into its tile against the largest scale so far (a power of two, which the accumulators follow as they follow the
 //    maximum): 11 bits of every value whose scale is within 2^-21 of the largest, and an absolute error below 2^-31 of the largest
-//    value behind that.
+//    value behind that.  Where a block holds keys that some row does not see, a value is against the largest scale up to its own key (a
+//    row that sees it sees those too), and what that is below the largest that the row sees goes into the row's probability: what a row
+//    does not see, however large, costs it nothing.
 //
 // Bound: a group's way through a block.  Clocks per block of 64 keys, bf16 heads of 64 (two CTAs per SM) / of 128 / 8 bits of 128: scores to
 // come 510 / 570 / 630, from tensor memory 250 / 150 / 290, maximum 300, product before to end 270 / 190 / 290, exponentials and their way
@@ -865,7 +867,9 @@ struct ChunkShape {
     static constexpr int RST = 2;
     static constexpr int O_KS = O_RAW + (E4M3 ? RST * RAW : 0);          // [8][128] key scales * scale_log2
     static constexpr int O_RF = O_KS + (E4M3 ? 8 * PT_KEYS * 4 : 0);     // [128] row factors
-    static constexpr int O_BARS = O_RF + (E4M3 ? PT_ROWS * 4 : 0);
+    static constexpr int O_EX = O_RF + (E4M3 ? PT_ROWS * 4 : 0);         // [2][128] exponents of values in blocks at the edge
+    static constexpr int O_SEEN = O_EX + (E4M3 ? 2 * PT_KEYS * 4 : 0);   // [2][128] the largest that a row has seen there
+    static constexpr int O_BARS = O_SEEN + (E4M3 ? 2 * PT_ROWS * 4 : 0);
     // (bf16 heads of 64: exactly what lets two CTAs share an SM; 256 bytes of barriers behind the tiles or in the alignment's pad)
     static constexpr int SMEM = 1024 + O_BARS + (TS ? 640 : 0);
     static constexpr int PER_SM = TS ? 1 : 2;
@@ -1065,7 +1069,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     uint64_t* ks_full = bars + 60;    // 8: what the softmax warps read of a block's scales.  (Not k_full, which may be a whole round ahead of them.)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* bad_value = abort_flag + 1;                              // a value that is not finite has been set to zero
-    volatile int* v_exponent = abort_flag + 2;                             // (8 bits) the last block's reference
+    volatile int* v_exponent = abort_flag + 2;                             // (8 bits) the reference of the last block that all rows see
     volatile int* is_last = abort_flag + 3;                                // this CTA was the last with its piece of a tile
     float* v_moved = reinterpret_cast<float*>(tmem_slot + 6);              // (8 bits) [8]: 2^(reference before - reference) of a block
     uint32_t* warp_most = tmem_slot + 14;                                  // (8 bits) [2][4]
@@ -1279,6 +1283,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const uint32_t ts = tS + lane_base + (uint32_t)(b * 64), to = tO + lane_base + (uint32_t)(b * 64 * NH);
         float m = -INFINITY, l = 0.f, c1 = p.scale_log2;
         bool ok = true;
+        // (8 bits) this row's reference of value scales, once there is one of its own: the others have v_exponent
+        int* seen_exponent = reinterpret_cast<int*>(smem + Sh::O_SEEN) + b * PT_ROWS + r;
+        if (E4M3) *seen_exponent = -1;
         uint32_t v[2][32];
         if (Sh::TS && !E4M3 && nkv > 0 && b == 0) {                         // the rows to tensor memory
             ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag));
@@ -1355,6 +1362,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 m = m_new;
             }
             if (E4M3) alpha *= moved;
+            const int* exponents = reinterpret_cast<const int*>(smem + Sh::O_EX) + ((from + j - edge0) & 1) * PT_KEYS + b * 64;
+            if (E4M3 && edge) {
+                const int before = *seen_exponent < 0 ? *v_exponent : *seen_exponent;
+                const int its_exponent = lim < 0 ? before : max(before, exponents[min(lim, 63)]);
+                *seen_exponent = its_exponent;
+                alpha *= power_of_two(max(before - its_exponent, -126));
+            }
             const bool move = __any_sync(0xffffffffu, alpha != 1.0f);
             if (j > 0 && !mbar_wait(&o_full[b], (uint32_t)((j - 1) & 1), abort_flag)) { ok = false; break; }
             // (a row that has seen no key yet, and sees none here)
@@ -1385,6 +1399,19 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
             }
             if (Sh::TS) tmem_st32(tP + lane_base + (uint32_t)(b * 32), all);
+            if (E4M3 && edge && __any_sync(0xffffffffu, exponents[0] < *seen_exponent)) {
+                const int its_exponent = *seen_exponent;
+                tmem_st_wait();
+                tmem_ld32(tP + lane_base + (uint32_t)(b * 32), v[0]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int2 x = *reinterpret_cast<const int2*>(exponents + 2 * i);
+                    const float2 pr = f16_floats(v[0][i]);
+                    v[0][i] = f16_pair(pr.x * power_of_two(min(max(x.x - its_exponent, -127), 0)), pr.y * power_of_two(min(max(x.y - its_exponent, -127), 0)));
+                }
+                tmem_st32(tP + lane_base + (uint32_t)(b * 32), v[0]);
+            }
             l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
             if (move && j > 0) {
                 tc_fence_after();
@@ -1411,15 +1438,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (ok) stat[b * PT_ROWS + r] = make_float2(m, l);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const bool none = pos < 0;                                          // a row without a key
-        float M = -INFINITY, L = 0.f, w0 = 0.f, w1 = 0.f;
+        float M = -INFINITY, L = 0.f, w0 = 0.f, w1 = 0.f, unit = 1.f;
         int last = 1;                                                       // this CTA has the tile's result
         if (ok) {
             const float2 s0 = stat[r], s1 = stat[PT_ROWS + r];
             M = fmaxf(s0.x, s1.x) + (E4M3 ? PT_SLACK + PT_UP : 0.f);         // (products and their scale within float32)
             const float e0 = s0.y == 0.f ? 0.f : ex2_approx(s0.x - M), e1 = s1.y == 0.f ? 0.f : ex2_approx(s1.x - M);
             L = s0.y * e0 + s1.y * e1;
-            const float unit = E4M3 ? exp2f((float)(*v_exponent - 127 - 6)) : 1.f;
-            w0 = e0 * unit; w1 = e1 * unit;
+            w0 = e0; w1 = e1;
+            if (E4M3) {                                                     // (by itself: a product with w may be no number that float32 has)
+                const int* x = reinterpret_cast<const int*>(smem + Sh::O_SEEN) + r;
+                const int x0 = x[0] < 0 ? *v_exponent : x[0], x1 = x[PT_ROWS] < 0 ? *v_exponent : x[PT_ROWS], most = max(x0, x1);
+                w0 *= power_of_two(max(x0 - most, -127)); w1 *= power_of_two(max(x1 - most, -127));
+                unit = exp2f((float)(most - 127 - 6));
+            }
         }
         tc_fence_after();
         // columns 64 c + 32 b .. of this row, against M
@@ -1442,8 +1474,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     own(c);
 #pragma unroll
                     for (int d = 0; d < 8; ++d)
-                        __stcg(to16 + (16 * c + 8 * b + d) * PT_ROWS, make_float4(__uint_as_float(v[0][4 * d]), __uint_as_float(v[0][4 * d + 1]),
-                                                                                  __uint_as_float(v[0][4 * d + 2]), __uint_as_float(v[0][4 * d + 3])));
+                        __stcg(to16 + (16 * c + 8 * b + d) * PT_ROWS, make_float4(__uint_as_float(v[0][4 * d]) * unit, __uint_as_float(v[0][4 * d + 1]) * unit,
+                                                                                  __uint_as_float(v[0][4 * d + 2]) * unit, __uint_as_float(v[0][4 * d + 3]) * unit));
                 }
                 if (b == 0) __stcg(pp.part_ml + (long long)blockIdx.x * PT_ROWS + r, make_float2(M, L));
                 if (warp == 2 && lane == 0) pp.bad[blockIdx.x] = *bad_value;
@@ -1498,7 +1530,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         }
                     }
                 }
-                auto out = [&](int e) { return none ? 0.f : __uint_as_float(v[0][e]) * inv; };
+                auto out = [&](int e) { return none ? 0.f : __uint_as_float(v[0][e]) * inv * (pieces == 1 ? unit : 1.f); };
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
                     *reinterpret_cast<uint4*>(row + c * PT_TILE + (((4 * b + d) ^ (r & 7)) << 4)) =
@@ -1607,18 +1639,31 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (lane == 0) w4[q] = most;
             if (!all_of(ok, 2, 128)) return false;
             const int now = max(reference, (int)max(max(w4[0], w4[1]), max(w4[2], w4[3])));
+            int its = now;
             reinterpret_cast<float*>(smem + Sh::O_KS)[(j & 7) * PT_KEYS + t] = ks_new * p.scale_log2;
+            const bool at_edge = from + j >= edge0;
+            if (at_edge) {
+                // so far up to this key
+                its = fin_next ? (int)ve : 0;
+#pragma unroll 1
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int x = __shfl_up_sync(0xffffffffu, its, o);
+                    if (lane >= o) its = max(its, x);
+                }
+                its = max(its, reference);
+                for (int w = 0; w < 3; ++w) if (w < q) its = max(its, (int)w4[w]);
+                reinterpret_cast<int*>(smem + Sh::O_EX)[((from + j - edge0) & 1) * PT_KEYS + t] = its;       // (there are two such blocks at most)
+            }
             if (t == 0) {
-                const int d = now - reference;                              // (an accumulator that is still empty may be scaled by anything)
-                v_moved[j & 7] = d == 0 ? 1.f : d > 126 ? 0.f : __uint_as_float((uint32_t)(127 - d) << 23);
-                *v_exponent = now;
+                v_moved[j & 7] = at_edge ? 1.f : power_of_two(max(reference - now, -126));                   // (at the edge: a row's own)
+                if (!at_edge) *v_exponent = now;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&ks_full[j & 7]);
             reference = now;
             // code * scale * 2^(6 - reference), in two steps: 2^(127 - reference) alone may be no normal number
-            const int half_way = (127 - now) / 2;
-            f_next = fin_next ? vs * __uint_as_float((uint32_t)(127 + half_way) << 23) * __uint_as_float((uint32_t)(133 + 127 - now - half_way) << 23) : vs;
+            const int half_way = (127 - its) / 2;
+            f_next = fin_next ? vs * power_of_two(half_way) * power_of_two(133 - its - half_way) : vs;
             return true;
         };
         // a row's 16-byte pieces in an order that differs from thread to thread: eight of them read 128 different bytes of banks
