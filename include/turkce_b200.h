@@ -220,7 +220,8 @@ int tb_attention_bwd(const void* d_Q, const void* d_K, const void* d_V, const vo
  * with them, so that its new rows sit at positions kv_len[s] - n .. kv_len[s] - 1.  A sequence may have no new row.  Rows
  * behind q_start[seqs] are left as they are.
  * A page outside the pool, a position or a length outside what the call allows is left out and reported by the next
- * tb_check (code 71 or 75: page, 72 or 76: length or position); nothing outside the arrays is read or written. */
+ * tb_check (code 71 or 75: page, 72 or 76: length or position); nothing outside the arrays is read or written.  Attention cannot
+ * leave a page out of a softmax: rows that see a key in a page outside the pool are NaN, and so is their lse. */
 #define TB_KV_BF16 0
 #define TB_KV_E4M3 1
 typedef struct TbKvCache {

@@ -149,3 +149,29 @@ def test_chunks_of_values_at_the_ends_of_their_range(tb, dim, exponent):
     bound = 2.0 ** -8 * np.abs(want) + (2 * 2.0 ** -11 * 1.01 + 2 * score[..., None] + 2.0 ** -15) * spread + lost + 2.0 ** -133
     assert (np.abs(got - want) <= bound).all(), np.nanmax(np.abs(got - want) / bound)
     assert (np.abs(lse - want_lse) <= score + 2.0 ** -15 + 2.0 ** -20 * (1 + np.abs(want_lse))).all()
+
+
+# ---------------------------------------------------------------------------------------------- pages outside the pool
+
+@pytest.mark.parametrize("bad", [-1, 1 << 20, 0x7fffffff])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("dim,page", [(48, 16), (64, 64), (128, 16)])
+@pytest.mark.parametrize("new,kv", [(1, 200), (3, 5000), (40, 200), (40, 40), (200, 3000)])
+def test_rows_that_see_a_page_outside_the_pool_are_nan(tb, e4m3, dim, page, new, kv, bad):
+    """Nothing takes the page's place: a result that looked right would hold some other sequence's values.  Rows in front of the page, and other
+    sequences, have the same bits as without it."""
+    b = Batch(e4m3, [2, new, 1], [70, kv, 30], 2, dim, page, seed=dim + new)
+    clean = attend(b, 4, seed=25)
+    for piece in {(kv - 1) // page, (kv - 1) // page // 2}:
+        b.table_dev.copy_(torch.from_numpy(b.table.astype(np.int32)))
+        b.table_dev[1, piece] = bad
+        q, got, lse = attend(b, 4, seed=25, check=False)
+        with pytest.raises(tb.TbError, match="code 75"):
+            tb.sync_check()
+        sees = np.zeros(b.rows, bool)
+        sees[2:2 + new] = kv - new + np.arange(new) >= piece * page
+        assert np.isnan(got[sees]).all() and np.isnan(lse[sees]).all()
+        assert (got[~sees] == clean[1][~sees]).all() and (lse[~sees] == clean[2][~sees]).all()
+    b.table_dev.copy_(torch.from_numpy(b.table.astype(np.int32)))
+    again = attend(b, 4, seed=25)                               # (and nothing of it stays)
+    assert (again[1] == clean[1]).all() and (again[2] == clean[2]).all()

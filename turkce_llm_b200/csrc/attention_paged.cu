@@ -172,6 +172,19 @@ __device__ __forceinline__ int row_blocks(const PagedAttParams& p, bool ok, int 
     return ok && n > 0 && n * p.group <= PA_ROWS ? max(1, (kv + KEYS - 1) / KEYS) : 0;
 }
 
+// A page outside the pool: what takes the place of its keys is NaN (as bf16 and as 8-bit codes), of its values zeros.  Rows that see such a key are
+// NaN, and no other sequence's values are in them.  By a whole warp; `bad` has a bit for each of the block's pieces; the fence is for the
+// tensor cores, and for the copies that overwrite this next.  (A call: inside its loop it cost single tokens in pages of 16 keys 5 %.)
+constexpr uint32_t PA_NAN = 0x7fff7fffu;
+__device__ __noinline__ void fill_pieces(uint8_t* tile, unsigned bad, int piece_bytes, uint32_t word) {
+    const int lane = threadIdx.x & 31;
+    for (; bad != 0u; bad &= bad - 1u)
+        for (int x = lane * 16; x < piece_bytes; x += 32 * 16)
+            *reinterpret_cast<uint4*>(tile + (__ffs(bad) - 1) * piece_bytes + x) = make_uint4(word, word, word, word);
+    fence_proxy_async();
+    __syncwarp();
+}
+
 template <int NH, bool E4M3>
 __global__ void __launch_bounds__(PA_THREADS, (RowsShape<NH, E4M3>::PER_SM))
 paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedAttParams p) {
@@ -286,7 +299,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 const int pg = table[piece >> per_page_shift];
                 if ((unsigned)pg < (unsigned)p.v.pages) return pg;
                 atomicExch(p.err, 75);
-                return 0;
+                return -1;
             };
             // the table is read 32 pieces at a time, one round ahead
             int held = b * pieces, now = 0, next = 0;
@@ -297,9 +310,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 runs = (int)((at_block - b + blocks - 1) / per) - c0 + 1;
             }
             const int b_begin = b;
+            bool any_bad = __any_sync(0xffffffffu, now < 0);
             for (; b < b_end; ++b) {
                 const int at = b * pieces;
-                if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
+                if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); any_bad = __any_sync(0xffffffffu, now < 0); }
                 const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
                 const int count = max(0, min(pieces, last_piece - at));      // copies of this block
                 if (!slot_free()) break;
@@ -307,17 +321,26 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 uint8_t* tile = smem + st * Sh::STAGE;
                 uint64_t* bar = &full[st];
                 const bool first = b == b_begin;
+                int copies = count;
+                if (any_bad) {
+                    const unsigned bad = __ballot_sync(0xffffffffu, lane < count && pg < 0);
+                    copies -= __popc(bad);
+                    for (int c = 0; c < (E4M3 ? 1 : NH); ++c) {
+                        fill_pieces(tile + c * Sh::BLOCK, bad, piece_keys * Sh::ROW_BYTES, PA_NAN);
+                        fill_pieces(tile + Sh::TILE + c * Sh::BLOCK, bad, piece_keys * Sh::ROW_BYTES, 0u);
+                    }
+                }
                 if (lane == 0) {
                     int4* what = reinterpret_cast<int4*>(smem + Sh::O_WHAT + st * Sh::WHAT);
                     what[0] = make_int4((first ? PA_FIRST : 0) | (b == b_end - 1 ? PA_LAST : 0) | (runs == 1 ? PA_FINAL : 0) | s << 16, b * KEYS, q0, n);
                     what[1] = make_int4(kv, h, c0, runs);
-                    mbar_expect_tx(bar, (uint32_t)(count * piece_keys * (2 * Sh::TILE / KEYS) + (first ? n * p.group * p.v.hd * 2 : 0)));
+                    mbar_expect_tx(bar, (uint32_t)(copies * piece_keys * (2 * Sh::TILE / KEYS) + (first ? n * p.group * p.v.hd * 2 : 0)));
                 }
                 __syncwarp();
                 if (first && lane < n)
                     bulk_load(smem + Sh::O_Q + st * Sh::Q_BYTES + lane * p.group * p.v.hd * 2,
                               p.Q + (long long)(q0 + lane) * p.ld_q + (long long)h * p.group * p.v.hd, (uint32_t)(p.group * p.v.hd * 2), bar);
-                if (lane < count) {
+                if (lane < count && pg >= 0) {
                     const int block = pg * heads + h, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift;
                     const int o = lane << piece_shift;
 #pragma unroll
@@ -333,7 +356,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
                     for (int x = 0; x < KEYS / 64; ++x) {
                         const int four = x * 32 + lane, key = (four & (KEYS / 4 - 1)) * 4, piece = key >> piece_shift;
-                        const int block = __shfl_sync(0xffffffffu, pg, piece) * heads + h;
+                        const int block = max(__shfl_sync(0xffffffffu, pg, piece), 0) * heads + h;       // (no matter which, beside codes of NaN and 0)
                         const int r0 = (((at + piece) & ((1 << per_page_shift) - 1)) << piece_shift) + (key & (piece_keys - 1));
                         if (piece < count) copy_async16(sc + four * 4, (four < KEYS / 4 ? p.ks : p.vs) + ((long long)block << p.v.page_shift) + r0);
                     }
@@ -653,7 +676,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                             const int key = t0 + t + 2 * c + (e & 1);
                             if (key > pos[e >> 1]) continue;
                             const long long at = row_of(key);
-                            if (at >= 0) add_sums(sum[e >> 1], make_float2(z[e] * (p.ks[at] * row_factor[e >> 1]), 1.f));
+                            const float scale = at < 0 ? __uint_as_float(0x7fffffffu) : p.ks[at];        // (a page outside the pool: NaN)
+                            add_sums(sum[e >> 1], make_float2(z[e] * (scale * row_factor[e >> 1]), 1.f));
                         }
                     }
                 }
@@ -1104,10 +1128,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int pg = table[piece >> per_page_shift];
         if ((unsigned)pg < (unsigned)p.v.pages) return pg;
         atomicExch(p.err, 75);
-        return 0;
+        return -1;
     };
     int held = piece0, now = 0, next = 0;
     if (warp == 0 && nkv > 0) { now = page_at(piece0 + lane); next = page_at(piece0 + 32 + lane); }
+    bool any_bad = __any_sync(0xffffffffu, now < 0);
 
     if (threadIdx.x == 32 * 2) {
         mbar_init(q_full, 1); mbar_init(q_ready, 4); mbar_init(v_land, 1);
@@ -1142,39 +1167,50 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (E4M3) {
             for (int j = 0; j < nkv; ++j) {
                 const int at = piece0 + j * page_pieces, st = j % KST, rs = j % Sh::RST, o = lane << piece_shift;
-                if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
+                if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); any_bad = __any_sync(0xffffffffu, now < 0); }
                 const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
                 const int count = min(page_pieces, last_piece - at);
+                const unsigned bad = any_bad ? __ballot_sync(0xffffffffu, lane < count && pg < 0) : 0u;
+                const int copies = count - __popc(bad);
+                const bool copied = lane < count && pg >= 0;
                 const int block = pg * p.v.heads + head, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift;
                 ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], (uint32_t)((j / KST) & 1) ^ 1u, abort_flag));
                 if (!ok) break;
-                if (lane == 0) mbar_expect_tx(&k_full[st], (uint32_t)(count * piece_keys * 128));
+                if (bad != 0u) fill_pieces(sK + st * Sh::K_TILE, bad, piece_keys * 128, PA_NAN);
+                if (lane == 0) mbar_expect_tx(&k_full[st], (uint32_t)(copies * piece_keys * 128));
                 __syncwarp();
-                if (lane < count) tma_load_3d(sK + st * Sh::K_TILE + o * 128, &tmK, &k_full[st], 0, r0, block);
+                if (copied) tma_load_3d(sK + st * Sh::K_TILE + o * 128, &tmK, &k_full[st], 0, r0, block);
                 __syncwarp();
                 ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[rs], (uint32_t)((j / Sh::RST) & 1) ^ 1u, abort_flag));
                 if (!ok) break;
-                if (lane == 0) mbar_expect_tx(&raw_full[rs], (uint32_t)(count * piece_keys * 64 * NH));
+                if (bad != 0u) fill_pieces(smem + Sh::O_RAW + rs * Sh::RAW, bad, piece_keys * 64 * NH, 0u);
+                if (lane == 0) mbar_expect_tx(&raw_full[rs], (uint32_t)(copies * piece_keys * 64 * NH));
                 __syncwarp();
-                if (lane < count) tma_load_3d(smem + Sh::O_RAW + rs * Sh::RAW + o * 64 * NH, &tmV, &raw_full[rs], 0, r0, block);
+                if (copied) tma_load_3d(smem + Sh::O_RAW + rs * Sh::RAW + o * 64 * NH, &tmV, &raw_full[rs], 0, r0, block);
                 __syncwarp();
             }
         }
         for (int j = 0; j < nkv && ok && !E4M3; ++j) {
             const int at = piece0 + j * page_pieces;
-            if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); }
+            if (at >= held + 32) { held += 32; now = next; next = page_at(held + 32 + lane); any_bad = __any_sync(0xffffffffu, now < 0); }
             const int pg = __shfl_sync(0xffffffffu, now, (at - held + lane) & 31);
             const int count = min(page_pieces, last_piece - at);
-            const int block = pg * p.v.heads + head, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift, o = lane << piece_shift;
+            const unsigned bad = any_bad ? __ballot_sync(0xffffffffu, lane < count && pg < 0) : 0u;
+            const int copies = count - __popc(bad);
+            const bool copied = lane < count && pg >= 0;
+            const int block = pg * p.v.heads + head, r0 = ((at + lane) & ((1 << per_page_shift) - 1)) << piece_shift;
+            const int o = lane << piece_shift;
             const int st = j % KST;
             {
                 const int vst = j % VST;
                 ok = mbar_wait(&k_empty[st], (uint32_t)((j / KST) & 1) ^ 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                if (lane == 0) mbar_expect_tx(&k_full[st], (uint32_t)(count * piece_keys * 128 * NH));
+                if (bad != 0u)
+                    for (int c = 0; c < NH; ++c) fill_pieces(sK + (st * NH + c) * PT_TILE, bad, piece_keys * 128, PA_NAN);
+                if (lane == 0) mbar_expect_tx(&k_full[st], (uint32_t)(copies * piece_keys * 128 * NH));
                 __syncwarp();
-                if (lane < count)
+                if (copied)
                     for (int c = 0; c < NH; ++c) tma_load_3d(sK + (st * NH + c) * PT_TILE + o * 128, &tmK, &k_full[st], c * 64, r0, block);
                 ok = mbar_wait(&v_empty[vst], (uint32_t)((j / VST) & 1) ^ 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -1182,9 +1218,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 const bool edge = from + j >= edge0;
                 uint64_t* bar = edge ? v_land : &v_full[vst];
                 uint8_t* tile_v = sV + vst * NH * PT_TILE;
-                if (lane == 0) mbar_expect_tx(bar, (uint32_t)(count * piece_keys * 128 * NH));
+                if (bad != 0u)
+                    for (int c = 0; c < NH; ++c) fill_pieces(tile_v + c * PT_TILE, bad, piece_keys * 128, 0u);
+                if (lane == 0) mbar_expect_tx(bar, (uint32_t)(copies * piece_keys * 128 * NH));
                 __syncwarp();
-                if (lane < count)
+                if (copied)
                     for (int c = 0; c < NH; ++c) tma_load_3d(tile_v + c * PT_TILE + o * 128, &tmV, bar, c * 64, r0, block);
                 if (edge) {
                     ok = mbar_wait(v_land, (uint32_t)(landed & 1), abort_flag);
@@ -1616,7 +1654,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const int key = (from + j) * PT_KEYS + t;
             if (j >= nkv || key > last_pos) return -1;
             const int pg = table[key >> p.v.page_shift];
-            return (unsigned)pg < (unsigned)p.v.pages ? pg : 0;             // (the producer reports it)
+            return (unsigned)pg < (unsigned)p.v.pages ? pg : 0;             // (the producer reports it; codes of NaN and 0 have any scale)
         };
         float ks_new = 0.f, vs_new = 0.f;
         auto load_scales = [&](int j, int pg) {

@@ -132,7 +132,8 @@ int device_error_result(DeviceCtx* ctx) {
         // gave up may have left them half-way
         cudaMemset(ctx->d_err, 0, 1024);
         // (codes of arguments that only the device sees: the kernel has left them out and gone on)
-        const char* what = h == 71 || h == 75   ? "a page table names a page outside the pool"
+        const char* what = h == 71              ? "a page table names a page outside the pool"
+                           : h == 75            ? "a page table names a page outside the pool; rows that see it are NaN"
                            : h == 72 || h == 76 ? "a length or position of a batch is outside what its call allows"
                            : h == 81            ? "a length or index of the rules on logits is outside its array"
                                                 : nullptr;
