@@ -48,7 +48,8 @@ int tb_device_count(void);
 const char* tb_last_error(void);
 /* Number of kernels this library has launched on the current device so far. */
 long long tb_launch_count(void);
-/* Waits for `stream` and reports a kernel that gave up on a bounded wait. */
+/* Waits for `stream` and reports a kernel that gave up on a bounded wait, or, where there is none, one that found an argument on
+ * the device outside its array.  Each is told once; a failed wait comes first, the argument with the next call. */
 int tb_check(void* stream);
 /* cuda_shutdown (cuda/cuda_backend.h:33): frees the library's scratch memory. */
 int tb_shutdown(void);

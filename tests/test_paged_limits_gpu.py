@@ -175,3 +175,30 @@ def test_rows_that_see_a_page_outside_the_pool_are_nan(tb, e4m3, dim, page, new,
     b.table_dev.copy_(torch.from_numpy(b.table.astype(np.int32)))
     again = attend(b, 4, seed=25)                               # (and nothing of it stays)
     assert (again[1] == clean[1]).all() and (again[2] == clean[2]).all()
+
+
+def test_a_bad_page_is_told_by_the_check_alone_and_once(tb):
+    """Calls that check their own work on the host neither fail for it nor take it away; a batch's bad length on one stream leaves the tickets of
+    a head on another alone (its choice is the same before and after)."""
+    b = Batch(False, [1, 1], [40, 50], 2, 64, 16, seed=2)
+    b.table_dev[1, 2] = -3
+    x = torch.randn(4, 128, device="cuda").to(torch.bfloat16)
+    e = torch.randn(1000, 128, device="cuda").to(torch.bfloat16)
+    tok = torch.zeros(4, dtype=torch.int32, device="cuda")
+    tb.lmhead_argmax_bf16(x, e, tok)
+    before = tok.clone()
+    attend(b, 2, seed=8, check=False)
+    torch.cuda.synchronize()
+    A, B, C = np.ones((64, 32), np.float32), np.ones((32, 48), np.float32), np.zeros((64, 48), np.float32)
+    tb.matmul_host(A, B, C, 64, 32, 48)
+    assert (C == 32).all()
+    other = torch.cuda.Stream()
+    for _ in range(20):
+        with torch.cuda.stream(other):
+            tb.lmhead_argmax_bf16(x, e, tok)
+        attend(b, 2, seed=8, check=False)
+        with pytest.raises(tb.TbError, match="code 75"):
+            tb.sync_check()
+        tb.sync_check()
+    torch.cuda.synchronize()
+    assert torch.equal(tok, before)

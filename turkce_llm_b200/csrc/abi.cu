@@ -37,7 +37,7 @@ long long tb_launch_count(void) {
 int tb_check(void* stream) {
     DeviceCtx* ctx;
     TB_TRY(get_ctx(&ctx));
-    return check_device_error(ctx, S(stream));
+    return check_device_error(ctx, S(stream), true);
 }
 
 int tb_shutdown(void) {

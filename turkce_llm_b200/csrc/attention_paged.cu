@@ -234,7 +234,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
                 for (int i = 0; i < PA_SCAN; ++i) {
                     const bool ok = batch_ok(p, q[i], q[i + 1], kv[i]);
-                    if (!ok && a + i < seqs) atomicExch(p.err, 76);
+                    if (!ok && a + i < seqs) report_argument(p.err, 76);
                     nb[i] = a + i < seqs ? row_blocks<KEYS>(p, ok, q[i + 1] - q[i], kv[i]) : 0;
                     mine += nb[i];
                 }
@@ -289,7 +289,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         while (ok && s < seqs && (p.whole || left > 0)) {
             int q0, n, kv;
             const bool fine = batch_of(p, s, q0, n, kv);
-            if (!fine && p.whole && lane == 0) atomicExch(p.err, 76);
+            if (!fine && p.whole && lane == 0) report_argument(p.err, 76);
             const int blocks = row_blocks<KEYS>(p, fine, n, kv);
             const int b_end = p.whole ? blocks : (int)min((long long)blocks, b + left);
             const int* table = p.v.table + (long long)s * p.v.table_ld;
@@ -298,7 +298,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 if (piece >= last_piece) return 0;
                 const int pg = table[piece >> per_page_shift];
                 if ((unsigned)pg < (unsigned)p.v.pages) return pg;
-                atomicExch(p.err, 75);
+                report_argument(p.err, 75);
                 return -1;
             };
             // the table is read 32 pieces at a time, one round ahead
@@ -1127,7 +1127,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (piece >= last_piece) return 0;
         const int pg = table[piece >> per_page_shift];
         if ((unsigned)pg < (unsigned)p.v.pages) return pg;
-        atomicExch(p.err, 75);
+        report_argument(p.err, 75);
         return -1;
     };
     int held = piece0, now = 0, next = 0;

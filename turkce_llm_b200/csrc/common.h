@@ -10,6 +10,8 @@
 #include <functional>
 #include <vector>
 
+#include "error_words.h"
+
 namespace tb {
 
 typedef __nv_bfloat16 bf16;
@@ -73,9 +75,8 @@ struct ProfRec { const char* tag; cudaEvent_t ev; cudaEvent_t ev_end; double flo
 struct DeviceCtx {
     int device = -1;
     int sm_count = 0;
-    int* d_err = nullptr;
-    // device error word written by kernels whose bounded waits ran out
-    unsigned int* d_tickets = nullptr;   // 32 zeroed words behind the error word, for single-launch tickets
+    int* d_err = nullptr;          // error words (error_words.h): kernels whose bounded waits ran out, arguments that only the device sees
+    unsigned int* d_tickets = nullptr;   // 32 zeroed words behind the error words, for single-launch tickets
     unsigned long long* d_best = nullptr; // 64 zeroed words for the fused LM head's packed maxima
     void* scratch = nullptr;       // growable scratch (operand packing, split-K partials)
     size_t scratch_bytes = 0;
@@ -95,12 +96,13 @@ const char* prof_intern(const char* text);
 int get_ctx(DeviceCtx** out);
 // Makes sure the scratch buffer holds at least `bytes`; may reallocate (synchronises).
 int ensure_scratch(DeviceCtx* ctx, size_t bytes);
-// Reads and clears the device error word (synchronises the stream first).
-int check_device_error(DeviceCtx* ctx, cudaStream_t stream);
-// The same in two halves, for a caller that waits for the stream itself in between: the word's copy to the host is issued
+// Reads the device's error words (synchronises the stream first) and clears what it tells of: a kernel that gave up on a wait, and with
+// `arguments` one that found an argument outside its array.  Calls that check their own work only leave the second for tb_check.
+int check_device_error(DeviceCtx* ctx, cudaStream_t stream, bool arguments = false);
+// The same in two halves, for a caller that waits for the stream itself in between: the words' copy to the host is issued
 // / what it brought is looked at.
 int device_error_request(DeviceCtx* ctx, cudaStream_t stream);
-int device_error_result(DeviceCtx* ctx);
+int device_error_result(DeviceCtx* ctx, bool arguments = false, cudaStream_t stream = nullptr);
 
 // ---- GEMM on BF16 operands (gemm_tcgen05.cu)
 enum GemmKind { GEMM_NN = 0, GEMM_NT = 1, GEMM_TN = 2 };
@@ -344,6 +346,8 @@ inline cudaError_t launch_kernel_early(void (*kernel)(KArgs...), dim3 grid, dim3
 #ifdef __CUDACC__
 // waits until every kernel this launch depends on has completed and its writes are visible
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// an argument that only the device sees is outside its array: the next tb_check tells its code
+__device__ __forceinline__ void report_argument(int* err, int code) { atomicExch(err + offsetof(ErrorWords, argument) / sizeof(int), code); }
 // lets the next kernel of the stream start launching
 __device__ __forceinline__ void pdl_launch_dependents_now() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() {

@@ -47,9 +47,9 @@ int get_ctx(DeviceCtx** out) {
                 const int n = atoi(e);
                 if (n > 0 && n < c->sm_count - 8) c->sm_count -= n;
             }
-            TB_CUDA(cudaMalloc(&c->d_err, 1024));
-            TB_CUDA(cudaMemset(c->d_err, 0, 1024));
-            c->d_tickets = reinterpret_cast<unsigned int*>(c->d_err + 32);
+            TB_CUDA(cudaMalloc(&c->d_err, kErrorBytes));
+            TB_CUDA(cudaMemset(c->d_err, 0, kErrorBytes));
+            c->d_tickets = reinterpret_cast<unsigned int*>(c->d_err) + kErrorTickets / 4;
             c->d_best = reinterpret_cast<unsigned long long*>(c->d_err + 64);
             c->scratch = nullptr;
             c->scratch_bytes = 0;
@@ -110,48 +110,44 @@ void prof_close(DeviceCtx* ctx, cudaStream_t stream) {
 }
 
 namespace {
-// where a calling thread receives the error word: pinned, so that the copy waits for nothing but its stream (the same copy
+// where a calling thread receives the error words: pinned, so that the copy waits for nothing but its stream (the same copy
 // to pageable memory took 12 us after the stream had drained)
 struct ErrWord {
-    int* p = nullptr;
+    ErrorWords* p = nullptr;
     ~ErrWord() { if (p) cudaFreeHost(p); }
 };
 thread_local ErrWord t_err;
+
+// (an argument's code that another stream has left since stays)
+__global__ void clear_word_kernel(int* word, int code) { atomicCAS(word, code, 0); }
 }  // namespace
 
 int device_error_request(DeviceCtx* ctx, cudaStream_t stream) {
-    if (!t_err.p) TB_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&t_err.p), sizeof(int), cudaHostAllocPortable));
-    TB_CUDA(cudaMemcpyAsync(t_err.p, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost, stream));
+    if (!t_err.p) TB_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&t_err.p), sizeof(ErrorWords), cudaHostAllocPortable));
+    TB_CUDA(cudaMemcpyAsync(t_err.p, ctx->d_err, sizeof(ErrorWords), cudaMemcpyDeviceToHost, stream));
     return 0;
 }
 
-int device_error_result(DeviceCtx* ctx) {
-    const int h = *static_cast<volatile int*>(t_err.p);
-    if (h != 0) {
-        // the ticket words and packed maxima behind the error word go back to zero as well: a kernel that
-        // gave up may have left them half-way
-        cudaMemset(ctx->d_err, 0, 1024);
-        // (codes of arguments that only the device sees: the kernel has left them out and gone on)
-        const char* what = h == 71              ? "a page table names a page outside the pool"
-                           : h == 75            ? "a page table names a page outside the pool; rows that see it are NaN"
-                           : h == 72 || h == 76 ? "a length or position of a batch is outside what its call allows"
-                           : h == 81            ? "a length or index of the rules on logits is outside its array"
-                                                : nullptr;
-        if (what) {
-            set_error("%s (code %d); what it concerns was left out", what, h);
-            return -3;
-        }
-        const char* who = h == 1 ? "TMA producer" : h == 2 ? "MMA issuer" : h == 3 ? "epilogue" : "kernel";
-        set_error("a kernel gave up on a bounded wait (%s, code %d); its output is invalid", who, h);
+int device_error_result(DeviceCtx* ctx, bool arguments, cudaStream_t stream) {
+    const volatile ErrorWords* w = t_err.p;
+    const ErrorReport r = error_report({w->wait, w->argument}, arguments);
+    if (r.code == 0) return 0;
+    if (!r.wait) {
+        clear_word_kernel<<<1, 1, 0, stream>>>(ctx->d_err + r.word / 4, r.code);
+        set_error("%s (code %d)", argument_error(r.code), r.code);
         return -3;
     }
-    return 0;
+    cudaMemset(ctx->d_err + r.word / 4, 0, sizeof(int));
+    if (r.tickets) cudaMemset(ctx->d_tickets, 0, kErrorBytes - kErrorTickets);
+    const char* who = r.code == 1 ? "TMA producer" : r.code == 2 ? "MMA issuer" : r.code == 3 ? "epilogue" : "kernel";
+    set_error("a kernel gave up on a bounded wait (%s, code %d); its output is invalid", who, r.code);
+    return -3;
 }
 
-int check_device_error(DeviceCtx* ctx, cudaStream_t stream) {
+int check_device_error(DeviceCtx* ctx, cudaStream_t stream, bool arguments) {
     TB_TRY(device_error_request(ctx, stream));
     TB_CUDA(cudaStreamSynchronize(stream));
-    return device_error_result(ctx);
+    return device_error_result(ctx, arguments, stream);
 }
 
 }  // namespace tb

@@ -162,12 +162,12 @@ kv_append_kernel(const AppendParams p) {
     if (mine_of.s < 0 || lane >= count) {
         my_pos = -1;
     } else if (my_pos < 0 || my_pos >= (long long)p.v.table_ld << p.v.page_shift || (p.half > 0 && my_pos >= p.positions)) {
-        atomicExch(p.err, 72);
+        report_argument(p.err, 72);
         my_pos = -1;
     } else {
         const int page = p.v.table[(long long)mine_of.s * p.v.table_ld + (my_pos >> p.v.page_shift)];
         if ((unsigned)page < (unsigned)p.v.pages) my_slot = ((long long)page * G << p.v.page_shift) + (my_pos & ((1 << p.v.page_shift) - 1));
-        else atomicExch(p.err, 71);
+        else report_argument(p.err, 71);
     }
     // (halves) partners are read from the other thread's place in the ring, all eight at once where they are a whole number of threads apart
     const bool by_lane = HALVES && (p.half & 7) == 0;
@@ -325,11 +325,11 @@ kv_read_kernel(const ReadParams p) {
     if (mine_of.s >= 0 && lane < count) {
         const long long t = (long long)row0 + lane - p.start[mine_of.s] + mine_of.len;
         if (t < 0 || t >= (long long)p.v.table_ld << p.v.page_shift) {
-            atomicExch(p.err, 72);
+            report_argument(p.err, 72);
         } else {
             const int page = p.v.table[(long long)mine_of.s * p.v.table_ld + (t >> p.v.page_shift)];
             if ((unsigned)page < (unsigned)p.v.pages) my_slot = ((long long)page * G << p.v.page_shift) + (t & ((1 << p.v.page_shift) - 1));
-            else atomicExch(p.err, 71);
+            else report_argument(p.err, 71);
         }
     }
     // All (row, group of heads) pairs of the warp, four of them on their way at a time

@@ -82,7 +82,7 @@ logit_rules_kernel(const LogitParams p) {
     if (r.bias_start) {
         b0 = r.bias_start[row]; b1 = r.bias_start[row + 1];
         if (b0 < 0 || b1 < b0 || b1 > r.bias_entries) {
-            if (tid == 0) atomicExch(p.err, 81);
+            if (tid == 0) report_argument(p.err, 81);
             b0 = b1 = 0;
         }
     }
@@ -95,7 +95,7 @@ logit_rules_kernel(const LogitParams p) {
     if (r.mask) {
         const int m = r.mask_row ? r.mask_row[row] : row;
         if (m >= r.masks || m < -1) {
-            if (tid == 0) atomicExch(p.err, 81);
+            if (tid == 0) report_argument(p.err, 81);
         } else if (m >= 0) {
             mask = r.mask + (long long)m * r.mask_ld;
         }
@@ -128,7 +128,7 @@ logit_rules_kernel(const LogitParams p) {
                 if (!at || (which == 0 && rep == 1.0f)) return;
                 int len = lens[which];
                 if (len < 0 || len > ld) {
-                    if (tid == 0) atomicExch(p.err, 81);
+                    if (tid == 0) report_argument(p.err, 81);
                     len = min(max(len, 0), ld);
                 }
                 auto one = [&](uint32_t id) {

@@ -169,7 +169,7 @@ def init(device=0):
 
 
 def sync_check():
-    """Waits for the current stream and raises if a kernel reported a failed bounded wait."""
+    """Waits for the current stream and raises if a kernel reported a failed bounded wait or an argument outside its array."""
     check(load().tb_check(_stream()))
 
 
