@@ -242,7 +242,8 @@ typedef struct TbKvCache {
  * contexts are the caller's; rot_dim 0: no rotation), q leaves as bf16 [rows, q_heads * head_dim] (leading dimension ld_q, a
  * multiple of 8), k and v go to their places in the cache.  Float32 arithmetic.  TB_KV_E4M3: scale = max(largest
  * magnitude of the row / 448, 2^-126), codes are the nearest to value / scale, halves to the even code; a row with an
- * infinity or NaN in it reads back as NaN.  q_heads a multiple of heads.  d_Q must not lie over d_qkv. */
+ * infinity or NaN in it reads back as NaN.  q_heads a multiple of heads.  d_Q, d_qkv and the pools must not lie over one another; rows side by side
+ * in one matrix do not. */
 int tb_kv_append(const TbKvCache* cache, const int32_t* d_q_start, const int32_t* d_kv_len, const void* d_qkv, int qkv_bf16,
                  int64_t ld_qkv, int rows, int q_heads, const float* d_cos, const float* d_sin, int positions, int rot_dim,
                  int rope_form, void* d_Q, int64_t ld_q, void* stream);
@@ -250,7 +251,7 @@ int tb_kv_append(const TbKvCache* cache, const int32_t* d_q_start, const int32_t
 /* Rows of the cache as bf16 (code * scale, rounded once): rows start[s] .. start[s + 1] - 1 of d_K and d_V receive keys and values
  * first[s], first[s] + 1, .. of sequence s (first NULL: from 0).  Head h of row r goes to r * ld_row + h * ld_head
  * (multiples of 8): ld_head = head_dim gives [rows, heads * head_dim], ld_head = rows * head_dim one matrix per head as
- * tb_attention_fwd reads them.  d_K or d_V may be NULL. */
+ * tb_attention_fwd reads them.  d_K or d_V may be NULL; they must not lie over one another or the pools. */
 int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_first, int rows, void* d_K, void* d_V,
                int64_t ld_row, int64_t ld_head, void* stream);
 
@@ -266,6 +267,7 @@ int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_
  * call may be replayed with any lengths within them).  d_workspace: 16-byte aligned (NULL where the call needs none), zero before its
  * first use; every call leaves it ready for the next one, of whatever sizes and types.  tb_attention_paged_workspace(..): bytes that no
  * batch of the cache's sequences with no more rows, new rows and keys needs more than; a larger one is refused.
+ * Result, lse and workspace must not lie over one another, the queries or the pools.
  * Calls that can overlap on the GPU need one each.  (After a call that reported a failed wait: zero it again.) */
 int64_t tb_attention_paged_workspace(const TbKvCache* cache, int rows, int q_heads, int max_q, int max_kv);
 int tb_attention_paged(const TbKvCache* cache, const int32_t* d_q_start, const int32_t* d_kv_len, const void* d_Q, int64_t ld_q,

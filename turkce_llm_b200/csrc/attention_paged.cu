@@ -1914,7 +1914,14 @@ int tb_attention_paged(const TbKvCache* cache, const int32_t* d_q_start, const i
     TB_CHECK(((reinterpret_cast<uintptr_t>(d_Q) | reinterpret_cast<uintptr_t>(d_att) | reinterpret_cast<uintptr_t>(d_workspace)) & 15u) == 0,
              "tb_attention_paged: rows and workspace must be 16-byte aligned");
     TB_CHECK(scale > 0.f && scale < INFINITY, "tb_attention_paged: scale must be positive and finite");
-    TB_CHECK(d_Q != d_att, "tb_attention_paged: the result must not lie over the queries");
+    const RowSpan q = {d_Q, rows, width * 2, ld_q * 2}, att = {d_att, rows, width * 2, ld_att * 2}, lse = {d_lse, 1, (long long)rows * q_heads * 4, 0};
+    const RowSpan room = {workspace_bytes > 0 ? d_workspace : nullptr, 1, workspace_bytes, 0};
+    TB_CHECK(!spans_overlap(q, att), "tb_attention_paged: the result must not lie over the queries");
+    TB_CHECK(!spans_overlap(lse, q) && !spans_overlap(lse, att), "tb_attention_paged: the sums must not lie over the queries or the result");
+    TB_CHECK(!spans_overlap(room, q) && !spans_overlap(room, att) && !spans_overlap(room, lse),
+             "tb_attention_paged: the workspace must not lie over the queries, the result or the sums");
+    TB_CHECK(!over_pools(cache, att) && !over_pools(cache, lse) && !over_pools(cache, room),
+             "tb_attention_paged: the result, the sums and the workspace must not lie over the pools");
     DeviceCtx* ctx;
     TB_TRY(get_ctx(&ctx));
     return launch_attention_paged(ctx, cache, d_q_start, d_kv_len, static_cast<const bf16*>(d_Q), ld_q, rows, q_heads, std::min(max_q, rows),

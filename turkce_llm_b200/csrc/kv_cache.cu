@@ -456,10 +456,13 @@ int tb_kv_append(const TbKvCache* cache, const int32_t* d_q_start, const int32_t
     TB_CHECK(ld_q >= (long long)q_heads * cache->head_dim && ld_q % 8 == 0, "tb_kv_append: ld_q must be a multiple of 8 and at least %lld (got %lld)",
              (long long)q_heads * cache->head_dim, (long long)ld_q);
     TB_CHECK(((reinterpret_cast<uintptr_t>(d_qkv) | reinterpret_cast<uintptr_t>(d_Q)) & 15u) == 0, "tb_kv_append: rows must be 16-byte aligned");
-    TB_CHECK(rows == 0 || d_Q != d_qkv, "tb_kv_append: the queries must not lie over the rows they come from");
+    const RowSpan from = {d_qkv, rows, width * (qkv_bf16 ? 2 : 4), ld_qkv * (qkv_bf16 ? 2 : 4)};
+    const RowSpan to = {d_Q, rows, (long long)q_heads * cache->head_dim * 2, ld_q * 2};
+    TB_CHECK(!spans_overlap(from, to), "tb_kv_append: the queries must not lie over the rows they come from");
     TB_CHECK(rot_dim >= 0 && rot_dim <= cache->head_dim && rot_dim % 2 == 0, "tb_kv_append: rot_dim must be even and at most head_dim (got %d)", rot_dim);
     TB_CHECK(rope_form == TB_ROPE_PAIRS || rope_form == TB_ROPE_HALVES, "tb_kv_append: unknown rotation form %d", rope_form);
     TB_CHECK(rot_dim == 0 || (d_cos && d_sin && positions > 0), "tb_kv_append: a rotation needs both tables");
+    TB_CHECK(!over_pools(cache, from) && !over_pools(cache, to), "tb_kv_append: the rows must not lie over the pools");
     if (rows == 0) return 0;
     DeviceCtx* ctx;
     TB_TRY(get_ctx(&ctx));
@@ -473,13 +476,18 @@ int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_
     TB_CHECK(rows >= 0, "tb_kv_read: rows must not be negative");
     TB_CHECK(d_start, "tb_kv_read: NULL row starts");
     TB_CHECK(d_K || d_V, "tb_kv_read: both outputs are NULL");
-    TB_CHECK(rows == 0 || d_K != d_V, "tb_kv_read: the two outputs lie over one another");
     TB_CHECK(ld_row >= cache->head_dim && ld_row % 8 == 0 && ld_head >= cache->head_dim && ld_head % 8 == 0,
              "tb_kv_read: ld_row and ld_head must be multiples of 8 and at least head_dim (got %lld, %lld)", (long long)ld_row,
              (long long)ld_head);
     TB_CHECK(ld_row >= (cache->heads - 1) * ld_head + cache->head_dim || ld_head >= (rows - 1LL) * ld_row + cache->head_dim,
              "tb_kv_read: rows of ld_row %lld and heads of ld_head %lld lie over one another", (long long)ld_row, (long long)ld_head);
     TB_CHECK(((reinterpret_cast<uintptr_t>(d_K) | reinterpret_cast<uintptr_t>(d_V)) & 15u) == 0, "tb_kv_read: outputs must be 16-byte aligned");
+    TB_CHECK(!d_K || !d_V || !heads_overlap(d_K, d_V, rows, ld_row * 2, cache->heads, ld_head * 2, cache->head_dim * 2LL),
+             "tb_kv_read: the two outputs lie over one another");
+    for (void* out : {d_K, d_V})
+        for (int h = 0; h < cache->heads; ++h)
+            TB_CHECK(!out || !over_pools(cache, {static_cast<const char*>(out) + h * ld_head * 2, rows, cache->head_dim * 2LL, ld_row * 2}),
+                     "tb_kv_read: the outputs must not lie over the pools");
     if (rows == 0) return 0;
     DeviceCtx* ctx;
     TB_TRY(get_ctx(&ctx));

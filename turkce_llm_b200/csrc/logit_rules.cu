@@ -6,6 +6,7 @@
 #include "../../include/turkce_b200.h"
 #include "common.h"
 #include "logit_rules.h"
+#include "overlap.h"
 
 #include <algorithm>
 
@@ -251,11 +252,8 @@ extern "C" int tb_logits_adjust(const TbLogitRules* rules, const float* d_logits
     TB_CHECK(d_logits && d_out, "tb_logits_adjust: NULL logits");
     TB_CHECK(ld_logits >= vocab && ld_out >= vocab, "tb_logits_adjust: leading dimensions must be at least vocab");
     TB_CHECK(d_out != d_logits || ld_out == ld_logits, "tb_logits_adjust: in place, both leading dimensions must be the same");
-    if (d_out != d_logits) {
-        const uintptr_t a0 = reinterpret_cast<uintptr_t>(d_logits), a1 = a0 + ((rows - 1) * ld_logits + vocab) * 4;
-        const uintptr_t b0 = reinterpret_cast<uintptr_t>(d_out), b1 = b0 + ((rows - 1) * ld_out + vocab) * 4;
-        TB_CHECK(a1 <= b0 || b1 <= a0, "tb_logits_adjust: the output overlaps the logits");
-    }
+    TB_CHECK(d_out == d_logits || !spans_overlap({d_logits, rows, vocab * 4LL, ld_logits * 4}, {d_out, rows, vocab * 4LL, ld_out * 4}),
+             "tb_logits_adjust: the output overlaps the logits");
     const TbLogitRules& r = *rules;
     TB_CHECK(!r.prompt || (r.prompt_len && r.prompt_ld > 0 && r.prompt_ld < (1 << 29)), "tb_logits_adjust: prompt ids need lengths and a leading dimension below 2^29");
     TB_CHECK(!r.output || (r.output_len && r.output_ld > 0 && r.output_ld < (1 << 29)), "tb_logits_adjust: output ids need lengths and a leading dimension below 2^29");

@@ -2,6 +2,7 @@
 #pragma once
 #include "../../include/turkce_b200.h"
 #include "common.h"
+#include "overlap.h"
 
 namespace tb {
 
@@ -12,6 +13,15 @@ struct PagedView {
 
 // host: the checks that every entry point makes of a cache
 int check_cache(const TbKvCache* c, const char* who);
+// host: whether rows lie over one of the cache's pools
+inline bool over_pools(const TbKvCache* c, RowSpan rows) {
+    const long long n = (long long)c->pages * c->heads * c->page_size, bytes = n * c->head_dim * (c->type == TB_KV_E4M3 ? 1 : 2);
+    for (const void* pool : {c->K, c->V})
+        if (spans_overlap({pool, 1, bytes, bytes}, rows)) return true;
+    for (const void* scales : {c->k_scale, c->v_scale})
+        if (spans_overlap({scales, 1, n * 4, n * 4}, rows)) return true;
+    return false;
+}
 inline int page_shift_of(int page_size) {
     int s = 0;
     while ((1 << s) < page_size) ++s;
