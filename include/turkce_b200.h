@@ -260,7 +260,7 @@ int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_
  * d_Q, d_att: bf16 [rows, q_heads * head_dim] (leading dimensions multiples of 8); at most 128 query heads share a key head;
  * scale positive.  d_lse (optional): float [rows, q_heads], natural
  * log of the row's sum of exponentials.  Keys behind a row's position have no influence on it, whatever they hold.  A row without
- * any key (kv_len below the number of new rows) gets zeros and lse -infinity.
+ * any key (kv_len below the number of new rows) gets zeros and lse -infinity.  Keys that score minus infinity have no weight beside others.
  * 8-bit rows: scores are exact but for 2^-21 of a row's largest query element; next to a row's largest probability those of 2^-32 of it
  * and more count, and values of 2^-31 of the sequence's largest scale and more.
  * max_q and max_kv bound the new rows and the keys of any one sequence (host numbers: they size the launch, and a captured

@@ -202,3 +202,30 @@ def test_a_bad_page_is_told_by_the_check_alone_and_once(tb):
         tb.sync_check()
     torch.cuda.synchronize()
     assert torch.equal(tok, before)
+
+
+# ---------------------------------------------------------------------------------------------- scores of minus infinity
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 3, 40])
+@pytest.mark.parametrize("kv", [300, 4000])
+def test_keys_of_minus_infinity_have_no_weight(tb, e4m3, dim, new, kv):
+    """The first keys, whole blocks of them, score minus infinity: the result is that of the others alone."""
+    cut = kv - 90
+    b = Batch(e4m3, [new], [kv], 1, dim, 16, seed=kv)
+    page, slot = at(b, 0, np.arange(cut))
+    if e4m3:
+        b.host["k"][page, 0, slot] = 0
+        b.host["k"][page, 0, slot, 0] = 0xb8                    # -1 times an infinite scale
+        b.host["k_scale"][page, 0, slot] = np.inf
+    else:
+        b.host["k"][page, 0, slot, 0] = -float("inf")
+    upload(b)
+    q = torch.randn(new + 3, 2 * dim).to(torch.bfloat16)
+    q[:, ::dim] = q[:, ::dim].abs() + 1
+    rows, got, lse = attend(b, 2, seed=26, q=q)
+    k, v = b.sequence("k", 0)[cut:], b.sequence("v", 0)[cut:]
+    want, want_lse, spread, size = plain.attention(rows, k, v, np.arange(90 - new, 90), dim ** -0.5)
+    assert plain.within(got, want, spread, size, dim) <= 1.0
+    assert (np.abs(lse - want_lse) <= (dim + 4) * 2.0 ** -24 * size + 2.0 ** -20 * (1 + np.abs(want_lse))).all()

@@ -83,6 +83,9 @@ __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0
 // conversions (43 % of the issue slots of 12 warps that wait for one another's loads).  A call of 40 us loses 4 us before its first block is
 // there and 2 to 4 us to the spread of its CTAs' ends.
 constexpr float PA_UP = 13.f;
+// The reference of a row that has seen no key yet, or keys that score minus infinity alone: lower than any score, but a number, so that minus
+// infinity is below it and not beside it.
+constexpr float PA_LOW = -3.0e38f;
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = (PA_WARPS + 1) * 32;
 constexpr int PA_SCAN = 4;               // sequences per lane of one look at the batch
@@ -461,7 +464,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                                 qf[b][g][x + 2 * j] = odd ? f16_pair(f.x, f.y) : f16_pair(f.x * down, f.y * down);
                             }
                 }
-                m[x] = -INFINITY; l[x] = 0.f;
+                m[x] = PA_LOW; l[x] = 0.f;
             }
             if (E4M3) {
                 const float vs = reinterpret_cast<const float*>(smem + Sh::O_SCALE + st * Sh::SCALES)[KEYS];
@@ -559,9 +562,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 if (E4M3) { f = parts[8 * t + 2 * c]; g = parts[8 * t + 2 * c + 1]; }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    // (a row that has seen no key yet: its maximum is -infinity, and so are its scores)
-                    const float base = edge && m[h] == -INFINITY ? 0.f : m[h];
-                    float p0 = ex2_approx(z[t][2 * h] - base), p1 = ex2_approx(z[t][2 * h + 1] - base);
+                    float p0 = ex2_approx(z[t][2 * h] - m[h]), p1 = ex2_approx(z[t][2 * h + 1] - m[h]);
                     if (E4M3) {
                         // (a key that the row does not see may have any scale)
                         const bool no0 = edge && z[t][2 * h] == -INFINITY, no1 = edge && z[t][2 * h + 1] == -INFINITY;
@@ -1132,7 +1133,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     };
     int held = piece0, now = 0, next = 0;
     if (warp == 0 && nkv > 0) { now = page_at(piece0 + lane); next = page_at(piece0 + 32 + lane); }
-    bool any_bad = __any_sync(0xffffffffu, now < 0);
 
     if (threadIdx.x == 32 * 2) {
         mbar_init(q_full, 1); mbar_init(q_ready, 4); mbar_init(v_land, 1);
@@ -1158,7 +1158,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 
     if (warp == 0) {
         // ---- producer: a lane per piece of a page
-        bool ok = true;
+        bool ok = true, any_bad = __any_sync(0xffffffffu, now < 0);
         if (lane == 0 && nkv > 0) {
             mbar_expect_tx(q_full, (uint32_t)(NH * pp.tokens * p.group * 128));
             for (int c = 0; c < NH; ++c) tma_load_3d(sQ + c * PT_TILE, &tmQ, q_full, c * 64, head * p.group, q0 + tok0);
@@ -1319,7 +1319,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const bool mine = r < tokens * p.group;
         const uint32_t lane_base = (uint32_t)(q * 32) << 16;
         const uint32_t ts = tS + lane_base + (uint32_t)(b * 64), to = tO + lane_base + (uint32_t)(b * 64 * NH);
-        float m = -INFINITY, l = 0.f, c1 = p.scale_log2;
+        float m = PA_LOW, l = 0.f, c1 = p.scale_log2;
         bool ok = true;
         // (8 bits) this row's reference of value scales, once there is one of its own: the others have v_exponent
         int* seen_exponent = reinterpret_cast<int*>(smem + Sh::O_SEEN) + b * PT_ROWS + r;
@@ -1409,8 +1409,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             const bool move = __any_sync(0xffffffffu, alpha != 1.0f);
             if (j > 0 && !mbar_wait(&o_full[b], (uint32_t)((j - 1) & 1), abort_flag)) { ok = false; break; }
-            // (a row that has seen no key yet, and sees none here)
-            const float nm = edge && lim < 0 && m == -INFINITY ? 0.f : -m;
+            // (a row that sees no key of this half: minus infinity against anything.  Against m as well is as right, and costs a spilled register.)
+            const float nm = lim < 0 ? 0.f : -m;
             const float2 c2 = make_float2(c1, c1), nm2 = make_float2(nm, nm);
             float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             uint8_t* prow = sP + b * PT_TILE + r * 128;
