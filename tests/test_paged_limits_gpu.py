@@ -229,3 +229,29 @@ def test_keys_of_minus_infinity_have_no_weight(tb, e4m3, dim, new, kv):
     want, want_lse, spread, size = plain.attention(rows, k, v, np.arange(90 - new, 90), dim ** -0.5)
     assert plain.within(got, want, spread, size, dim) <= 1.0
     assert (np.abs(lse - want_lse) <= (dim + 4) * 2.0 ** -24 * size + 2.0 ** -20 * (1 + np.abs(want_lse))).all()
+
+
+# ---------------------------------------------------------------------------------------------- 8-bit codes
+
+@pytest.mark.parametrize("exponent", [-126, -123, -118, -112, -104, -100, -99, -40, 100, 118])
+def test_codes_of_rows_of_any_size_are_the_nearest(tb, exponent):
+    """Elements next to the middles of two codes, in rows whose scale is anywhere in the range: bit for bit."""
+    rng = np.random.default_rng(exponent + 200)
+    rows, dim = 400, 64
+    b = Batch(True, [rows], [rows], 1, dim, 16, seed=0)
+    scale = np.ldexp((1 + rng.random(rows)).astype(np.float32), exponent)
+    big = np.minimum(scale.astype(np.float64) * 448, np.finfo(np.float32).max).astype(np.float32)
+    scale = np.maximum((big.astype(np.float64) / 448).astype(np.float32), np.float32(2.0 ** -126))
+    middles = (plain.E4M3[1:] + plain.E4M3[:-1]) / 2
+    x = (rng.choice(middles, (rows, dim)) * scale[:, None].astype(np.float64)).astype(np.float32)
+    x = (x.view(np.int32) + rng.integers(-1, 2, x.shape).astype(np.int32)).view(np.float32) * rng.choice([-1, 1], x.shape).astype(np.float32)
+    x[:, 5] = big
+    qkv = torch.zeros(rows, 3 * dim)
+    qkv[:, 2 * dim:] = torch.from_numpy(x)
+    q = torch.empty(rows, dim, dtype=torch.bfloat16, device="cuda")
+    b.cache.append(qkv.cuda(), q, b.q_start, b.kv_len)
+    tb.sync_check()
+    page, slot = at(b, 0, np.arange(rows))
+    assert (b.dev["v_scale"].cpu().numpy()[page, 0, slot] == scale).all()
+    codes = b.dev["v"].view(torch.uint8).cpu().numpy()[page, 0, slot]
+    assert (codes == plain.e4m3_codes(x, scale[:, None])).all(), (codes != plain.e4m3_codes(x, scale[:, None])).sum()

@@ -283,10 +283,16 @@ kv_append_kernel(const AppendParams p) {
             } else {
                 float inverse;
                 const float scale = e4m3_scale(__uint_as_float(big), &inverse);
+                float by = scale;
+                if (scale < E4M3_SMALL) {                        // (remainders would be below what float32 has: all of it 2^64 times as large)
+                    by *= 0x1p64f; inverse *= 0x1p-64f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] *= 0x1p64f;
+                }
                 uint32_t q[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    q[k] = e4m3_pair(quotient_to_odd(x[2 * k], scale, inverse), quotient_to_odd(x[2 * k + 1], scale, inverse));
+                    q[k] = e4m3_pair(quotient_to_odd(x[2 * k], by, inverse), quotient_to_odd(x[2 * k + 1], by, inverse));
                 *reinterpret_cast<uint2*>(static_cast<uint8_t*>(key ? p.K : p.V) + at * hd + e0) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
                 if (e0 == 0) (key ? p.ks : p.vs)[at] = scale;
             }

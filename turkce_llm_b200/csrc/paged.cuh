@@ -57,7 +57,9 @@ __device__ __forceinline__ int sequence_of(const int* __restrict__ start, int se
 
 // x / scale on its way to the nearest 8-bit float (4 exponent bits, 3 of significand; halves to the even one): a float32 that lies on the
 // same side of every middle of two codes as the true quotient.  By Markstein's correction of a quotient from its remainder, q is within a unit of its last place of that, its remainder tells on which
-// side, and a number strictly between two floats becomes the one of them whose last bit is set, which no middle has.
+// side, and a number strictly between two floats becomes the one of them whose last bit is set, which no middle has.  Where q is a middle, its
+// remainder has to be exact: with a scale of 2^-100 and more (E4M3_SMALL) it is a multiple of 2^-133, which float32 has.
+constexpr float E4M3_SMALL = 0x1p-100f;
 __device__ __forceinline__ float quotient_to_odd(float x, float scale, float inverse) {
     const float q0 = x * inverse;
     const float q = __fmaf_rn(__fmaf_rn(-q0, scale, x), inverse, q0);
