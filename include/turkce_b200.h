@@ -288,7 +288,7 @@ int tb_attention_paged(const TbKvCache* cache, const int32_t* d_q_start, const i
 typedef struct TbLogitRules {
     const uint32_t* prompt; const int32_t* prompt_len;     /* [rows][prompt_ld]: the first prompt_len[s] ids of row s */
     const uint32_t* output; const int32_t* output_len;     /* [rows][output_ld] */
-    const float *repetition, *frequency, *presence;        /* [rows]; repetition > 0, 1 for none */
+    const float *repetition, *frequency, *presence;        /* [rows]; repetition 2^-32 .. 2^32, 1 for none */
     const int32_t* bias_start; const uint32_t* bias_id; const float* bias_value;   /* entries bias_start[s] .. bias_start[s + 1] - 1 */
     const uint32_t* mask; const int32_t* mask_row;         /* [masks][mask_ld] words, bit v % 32 of word v / 32 set: allowed; mask_row
                                                               [rows]: the row's mask, -1 for none (NULL: mask s for row s) */
@@ -296,7 +296,8 @@ typedef struct TbLogitRules {
 } TbLogitRules;
 
 /* d_out may be d_logits (in place) or another matrix that does not overlap it.  Ids of a row number less than 2^29; a length or an
- * index outside its array is cut to it or left out, and reported by the next tb_check (code 81). */
+ * index outside its array is cut to it or left out, a repetition penalty outside its range is left out, and both are reported by the
+ * next tb_check (code 81). */
 int tb_logits_adjust(const TbLogitRules* rules, const float* d_logits, int64_t ld_logits, float* d_out, int64_t ld_out, int rows,
                      int vocab, void* stream);
 

@@ -33,7 +33,7 @@ inline const char* argument_error(int code) {
     return code == 71                 ? "a page table names a page outside the pool; its rows were left out"
            : code == 75               ? "a page table names a page outside the pool; rows that see it are NaN"
            : code == 72 || code == 76 ? "a length or position of a batch is outside what its call allows; its rows were left out"
-           : code == 81               ? "a length or index of the rules on logits is outside its array; what it concerns was left out"
+           : code == 81               ? "a length, index or penalty of the rules on logits is outside its range; what it concerns was left out"
                                       : "an argument on the device is outside its array";
 }
 

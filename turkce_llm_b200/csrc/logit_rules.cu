@@ -22,6 +22,7 @@ constexpr uint32_t LR_COUNT = 0x1fffffffu;
 constexpr int LR_IDS = 2;                        // ids of the prompt and of the output that a thread asks for at once
 constexpr uint32_t LR_NONE = 0xffffffffu;
 constexpr int LR_AGAIN = 64;
+constexpr float LR_LEAST = 0x1p-32f, LR_MOST = 0x1p32f;          // repetition penalties
 constexpr int LR_ROUNDS = kLogitSlice / (LR_THREADS * 4);
 
 struct LogitParams {
@@ -77,7 +78,9 @@ logit_rules_kernel(const LogitParams p) {
     early(r.prompt, r.prompt_ld, ids[0]);
     early(r.output, r.output_ld, ids[1]);
     int lens[2] = {r.prompt ? r.prompt_len[row * r.prompt_len_stride] : 0, r.output ? r.output_len[row * r.output_len_stride] : 0};
-    const float rep = r.repetition ? r.repetition[row] : 1.0f, freq = r.frequency ? r.frequency[row] : 0.0f,
+    float rep = r.repetition ? r.repetition[row] : 1.0f;
+    rep = rep >= LR_LEAST && rep <= LR_MOST ? rep : 1.0f;        // (its inverse or a remainder may be outside float32; or it is none)
+    const float freq = r.frequency ? r.frequency[row] : 0.0f,
                 pres = r.presence ? r.presence[row] : 0.0f;
     int b0 = 0, b1 = 0;
     if (r.bias_start) {
@@ -179,10 +182,12 @@ logit_rules_kernel(const LogitParams p) {
         }
     }
     const float inverse = __frcp_rn(rep);
+    if (tid == 0 && r.repetition && rep == 1.0f && r.repetition[row] != 1.0f) report_argument(p.err, 81);       // (read again: not to be held)
     auto rule = [&](float x, uint32_t w, int t) -> float {
         if (counts && (w & (LR_COUNT | LR_PROMPT)) != 0u) {
-            // x / rep by Markstein's correction (a quotient by the correctly rounded reciprocal, and what its remainder adds, both fused),
-            // x * rep of what is not positive
+            // x / rep by Markstein's correction (a quotient by the correctly rounded reciprocal, and what its remainder adds, both fused):
+            // the nearest number while the remainder is one that float32 has, else two units in the last place from it at most; x * rep of
+            // what is not positive
             const float q = x * inverse, y = __fmaf_rn(__fmaf_rn(-q, rep, x), inverse, q);
             x = x > 0.0f ? (q < INFINITY ? y : q) : x * rep;
             if ((w & LR_COUNT) != 0u) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)(w & LR_COUNT))), pres);

@@ -15,7 +15,7 @@ class LogitRules:
     """Rules for `rows` rows of `vocab` logits; every one may be None.
 
     prompt, output: int32 (or uint32) [rows, ids] with prompt_len, output_len int32 [rows]; repetition, frequency, presence:
-    float32 [rows]; bias_start int32 [rows + 1] into bias_id (int32) and bias_value (float32); mask: int32 [masks, words of 32
+    float32 [rows], repetition from 2^-32 to 2^32; bias_start int32 [rows + 1] into bias_id (int32) and bias_value (float32); mask: int32 [masks, words of 32
     tokens], a set bit allows the token, with mask_row int32 [rows] (-1: no mask; None: mask s for row s)."""
 
     def __init__(self, rows, vocab, prompt=None, prompt_len=None, output=None, output_len=None, repetition=None, frequency=None,
