@@ -67,3 +67,23 @@ def test_a_penalty_outside_its_range_is_left_out_and_reported(tb, repetition):
     with pytest.raises(tb.TbError, match="code 81"):
         tb.sync_check()
     assert z[0].tolist() == [0.5, -3.0, 0.25, -1.0] and z[1].tolist() == [0.75, -4.0, 0.25, float(np.float32(1e-38) / np.float32(2))]
+
+
+def test_empty_arrays_are_no_way_around_a_rule(tb):
+    """A mask without words or rows is refused, starts that speak of entries where there are none are reported."""
+    from turkce_llm_b200.logit_rules import LogitRules
+    for shape in ((0, 4), (3, 0), (2, 4), (3, 3)):
+        with pytest.raises(tb.TbError, match="masks have to have"):
+            LogitRules(3, 100, mask=torch.zeros(shape, dtype=torch.int32, device="cuda"))
+    for shape in ((0, 4), (1, 0)):
+        with pytest.raises(tb.TbError, match="masks have to have"):
+            LogitRules(3, 100, mask=torch.zeros(shape, dtype=torch.int32, device="cuda"), mask_row=dev(0, 0, 0))
+    z = torch.randn(2, 100, device="cuda")
+    before = z.clone()
+    none = dict(bias_id=torch.zeros(0, dtype=torch.int32, device="cuda"), bias_value=torch.zeros(0, device="cuda"))
+    LogitRules(2, 100, bias_start=dev(0, 0, 0), **none).apply(z)
+    tb.sync_check()
+    LogitRules(2, 100, bias_start=dev(0, 2, 2), **none).apply(z)
+    with pytest.raises(tb.TbError, match="code 81"):
+        tb.sync_check()
+    assert torch.equal(z, before)

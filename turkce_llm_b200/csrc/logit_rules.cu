@@ -270,7 +270,7 @@ extern "C" int tb_logits_adjust(const TbLogitRules* rules, const float* d_logits
     a.prompt = r.prompt; a.prompt_len = r.prompt_len; a.prompt_ld = r.prompt_ld; a.prompt_len_stride = 1;
     a.output = r.output; a.output_len = r.output_len; a.output_ld = r.output_ld; a.output_len_stride = 1;
     a.repetition = r.repetition; a.frequency = r.frequency; a.presence = r.presence;
-    a.bias_start = r.bias_entries > 0 ? r.bias_start : nullptr; a.bias_id = r.bias_id; a.bias_value = r.bias_value; a.bias_entries = r.bias_entries;
+    a.bias_start = r.bias_start; a.bias_id = r.bias_id; a.bias_value = r.bias_value; a.bias_entries = r.bias_entries;
     a.mask = r.mask; a.mask_row = r.mask_row; a.masks = r.masks; a.mask_ld = r.mask_ld;
     DeviceCtx* ctx;
     TB_TRY(get_ctx(&ctx));

@@ -44,6 +44,8 @@ class LogitRules:
                 raise lib.TbError("ids need their lengths, biases their starts, ids and values")
         if mask_row is not None and mask is None:
             raise lib.TbError("mask_row needs masks")
+        if mask is not None and rows and (mask.shape[1] < -(-vocab // 32) or mask.shape[0] < (rows if mask_row is None else 1)):
+            raise lib.TbError("masks have to have %d words each, and without mask_row one for each of the %d rows" % (-(-vocab // 32), rows))
         self._kept = (prompt, prompt_len, output, output_len, repetition, frequency, presence, bias_start, bias_id, bias_value, mask, mask_row)
         width = lambda t: t.shape[1] if t is not None else 0  # noqa: E731
         self._struct = lib.LogitRulesStruct(*[lib._ptr(t) if t is not None and t.numel() else None for t in self._kept], width(prompt),
