@@ -231,6 +231,25 @@ def test_keys_of_minus_infinity_have_no_weight(tb, e4m3, dim, new, kv):
     assert (np.abs(lse - want_lse) <= (dim + 4) * 2.0 ** -24 * size + 2.0 ** -20 * (1 + np.abs(want_lse))).all()
 
 
+# ---------------------------------------------------------------------------------------------- many rows
+
+def test_more_tiles_than_65535(tb):
+    """128 heads over one key head: a tile is one token.  A prompt of 65,600 of them, a row here and there against the formula."""
+    new, H, dim = 65600, 128, 16
+    b = Batch(False, [new], [new], 1, dim, 256, seed=6)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(new, H * dim, device="cuda", generator=g).to(torch.bfloat16)
+    att, lse = torch.empty_like(q), torch.empty(new, H, device="cuda")
+    b.cache.attend(q, att, b.q_start, b.kv_len, new, new, lse=lse, workspace=b.cache.workspace(H, new, new, new))
+    tb.sync_check()
+    k, v = b.sequence("k", 0), b.sequence("v", 0)
+    for r in (0, 1, 127, 40000, new - 1):
+        rows = q[r].double().cpu().numpy().reshape(1, H, dim)
+        want, want_lse, spread, size = plain.attention(rows, k, v, np.array([r]), dim ** -0.5)
+        assert plain.within(att[r].double().cpu().numpy().reshape(1, H, dim), want, spread, size, dim) <= 1.0
+        assert (np.abs(lse[r].cpu().numpy() - want_lse[0]) <= (dim + 4) * 2.0 ** -24 * size[0] + 2.0 ** -20 * (1 + np.abs(want_lse[0]))).all()
+
+
 # ---------------------------------------------------------------------------------------------- 8-bit codes
 
 @pytest.mark.parametrize("exponent", [-126, -123, -118, -112, -104, -100, -99, -40, 100, 118])

@@ -1110,7 +1110,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         s = a.x; head = a.y; tile = a.z; from = a.w; to = b.x; first_unit = b.y; pieces = b.z;
     } else {
         // the heaviest tiles of all sequences first
-        s = (int)(blockIdx.x / (unsigned)p.v.heads); head = (int)(blockIdx.x % (unsigned)p.v.heads); tile = pp.tiles - 1 - (int)blockIdx.y;
+        s = (int)(blockIdx.x / (unsigned)p.v.heads); head = (int)(blockIdx.x % (unsigned)p.v.heads);
+        tile = pp.tiles - 1 - (int)(blockIdx.z * gridDim.y + blockIdx.y);
+        if (tile < 0) return;
     }
     int q0, n, kv;
     const bool fine = batch_of(p, s, q0, n, kv);                           // (paged_rows_kernel reports it)
@@ -1809,10 +1811,7 @@ int plan_chunks(DeviceCtx* ctx, const PagedAttParams& p, const PagedPlan& pl, ui
     pp->units = reinterpret_cast<ChunkUnit*>(pp->bad + pl.most_units);
     pp->part_ml = reinterpret_cast<float2*>(pp->units + pl.most_units);
     pp->part_o = reinterpret_cast<float4*>(pp->part_ml + (size_t)pl.most_pieces * PT_ROWS);
-    if (!pp->planned) {
-        TB_CHECK(pp->tiles <= 65535, "tb_attention_paged: max_q %d is too much for one launch", p.max_q);
-        return 0;
-    }
+    if (!pp->planned) return 0;
     prof_mark(ctx, "paged_plan", 0.0, 0.0, st);
     TB_CUDA(launch_kernel(paged_plan_kernel, dim3(1), dim3(PL_THREADS), 0, st, *pp));
     ctx->launches++;
@@ -1835,7 +1834,9 @@ int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedChunkParams& pp
         attr_set[ctx->device & 63] = true;
     }
     prof_mark(ctx, "paged_chunk", 4.0 * p.rows * p.H * (double)p.max_kv * c->head_dim, 0.0, st);
-    const dim3 grid = pp.planned ? dim3(pp.most_units) : dim3((unsigned)c->heads * (unsigned)c->seqs, pp.tiles);
+    // (rows * q_heads is below 2^31, so that there are no more than 2^24 tiles)
+    const unsigned layer = std::min(pp.tiles, 65535);
+    const dim3 grid = pp.planned ? dim3(pp.most_units) : dim3((unsigned)c->heads * (unsigned)c->seqs, layer, ((unsigned)pp.tiles + layer - 1) / layer);
     TB_CUDA(launch_kernel_early(paged_chunk_kernel<NH, E4M3>, grid, dim3(Sh::THREADS), Sh::SMEM, st, tmQ, tmK, tmV, static_cast<const uint8_t*>(c->V), pp));
     ctx->launches++;
     prof_close(ctx, st);
