@@ -250,6 +250,16 @@ def test_more_tiles_than_65535(tb):
         assert (np.abs(lse[r].cpu().numpy() - want_lse[0]) <= (dim + 4) * 2.0 ** -24 * size[0] + 2.0 ** -20 * (1 + np.abs(want_lse[0]))).all()
 
 
+def test_profile_claims_no_work_that_only_the_device_knows(tb):
+    """Both kernels of a call claimed all rows times the largest number of keys."""
+    b = Batch(False, [40, 1], [300, 200], 2, 64, 16, seed=1)
+    tb.profile_begin()
+    attend(b, 2, seed=1, max_kv=16 * b.table.shape[1])
+    seen = tb.profile_end()
+    assert {"paged_rows", "paged_chunk"} <= set(seen)
+    assert all(seen[n]["flops"] == 0 and seen[n]["bytes"] == 0 for n in seen if n.startswith("paged"))
+
+
 # ---------------------------------------------------------------------------------------------- 8-bit codes
 
 @pytest.mark.parametrize("exponent", [-126, -123, -118, -112, -104, -100, -99, -40, 100, 118])

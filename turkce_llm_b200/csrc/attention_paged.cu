@@ -1786,7 +1786,7 @@ int launch_rows(DeviceCtx* ctx, const TbKvCache* c, const PagedAttParams& p, cud
         TB_CUDA(cudaFuncSetAttribute(paged_rows_kernel<NH, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
         attr_set[ctx->device & 63] = true;
     }
-    prof_mark(ctx, "paged_rows", 4.0 * p.rows * p.H * (double)p.max_kv * c->head_dim, 0.0, st);
+    prof_mark(ctx, "paged_rows", 0.0, 0.0, st);          // (how much of the batch is whose, and how long it is, only the device knows)
     TB_CUDA(launch_kernel_early(paged_rows_kernel<NH, E4M3>, dim3(p.grid), dim3(PA_THREADS), Sh::SMEM, st, tmK, tmV, p));
     ctx->launches++;
     prof_close(ctx, st);
@@ -1833,7 +1833,7 @@ int launch_chunks(DeviceCtx* ctx, const TbKvCache* c, const PagedChunkParams& pp
         TB_CUDA(cudaFuncSetAttribute(paged_chunk_kernel<NH, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
         attr_set[ctx->device & 63] = true;
     }
-    prof_mark(ctx, "paged_chunk", 4.0 * p.rows * p.H * (double)p.max_kv * c->head_dim, 0.0, st);
+    prof_mark(ctx, "paged_chunk", 0.0, 0.0, st);
     // (rows * q_heads is below 2^31, so that there are no more than 2^24 tiles)
     const unsigned layer = std::min(pp.tiles, 65535);
     const dim3 grid = pp.planned ? dim3(pp.most_units) : dim3((unsigned)c->heads * (unsigned)c->seqs, layer, ((unsigned)pp.tiles + layer - 1) / layer);
