@@ -152,9 +152,6 @@ __device__ __forceinline__ void add_sums(float2& to, float2 x) {
     to = make_float2(top, to.y * ex2_approx(to.x - base) + x.y * ex2_approx(x.x - base));
 }
 
-__device__ __forceinline__ void copy_async16(void* to_shared, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to_shared)), "l"(from) : "memory");
-}
 // an arrival when this thread's copies so far are there (the barrier's count has room for it)
 __device__ __forceinline__ void copy_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -903,7 +900,7 @@ struct ChunkShape {
 };
 
 // A piece of a tile's keys, [blocks from, to): what one CTA does.  first, pieces: the tile's pieces are units first .. first + pieces - 1.
-struct ChunkUnit { int s, head, tile, from, to, first, pieces, unused; };
+struct alignas(16) ChunkUnit { int s, head, tile, from, to, first, pieces; };
 
 struct PagedChunkParams {
     PagedAttParams a;
@@ -929,6 +926,7 @@ __device__ __forceinline__ int tile_blocks(int n, int kv, int tile, int tokens) 
 // How few tiles are cut into pieces: by the number of pieces of the longest one for which (rounds of CTAs) * (blocks of a piece and what a
 // piece costs beside them) is least.  One block of threads, some microseconds; where there are tiles enough (the host's bound), they are
 // not cut and this does not run.
+static_assert(sizeof(ChunkUnit) == 32, "room for units: paged_plan.h");
 constexpr int PL_THREADS = 512;
 __global__ void __launch_bounds__(PL_THREADS)
 paged_plan_kernel(const PagedChunkParams pp) {
@@ -1027,7 +1025,7 @@ paged_plan_kernel(const PagedChunkParams pp) {
             if (u >= pp.most_units) continue;
             ChunkUnit c;
             c.s = seq[t]; c.head = head; c.tile = idx[t]; c.from = min(i * per, nb[t]); c.to = min((i + 1) * per, nb[t]);
-            c.first = u - i; c.pieces = pieces; c.unused = 0;
+            c.first = u - i; c.pieces = pieces;
             pp.units[u] = c;
             pp.arrived[u] = 0u;
         }

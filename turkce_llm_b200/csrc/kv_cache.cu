@@ -56,9 +56,6 @@ struct AppendParams {
 
 // eight elements as they lie in memory, and as float32
 template <bool BF16_IN> struct Raw8 { uint4 w[BF16_IN ? 1 : 2]; };
-__device__ __forceinline__ void copy_async16(void* to_shared, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to_shared)), "l"(from) : "memory");
-}
 __device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }

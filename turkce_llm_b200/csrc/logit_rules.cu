@@ -77,7 +77,7 @@ logit_rules_kernel(const LogitParams p) {
     };
     early(r.prompt, r.prompt_ld, ids[0]);
     early(r.output, r.output_ld, ids[1]);
-    int lens[2] = {r.prompt ? r.prompt_len[row * r.prompt_len_stride] : 0, r.output ? r.output_len[row * r.output_len_stride] : 0};
+    int lens[2] = {r.prompt ? r.prompt_len[row] : 0, r.output ? r.output_len[row] : 0};
     float rep = r.repetition ? r.repetition[row] : 1.0f;
     rep = rep >= LR_LEAST && rep <= LR_MOST ? rep : 1.0f;        // (its inverse or a remainder may be outside float32; or it is none)
     const float freq = r.frequency ? r.frequency[row] : 0.0f,
@@ -267,8 +267,8 @@ extern "C" int tb_logits_adjust(const TbLogitRules* rules, const float* d_logits
     TB_CHECK(!r.mask || (r.masks > 0 && r.mask_ld >= (vocab + 31) / 32), "tb_logits_adjust: masks need %d words each", (vocab + 31) / 32);
     TB_CHECK(!r.mask || r.mask_row || r.masks >= rows, "tb_logits_adjust: %d masks for %d rows need mask_row", r.masks, rows);
     LogitRuleArgs a;
-    a.prompt = r.prompt; a.prompt_len = r.prompt_len; a.prompt_ld = r.prompt_ld; a.prompt_len_stride = 1;
-    a.output = r.output; a.output_len = r.output_len; a.output_ld = r.output_ld; a.output_len_stride = 1;
+    a.prompt = r.prompt; a.prompt_len = r.prompt_len; a.prompt_ld = r.prompt_ld;
+    a.output = r.output; a.output_len = r.output_len; a.output_ld = r.output_ld;
     a.repetition = r.repetition; a.frequency = r.frequency; a.presence = r.presence;
     a.bias_start = r.bias_start; a.bias_id = r.bias_id; a.bias_value = r.bias_value; a.bias_entries = r.bias_entries;
     a.mask = r.mask; a.mask_row = r.mask_row; a.masks = r.masks; a.mask_ld = r.mask_ld;

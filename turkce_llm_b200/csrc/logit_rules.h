@@ -1,5 +1,5 @@
-// The rules on logits as the library's own callers give them (the entry point's arrays, and a step between a row's lengths, 0
-// where all rows share one), and how rows are cut into slices.  The slices are host arithmetic without CUDA types.
+// The rules on logits as their kernel has them (the entry point's arrays), and how rows are cut into slices.  The slices are host arithmetic
+// without CUDA types.
 #pragma once
 #include <cstdint>
 
@@ -7,7 +7,8 @@ namespace tb {
 
 constexpr int kLogitSlice = 4096;         // most columns per CTA: four per thread in two rounds
 
-// Columns of the vocabulary per CTA: a multiple of 32 (a mask word belongs to one CTA) up to 4096.  As many as give every SM
+// Columns of the vocabulary per CTA: a multiple of 32 up to 4096, a few words of a mask.  (Where slices begin in front of it, at a whole
+// 16-byte piece of the logits, two CTAs read the word between them.)  As many as give every SM
 // four CTAs, so that few rows spread over the chip and many rows do not read their ids more often than needed.
 inline int logit_rules_slice(int rows, int V, int sms) {
     const long long want = 4LL * sms;
@@ -18,8 +19,8 @@ inline int logit_rules_slice(int rows, int V, int sms) {
 }
 
 struct LogitRuleArgs {
-    const uint32_t* prompt = nullptr; const int* prompt_len = nullptr; int prompt_ld = 0, prompt_len_stride = 1;
-    const uint32_t* output = nullptr; const int* output_len = nullptr; int output_ld = 0, output_len_stride = 1;
+    const uint32_t* prompt = nullptr; const int* prompt_len = nullptr; int prompt_ld = 0;
+    const uint32_t* output = nullptr; const int* output_len = nullptr; int output_ld = 0;
     const float *repetition = nullptr, *frequency = nullptr, *presence = nullptr;
     const int* bias_start = nullptr; const uint32_t* bias_id = nullptr; const float* bias_value = nullptr; int bias_entries = 0;
     const uint32_t* mask = nullptr; const int* mask_row = nullptr; int masks = 0, mask_ld = 0;

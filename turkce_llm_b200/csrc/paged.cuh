@@ -94,6 +94,10 @@ __device__ __forceinline__ float2 e4m3_floats(uint32_t two) {
     asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(f.x), "=f"(f.y) : "r"(h));
     return f;
 }
+// 16 bytes on their way to shared memory, by this thread
+__device__ __forceinline__ void copy_async16(void* to_shared, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to_shared)), "l"(from) : "memory");
+}
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
