@@ -151,6 +151,30 @@ def test_chunks_of_values_at_the_ends_of_their_range(tb, dim, exponent):
     assert (np.abs(lse - want_lse) <= score + 2.0 ** -15 + 2.0 ** -20 * (1 + np.abs(want_lse))).all()
 
 
+def test_a_value_above_float32_counts_once(tb):
+    """A code times a scale of 2^121 is more than float32 has, its product with a small probability is not; beside a code that is none in another
+    column (such codes are added by themselves)."""
+    b = Batch(True, [40], [240], 1, 64, 16, seed=7)
+    page, slot = at(b, 0, np.arange(240))
+    b.host["k"][page, 0, slot] = 0
+    b.host["k_scale"][page, 0, slot] = 1.0
+    b.host["k"][page[210], 0, slot[210], 0] = 0xfe              # -448
+    b.host["k_scale"][page[210], 0, slot[210]] = np.float32(20 * np.log(2) / 448 * 8)
+    b.host["v"][page[210], 0, slot[210]] = 0x7e                 # 448
+    b.host["v_scale"][page[210], 0, slot[210]] = 2.0 ** 121
+    b.host["v"][page[205], 0, slot[205], 7] = 0x7f
+    upload(b)
+    q = torch.zeros(43, 64, dtype=torch.bfloat16)
+    q[:, 0] = 1.0
+    _, got, _ = attend(b, 1, seed=28, q=q)
+    seen = np.arange(210, 240)                                  # rows that see it: 2^-20 of its value over the other keys' number
+    want = 448.0 * 2.0 ** 121 * 2.0 ** -20 / (seen + 2.0 ** -20)
+    got = got[10:, 0]
+    assert np.isnan(got[:, 7]).all()
+    # (the score 2^-17 of itself off by float32 and the scale's rounding, f16 twice, bf16)
+    assert (np.abs(np.delete(got, 7, axis=1) / want[:, None] - 1) <= 2.0 ** -8 + 2 * 2.0 ** -11 + 2.0 ** -14).all()
+
+
 # ---------------------------------------------------------------------------------------------- pages outside the pool
 
 @pytest.mark.parametrize("bad", [-1, 1 << 20, 0x7fffffff])

@@ -1055,8 +1055,10 @@ __device__ __forceinline__ void add_what_is_not_finite(const PagedAttParams& p, 
 #pragma unroll 1
         for (int d = 0; d < p.v.hd; ++d) {
             if (((d >> 5) & 1) != b) continue;
-            const float x = E4M3 ? e4m3_floats(V[at * p.v.hd + d]).x * scale : __bfloat162float(reinterpret_cast<const bf16*>(V)[at * p.v.hd + d]);
-            if (fabsf(x) < INFINITY) continue;
+            // (8 bits: a code and a scale that are numbers are in the product, even if theirs is more than float32 has)
+            const float value = E4M3 ? e4m3_floats(V[at * p.v.hd + d]).x : __bfloat162float(reinterpret_cast<const bf16*>(V)[at * p.v.hd + d]);
+            if (fabsf(value) < INFINITY && fabsf(scale) < INFINITY) continue;
+            const float x = value * scale;
             bf16* o = reinterpret_cast<bf16*>(row + (d >> 6) * PT_TILE + ((((d & 63) >> 3) ^ (r & 7)) << 4)) + (d & 7);
             *o = __float2bfloat16_rn(__bfloat162float(*o) + x);
         }
