@@ -261,8 +261,12 @@ int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_
  * scale positive.  d_lse (optional): float [rows, q_heads], natural
  * log of the row's sum of exponentials.  Keys behind a row's position have no influence on it, whatever they hold.  A row without
  * any key (kv_len below the number of new rows) gets zeros and lse -infinity.  Keys that score minus infinity have no weight beside others.
- * 8-bit rows: scores are exact but for 2^-21 of a row's largest query element; next to a row's largest probability those of 2^-32 of it
- * and more count, and values of 2^-31 of the sequence's largest scale and more.
+ * Arithmetic: scores, sums and accumulators are float32.  Probabilities are rounded in front of their product with the values, to bf16 (half a
+ * step: 2^-8) beside bf16 values, to f16 (2^-11) beside 8-bit ones; the sum beside them is not.  8-bit rows: a query's elements count down to
+ * 2^-21 of its largest.  Up to 16 query rows per key head (new tokens times the heads that share it): a score carries its value's scale, and
+ * is off by 2^-17 (in log2) by that; a product of probability and scale counts down to 2^-38 of the row's largest.  More rows: a value is
+ * rounded to f16 against the largest scale that the row sees (2^-11 of it, 2^-31 of that scale where it is small); probabilities count down
+ * to 2^-32 of the largest, in the blocks of 128 keys that not all rows see together with what the key's scale lacks to that largest one.
  * max_q and max_kv bound the new rows and the keys of any one sequence (host numbers: they size the launch, and a captured
  * call may be replayed with any lengths within them).  d_workspace: 16-byte aligned (NULL where the call needs none), zero before its
  * first use; every call leaves it ready for the next one, of whatever sizes and types.  tb_attention_paged_workspace(..): bytes that no

@@ -79,8 +79,8 @@ __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0
 // behind it p' may be no number that float32 has, and the sum would lose a key whose value is small beside another.  (A row of zeros has
 // the smallest scale there is, 2^-126.)  Rows that have seen such a key get their sum at the item's end, from the keys once more.
 //
-// Bound: memory; 64 sequences of 16,000 keys, 6 heads of 64: bf16 6.7 TB/s, 8 bits 5.2 TB/s, there by the instructions around the
-// conversions (43 % of the issue slots of 12 warps that wait for one another's loads).  A call of 40 us loses 4 us before its first block is
+// Bound: memory; 64 sequences of 16,000 keys, 6 heads of 64: bf16 6.7 TB/s, 8 bits 5.1 TB/s, there by the instructions around the
+// conversions (42 % of the issue slots of 12 warps that wait for one another's loads; 120 bytes of registers spilled).  A call of 40 us loses 4 us before its first block is
 // there and 2 to 4 us to the spread of its CTAs' ends.
 constexpr float PA_UP = 13.f;
 // The reference of a row that has seen no key yet, or keys that score minus infinity alone: lower than any score, but a number, so that minus
@@ -351,7 +351,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 }
                 if (E4M3) {
                     // four scales per copy: of keys, then of values.  (A bulk copy per piece of a page and array: 225 us instead of 192 for
-                    // 64 sequences of 16,000 keys in pages of 16, 6 heads of 64; 163 instead of 162 in pages of 64.)
+                    // 64 sequences of 16,000 keys in pages of 16, 6 heads of 64; as fast in pages of 64.)
                     float* sc = reinterpret_cast<float*>(smem + Sh::O_SCALE + st * Sh::SCALES);
 #pragma unroll
                     for (int x = 0; x < KEYS / 64; ++x) {
@@ -867,7 +867,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 // Bound: a group's way through a block.  Clocks per block of 64 keys, bf16 heads of 64 (two CTAs per SM) / of 128 / 8 bits of 128: scores to
 // come 510 / 570 / 630, from tensor memory 250 / 150 / 290, maximum 300, product before to end 270 / 190 / 290, exponentials and their way
 // back 1,680 / 1,140 / 1,250.  Neither fewer loads, nor a quarter of the products, nor no exponentials at all change the total by more than
-// 10 %.  2 x 512 rows of 8 heads of 128 behind 32,000 keys: bf16 158 us (856 TFLOP/s), 8 bits 196 us (690 TFLOP/s).
+// 10 %.  2 x 512 rows of 8 heads of 128 behind 32,000 keys: bf16 159 us (851 TFLOP/s), 8 bits 200 us (675 TFLOP/s; 196 before every row had
+// its own largest scale at the edge).
 //
 // A row's reference m follows its largest score only when that lies more than PT_SLACK above it (log2): every sum and product is against
 // the same m, so the result is the same, probabilities reach 2^8 at most, and the accumulators are seldom scaled (104 -> 94.6 us).
