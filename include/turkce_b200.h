@@ -264,7 +264,8 @@ int tb_kv_read(const TbKvCache* cache, const int32_t* d_start, const int32_t* d_
  * Arithmetic: scores, sums and accumulators are float32.  Probabilities are rounded in front of their product with the values, to bf16 (half a
  * step: 2^-8) beside bf16 values, to f16 (2^-11) beside 8-bit ones; the sum beside them is not.  8-bit rows: a query's elements count down to
  * 2^-21 of its largest.  Up to 16 query rows per key head (new tokens times the heads that share it): a score carries its value's scale, and
- * is off by 2^-17 (in log2) by that; a product of probability and scale counts down to 2^-38 of the row's largest.  More rows: a value is
+ * is off by 2^-17 (in log2) by that; a product of probability and scale counts down to 2^-38 of the row's largest (values of rows with the
+ * smallest scale, 2^-126, may count as zeros).  More rows: a value is
  * rounded to f16 against the largest scale that the row sees (2^-11 of it, 2^-31 of that scale where it is small); probabilities count down
  * to 2^-32 of the largest, in the blocks of 128 keys that not all rows see together with what the key's scale lacks to that largest one.
  * max_q and max_kv bound the new rows and the keys of any one sequence (host numbers: they size the launch, and a captured

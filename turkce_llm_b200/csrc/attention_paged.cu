@@ -75,9 +75,10 @@ __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0
 // Codes become f16, which holds each of them, against queries in f16 (a row scaled by a power of two).  The exponent e of a value's scale is
 // added to the score before the maximum is taken, so that probabilities, which become f16, carry it: p' = 2^(s + e - m), against 2^-13 of
 // the largest: at most 2^15 with what is left of the scale, and products of probability and scale down to 2^-38 of the largest count.  The sum
-// takes the exponent back, l = sum of p' 2^(B - e) with B the exponent at the item's first key.  That holds while every e lies within NEAR of B;
-// behind it p' may be no number that float32 has, and the sum would lose a key whose value is small beside another.  (A row of zeros has
-// the smallest scale there is, 2^-126.)  Rows that have seen such a key get their sum at the item's end, from the keys once more.
+// takes the exponent back, l = sum of p' 2^(B - e) with B the largest exponent of the item's first 32 keys, of those that all its rows see.  That
+// holds while every e lies within NEAR of B; behind it p' may be no number that float32 has, and the sum would lose a key whose value is
+// small beside another.  Rows that have seen such a key get their sum at the item's end, from the keys once more (64 sequences of 16,000
+// keys: 820 us).  Rows of zeros, which have the smallest scale there is (SCALE_LEAST), count as B - NEAR: what is lost is below 2^-117.
 //
 // Bound: memory; 64 sequences of 16,000 keys, 6 heads of 64: bf16 6.7 TB/s, 8 bits 5.1 TB/s, there by the instructions around the
 // conversions (42 % of the issue slots of 12 warps that wait for one another's loads; 120 bytes of registers spilled).  A call of 40 us loses 4 us before its first block is
@@ -142,6 +143,7 @@ __device__ __forceinline__ float power_of_two(int n) { return __uint_as_float((u
 // The exponent of a value's scale as float32 keeps it: a scale is 2^(exponent - 127) * part with |part| < 2, below 4 where it is above 2^126.
 // 0: infinity or NaN, their own part with any exponent.
 constexpr int NEAR = 40;
+constexpr float SCALE_LEAST = 0x1p-126f;
 __device__ __forceinline__ int scale_exponent(float s) {
     const int e = (int)(__float_as_uint(s) >> 23) & 255;
     return e == 255 ? 0 : min(max(e, 1), 253);
@@ -464,8 +466,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 m[x] = PA_LOW; l[x] = 0.f;
             }
             if (E4M3) {
-                const float vs = reinterpret_cast<const float*>(smem + Sh::O_SCALE + st * Sh::SCALES)[KEYS];
-                if (lane <= K_FAR) known[lane] = lane == K_BASE ? max(scale_exponent(vs), 1) : lane == K_FIRST ? what.y : 0x7fffffff;
+                const float vs = reinterpret_cast<const float*>(smem + Sh::O_SCALE + st * Sh::SCALES)[KEYS + lane];
+                const int base = __reduce_max_sync(0xffffffffu, (lane == 0 || what.y + lane <= first_pos) && vs > SCALE_LEAST ? scale_exponent(vs) : 0);
+                if (lane <= K_FAR) known[lane] = lane == K_BASE ? max(base, 1) : lane == K_FIRST ? what.y : 0x7fffffff;
                 __syncwarp();
             }
 #pragma unroll
@@ -482,7 +485,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     const float vs = sc[KEYS + lane];
                     const int B = known[K_BASE];
                     int e = scale_exponent(vs);
-                    e = e == 0 ? B : e;
+                    e = e == 0 ? B : vs == SCALE_LEAST ? max(B - NEAR, 1) : e;
                     const int off = e - B, near = min(max(off, -NEAR), NEAR);
                     parts[lane] = make_float4(sc[lane], __uint_as_float(0x4b000000u | (uint32_t)e) - 8388735.0f /* e - 127 */, vs * power_of_two(127 - e),
                                               power_of_two(-near));
