@@ -308,3 +308,23 @@ def test_codes_of_rows_of_any_size_are_the_nearest(tb, exponent):
     assert (b.dev["v_scale"].cpu().numpy()[page, 0, slot] == scale).all()
     codes = b.dev["v"].view(torch.uint8).cpu().numpy()[page, 0, slot]
     assert (codes == plain.e4m3_codes(x, scale[:, None])).all(), (codes != plain.e4m3_codes(x, scale[:, None])).sum()
+
+
+@pytest.mark.parametrize("new", [1, 8, 40])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [2.0 ** 126, 1.5 * 2.0 ** 127])
+def test_the_largest_queries_of_8_bit_rows(tb, dim, new, size):
+    """A query element as large as bf16 has: the scores are numbers, and one key has all of the weight."""
+    b = Batch(True, [new], [200 + new], 1, dim, 16, seed=8)
+    page, slot = at(b, 0, np.arange(200 + new))
+    b.host["k_scale"][page, 0, slot] = 2.0 ** -12
+    b.host["k"][page, 0, slot, 3] = np.random.default_rng(2).permutation(200 + new) % 100   # (the largest of them: 99, twice at most)
+    b.host["k"][page[150], 0, slot[150], 3] = 0x7e
+    upload(b)
+    q = torch.randn(new + 3, 2 * dim).to(torch.bfloat16)
+    q[:, 3] = q[:, dim + 3] = size
+    _, got, lse = attend(b, 2, seed=29, q=q)
+    want = b.sequence("v", 0)[150, 0]
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want)).all()
+    score = float(torch.tensor(size).to(torch.bfloat16)) * 448 * 2.0 ** -12 * dim ** -0.5
+    assert (np.abs(lse / score - 1) <= 2.0 ** -18).all()

@@ -84,9 +84,9 @@ __device__ __forceinline__ bool batch_of(const PagedAttParams& p, int s, int& q0
 // conversions (42 % of the issue slots of 12 warps that wait for one another's loads; 120 bytes of registers spilled).  A call of 40 us loses 4 us before its first block is
 // there and 2 to 4 us to the spread of its CTAs' ends.
 constexpr float PA_UP = 13.f;
-// The reference of a row that has seen no key yet, or keys that score minus infinity alone: lower than any score, but a number, so that minus
+// The reference of a row that has seen no key yet, or keys that score minus infinity alone: no score is lower, but it is a number, so that minus
 // infinity is below it and not beside it.
-constexpr float PA_LOW = -3.0e38f;
+constexpr float PA_LOW = -3.402823466e38f;
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = (PA_WARPS + 1) * 32;
 constexpr int PA_SCAN = 4;               // sequences per lane of one look at the batch
@@ -445,13 +445,13 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                         }
                     }
                 if (E4M3) {
-                    // as f16, the row scaled by a power of two so that its largest magnitude lies in [1, 2): exact but for what is
-                    // less than 2^-24 of it
+                    // as f16, the row scaled by a power of two so that its largest magnitude lies in [1, 2), or below 4: exact but for
+                    // what is less than 2^-24 of it
                     big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
                     big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                    const int e = max((int)(big >> 7), 1);                             // (biased; 255: infinity or NaN)
-                    const float down = __uint_as_float((uint32_t)min(254 - e, 253) << 23), up = __uint_as_float((uint32_t)e << 23);
-                    const bool odd = e >= 254;                                         // (2^(127 - e) would be no normal number)
+                    const bool odd = big >> 7 == 255u;                                 // (an infinity or NaN)
+                    const int e = min(max((int)(big >> 7), 1), 253);                   // (2^(127 - e) and its inverse are normal numbers)
+                    const float down = power_of_two(127 - e), up = power_of_two(e - 127);
                     row_factor[x] = odd ? p.scale_log2 : p.scale_log2 * up;
 #pragma unroll
                     for (int b = 0; b < NH; ++b)
@@ -657,6 +657,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll 1
                     for (int t = 0; t < KW; t += 8) {
                         // (lane (r, c): elements 16 c .. of key t0 + t + r; products with keys t0 + t + 2 c and the next)
+                        __syncwarp();
                         auto row_of = [&](int key) -> long long {
                             const int page = key <= last_pos ? table[key >> p.v.page_shift] : -1;
                             if ((unsigned)page >= (unsigned)p.v.pages) return -1;
